@@ -1280,6 +1280,281 @@ at::Tensor Hif8EmbeddingLookupMeta(const at::Tensor &ids, const at::Tensor &weig
   return at::empty(shape, weight.options().dtype(at::kBFloat16));
 }
 
+// ------------------------------------------------ rows of the KV cache
+// Attention of drafted tokens, decode attention with key weights, key weights of
+// many rows, acceptance of drafts and eviction.
+
+struct PagedOperands {
+  int64_t kv_heads, d, dv, block_size, num_blocks, max_blocks;
+  int bt_code;
+};
+
+// Checks the caches, the table and the request lengths that these operators share.
+PagedOperands CheckPaged(const at::Tensor &key_cache, const at::Tensor *value_cache, const at::Tensor &block_table,
+                         const at::Tensor &lens, const char *lens_name, int64_t batch, int64_t max_seq_len) {
+  TORCH_CHECK(key_cache.dim() == 4 && (!value_cache || value_cache->dim() == 4),
+              "caches must have shape [num_blocks, block_size, num_kv_heads, width]");
+  PagedOperands o{};
+  o.kv_heads = key_cache.size(2);
+  o.d = key_cache.size(3) - 4;
+  CheckCache(key_cache, "key_cache", o.kv_heads, o.d + 4);
+  TORCH_CHECK(o.d > 0, "key_cache rows are too short");
+  const auto device = key_cache.device();
+  if (value_cache) {
+    o.dv = value_cache->size(3) - 4;
+    CheckCache(*value_cache, "value_cache", o.kv_heads, o.dv + 4);
+    TORCH_CHECK(o.dv > 0, "value_cache rows are too short");
+    TORCH_CHECK(value_cache->size(0) == key_cache.size(0) && value_cache->size(1) == key_cache.size(1),
+                "key_cache and value_cache must have the same blocks");
+    CheckSameDevice(*value_cache, device, "value_cache");
+  }
+  CheckContiguousDevice(block_table, "block_table");
+  o.bt_code = IndexCode(block_table, "block_table");
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) >= batch && block_table.size(1) > 0,
+              "block_table must have shape [batch, max_blocks]");
+  CheckSameDevice(block_table, device, "block_table");
+  CheckContiguousDevice(lens, lens_name);
+  TORCH_CHECK(lens.scalar_type() == at::ScalarType::Int, lens_name, " must have dtype torch.int32");
+  TORCH_CHECK(lens.dim() == 1 && lens.numel() >= batch, lens_name, " must contain one length per request");
+  CheckSameDevice(lens, device, lens_name);
+  o.block_size = key_cache.size(1);
+  o.num_blocks = key_cache.size(0);
+  o.max_blocks = block_table.size(1);
+  TORCH_CHECK(max_seq_len >= 0 && max_seq_len <= o.max_blocks * o.block_size,
+              "max_seq_len must be within the block table capacity");
+  return o;
+}
+
+void CheckQuery(const at::Tensor &query, const PagedOperands &o, const at::Device &device) {
+  CheckContiguousDevice(query, "query");
+  TORCH_CHECK(query.scalar_type() == at::ScalarType::Half || query.scalar_type() == at::ScalarType::BFloat16,
+              "query must have dtype torch.float16 or torch.bfloat16");
+  TORCH_CHECK(query.dim() == 3, "query must have shape [tokens, num_heads, head_size]");
+  TORCH_CHECK(query.size(1) > 0 && query.size(2) == o.d, "query head size must match the key cache");
+  TORCH_CHECK(query.size(1) % o.kv_heads == 0, "num_heads must be divisible by num_kv_heads");
+  CheckSameDevice(query, device, "query");
+}
+
+int64_t CheckStartLoc(const at::Tensor &query_start_loc, const at::Device &device) {
+  CheckContiguousDevice(query_start_loc, "query_start_loc");
+  TORCH_CHECK(query_start_loc.scalar_type() == at::ScalarType::Int && query_start_loc.dim() == 1 &&
+                  query_start_loc.numel() >= 1,
+              "query_start_loc must be an int32 tensor [batch + 1]");
+  CheckSameDevice(query_start_loc, device, "query_start_loc");
+  return query_start_loc.numel() - 1;
+}
+
+void CheckKeyWeights(const at::Tensor &w, int64_t batch, int64_t kv_heads, int64_t max_seq_len,
+                     const at::Device &device) {
+  CheckContiguousDevice(w, "key_weights");
+  TORCH_CHECK(w.scalar_type() == at::ScalarType::Float, "key_weights must have dtype torch.float32");
+  TORCH_CHECK(w.dim() == 3 && w.size(0) >= batch && w.size(1) == kv_heads && w.size(2) >= max_seq_len,
+              "key_weights must have shape [batch, num_kv_heads, at least max_seq_len]");
+  CheckSameDevice(w, device, "key_weights");
+}
+
+at::Tensor Workspace(size_t bytes, const at::Tensor &like) {
+  return bytes ? at::empty({int64_t(bytes)}, like.options().dtype(at::ScalarType::Byte)) : at::Tensor();
+}
+
+void *WorkspacePtr(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+at::Tensor Hif8TreeAttention(const at::Tensor &query, const at::Tensor &key_cache, const at::Tensor &value_cache,
+                             const at::Tensor &block_table, const at::Tensor &query_start_loc,
+                             const at::Tensor &context_lens, const at::Tensor &tree_mask, double scale,
+                             int64_t max_query_len, int64_t max_seq_len) {
+  const int64_t batch = CheckStartLoc(query_start_loc, key_cache.device());
+  const auto o = CheckPaged(key_cache, &value_cache, block_table, context_lens, "context_lens", batch, max_seq_len);
+  CheckQuery(query, o, key_cache.device());
+  CheckContiguousDevice(tree_mask, "tree_mask");
+  TORCH_CHECK(tree_mask.scalar_type() == at::ScalarType::Bool || tree_mask.scalar_type() == at::ScalarType::Byte,
+              "tree_mask must have dtype torch.bool or torch.uint8");
+  TORCH_CHECK(max_query_len >= 0, "max_query_len must be non-negative");
+  TORCH_CHECK(tree_mask.dim() == 2 && tree_mask.size(0) == query.size(0) && tree_mask.size(1) >= max_query_len,
+              "tree_mask must have shape [tokens, at least max_query_len]");
+  CheckSameDevice(tree_mask, key_cache.device(), "tree_mask");
+  const c10::OptionalDeviceGuard guard(query.device());
+  auto out = at::empty({query.size(0), query.size(1), o.dv}, query.options());
+  if (batch == 0 || query.size(0) == 0 || max_query_len == 0) return out;
+  const size_t bytes = hif8_tree_attention_workspace_size(batch, query.size(1), o.kv_heads, o.d, o.dv, query.size(0),
+                                                          max_query_len, max_seq_len);
+  const auto ws = Workspace(bytes, query);
+  CheckStatus(hif8_tree_attention(query.data_ptr(), DtypeCode(query.scalar_type()), key_cache.data_ptr<uint8_t>(),
+                                  value_cache.data_ptr<uint8_t>(), o.num_blocks, o.block_size, o.kv_heads, o.d, o.dv,
+                                  block_table.data_ptr(), o.bt_code, o.max_blocks, query_start_loc.data_ptr<int32_t>(),
+                                  context_lens.data_ptr<int32_t>(), static_cast<const uint8_t *>(tree_mask.data_ptr()),
+                                  tree_mask.size(1), batch, query.size(1), query.size(0), max_query_len, max_seq_len,
+                                  float(scale), out.data_ptr(), WorkspacePtr(ws), bytes, CurrentStream(query.device())),
+              "hif8_tree_attention");
+  return out;
+}
+
+at::Tensor Hif8PagedDecodeAttentionWeights(const at::Tensor &query, const at::Tensor &key_cache,
+                                           const at::Tensor &value_cache, const at::Tensor &block_table,
+                                           const at::Tensor &seq_lens, const at::Tensor &key_weights, double scale,
+                                           int64_t max_seq_len, bool accumulate) {
+  TORCH_CHECK(query.dim() == 3, "query must have shape [batch, num_heads, head_size]");
+  const int64_t batch = query.size(0);
+  const auto o = CheckPaged(key_cache, &value_cache, block_table, seq_lens, "seq_lens", batch, max_seq_len);
+  CheckQuery(query, o, key_cache.device());
+  CheckKeyWeights(key_weights, batch, o.kv_heads, max_seq_len, key_cache.device());
+  MarkChanged(key_weights);
+  const c10::OptionalDeviceGuard guard(query.device());
+  auto out = at::empty({batch, query.size(1), o.dv}, query.options());
+  if (batch == 0) return out;
+  const size_t bytes =
+      hif8_paged_decode_attention_weights_workspace_size(batch, query.size(1), o.kv_heads, o.d, o.dv, max_seq_len);
+  const auto ws = Workspace(bytes, query);
+  CheckStatus(hif8_paged_decode_attention_weights(
+                  query.data_ptr(), DtypeCode(query.scalar_type()), key_cache.data_ptr<uint8_t>(),
+                  value_cache.data_ptr<uint8_t>(), o.num_blocks, o.block_size, o.kv_heads, o.d, o.dv,
+                  block_table.data_ptr(), o.bt_code, o.max_blocks, seq_lens.data_ptr<int32_t>(), batch, query.size(1),
+                  max_seq_len, float(scale), out.data_ptr(), key_weights.data_ptr<float>(), key_weights.size(2),
+                  accumulate ? 1 : 0, WorkspacePtr(ws), bytes, CurrentStream(query.device())),
+              "hif8_paged_decode_attention_weights");
+  return out;
+}
+
+void Hif8KeyWeights(const at::Tensor &query, const at::Tensor &key_cache, const at::Tensor &block_table,
+                    const at::Tensor &query_start_loc, const at::Tensor &seq_lens, const at::Tensor &key_weights,
+                    double scale, int64_t max_query_len, int64_t max_seq_len, bool causal, bool accumulate) {
+  const int64_t batch = CheckStartLoc(query_start_loc, key_cache.device());
+  const auto o = CheckPaged(key_cache, nullptr, block_table, seq_lens, "seq_lens", batch, max_seq_len);
+  CheckQuery(query, o, key_cache.device());
+  CheckKeyWeights(key_weights, batch, o.kv_heads, max_seq_len, key_cache.device());
+  TORCH_CHECK(max_query_len >= 0, "max_query_len must be non-negative");
+  MarkChanged(key_weights);
+  if (batch == 0) return;
+  const c10::OptionalDeviceGuard guard(query.device());
+  const size_t bytes = hif8_key_weights_workspace_size(batch, query.size(1), o.kv_heads, o.d, query.size(0),
+                                                       max_query_len, max_seq_len);
+  const auto ws = Workspace(bytes, query);
+  CheckStatus(hif8_key_weights(query.data_ptr(), DtypeCode(query.scalar_type()), key_cache.data_ptr<uint8_t>(),
+                               o.num_blocks, o.block_size, o.kv_heads, o.d, block_table.data_ptr(), o.bt_code,
+                               o.max_blocks, query_start_loc.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), batch,
+                               query.size(1), query.size(0), max_query_len, max_seq_len, float(scale), causal ? 1 : 0,
+                               key_weights.data_ptr<float>(), key_weights.size(2), accumulate ? 1 : 0,
+                               WorkspacePtr(ws), bytes, CurrentStream(query.device())),
+              "hif8_key_weights");
+}
+
+at::Tensor Hif8AcceptDrafts(at::TensorList caches, const at::Tensor &block_table, const at::Tensor &context_lens,
+                            const at::Tensor &accepted, const at::Tensor &accepted_counts) {
+  TORCH_CHECK(!caches.empty(), "hif8_accept_drafts needs at least one cache");
+  TORCH_CHECK(accepted.dim() == 2 && accepted.scalar_type() == at::ScalarType::Int,
+              "accepted must be an int32 tensor [batch, width]");
+  const int64_t batch = accepted.size(0);
+  std::vector<void *> ptrs;
+  std::vector<int64_t> row_bytes;
+  for (const auto &c : caches) {
+    TORCH_CHECK(c.dim() == 4, "caches must have shape [num_blocks, block_size, num_kv_heads, width]");
+    const auto o = CheckPaged(c, nullptr, block_table, context_lens, "context_lens", batch, 0);
+    TORCH_CHECK(c.size(0) == caches[0].size(0) && c.size(1) == caches[0].size(1),
+                "all caches must have the same blocks");
+    ptrs.push_back(c.data_ptr());
+    row_bytes.push_back(o.kv_heads * (o.d + 4));
+    MarkChanged(c);
+  }
+  const auto device = caches[0].device();
+  CheckContiguousDevice(accepted, "accepted");
+  CheckContiguousDevice(accepted_counts, "accepted_counts");
+  TORCH_CHECK(accepted_counts.scalar_type() == at::ScalarType::Int && accepted_counts.dim() == 1 &&
+                  accepted_counts.numel() >= batch,
+              "accepted_counts must contain one int32 count per request");
+  CheckSameDevice(accepted, device, "accepted");
+  CheckSameDevice(accepted_counts, device, "accepted_counts");
+  const c10::OptionalDeviceGuard guard(device);
+  auto lens = at::empty({batch}, context_lens.options());
+  if (batch == 0) return lens;
+  CheckStatus(hif8_accept_drafts(ptrs.data(), row_bytes.data(), int64_t(ptrs.size()), caches[0].size(0),
+                                 caches[0].size(1), block_table.data_ptr(), IndexCode(block_table, "block_table"),
+                                 block_table.size(1), context_lens.data_ptr<int32_t>(),
+                                 accepted.numel() ? accepted.data_ptr<int32_t>() : nullptr, accepted.size(1),
+                                 accepted_counts.data_ptr<int32_t>(), batch, lens.data_ptr<int32_t>(),
+                                 CurrentStream(device)),
+              "hif8_accept_drafts");
+  return lens;
+}
+
+at::Tensor Hif8KVEvict(const at::Tensor &key_cache, const at::Tensor &value_cache, const at::Tensor &block_table,
+                       const at::Tensor &seq_lens, const at::Tensor &key_weights,
+                       const c10::optional<at::Tensor> &positions, const c10::optional<at::Tensor> &keep,
+                       int64_t keep_all, int64_t sinks, const c10::optional<at::Tensor> &protect_from,
+                       int64_t max_seq_len) {
+  TORCH_CHECK(key_weights.dim() == 3, "key_weights must have shape [batch, num_kv_heads, at least max_seq_len]");
+  TORCH_CHECK(seq_lens.dim() == 1, "seq_lens must contain one length per request");
+  const int64_t batch = seq_lens.size(0);
+  const auto o = CheckPaged(key_cache, &value_cache, block_table, seq_lens, "seq_lens", batch, max_seq_len);
+  const auto device = key_cache.device();
+  CheckKeyWeights(key_weights, batch, o.kv_heads, max_seq_len, device);
+  if (positions.has_value()) {
+    CheckContiguousDevice(*positions, "positions");
+    TORCH_CHECK(positions->scalar_type() == at::ScalarType::Int && positions->sizes() == key_weights.sizes(),
+                "positions must be an int32 tensor of the shape of key_weights");
+    CheckSameDevice(*positions, device, "positions");
+    MarkChanged(*positions);
+  }
+  for (const auto *t : {&keep, &protect_from}) {
+    if (!t->has_value()) continue;
+    CheckContiguousDevice(**t, "keep / protect_from");
+    TORCH_CHECK((*t)->scalar_type() == at::ScalarType::Int && (*t)->dim() == 1 && (*t)->numel() >= batch,
+                "keep / protect_from must contain one int32 value per request");
+    CheckSameDevice(**t, device, "keep / protect_from");
+  }
+  MarkChanged(key_cache);
+  MarkChanged(value_cache);
+  MarkChanged(key_weights);
+  const c10::OptionalDeviceGuard guard(device);
+  auto lens = at::empty({batch}, seq_lens.options());
+  if (batch == 0) return lens;
+  const size_t bytes = hif8_kv_evict_workspace_size(batch, o.kv_heads, max_seq_len > 0 ? max_seq_len : 1);
+  const auto ws = Workspace(bytes, key_cache);
+  CheckStatus(hif8_kv_evict(key_cache.data_ptr<uint8_t>(), value_cache.data_ptr<uint8_t>(), o.num_blocks, o.block_size,
+                            o.kv_heads, o.d, o.dv, block_table.data_ptr(), o.bt_code, o.max_blocks,
+                            seq_lens.data_ptr<int32_t>(), batch, max_seq_len, key_weights.data_ptr<float>(),
+                            positions.has_value() ? positions->data_ptr<int32_t>() : nullptr, key_weights.size(2),
+                            keep.has_value() ? keep->data_ptr<int32_t>() : nullptr, keep_all, sinks,
+                            protect_from.has_value() ? protect_from->data_ptr<int32_t>() : nullptr,
+                            lens.data_ptr<int32_t>(), WorkspacePtr(ws), bytes, CurrentStream(device)),
+              "hif8_kv_evict");
+  return lens;
+}
+
+at::Tensor Hif8TreeAttentionMeta(const at::Tensor &query, const at::Tensor &, const at::Tensor &value_cache,
+                                 const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                 double, int64_t, int64_t) {
+  return at::empty({query.size(0), query.size(1), value_cache.size(3) - 4}, query.options());
+}
+
+at::Tensor Hif8PagedDecodeAttentionWeightsMeta(const at::Tensor &query, const at::Tensor &,
+                                               const at::Tensor &value_cache, const at::Tensor &, const at::Tensor &,
+                                               const at::Tensor &key_weights, double, int64_t, bool) {
+  MarkChanged(key_weights);
+  return at::empty({query.size(0), query.size(1), value_cache.size(3) - 4}, query.options());
+}
+
+void Hif8KeyWeightsMeta(const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                        const at::Tensor &, const at::Tensor &key_weights, double, int64_t, int64_t, bool, bool) {
+  MarkChanged(key_weights);
+}
+
+at::Tensor Hif8AcceptDraftsMeta(at::TensorList caches, const at::Tensor &, const at::Tensor &context_lens,
+                                const at::Tensor &accepted, const at::Tensor &) {
+  for (const auto &c : caches) MarkChanged(c);
+  return at::empty({accepted.size(0)}, context_lens.options());
+}
+
+at::Tensor Hif8KVEvictMeta(const at::Tensor &key_cache, const at::Tensor &value_cache, const at::Tensor &,
+                           const at::Tensor &seq_lens, const at::Tensor &key_weights,
+                           const c10::optional<at::Tensor> &positions, const c10::optional<at::Tensor> &, int64_t,
+                           int64_t, const c10::optional<at::Tensor> &, int64_t) {
+  MarkChanged(key_cache);
+  MarkChanged(value_cache);
+  MarkChanged(key_weights);
+  if (positions.has_value()) MarkChanged(*positions);
+  return at::empty({seq_lens.size(0)}, seq_lens.options());
+}
+
 // The decode glue ops (shapes and dtypes of the CUDA implementations above).
 at::Tensor Hif8AddRmsNormMeta(at::Tensor &h, const c10::optional<at::Tensor> &, const at::Tensor &, double) {
   return at::empty_like(h);
@@ -1363,6 +1638,11 @@ TORCH_LIBRARY(vllm_ascend_hif8, m) {
   m.def("hif8_kv_cache_write(Tensor key, Tensor value, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor slot_mapping, Tensor key_scale, Tensor value_scale, Tensor(c!)? invalid_slots=None) -> ()");
   m.def("hif8_paged_decode_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor seq_lens, float scale, int max_seq_len) -> Tensor");
   m.def("hif8_paged_prefill_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor query_start_loc, Tensor seq_lens, float scale, int max_query_len, int max_seq_len, bool causal=True) -> Tensor");
+  m.def("hif8_tree_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor query_start_loc, Tensor context_lens, Tensor tree_mask, float scale, int max_query_len, int max_seq_len) -> Tensor");
+  m.def("hif8_paged_decode_attention_weights(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor seq_lens, Tensor(a!) key_weights, float scale, int max_seq_len, bool accumulate=True) -> Tensor");
+  m.def("hif8_key_weights(Tensor query, Tensor key_cache, Tensor block_table, Tensor query_start_loc, Tensor seq_lens, Tensor(a!) key_weights, float scale, int max_query_len, int max_seq_len, bool causal=True, bool accumulate=True) -> ()");
+  m.def("hif8_accept_drafts(Tensor(a!)[] caches, Tensor block_table, Tensor context_lens, Tensor accepted, Tensor accepted_counts) -> Tensor");
+  m.def("hif8_kv_evict(Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor block_table, Tensor seq_lens, Tensor(c!) key_weights, Tensor(d!)? positions, Tensor? keep, int keep_all, int sinks, Tensor? protect_from, int max_seq_len) -> Tensor");
   m.def("hif8_embedding_lookup(Tensor input_ids, Tensor weight, Tensor weight_scale, Tensor(a!)? invalid_ids=None) -> Tensor");
   m.def("hif8_dynamic_quant(Tensor x) -> (Tensor, Tensor)");
   m.def("soft_hif8_fused_gemm(Tensor activation, Tensor weight, Tensor channel_scale, Tensor? bias, ScalarType output_dtype) -> Tensor");
@@ -1397,6 +1677,11 @@ TORCH_LIBRARY_IMPL(vllm_ascend_hif8, CUDA, m) {
   m.impl("hif8_kv_cache_write", &Hif8KVCacheWrite);
   m.impl("hif8_paged_decode_attention", &Hif8PagedDecodeAttention);
   m.impl("hif8_paged_prefill_attention", &Hif8PagedPrefillAttention);
+  m.impl("hif8_tree_attention", &Hif8TreeAttention);
+  m.impl("hif8_paged_decode_attention_weights", &Hif8PagedDecodeAttentionWeights);
+  m.impl("hif8_key_weights", &Hif8KeyWeights);
+  m.impl("hif8_accept_drafts", &Hif8AcceptDrafts);
+  m.impl("hif8_kv_evict", &Hif8KVEvict);
   m.impl("hif8_embedding_lookup", &Hif8EmbeddingLookup);
   m.impl("hif8_dynamic_quant", &Hif8DynamicQuant);
   m.impl("soft_hif8_fused_gemm", &SoftHif8FusedGemm);
@@ -1430,6 +1715,11 @@ TORCH_LIBRARY_IMPL(vllm_ascend_hif8, Meta, m) {
   m.impl("hif8_kv_cache_write", &Hif8KVCacheWriteMeta);
   m.impl("hif8_paged_decode_attention", &Hif8PagedDecodeAttentionMeta);
   m.impl("hif8_paged_prefill_attention", &Hif8PagedPrefillAttentionMeta);
+  m.impl("hif8_tree_attention", &Hif8TreeAttentionMeta);
+  m.impl("hif8_paged_decode_attention_weights", &Hif8PagedDecodeAttentionWeightsMeta);
+  m.impl("hif8_key_weights", &Hif8KeyWeightsMeta);
+  m.impl("hif8_accept_drafts", &Hif8AcceptDraftsMeta);
+  m.impl("hif8_kv_evict", &Hif8KVEvictMeta);
   m.impl("hif8_embedding_lookup", &Hif8EmbeddingLookupMeta);
   m.impl("hif8_dynamic_quant", &Hif8DynamicQuantMeta);
   m.impl("soft_hif8_fused_gemm", &FusedLinearMeta);

@@ -28,7 +28,8 @@ ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
 HIP_SOURCES = ["capi.hip", "static_quant.hip", "gemv.hip", "gemm.hip", "gemm_skinny.hip",
                "static_operand.hip", "linear_api.hip", "kv_cache.hip",
-               "embedding.hip", "model_ops.hip", "gdn_prefill.hip", "prefill_attention.hip"]
+               "embedding.hip", "model_ops.hip", "gdn_prefill.hip", "prefill_attention.hip",
+               "row_attention.hip", "key_weights.hip", "cache_edit.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",

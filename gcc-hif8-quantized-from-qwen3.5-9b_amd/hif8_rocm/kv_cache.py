@@ -359,13 +359,360 @@ def paged_attention(
         int(max_seq_len), bool(causal))
 
 
+def _device_lengths(lens, name: str, device) -> tuple[torch.Tensor, list[int] | None]:
+    """Request lengths as an int32 device tensor, and as host integers where they came so."""
+    if isinstance(lens, torch.Tensor):
+        return lens.to(device=device, dtype=torch.int32).contiguous(), None
+    host = [int(v) for v in lens]
+    if any(v < 0 for v in host):
+        raise ValueError(f"{name} must be non-negative")
+    return torch.tensor(host, dtype=torch.int32).to(device), host
+
+
+def _device_table(block_table: torch.Tensor, batch: int, device) -> torch.Tensor:
+    if block_table.ndim != 2 or block_table.shape[0] < batch:
+        raise ValueError("block_table must have shape [batch, max_blocks]")
+    table = block_table[:batch]
+    if table.dtype not in (torch.int32, torch.int64):
+        table = table.to(torch.int64)
+    return table.to(device).contiguous()
+
+
+def _request_rows(query, query_lens, query_start_loc, max_query_len, validate: bool):
+    """(query_start_loc on the device, batch, max_query_len, host query lengths or None)."""
+    if (query_lens is None) == (query_start_loc is None):
+        raise ValueError("pass exactly one of query_lens and query_start_loc")
+    if query_lens is not None:
+        host = [int(v) for v in query_lens]
+        if any(v < 0 for v in host) or sum(host) != query.shape[0]:
+            raise ValueError("query_lens must describe every query row")
+        loc = torch.tensor([0] + host, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(query.device)
+        longest = max(host, default=0)
+        if max_query_len is None:
+            max_query_len = longest
+        elif max_query_len < longest:
+            raise ValueError(f"max_query_len ({max_query_len}) is smaller than a request's query length ({longest})")
+        return loc, len(host), int(max_query_len), host
+    if query_start_loc.ndim != 1 or query_start_loc.numel() < 1:
+        raise ValueError("query_start_loc must have shape [batch + 1]")
+    loc = query_start_loc.to(device=query.device, dtype=torch.int32).contiguous()
+    batch = loc.numel() - 1
+    if max_query_len is None or (validate and batch):
+        longest = int((loc[1:] - loc[:-1]).max().item()) if batch else 0
+        if max_query_len is None:
+            max_query_len = longest
+        elif longest > max_query_len:
+            raise ValueError(f"max_query_len ({max_query_len}) is smaller than a request's query length ({longest})")
+    return loc, batch, int(max_query_len), None
+
+
+def _check_pages(lens: torch.Tensor, table: torch.Tensor, max_seq_len: int, block_size: int, blocks: int) -> None:
+    """Host check of what the kernels only skip: lengths past max_seq_len, block ids outside the cache."""
+    if not lens.numel() or max_seq_len <= 0:
+        if lens.numel() and bool((lens > max_seq_len).any()):
+            raise ValueError("max_seq_len is smaller than a sequence length")
+        return
+    if bool((lens > max_seq_len).any()):
+        raise ValueError("max_seq_len is smaller than a sequence length")
+    needed = (max_seq_len + block_size - 1) // block_size
+    used = torch.arange(needed, device=table.device)[None, :] * block_size < lens[:, None].to(torch.int64)
+    ids = table[:, :needed].to(torch.int64)
+    if bool(((ids < 0) | (ids >= blocks))[used].any()):
+        raise IndexError("block_table references a block outside the cache")
+
+
+def tree_attention(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    context_lens: Sequence[int] | torch.Tensor,
+    tree_mask: torch.Tensor,
+    *,
+    scale: float,
+    query_lens: Sequence[int] | None = None,
+    query_start_loc: torch.Tensor | None = None,
+    max_query_len: int | None = None,
+    max_seq_len: int | None = None,
+    validate: bool = True,
+) -> torch.Tensor:
+    """Attention of a tree of drafted tokens per request: ``query`` ``[T, Hq, D]`` -> ``[T, Hq, Dv]``.
+
+    No counterpart in the reference: the verification step of speculative
+    decoding.  Request b has ``context_lens[b]`` cached tokens and
+    ``query_lens[b]`` drafts, whose K and V :func:`write_kv_cache` has put
+    behind them, at cache rows ``context_lens[b] + j``.  Draft i sees every
+    context row and the drafts j of its request where ``tree_mask[row, j]``
+    (bool or uint8, ``[T, at least max_query_len]``) is set: its ancestors and,
+    usually, itself.  A draft that sees nothing gets zeros; what is not seen
+    has no influence, NaN and infinities included.
+
+    The request split is given as for :func:`paged_attention`.  ``max_seq_len``
+    bounds ``context_lens[b] + query_lens[b]``; with device tensors pass it and
+    ``max_query_len`` and ``validate=False`` to avoid host synchronisations.
+    """
+    _check_caches(key_cache, value_cache)
+    if query.ndim != 3:
+        raise ValueError("query must have shape [tokens, num_heads, head_size]")
+    if query.shape[1] % key_cache.shape[2]:
+        raise ValueError("num_heads must be divisible by num_kv_heads")
+    if tree_mask.dtype not in (torch.bool, torch.uint8):
+        raise TypeError(f"tree_mask must be bool or uint8, got {tree_mask.dtype}")
+    loc, batch, max_query_len, _ = _request_rows(query, query_lens, query_start_loc, max_query_len, validate)
+    if tree_mask.ndim != 2 or tree_mask.shape[0] != query.shape[0] or tree_mask.shape[1] < max_query_len:
+        raise ValueError("tree_mask must have shape [tokens, at least max_query_len]")
+    lens, host = _device_lengths(context_lens, "context_lens", query.device)
+    if lens.ndim != 1 or (lens.numel() < batch if host is None else lens.numel() != batch):
+        raise ValueError("one context length is required per request")
+    total = lens[:batch] + (loc[1:] - loc[:-1]) if max_seq_len is None or validate else None
+    if max_seq_len is None:
+        max_seq_len = int(total.max().item()) if batch else 0
+    if max_seq_len > block_table.shape[1] * key_cache.shape[1]:
+        raise ValueError("block_table has too few entries for a sequence length")
+    table = _device_table(block_table, batch, query.device)
+    if validate and batch:
+        _check_pages(total, table, max_seq_len, key_cache.shape[1], key_cache.shape[0])
+    extension = native.load_extension()
+    return native._operator("hif8_tree_attention", extension)(
+        query.contiguous(), key_cache, value_cache, table, loc, lens, tree_mask.to(query.device).contiguous(),
+        float(scale), max_query_len, int(max_seq_len))
+
+
+def accept_drafts(
+    key_caches: torch.Tensor | Sequence[torch.Tensor],
+    value_caches: torch.Tensor | Sequence[torch.Tensor],
+    block_table: torch.Tensor,
+    context_lens: Sequence[int] | torch.Tensor,
+    accepted: torch.Tensor,
+    accepted_counts: Sequence[int] | torch.Tensor,
+    *,
+    validate: bool = True,
+) -> torch.Tensor:
+    """Moves the rows of accepted drafts to the end of each request's context, in place.
+
+    No counterpart in the reference; follows :func:`tree_attention`.  Row
+    ``context_lens[b] + accepted[b, i]`` of every cache moves to row
+    ``context_lens[b] + i`` for ``i < accepted_counts[b]``.  ``accepted``
+    (int32, ``[B, width]``) lists draft indices in strictly rising order, the
+    path from the root (every parent precedes its children).  The caches are
+    one layer's pair or the pairs of all layers, which share ``block_table``;
+    all move in one launch.  Returns the new lengths, int32 ``[B]``, on the
+    device.  The pages must belong to one request each.
+
+    ``validate`` checks counts, order and pages on the host.
+    """
+    keys = [key_caches] if isinstance(key_caches, torch.Tensor) else list(key_caches)
+    values = [value_caches] if isinstance(value_caches, torch.Tensor) else list(value_caches)
+    if not keys or len(keys) != len(values):
+        raise ValueError("accept_drafts needs a value cache for every key cache")
+    for k, v in zip(keys, values):
+        _check_caches(k, v)
+        if k.shape[:2] != keys[0].shape[:2]:
+            raise ValueError("all caches must have the same blocks")
+    device = keys[0].device
+    if accepted.ndim != 2:
+        raise ValueError("accepted must have shape [batch, width]")
+    if accepted.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"accepted must be int32 or int64, got {accepted.dtype}")
+    batch, width = accepted.shape
+    lens, host = _device_lengths(context_lens, "context_lens", device)
+    counts, _ = _device_lengths(accepted_counts, "accepted_counts", device)
+    if lens.ndim != 1 or lens.numel() < batch or (host is not None and len(host) != batch):
+        raise ValueError("one context length is required per request")
+    if counts.ndim != 1 or counts.numel() < batch:
+        raise ValueError("one accepted count is required per request")
+    path = accepted.to(device=device, dtype=torch.int32).contiguous()
+    table = _device_table(block_table, batch, device)
+    if validate and batch:
+        live = torch.arange(width, device=device) < counts[:batch, None]
+        if bool((counts[:batch] > width).any()) or bool((counts[:batch] < 0).any()):
+            raise ValueError("accepted_counts must be within the width of accepted")
+        before = torch.nn.functional.pad(path, (1, 0), value=-1)[:, :-1]
+        if bool(((path <= before) & live).any()):
+            raise ValueError("accepted must list draft indices in strictly rising order")
+        if width:
+            last = (torch.where(live, path, -1).amax(dim=1) + 1 + lens[:batch]).to(torch.int32)
+            most = int(last.max().item())
+            if most > table.shape[1] * keys[0].shape[1]:
+                raise ValueError("block_table has too few entries for an accepted draft")
+            _check_pages(last, table, most, keys[0].shape[1], keys[0].shape[0])
+    extension = native.load_extension()
+    return native._operator("hif8_accept_drafts", extension)(keys + values, table, lens, path, counts)
+
+
+def paged_decode_attention_weights(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: Sequence[int] | torch.Tensor,
+    key_weights: torch.Tensor,
+    *,
+    scale: float,
+    accumulate: bool = True,
+    max_seq_len: int | None = None,
+    validate: bool = True,
+) -> torch.Tensor:
+    """:func:`paged_decode_attention` that also keeps the weight every cached row got.
+
+    No counterpart in the reference; feeds :func:`evict_kv_rows`.
+    ``key_weights`` (float32 ``[B, Hkv, at least max_seq_len]``, contiguous)
+    receives, in place, the sum of the row's softmax weights over the query
+    heads of each KV head: added, or stored with ``accumulate=False``.  Entries
+    from ``seq_lens[b]`` on are left as they were.
+    """
+    _check_caches(key_cache, value_cache)
+    if query.ndim != 3:
+        raise ValueError("query must have shape [tokens, num_heads, head_size]")
+    batch = query.shape[0]
+    if query.shape[1] % key_cache.shape[2]:
+        raise ValueError("num_heads must be divisible by num_kv_heads")
+    lens, table, max_seq_len = _weighted_request(key_cache, block_table, seq_lens, key_weights, batch, max_seq_len,
+                                                 validate)
+    extension = native.load_extension()
+    return native._operator("hif8_paged_decode_attention_weights", extension)(
+        query.contiguous(), key_cache, value_cache, table, lens, key_weights, float(scale), max_seq_len,
+        bool(accumulate))
+
+
+def _weighted_request(key_cache, block_table, seq_lens, key_weights, batch: int, max_seq_len, validate: bool):
+    """The checks that the calls with ``key_weights`` share: (seq_lens, block table, max_seq_len)."""
+    if key_weights.dtype != torch.float32:
+        raise TypeError(f"key_weights must be float32, got {key_weights.dtype}")
+    if not key_weights.is_contiguous():
+        raise ValueError("key_weights must be contiguous")
+    lens, host = _device_lengths(seq_lens, "sequence lengths", key_cache.device)
+    if lens.ndim != 1 or (lens.numel() < batch if host is None else lens.numel() != batch):
+        raise ValueError("one sequence length is required per request")
+    lens = lens[:batch]
+    if max_seq_len is None:
+        max_seq_len = (max(host, default=0) if host is not None else int(lens.max().item())) if batch else 0
+    if max_seq_len > block_table.shape[1] * key_cache.shape[1]:
+        raise ValueError("block_table has too few entries for a sequence length")
+    if key_weights.ndim != 3 or key_weights.shape[0] < batch or key_weights.shape[1] != key_cache.shape[2] or \
+            key_weights.shape[2] < max_seq_len:
+        raise ValueError("key_weights must have shape [batch, num_kv_heads, at least max_seq_len]")
+    table = _device_table(block_table, batch, key_cache.device)
+    if validate and batch:
+        _check_pages(lens, table, int(max_seq_len), key_cache.shape[1], key_cache.shape[0])
+    return lens, table, int(max_seq_len)
+
+
+def accumulate_key_weights(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: Sequence[int] | torch.Tensor,
+    key_weights: torch.Tensor,
+    *,
+    scale: float,
+    query_lens: Sequence[int] | None = None,
+    query_start_loc: torch.Tensor | None = None,
+    causal: bool = True,
+    accumulate: bool = True,
+    max_query_len: int | None = None,
+    max_seq_len: int | None = None,
+    validate: bool = True,
+) -> None:
+    """Adds up the softmax weight that many query rows give every cached row, in place.
+
+    The multi-row form of :func:`paged_decode_attention_weights`, for a prompt
+    (or the last rows of one) before :func:`evict_kv_rows`; it reads the key
+    cache alone and returns nothing.  Request b's query rows are the last
+    positions of its ``seq_lens[b]`` cached tokens, given and masked as in
+    :func:`paged_attention`.  ``key_weights`` as there; with
+    ``accumulate=False`` the sums are stored instead of added.
+    """
+    if key_cache.dtype != torch.uint8 or key_cache.ndim != 4:
+        raise TypeError("key_cache must be a 4-D uint8 tensor")
+    if not key_cache.is_contiguous():
+        raise ValueError("key_cache must be contiguous")
+    if query.ndim != 3:
+        raise ValueError("query must have shape [tokens, num_heads, head_size]")
+    if query.shape[1] % key_cache.shape[2]:
+        raise ValueError("num_heads must be divisible by num_kv_heads")
+    loc, batch, max_query_len, _ = _request_rows(query, query_lens, query_start_loc, max_query_len, validate)
+    lens, table, max_seq_len = _weighted_request(key_cache, block_table, seq_lens, key_weights, batch, max_seq_len,
+                                                 validate)
+    extension = native.load_extension()
+    native._operator("hif8_key_weights", extension)(
+        query.contiguous(), key_cache, table, loc, lens, key_weights, float(scale), max_query_len, max_seq_len,
+        bool(causal), bool(accumulate))
+
+
+def evict_kv_rows(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: Sequence[int] | torch.Tensor,
+    key_weights: torch.Tensor,
+    keep: int | Sequence[int] | torch.Tensor,
+    *,
+    positions: torch.Tensor | None = None,
+    sinks: int = 0,
+    protect_from: Sequence[int] | torch.Tensor | None = None,
+    max_seq_len: int | None = None,
+    validate: bool = True,
+) -> torch.Tensor:
+    """Cuts each request's cache to its ``keep`` rows of largest accumulated weight, in place.
+
+    No counterpart in the reference.  Every KV head keeps its own rows:
+    protected ones first (position below ``sinks``, or from ``protect_from[b]``
+    on), then by falling ``key_weights``, NaN last, ties by the lower row.
+    With ``n = min(seq_lens[b], keep)`` the r-th dropped row before row n
+    receives the r-th kept row from row n on - codes, scale, weight and
+    position - and the other kept rows stay where they are, so attention over
+    the first n rows is attention over the kept ones.  Weights from row n to
+    the old length become zero.
+
+    ``positions`` (int32, the shape of ``key_weights``) holds each row's
+    position in the sequence and moves along; without it a row's index counts
+    as its position, as in a cache that was never cut.  Returns the new
+    lengths, int32 ``[B]``, on the device.  The pages must belong to one request.
+    """
+    _check_caches(key_cache, value_cache)
+    batch = len(seq_lens) if not isinstance(seq_lens, torch.Tensor) else seq_lens.numel()
+    lens, table, max_seq_len = _weighted_request(key_cache, block_table, seq_lens, key_weights, batch, max_seq_len,
+                                                 validate)
+    if positions is not None:
+        if positions.dtype != torch.int32 or positions.shape != key_weights.shape:
+            raise TypeError("positions must be int32 with the shape of key_weights")
+        if not positions.is_contiguous():
+            raise ValueError("positions must be contiguous")
+    if sinks < 0:
+        raise ValueError("sinks must not be negative")
+    keep_each, keep_all = None, 0
+    if isinstance(keep, int):
+        keep_all = keep
+    else:
+        keep_each, _ = _device_lengths(keep, "keep", key_cache.device)
+        if keep_each.ndim != 1 or keep_each.numel() < batch:
+            raise ValueError("one keep count is required per request")
+    if keep_all < 0 or (validate and keep_each is not None and bool((keep_each < 0).any())):
+        raise ValueError("keep must not be negative")
+    if protect_from is not None:
+        protect_from = torch.as_tensor(protect_from).to(device=key_cache.device, dtype=torch.int32).contiguous()
+        if protect_from.ndim != 1 or protect_from.numel() < batch:
+            raise ValueError("one protect_from position is required per request")
+    extension = native.load_extension()
+    return native._operator("hif8_kv_evict", extension)(
+        key_cache, value_cache, table, lens, key_weights, positions, keep_each, int(keep_all), int(sinks),
+        protect_from, max_seq_len)
+
+
+
 __all__ = [
     "HIF8_CACHE_DTYPE",
     "HIF8_SCALE_BYTES",
     "Hif8KVCacheLayout",
+    "accept_drafts",
+    "accumulate_key_weights",
+    "evict_kv_rows",
     "pack_kv_rows",
     "paged_attention",
     "paged_decode_attention",
+    "paged_decode_attention_weights",
+    "tree_attention",
     "unpack_kv_rows",
     "write_kv_cache",
 ]

@@ -385,6 +385,116 @@ int hif8_paged_prefill_attention(const void *query, int q_dtype, const uint8_t *
                                  size_t workspace_bytes, hif8_stream_t stream);
 
 /*
+ * Attention of a tree of drafted tokens over the paged HiF8 cache (no counterpart in
+ * the reference: speculative decoding's verification step).  Request b has
+ * context_lens[b] cached rows and n_b = query_start_loc[b + 1] - query_start_loc[b]
+ * drafts, whose K and V rows are already written behind them (cache rows
+ * context_lens[b] + j, by hif8_kv_cache_write).
+ *   query [total_query_tokens, num_heads, D] fp16/bf16, the drafts of request b at rows
+ *     query_start_loc[b] ..
+ *   tree_mask [total_query_tokens, mask_width] bytes: draft i of request b sees all its
+ *     context rows and the drafts j < min(n_b, mask_width) with a byte other than zero
+ *     in column j of its row (its ancestors and, usually, itself)
+ *   max_query_len >= every n_b, <= mask_width; max_seq_len >= every context_lens[b] + n_b
+ *     (lengths are clamped to it), <= max_blocks_per_seq * block_size
+ *   out [total_query_tokens, num_heads, Dv] in the query dtype: softmax(scale * q . K) V over
+ *     the rows seen, K and V dec(code) * row scale; a row that sees nothing gets zeros,
+ *     and what is not seen has no influence, whatever it holds.  Cache rows whose block id
+ *     lies outside [0, num_blocks) are left out.  Rows before query_start_loc[0] or from
+ *     query_start_loc[batch] on are not written.
+ *   workspace  at least hif8_tree_attention_workspace_size(...) bytes, 16-byte aligned; its
+ *              size depends on these arguments alone
+ */
+size_t hif8_tree_attention_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
+                                          int64_t head_size_v, int64_t total_query_tokens, int64_t max_query_len,
+                                          int64_t max_seq_len);
+int hif8_tree_attention(const void *query, int q_dtype, const uint8_t *key_cache, const uint8_t *value_cache,
+                        int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_size,
+                        int64_t head_size_v, const void *block_table, int block_table_dtype,
+                        int64_t max_blocks_per_seq, const int32_t *query_start_loc, const int32_t *context_lens,
+                        const uint8_t *tree_mask, int64_t mask_width, int64_t batch, int64_t num_heads,
+                        int64_t total_query_tokens, int64_t max_query_len, int64_t max_seq_len, float scale,
+                        void *out, void *workspace, size_t workspace_bytes, hif8_stream_t stream);
+
+/*
+ * hif8_paged_decode_attention that also accumulates the weight each cached row got (no
+ * counterpart in the reference): with p the softmax weights of request b,
+ *   key_weights[b, h, t] (+)= sum over the query heads of KV head h of p[head, t]
+ * for t < seq_lens[b]; later entries are left as they were.
+ *   key_weights [batch, num_kv_heads, weights_stride] float32, weights_stride >= max_seq_len
+ *   accumulate  0 stores the sums instead of adding them
+ * The other arguments are those of hif8_paged_decode_attention.
+ */
+size_t hif8_paged_decode_attention_weights_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                                                          int64_t head_size, int64_t head_size_v,
+                                                          int64_t max_seq_len);
+int hif8_paged_decode_attention_weights(const void *query, int q_dtype, const uint8_t *key_cache,
+                                        const uint8_t *value_cache, int64_t num_blocks, int64_t block_size,
+                                        int64_t num_kv_heads, int64_t head_size, int64_t head_size_v,
+                                        const void *block_table, int block_table_dtype, int64_t max_blocks_per_seq,
+                                        const int32_t *seq_lens, int64_t batch, int64_t num_heads,
+                                        int64_t max_seq_len, float scale, void *out, float *key_weights,
+                                        int64_t weights_stride, int accumulate, void *workspace,
+                                        size_t workspace_bytes, hif8_stream_t stream);
+
+/*
+ * The same weights of many query rows at once, from the key cache alone (a prompt, or the
+ * last rows of one):
+ *   key_weights[b, h, t] (+)= sum over request b's query rows i and the query heads of KV
+ *                             head h of softmax_t(scale * q_i . K_t), t < seq_lens[b]
+ * query, query_start_loc, seq_lens, max_query_len, max_seq_len and causal as in
+ * hif8_paged_prefill_attention; key_weights and accumulate as above.  A request without
+ * query rows adds (or stores) zeros.
+ */
+size_t hif8_key_weights_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
+                                       int64_t total_query_tokens, int64_t max_query_len, int64_t max_seq_len);
+int hif8_key_weights(const void *query, int q_dtype, const uint8_t *key_cache, int64_t num_blocks, int64_t block_size,
+                     int64_t num_kv_heads, int64_t head_size, const void *block_table, int block_table_dtype,
+                     int64_t max_blocks_per_seq, const int32_t *query_start_loc, const int32_t *seq_lens,
+                     int64_t batch, int64_t num_heads, int64_t total_query_tokens, int64_t max_query_len,
+                     int64_t max_seq_len, float scale, int causal, float *key_weights, int64_t weights_stride,
+                     int accumulate, void *workspace, size_t workspace_bytes, hif8_stream_t stream);
+
+/*
+ * Moves the rows of accepted drafts to the end of the context, in place, in any number of
+ * caches that share a block table (K and V of every layer), in one launch per 128 caches:
+ *   row context_lens[b] + accepted[b][i]  ->  row context_lens[b] + i,  i < accepted_counts[b]
+ *   caches [num_caches]  host array of device pointers; row_bytes[i] = Hkv * (D + 4) of cache i
+ *   accepted [batch, accepted_width] int32: draft indices in strictly rising order (a path
+ *     from the root: parents come before children); not rising, the rows' contents are
+ *     unspecified, the accesses stay inside the cache
+ *   new_lens [batch] int32 (may be NULL): context_lens[b] + accepted_counts[b]
+ * Rows outside the table or in a block outside [0, num_blocks) are skipped.  The pages
+ * that are written must belong to one request.
+ */
+int hif8_accept_drafts(void *const *caches, const int64_t *row_bytes, int64_t num_caches, int64_t num_blocks,
+                       int64_t block_size, const void *block_table, int block_table_dtype,
+                       int64_t max_blocks_per_seq, const int32_t *context_lens, const int32_t *accepted,
+                       int64_t accepted_width, const int32_t *accepted_counts, int64_t batch, int32_t *new_lens,
+                       hif8_stream_t stream);
+
+/*
+ * Cuts every request's cache to its `keep` rows of largest accumulated weight, per KV head
+ * and in place.  Rows are ranked by: protected rows first (position < sinks, or
+ * >= protect_from[b]), then falling key_weights, NaN last, ties by the lower row.  With
+ * n = min(seq_lens[b], keep), the r-th dropped row before row n receives the r-th kept row
+ * from row n on (codes, scale, weight and position; both counted in row order); the other
+ * kept rows stay where they are.  Weights of rows n .. seq_lens[b] - 1 become zero.
+ *   key_weights [batch, Hkv, weights_stride] float32; positions the same shape in int32, or
+ *     NULL (then a row's position is its index)
+ *   keep [batch] int32, or NULL for keep_all of every request; protect_from [batch] int32 or NULL
+ *   new_lens [batch] int32: n
+ * Rows in a block outside [0, num_blocks) are not copied.  Pages must belong to one request.
+ */
+size_t hif8_kv_evict_workspace_size(int64_t batch, int64_t num_kv_heads, int64_t max_seq_len);
+int hif8_kv_evict(uint8_t *key_cache, uint8_t *value_cache, int64_t num_blocks, int64_t block_size,
+                  int64_t num_kv_heads, int64_t head_size, int64_t head_size_v, const void *block_table,
+                  int block_table_dtype, int64_t max_blocks_per_seq, const int32_t *seq_lens, int64_t batch,
+                  int64_t max_seq_len, float *key_weights, int32_t *positions, int64_t weights_stride,
+                  const int32_t *keep, int64_t keep_all, int64_t sinks, const int32_t *protect_from,
+                  int32_t *new_lens, void *workspace, size_t workspace_bytes, hif8_stream_t stream);
+
+/*
  * Decode-step glue of the synthetic hybrid model (the end-to-end workload).
  * These have no counterpart among the reference's operators: they fuse the
  * bf16 / fp32 model parts that the reference leaves to vLLM (norms, the MLP
