@@ -10,7 +10,9 @@
 #include <stddef.h>
 
 #include <algorithm>
+#include <type_traits>
 
+#include "mfma_lookup.h"
 #include "row_attention.h"
 
 namespace hif8 {
@@ -112,6 +114,446 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
   }
 }
 
+// ---------------------------------------------------- on the matrix cores
+//
+// Head sizes 64, 128 and 256 (K and V alike), pages of a multiple of 16 rows.
+// A workgroup of four wavefronts owns (request, KV head, 16 kRB query rows,
+// split); its query rows are the (draft, head) pairs of the KV head, so every
+// cached code is decoded once for all of them.  It walks its split in tiles of
+// kT = 16384 / D cache rows, with two barriers per tile:
+//   * S^T = K Q^T: every wavefront takes a quarter of the tile's rows, loaded
+//     from HBM straight into the MFMA A operand (row = lane % 16, 16 codes per
+//     lane) and decoded in registers; Q is the B operand, held all along;
+//   * the row maxima meet in LDS; P = 2^(x + e - m) in fp16 goes to LDS, where e
+//     is the exponent of the row's V scale and its mantissa is multiplied in,
+//     so V itself stays the exact dec(code) and no scale is rounded;
+//   * O^T += V^T P^T: every wavefront takes 64 dims of 64 rows (all of the
+//     tile's at D = 256), 4 bytes of 16 rows per lane.
+// The next tile's K loads are issued as soon as S is done, its V loads after O.
+// sum_t P_t 2^-e_t is the softmax sum against the same maximum.
+constexpr float kLazy = 6.f;  // log2 headroom of the maximum: it moves in steps of more than 2^6
+
+struct RowTile {
+  int64_t magic;       // ceil(2^36 / (block_size / 16))
+  int rows_per_wg;     // 16 * kRB
+  int row_tiles;       // of the longest request
+};
+
+// Exponent, signed mantissa and 2^-exponent of a V row's scale.  Scales below
+// 2^-64 keep 2^-64 as exponent (and a mantissa below one); NaN and infinity
+// become the mantissa.
+__device__ __forceinline__ void split_scale(float s, float &e, float &mant, float &inv) {
+  const uint32_t u = __float_as_uint(s);
+  const int ex = int((u >> 23) & 0xFFu);
+  if (ex == 0xFF) {
+    e = 0.f;
+    mant = s;
+    inv = 1.f;
+  } else if (ex < 127 - 64) {
+    e = -64.f;
+    mant = s * 0x1p64f;
+    inv = 0x1p64f;
+  } else {
+    e = float(ex - 127);
+    mant = __uint_as_float((u & 0x807FFFFFu) | 0x3F800000u);
+    inv = __uint_as_float(uint32_t(254 - ex) << 23);
+    if (ex == 254) inv = 0x1p-127f;
+  }
+}
+
+template <int kD, bool kBf16, int kRB, bool kX, typename BtT>
+__global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(const RowAttnParams p,
+                                                                               const RowTile tile) {
+  constexpr int kRow = kD + 4;
+  constexpr int kT = 16384 / kD;          // cache rows of a tile
+  constexpr int kKB = kT / 64;            // 16-row blocks of a wavefront in S
+  constexpr int kQS = kD / 32;            // MFMA steps over the head dims
+  constexpr int kSlices = kD / 64;        // 64-dim slices of V
+  constexpr int kGroups = kT / 16;        // 16-row groups of a tile
+  constexpr int kRows = 16 * kRB;
+  constexpr int kPStride = kT + 8;        // fp16 values of a row of P in LDS
+  struct Smem {
+    uint32_t table[kLookupBytes / 4];     // at LDS byte 0: a lookup's address needs no addition
+    uint16_t pt[kRows * kPStride];
+    float top[4][kRows];
+  };
+  __shared__ __attribute__((aligned(16))) Smem sm;
+  const uint32_t table = lds_address(sm.table);
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const uint32_t lane4 = uint32_t(4 * lane);
+  // The KV heads and row tiles of one (request, split) read the same cache
+  // lines: their blocks are equal modulo 8, on one XCD.
+  const int inner = p.hkv * tile.row_tiles;
+  const int xcd = int(blockIdx.x) & 7, slot = int(blockIdx.x) >> 3;
+  const int outer = (slot / inner) * 8 + xcd;
+  if (outer >= p.batch * p.num_splits) return;  // padding block (uniform)
+  const int rt = (slot % inner) % tile.row_tiles, h = (slot % inner) / tile.row_tiles;
+  const int b = outer / p.num_splits, split = outer % p.num_splits;
+  int begin, count;
+  request_rows(p, b, begin, count);
+  const int rows = count * p.group;
+  const int ctx = clamp_rows(p.lens[b], p.max_len);
+  const int len = rows_seen(p, ctx, count);
+  const int t_begin = split * p.split_tokens, t_end = min(t_begin + p.split_tokens, len);
+  if (rt * kRows >= rows) return;  // uniform
+  if (t_begin >= t_end && !(split == 0 && p.num_splits == 1)) return;
+  const int ntiles = max(t_end - t_begin + kT - 1, 0) / kT;
+
+  // This lane's query rows (column n of every row block).
+  int qrow[kRB], head[kRB];
+  bool row_ok[kRB];
+#pragma unroll
+  for (int rb = 0; rb < kRB; ++rb) {
+    const int r = rt * kRows + 16 * rb + n;
+    row_ok[rb] = r < rows;
+    const int tok = row_ok[rb] ? r / p.group : 0;
+    qrow[rb] = begin + tok;
+    head[rb] = h * p.group + (row_ok[rb] ? r - tok * p.group : 0);
+  }
+
+  const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.bt_stride;
+  const uint32_t rec = uint32_t(p.hkv) * kRow;
+  const int bs16 = p.block_size >> 4;
+  // Lane i % kGroups looks up 16-row group i of a tile; the entry is loaded a
+  // tile ahead of its use.
+  auto group_of = [&](int t0) { return min(t0 + 16 * (lane & (kGroups - 1)), t_end - 1) >> 4; };
+  auto block_at = [&](int t0) {
+    const int gr = group_of(t0);
+    return int64_t(bt[int((uint64_t(gr) * uint64_t(tile.magic)) >> 36)]);
+  };
+  // Byte offset of the group's first row of this KV head, or -1.
+  auto offset_at = [&](int t0, int64_t blk) {
+    const int gr = group_of(t0);
+    const int in16 = gr - int((uint64_t(gr) * uint64_t(tile.magic)) >> 36) * bs16;
+    return blk >= 0 && blk < p.num_blocks && t0 + 16 * (lane & (kGroups - 1)) < t_end
+               ? (blk * p.block_size + 16 * in16) * int64_t(rec) + int64_t(h) * kRow
+               : int64_t(-1);
+  };
+  auto uniform_offset = [&](int64_t off, int group) {
+    const int lo = __builtin_amdgcn_readlane(int(uint64_t(off)), group);
+    const int hi = __builtin_amdgcn_readlane(int(uint64_t(off) >> 32), group);
+    return int64_t((uint64_t(uint32_t(hi)) << 32) | uint32_t(lo));
+  };
+
+  const int vslice = wave % kSlices, vgroup = wave / kSlices;
+  const uint32_t k_off = uint32_t(n) * rec + 16u * g;              // K: row n, codes 16 g + 64 i
+  uint32_t v_off[4], s_off[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v_off[e] = uint32_t(4 * g + e) * rec + uint32_t(64 * vslice + 4 * n);  // V: row 4 g + e, four dims
+    s_off[e] = uint32_t(4 * g + e) * rec + uint32_t(kD);                   // scale of row 4 g + e
+  }
+  typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+  lk_u32x4 kraw[kKB][kSlices];
+  float ks[kKB][4], vs[kKB][4];
+  uint32_t vraw[2][8];
+  int64_t off_lane = -1;   // group offsets of the tile whose K is in flight
+  uint32_t ok_groups = 0;  // its groups that lie in the cache, a bit each
+  auto load_k = [&]() {
+#pragma unroll
+    for (int kb = 0; kb < kKB; ++kb) {
+      const int64_t off = uniform_offset(off_lane, wave * kKB + kb);
+      const uint8_t *kp = p.key_cache + (off < 0 ? 0 : off), *vp = p.value_cache + (off < 0 ? 0 : off);
+#pragma unroll
+      for (int i = 0; i < kSlices; ++i) kraw[kb][i] = *reinterpret_cast<const u32x4_a4 *>(kp + k_off + 64 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ks[kb][e] = *reinterpret_cast<const float *>(kp + s_off[e]);
+        vs[kb][e] = *reinterpret_cast<const float *>(vp + s_off[e]);
+      }
+    }
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t off = uniform_offset(off_lane, 4 * vgroup + j);
+      const uint8_t *vp = p.value_cache + (off < 0 ? 0 : off);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        vraw[j >> 1][4 * (j & 1) + e] = *reinterpret_cast<const uint32_t *>(vp + v_off[e]);
+    }
+  };
+
+  int64_t blk_next = -1;
+  if (ntiles > 0) {
+    const int64_t blk = block_at(t_begin);
+    if (ntiles > 1) blk_next = block_at(t_begin + kT);
+    off_lane = offset_at(t_begin, blk);
+    ok_groups = uint32_t(__ballot(off_lane >= 0));
+    load_k();
+    load_v();
+  }
+  lk_u32x4 qf[kRB][kQS];
+#pragma unroll
+  for (int rb = 0; rb < kRB; ++rb) {
+    const uint16_t *q = static_cast<const uint16_t *>(p.query) + (size_t(qrow[rb]) * p.hq + head[rb]) * kD + 16 * g;
+#pragma unroll
+    for (int i = 0; i < kQS; ++i)  // step 2 i + s: dims 64 i + 16 g + 8 s + [0, 8)
+      qf[rb][i] = row_ok[rb] ? *reinterpret_cast<const lk_u32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1)) : lk_u32x4{0, 0, 0, 0};
+  }
+  fill_lookup<kBf16, kThreads>(sm.table, tid);
+  lk_f32x4 oacc[kRB][4];
+  float m[kRB], l[kRB];
+#pragma unroll
+  for (int rb = 0; rb < kRB; ++rb) {
+    m[rb] = -__builtin_inff();
+    l[rb] = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) oacc[rb][q] = lk_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  lds_barrier();
+
+  for (int it = 0; it < ntiles; ++it) {
+    const int t0 = t_begin + it * kT;
+    const uint32_t ok_now = ok_groups;
+    // Every row of the tile lies in the cache and every query row sees it (uniform).
+    const bool full = t0 + kT <= min(ctx, t_end) && (ok_now & ((1u << kGroups) - 1u)) == (1u << kGroups) - 1u;
+    // S^T of this wavefront's rows.
+    lk_f32x4 s[kRB][kKB];
+#pragma unroll
+    for (int kb = 0; kb < kKB; ++kb) {
+#pragma unroll
+      for (int rb = 0; rb < kRB; ++rb) s[rb][kb] = lk_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kQS; ++i) {
+        const lk_u32x4 w = kraw[kb][i >> 1];
+        const lk_u32x4 a = look8<false>(w[2 * (i & 1)], w[2 * (i & 1) + 1], lane4, table);
+#pragma unroll
+        for (int rb = 0; rb < kRB; ++rb) s[rb][kb] = mfma_16x16x32<kBf16>(a, qf[rb][i], s[rb][kb]);
+      }
+    }
+    float ksc[kKB][4], ve[kKB][4], vm[kKB][4], vi[kKB][4];
+#pragma unroll
+    for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ksc[kb][e] = ks[kb][e] * p.scale_log2;
+        split_scale(vs[kb][e], ve[kb][e], vm[kb][e], vi[kb][e]);
+      }
+    // The next tile's K, in flight from here to the next S.
+    if (it + 1 < ntiles) {
+      off_lane = offset_at(t0 + kT, blk_next);
+      ok_groups = uint32_t(__ballot(off_lane >= 0));
+      if (it + 2 < ntiles) blk_next = block_at(t0 + 2 * kT);
+      load_k();
+    }
+    // Logits (base 2), the rows each query row sees, and the tile's maxima.
+    uint32_t seen[kRB];  // bit 4 kb + e: this query row sees cache row 4 g + e of block kb
+    float y[kRB][kKB][4];
+#pragma unroll
+    for (int rb = 0; rb < kRB; ++rb) {
+      seen[rb] = 0xFFFFFFFFu;
+      if (!full) {
+        seen[rb] = 0;
+        const uint8_t *mrow = p.mask + (p.mask ? size_t(qrow[rb]) * p.mask_stride : 0);
+#pragma unroll
+        for (int kb = 0; kb < kKB; ++kb) {
+          const bool in = (ok_now >> (wave * kKB + kb)) & 1u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = t0 + 16 * (wave * kKB + kb) + 4 * g + e;
+            bool vis = in && t < t_end;
+            if (vis && t >= ctx) vis = mrow[t - ctx] != 0;
+            seen[rb] |= uint32_t(vis) << (4 * kb + e);
+          }
+        }
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int kb = 0; kb < kKB; ++kb) {
+        lk_f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool vis = (seen[rb] >> (4 * kb + e)) & 1u;
+          x[e] = vis ? s[rb][kb][e] * ksc[kb][e] : -__builtin_inff();
+          y[rb][kb][e] = x[e] + ve[kb][e];
+          top = fmaxf(top, y[rb][kb][e]);
+        }
+        if constexpr (kX) {
+          const int t = t0 + 16 * (wave * kKB + kb) + 4 * g;
+          if (row_ok[rb] && t < t_end)
+            *reinterpret_cast<lk_f32x4 *>(p.x + (size_t(qrow[rb]) * p.hq + head[rb]) * p.x_stride + t) = x;
+        }
+      }
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      if (g == 0) sm.top[wave][16 * rb + n] = top;
+    }
+    lds_barrier();
+#pragma unroll
+    for (int rb = 0; rb < kRB; ++rb) {
+      const float top = fmaxf(fmaxf(sm.top[0][16 * rb + n], sm.top[1][16 * rb + n]),
+                              fmaxf(sm.top[2][16 * rb + n], sm.top[3][16 * rb + n]));
+      const bool grow = top > m[rb] + kLazy;
+      if (__any(grow)) {
+        const float next = grow ? top : m[rb];
+        if (!__all(!grow || m[rb] == -__builtin_inff())) {
+          const float alpha = grow ? __builtin_amdgcn_exp2f(m[rb] - next) : 1.f;
+          l[rb] *= alpha;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) oacc[rb][q] *= alpha;
+        }
+        m[rb] = next;
+      }
+      const float ref = m[rb] == -__builtin_inff() ? 0.f : m[rb];
+#pragma unroll
+      for (int kb = 0; kb < kKB; ++kb) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float pw = __builtin_amdgcn_exp2f(y[rb][kb][e] - ref);
+          if (full) {
+            l[rb] = fmaf(pw, vi[kb][e], l[rb]);
+            w[e] = pw * vm[kb][e];
+          } else {
+            const bool vis = (seen[rb] >> (4 * kb + e)) & 1u;
+            l[rb] = vis ? fmaf(pw, vi[kb][e], l[rb]) : l[rb];
+            w[e] = vis ? pw * vm[kb][e] : 0.f;
+          }
+        }
+        const int j = wave * kKB + kb;
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        *reinterpret_cast<u32x2 *>(sm.pt + (16 * rb + n) * kPStride + 32 * (j >> 1) + 8 * g + 4 * (j & 1)) =
+            u32x2{uint32_t(float_to_f16_bits(w[0])) | (uint32_t(float_to_f16_bits(w[1])) << 16),
+                  uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
+      }
+    }
+    lds_barrier();
+    // O^T += V^T P^T: slots 8 g + e of a 32-row step are rows 4 g + e of its
+    // first 16, then of its second 16, as P lies in LDS.
+    if (!full) {
+      // Rows that are not there, then infinities and NaN among the drafts: a
+      // query row that does not see one must not meet it in the product.
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t &w = vraw[j >> 1][4 * (j & 1) + e];
+          const int t = t0 + 64 * vgroup + 16 * j + 4 * g + e;
+          if (!((ok_now >> (4 * vgroup + j)) & 1u) || t >= t_end) w = 0;
+          odd |= t >= ctx && some_not_finite(w);
+        }
+      if (__any(odd)) {
+#pragma unroll 1
+        for (int k = 0; k < 16; ++k) {
+          const int j = k >> 2, e = k & 3;
+          uint32_t w = 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w = i == k ? vraw[i >> 3][i & 7] : w;
+          const int t_lane = t0 + 64 * vgroup + 16 * j + 4 * g + e;
+#pragma unroll 1
+          for (int byte = 0; byte < 4; ++byte) {
+            const uint32_t c = (w >> (8 * byte)) & 0xFFu;
+            const bool bad = t_lane >= ctx && ((c & 0x7Fu) == 0x6Fu || c == 0x80u);
+            uint64_t left = __ballot(bad);
+            if (bad) w &= ~(0xFFu << (8 * byte));
+            while (left) {
+              const int src = __builtin_ctzll(left);
+              left &= left - 1;
+              const float v = __uint_as_float(decode_bits(uint32_t(__builtin_amdgcn_readlane(int(c), src))));
+              const int sg = src >> 4, sn = src & 15;       // row 4 sg + e, dims 64 vslice + 4 sn + byte
+              const int t = t0 + 64 * vgroup + 16 * j + 4 * sg + e;
+              const int at = 64 * vgroup + 32 * (j >> 1) + 8 * sg + 4 * (j & 1) + e;
+#pragma unroll
+              for (int rb = 0; rb < kRB; ++rb) {
+                // (t, dim) is element sn % 4 of accumulator `byte` in the lanes of group sn / 4.
+                const bool vis = g == (sn >> 2) && row_ok[rb] && p.mask[size_t(qrow[rb]) * p.mask_stride + (t - ctx)] != 0;
+                const uint16_t pb = sm.pt[(16 * rb + n) * kPStride + at];
+                const float add = vis ? ((pb & 0x8000u) ? -v : v) : 0.f;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                  for (int x = 0; x < 4; ++x)
+                    if (q == byte && x == (sn & 3) && vis) oacc[rb][q][x] += add;
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i == k) vraw[i >> 3][i & 7] = w;
+        }
+      }
+    }
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      lk_u32x4 pf[kRB];
+#pragma unroll
+      for (int rb = 0; rb < kRB; ++rb)
+        pf[rb] = *reinterpret_cast<const lk_u32x4 *>(sm.pt + (16 * rb + n) * kPStride + 64 * vgroup + 32 * hf + 8 * g);
+      auto column = [&](auto byte) {
+        constexpr int q = decltype(byte)::value;
+        const lk_u32x4 a = look_column<q, true>(vraw[hf], lane4, table);
+#pragma unroll
+        for (int rb = 0; rb < kRB; ++rb) oacc[rb][q] = mfma_16x16x32<false>(a, pf[rb], oacc[rb][q]);
+      };
+      column(std::integral_constant<int, 0>{});
+      column(std::integral_constant<int, 1>{});
+      column(std::integral_constant<int, 2>{});
+      column(std::integral_constant<int, 3>{});
+    }
+    if (it + 1 < ntiles) load_v();
+  }
+
+  // The wavefronts' shares of the softmax sum, and (D < 256) of O.
+  lds_barrier();
+#pragma unroll
+  for (int rb = 0; rb < kRB; ++rb) {
+    float lt = l[rb] + __shfl_xor(l[rb], 16, kWave);
+    lt += __shfl_xor(lt, 32, kWave);
+    if (g == 0) sm.top[wave][16 * rb + n] = lt;
+  }
+  lk_f32x4 *spill = reinterpret_cast<lk_f32x4 *>(sm.table);
+  if constexpr (kSlices < 4) {
+    if (vgroup > 0) {
+#pragma unroll
+      for (int rb = 0; rb < kRB; ++rb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          spill[(((vgroup - 1) * kSlices + vslice) * kRB * 4 + rb * 4 + q) * kWave + lane] = oacc[rb][q];
+    }
+  }
+  lds_barrier();
+  if constexpr (kSlices < 4) {
+    if (vgroup > 0) return;
+#pragma unroll
+    for (int og = 0; og < 4 / kSlices - 1; ++og)
+#pragma unroll
+      for (int rb = 0; rb < kRB; ++rb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) oacc[rb][q] += spill[((og * kSlices + vslice) * kRB * 4 + rb * 4 + q) * kWave + lane];
+  }
+#pragma unroll
+  for (int rb = 0; rb < kRB; ++rb) {
+    if (!row_ok[rb]) continue;
+    const float total = sm.top[0][16 * rb + n] + sm.top[1][16 * rb + n] + sm.top[2][16 * rb + n] + sm.top[3][16 * rb + n];
+    const size_t r = size_t(qrow[rb]) * p.hq + head[rb];
+    const int dim = 64 * vslice + 16 * g;  // element e of accumulator q: dim + 4 e + q
+    if (p.num_splits == 1) {
+      const float inv = total != 0.f ? 1.f / total : 0.f;
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        w[i] = uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i) & 3][i >> 1] * inv)) |
+               (uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i + 1) & 3][i >> 1] * inv)) << 16);
+      lk_u32x4 *o = reinterpret_cast<lk_u32x4 *>(static_cast<uint16_t *>(p.out) + r * kD + dim);
+      o[0] = lk_u32x4{w[0], w[1], w[2], w[3]};
+      o[1] = lk_u32x4{w[4], w[5], w[6], w[7]};
+    } else {
+      lk_f32x4 *po = reinterpret_cast<lk_f32x4 *>(p.part_o + (r * p.num_splits + split) * kD + dim);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) po[e] = lk_f32x4{oacc[rb][0][e], oacc[rb][1][e], oacc[rb][2][e], oacc[rb][3][e]};
+    }
+    if (g == 0 && vslice == 0) {
+      p.part_ml[2 * (r * p.num_splits + split)] = m[rb];
+      p.part_ml[2 * (r * p.num_splits + split) + 1] = total;
+    }
+  }
+}
+
 // Joins the splits of every query row and, where the call asks for them, adds
 // the heads' weights onto the cached rows:
 //   M = max_s m_s, L = sum_s 2^(m_s - M) l_s, out = sum_s 2^(m_s - M) O_s / L,
@@ -141,6 +583,7 @@ __device__ __forceinline__ void join_stats(const RowAttnParams &p, size_t r, int
   inv = total != 0.f ? 1.f / total : 0.f;
 }
 
+// dim_slices 0: the outputs are written already.
 template <bool kBf16>
 __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnParams p, int dim_slices) {
   __shared__ float red[kThreads / 16][kSliceDims + 4];
@@ -224,28 +667,82 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
 
 struct RowPlan {
   int split_tokens, num_splits;
+  int row_blocks;  // 16-row blocks of a workgroup on the matrix cores; 0: any-shape kernel
+  int row_tiles;
+  int64_t magic;
 };
 
-RowPlan plan_rows(int64_t total_q, int64_t heads, int64_t max_len) {
+// The matrix-core kernel's shapes; the query's and output's alignment comes on top.
+bool mfma_rows(int64_t d, int64_t dv, int64_t block_size, int64_t max_len) {
+  return (d == 64 || d == 128 || d == 256) && dv == d && block_size % 16 == 0 &&
+         (max_len / 16 + 1) * (block_size / 16) < (int64_t(1) << 36) && block_size / 16 < (int64_t(1) << 20);
+}
+
+RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int64_t hkv, int64_t d, int64_t block_size,
+                  int64_t max_query, int64_t max_len) {
   RowPlan pl{};
   const int64_t len = std::max<int64_t>(max_len, 1);
-  // About 2048 workgroups, at least 64 cache rows each.
-  int64_t splits = std::max<int64_t>(1, 2048 / std::max<int64_t>(total_q * heads, 1));
-  splits = std::min<int64_t>(splits, (len + 63) / 64);
-  splits = std::min<int64_t>(splits, kMaxSplits);
-  pl.split_tokens = int((len + splits - 1) / splits);
-  pl.num_splits = int((len + pl.split_tokens - 1) / pl.split_tokens);
+  if (!mfma) {
+    // About 2048 workgroups, at least 64 cache rows each.
+    int64_t splits = std::max<int64_t>(1, 2048 / std::max<int64_t>(total_q * heads, 1));
+    splits = std::min<int64_t>(splits, (len + 63) / 64);
+    splits = std::min<int64_t>(splits, kMaxSplits);
+    pl.split_tokens = int((len + splits - 1) / splits);
+    pl.num_splits = int((len + pl.split_tokens - 1) / pl.split_tokens);
+    return pl;
+  }
+  const int64_t rows = std::max<int64_t>(max_query, 1) * (heads / hkv);
+  pl.row_blocks = rows <= 16 ? 1 : rows <= 32 || d == 64 ? 2 : 4;
+  pl.row_tiles = int((rows + 16 * pl.row_blocks - 1) / (16 * pl.row_blocks));
+  pl.magic = ((int64_t(1) << 36) + block_size / 16 - 1) / (block_size / 16);
+  const int64_t tile = 16384 / d, tiles = (len + tile - 1) / tile;
+  // About 512 workgroups (two per CU), whole tiles each.
+  const int64_t items = batch * hkv * pl.row_tiles;
+  const int64_t splits = std::min<int64_t>(std::max<int64_t>(1, (512 + items - 1) / items), kMaxSplits);
+  const int64_t per = std::max<int64_t>((tiles + splits - 1) / splits, 1);
+  pl.split_tokens = int(per * tile);
+  pl.num_splits = int((tiles + per - 1) / per);
   return pl;
 }
 
 int64_t x_stride_of(int64_t max_len) { return (std::max<int64_t>(max_len, 1) + 63) / 64 * 64; }
 
-size_t row_workspace(int64_t total_q, int64_t heads, int64_t dv, int64_t max_len, bool weights) {
-  const RowPlan pl = plan_rows(total_q, heads, max_len);
-  size_t floats = size_t(total_q) * heads * pl.num_splits * size_t(dv + 2);
+// Bytes for either kernel: the query's alignment, which also decides, is not known here.
+size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv, int64_t d, int64_t dv,
+                     int64_t block_size, int64_t max_query, int64_t max_len, bool weights) {
+  int64_t splits = plan_rows(false, batch, total_q, heads, hkv, d, block_size, max_query, max_len).num_splits;
+  if (mfma_rows(d, dv, block_size, max_len))
+    splits = std::max<int64_t>(splits, plan_rows(true, batch, total_q, heads, hkv, d, block_size, max_query, max_len).num_splits);
+  size_t floats = size_t(total_q) * heads * splits * size_t(dv + 2);
   floats = (floats + 3) / 4 * 4;
   if (weights) floats += size_t(total_q) * heads * size_t(x_stride_of(max_len));
   return floats * sizeof(float);
+}
+
+template <int kD, bool kBf16, int kRB, typename BtT>
+void launch_rows(const RowAttnParams &p, const RowTile &tile, hipStream_t s) {
+  const int64_t outer = (int64_t(p.batch) * p.num_splits + 7) / 8 * 8;
+  const unsigned blocks = unsigned(outer * p.hkv * tile.row_tiles);
+  if (p.x) row_attention_mfma<kD, kBf16, kRB, true, BtT><<<blocks, kThreads, 0, s>>>(p, tile);
+  else row_attention_mfma<kD, kBf16, kRB, false, BtT><<<blocks, kThreads, 0, s>>>(p, tile);
+}
+
+template <bool kBf16, typename BtT>
+void launch_row_attention(const RowAttnParams &p, const RowPlan &pl, hipStream_t s) {
+  if (!pl.row_blocks) {
+    row_attention_any<kBf16, BtT><<<dim3(unsigned(p.total_q) * unsigned(p.hq), unsigned(p.num_splits)), kThreads, 0, s>>>(p);
+    return;
+  }
+  const RowTile tile{pl.magic, 16 * pl.row_blocks, pl.row_tiles};
+  const auto with_dim = [&](auto dim) {
+    constexpr int kD = decltype(dim)::value;
+    if (pl.row_blocks == 1) launch_rows<kD, kBf16, 1, BtT>(p, tile, s);
+    else if (kD == 64 || pl.row_blocks == 2) launch_rows<kD, kBf16, 2, BtT>(p, tile, s);
+    else launch_rows<kD, kBf16, kD == 64 ? 2 : 4, BtT>(p, tile, s);
+  };
+  if (p.d == 64) with_dim(std::integral_constant<int, 64>{});
+  else if (p.d == 128) with_dim(std::integral_constant<int, 128>{});
+  else with_dim(std::integral_constant<int, 256>{});
 }
 
 struct RowArgs {
@@ -258,7 +755,7 @@ struct RowArgs {
   int64_t max_blocks;
   const int32_t *start_loc, *lens;
   const uint8_t *mask;
-  int64_t mask_stride, batch, heads, total_q, max_len;
+  int64_t mask_stride, batch, heads, total_q, max_query, max_len;
   float scale;
   void *out;
   float *weights;
@@ -294,14 +791,16 @@ int row_attention(const char *name, const RowArgs &a) {
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: caches must be 4-byte aligned", name);
   if (!aligned(a.query, 2) || !aligned(a.out, 2))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: query/out must be 2-byte aligned", name);
-  const size_t need = row_workspace(a.total_q, a.heads, a.dv, a.max_len, a.weights != nullptr);
+  const size_t need = row_workspace(a.batch, a.total_q, a.heads, a.hkv, a.d, a.dv, a.block_size, a.max_query, a.max_len,
+                                    a.weights != nullptr);
   if (!a.workspace || a.workspace_bytes < need)
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes required (got %zu)", name, need,
                 a.workspace_bytes);
   if (!aligned(a.workspace, 16))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", name);
 
-  const RowPlan pl = plan_rows(a.total_q, a.heads, a.max_len);
+  const bool mfma = mfma_rows(a.d, a.dv, a.block_size, a.max_len) && aligned(a.query, 16) && aligned(a.out, 16);
+  const RowPlan pl = plan_rows(mfma, a.batch, a.total_q, a.heads, a.hkv, a.d, a.block_size, a.max_query, a.max_len);
   RowAttnParams p{};
   p.query = a.query;
   p.key_cache = a.key_cache;
@@ -336,21 +835,24 @@ int row_attention(const char *name, const RowArgs &a) {
     p.weights = a.weights;
     p.w_stride = a.w_stride;
   }
-  const int dim_slices = int((a.dv + kSliceDims - 1) / kSliceDims);
-  const int64_t out_blocks = int64_t(rows) * dim_slices;
-  const int64_t weight_blocks = a.weights ? a.batch * a.hkv * ((a.max_len + kWeightKeys - 1) / kWeightKeys) : 0;
-  if (out_blocks + weight_blocks > 0xFFFFFFFFll / kThreads)  // threads of one launch
+  // One split of the matrix-core kernel writes the outputs itself.
+  const int dim_slices = mfma && pl.num_splits == 1 ? 0 : int((a.dv + kSliceDims - 1) / kSliceDims);
+  const int64_t join_blocks = int64_t(rows) * dim_slices +
+                              (a.weights ? a.batch * a.hkv * ((a.max_len + kWeightKeys - 1) / kWeightKeys) : 0);
+  const int64_t attn_blocks =
+      mfma ? (a.batch * pl.num_splits + 7) / 8 * 8 * a.hkv * pl.row_tiles : int64_t(rows);
+  if (std::max(join_blocks, attn_blocks) > 0xFFFFFFFFll / kThreads)  // threads of one launch
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
   hipStream_t s = reinterpret_cast<hipStream_t>(a.stream);
   const bool bf16 = a.q_dtype == HIF8_DTYPE_BF16, i64 = a.bt_dtype == HIF8_INDEX_INT64;
-  const dim3 grid(unsigned(rows), unsigned(pl.num_splits));
-  if (bf16 && i64) row_attention_any<true, int64_t><<<grid, kThreads, 0, s>>>(p);
-  else if (bf16) row_attention_any<true, int32_t><<<grid, kThreads, 0, s>>>(p);
-  else if (i64) row_attention_any<false, int64_t><<<grid, kThreads, 0, s>>>(p);
-  else row_attention_any<false, int32_t><<<grid, kThreads, 0, s>>>(p);
-  const unsigned blocks = unsigned(out_blocks + weight_blocks);
-  if (bf16) row_attention_join<true><<<blocks, kThreads, 0, s>>>(p, dim_slices);
-  else row_attention_join<false><<<blocks, kThreads, 0, s>>>(p, dim_slices);
+  if (bf16 && i64) launch_row_attention<true, int64_t>(p, pl, s);
+  else if (bf16) launch_row_attention<true, int32_t>(p, pl, s);
+  else if (i64) launch_row_attention<false, int64_t>(p, pl, s);
+  else launch_row_attention<false, int32_t>(p, pl, s);
+  if (join_blocks > 0) {
+    if (bf16) row_attention_join<true><<<unsigned(join_blocks), kThreads, 0, s>>>(p, dim_slices);
+    else row_attention_join<false><<<unsigned(join_blocks), kThreads, 0, s>>>(p, dim_slices);
+  }
   return check_launch(name);
 }
 
@@ -360,13 +862,14 @@ int row_attention(const char *name, const RowArgs &a) {
 using namespace hif8;
 
 extern "C" size_t hif8_tree_attention_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
-                                                     int64_t head_size, int64_t head_size_v,
+                                                     int64_t head_size, int64_t head_size_v, int64_t block_size,
                                                      int64_t total_query_tokens, int64_t max_query_len,
                                                      int64_t max_seq_len) {
   if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || head_size_v <= 0 ||
-      total_query_tokens <= 0 || max_query_len <= 0 || max_seq_len < 0 || num_heads % num_kv_heads)
+      block_size <= 0 || total_query_tokens <= 0 || max_query_len <= 0 || max_seq_len < 0 || num_heads % num_kv_heads)
     return 0;
-  return row_workspace(total_query_tokens, num_heads, head_size_v, max_seq_len, false);
+  return row_workspace(batch, total_query_tokens, num_heads, num_kv_heads, head_size, head_size_v, block_size,
+                       max_query_len, max_seq_len, false);
 }
 
 extern "C" int hif8_tree_attention(const void *query, int q_dtype, const uint8_t *key_cache,
@@ -393,17 +896,18 @@ extern "C" int hif8_tree_attention(const void *query, int q_dtype, const uint8_t
   return row_attention(kName, RowArgs{query, q_dtype, key_cache, value_cache, num_blocks, block_size, num_kv_heads,
                                       head_size, head_size_v, block_table, block_table_dtype, max_blocks_per_seq,
                                       query_start_loc, context_lens, tree_mask, mask_width, batch, num_heads,
-                                      total_query_tokens, max_seq_len, scale, out, nullptr, 0, 0, workspace,
+                                      total_query_tokens, max_query_len, max_seq_len, scale, out, nullptr, 0, 0, workspace,
                                       workspace_bytes, stream});
 }
 
 extern "C" size_t hif8_paged_decode_attention_weights_workspace_size(int64_t batch, int64_t num_heads,
                                                                      int64_t num_kv_heads, int64_t head_size,
-                                                                     int64_t head_size_v, int64_t max_seq_len) {
-  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || head_size_v <= 0 || max_seq_len < 0 ||
-      num_heads % num_kv_heads)
+                                                                     int64_t head_size_v, int64_t block_size,
+                                                                     int64_t max_seq_len) {
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || head_size_v <= 0 || block_size <= 0 ||
+      max_seq_len < 0 || num_heads % num_kv_heads)
     return 0;
-  return row_workspace(batch, num_heads, head_size_v, max_seq_len, true);
+  return row_workspace(batch, batch, num_heads, num_kv_heads, head_size, head_size_v, block_size, 1, max_seq_len, true);
 }
 
 extern "C" int hif8_paged_decode_attention_weights(const void *query, int q_dtype, const uint8_t *key_cache,
@@ -422,6 +926,6 @@ extern "C" int hif8_paged_decode_attention_weights(const void *query, int q_dtyp
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: key_weights must be 4-byte aligned", kName);
   return row_attention(kName, RowArgs{query, q_dtype, key_cache, value_cache, num_blocks, block_size, num_kv_heads,
                                       head_size, head_size_v, block_table, block_table_dtype, max_blocks_per_seq,
-                                      nullptr, seq_lens, nullptr, 0, batch, num_heads, batch, max_seq_len, scale, out,
+                                      nullptr, seq_lens, nullptr, 0, batch, num_heads, batch, 1, max_seq_len, scale, out,
                                       key_weights, weights_stride, accumulate, workspace, workspace_bytes, stream});
 }

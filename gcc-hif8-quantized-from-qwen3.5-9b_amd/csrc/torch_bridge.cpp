@@ -1376,8 +1376,8 @@ at::Tensor Hif8TreeAttention(const at::Tensor &query, const at::Tensor &key_cach
   const c10::OptionalDeviceGuard guard(query.device());
   auto out = at::empty({query.size(0), query.size(1), o.dv}, query.options());
   if (batch == 0 || query.size(0) == 0 || max_query_len == 0) return out;
-  const size_t bytes = hif8_tree_attention_workspace_size(batch, query.size(1), o.kv_heads, o.d, o.dv, query.size(0),
-                                                          max_query_len, max_seq_len);
+  const size_t bytes = hif8_tree_attention_workspace_size(batch, query.size(1), o.kv_heads, o.d, o.dv, o.block_size,
+                                                          query.size(0), max_query_len, max_seq_len);
   const auto ws = Workspace(bytes, query);
   CheckStatus(hif8_tree_attention(query.data_ptr(), DtypeCode(query.scalar_type()), key_cache.data_ptr<uint8_t>(),
                                   value_cache.data_ptr<uint8_t>(), o.num_blocks, o.block_size, o.kv_heads, o.d, o.dv,
@@ -1403,7 +1403,8 @@ at::Tensor Hif8PagedDecodeAttentionWeights(const at::Tensor &query, const at::Te
   auto out = at::empty({batch, query.size(1), o.dv}, query.options());
   if (batch == 0) return out;
   const size_t bytes =
-      hif8_paged_decode_attention_weights_workspace_size(batch, query.size(1), o.kv_heads, o.d, o.dv, max_seq_len);
+      hif8_paged_decode_attention_weights_workspace_size(batch, query.size(1), o.kv_heads, o.d, o.dv, o.block_size,
+                                                         max_seq_len);
   const auto ws = Workspace(bytes, query);
   CheckStatus(hif8_paged_decode_attention_weights(
                   query.data_ptr(), DtypeCode(query.scalar_type()), key_cache.data_ptr<uint8_t>(),

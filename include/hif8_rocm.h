@@ -406,8 +406,8 @@ int hif8_paged_prefill_attention(const void *query, int q_dtype, const uint8_t *
  *              size depends on these arguments alone
  */
 size_t hif8_tree_attention_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
-                                          int64_t head_size_v, int64_t total_query_tokens, int64_t max_query_len,
-                                          int64_t max_seq_len);
+                                          int64_t head_size_v, int64_t block_size, int64_t total_query_tokens,
+                                          int64_t max_query_len, int64_t max_seq_len);
 int hif8_tree_attention(const void *query, int q_dtype, const uint8_t *key_cache, const uint8_t *value_cache,
                         int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_size,
                         int64_t head_size_v, const void *block_table, int block_table_dtype,
@@ -427,7 +427,7 @@ int hif8_tree_attention(const void *query, int q_dtype, const uint8_t *key_cache
  */
 size_t hif8_paged_decode_attention_weights_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
                                                           int64_t head_size, int64_t head_size_v,
-                                                          int64_t max_seq_len);
+                                                          int64_t block_size, int64_t max_seq_len);
 int hif8_paged_decode_attention_weights(const void *query, int q_dtype, const uint8_t *key_cache,
                                         const uint8_t *value_cache, int64_t num_blocks, int64_t block_size,
                                         int64_t num_kv_heads, int64_t head_size, int64_t head_size_v,

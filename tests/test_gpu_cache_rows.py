@@ -168,7 +168,7 @@ def test_tree_rows_outside_every_request_stay(native_ops, device):
     lib = ctypes.CDLL(str(PKG_ROOT / "hif8_rocm" / "libhif8_rocm.so"))
     lib.hif8_last_error.restype = ctypes.c_char_p
     size = lib.hif8_tree_attention_workspace_size
-    size.argtypes, size.restype = [ctypes.c_int64] * 8, ctypes.c_size_t
+    size.argtypes, size.restype = [ctypes.c_int64] * 9, ctypes.c_size_t
     i64, ptr, i32 = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int
     lib.hif8_tree_attention.argtypes = [ptr, i32, ptr, ptr] + [i64] * 5 + [ptr, i32, i64, ptr, ptr, ptr] + [i64] * 6 + \
         [ctypes.c_float, ptr, ptr, ctypes.c_size_t, ptr]
@@ -180,7 +180,7 @@ def test_tree_rows_outside_every_request_stay(native_ops, device):
         mask = torch.ones(14, 10, dtype=torch.bool, device=device)
         table = table.to(device)
         out = torch.full((14, 16, d), 7.0, dtype=torch.bfloat16, device=device)
-        need = size(1, 16, 4, d, d, 14, 10, 210)
+        need = size(1, 16, 4, d, d, bs, 14, 10, 210)
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
         st = lib.hif8_tree_attention(p(q), 1, p(kc), p(vc), kc.shape[0], bs, 4, d, d, p(table), 0, table.shape[1], p(loc),
