@@ -9,8 +9,9 @@
 #include <stddef.h>
 
 #include <algorithm>
+#include <type_traits>
 
-#include "hif8_common.h"
+#include "mfma_lookup.h"
 
 namespace hif8 {
 namespace {
@@ -29,6 +30,13 @@ struct WeightParams {
   int64_t bt_stride, num_blocks, w_stride;
   int block_size, hkv, hq, group, d, batch, total_q, max_len, causal, accumulate;
   float scale_log2;
+  // Matrix-core kernels.
+  float *part;                 // [key tiles, rows of this chunk * Hq, 2]: maximum, sum
+  float *part_w;               // [row splits, batch, Hkv, w_pad] sums, or null: straight into weights
+  int64_t magic, group_magic;  // ceil(2^36 / (block_size / 16)), ceil(2^32 / group)
+  int64_t w_pad;
+  int tok_lo, tok_hi;          // query tokens of this chunk
+  int tiles, row_splits, split_rows;
 };
 
 __device__ __forceinline__ int clamp_rows(int n, int most) { return n < 0 ? 0 : (n > most ? most : n); }
@@ -115,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void key_sums_any(const WeightParams p, i
   float *w = p.weights + (int64_t(b) * p.hkv + h) * p.w_stride;
   for (int t = 64 * tile + 16 * wave; t < min(64 * tile + 16 * wave + 16, len); ++t) {
     const int64_t blk = int64_t(bt[t / p.block_size]);
-    float sum = 0.f;
+    float sum = 0.f, block = 0.f;
     if (blk >= 0 && blk < p.num_blocks) {
       const uint8_t *kr = p.key_cache + ((blk * p.block_size + t % p.block_size) * p.hkv + h) * (p.d + 4);
       const float ksc = *reinterpret_cast<const float *>(kr + p.d) * p.scale_log2;
@@ -127,7 +135,8 @@ __global__ __launch_bounds__(kThreads) void key_sums_any(const WeightParams p, i
       }
       // The first query row that sees row t.
       const int first = p.causal ? max(0, t - (len - count)) : 0;
-      for (int i = first; i < count; ++i)
+      for (int i = first; i < count; ++i) {
+        float part = 0.f;  // a query token's heads, then the tokens: the sum of many small terms stays near
         for (int g = 0; g < p.group; ++g) {
           const size_t r = size_t(begin + i) * p.hq + h * p.group + g;
           const uint16_t *q = static_cast<const uint16_t *>(p.query) + r * p.d;
@@ -137,10 +146,414 @@ __global__ __launch_bounds__(kThreads) void key_sums_any(const WeightParams p, i
             const int dim = lane + kWave * j;
             if (dim < p.d) dot = fmaf(half_bits_to_float<kBf16>(q[dim]), kv[j], dot);
           }
-          sum += __builtin_amdgcn_exp2f(wave_sum(dot) * ksc - p.stat[2 * r]) * p.stat[2 * r + 1];
+          part += __builtin_amdgcn_exp2f(wave_sum(dot) * ksc - p.stat[2 * r]) * p.stat[2 * r + 1];
         }
+        block += part;
+        if ((i & 63) == 63) {
+          sum += block;
+          block = 0.f;
+        }
+      }
+      sum += block;
     }
     if (lane == 0) w[t] = p.accumulate ? w[t] + sum : sum;
+  }
+}
+
+// ---------------------------------------------------- on the matrix cores
+//
+// Head sizes 64, 128 and 256, pages of a multiple of 16 rows.  A workgroup of
+// four wavefronts owns 256 cached rows of a (request, KV head), 64 per
+// wavefront: their codes are decoded once into MFMA A operands (key =
+// lane % 16) that stay in registers, and the (token, head) rows of the queries
+// go by as B operands, 32 at a time through a ring in LDS filled by DMA in
+// operand order.  The keys are stationary because every query row then costs
+// one pass of 8 D / 256 LDS reads for 256 keys, and column sums need no
+// exchange.  Two passes over S = K Q^T:
+//   kSums false: per query row the maximum and the sum of 2^(x - maximum) over
+//     the 256 keys, joined over the wavefronts in LDS, to `part`;
+//   kSums true: with every row's maximum and sum known, each lane adds up
+//     2^(x - M) / L of its keys over the rows, joined over the lanes at the end.
+// A third small kernel joins `part` over the key tiles, a fourth the sums over
+// the row splits; all orders of summation are fixed.
+constexpr int kKeys = 256;    // cached rows of a workgroup
+constexpr int kStage = 32;    // query rows of a ring stage
+constexpr int kRing = 3;
+
+__device__ __forceinline__ void row_place(const WeightParams &p, int h, int r, int &tok, int &head) {
+  tok = int((uint64_t(uint32_t(r)) * uint64_t(p.group_magic)) >> 32);
+  head = h * p.group + (r - tok * p.group);
+}
+
+template <int kD, bool kBf16, bool kSums, typename BtT>
+__global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams p) {
+  constexpr int kRow = kD + 4;
+  constexpr int kQS = kD / 32;
+  constexpr int kSlices = kD / 64;
+  constexpr int kStageBytes = kStage * kD * 2;
+  constexpr int kDma = kQS / 2;  // DMA instructions of a wavefront per stage
+  static_assert(kRing * kStageBytes <= kLookupBytes, "the ring reuses the table's LDS");
+  struct Smem {
+    uint32_t table[kLookupBytes / 4];  // then the ring
+    float2 ml[2][4][kStage];           // a stage's (maximum, sum) per wavefront
+  };
+  __shared__ __attribute__((aligned(16))) Smem sm;
+  const uint32_t table = lds_address(sm.table);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+
+  // The key tiles of one (request, KV head, row split) read the same queries:
+  // their blocks are equal modulo 8, on one XCD.
+  const int xcd = int(blockIdx.x) & 7, slot = int(blockIdx.x) >> 3;
+  const int outer = (slot / p.tiles) * 8 + xcd;
+  if (outer >= p.batch * p.hkv * p.row_splits) return;  // padding block (uniform)
+  const int tile = slot % p.tiles;
+  const int h = outer % p.hkv, split = (outer / p.hkv) % p.row_splits, b = outer / (p.hkv * p.row_splits);
+  const int len = clamp_rows(p.lens[b], p.max_len);
+  const int t0 = tile * kKeys;
+  if (t0 >= len) return;  // uniform
+  int begin, count;
+  request_rows(p, b, begin, count);
+  // Query rows of this split and chunk that see row t0 or later.
+  const int shift = p.causal ? len - count : len;     // row i sees rows up to shift + i (causal)
+  const int first_tok = p.causal ? max(t0 - shift, 0) : 0;
+  const int lo_tok = max(first_tok, p.tok_lo - begin), hi_tok = min(count, p.tok_hi - begin);
+  const int64_t lo64 = max(int64_t(split) * p.split_rows, int64_t(max(lo_tok, 0)) * p.group);
+  const int64_t hi64 = min((int64_t(split) + 1) * p.split_rows, int64_t(max(hi_tok, 0)) * p.group);
+  const int r_lo = int(min(lo64, int64_t(0x7FFFFFFF))), r_hi = int(min(hi64, int64_t(0x7FFFFFFF)));
+  const int stages = r_hi > r_lo ? (r_hi - r_lo + kStage - 1) / kStage : 0;
+  const int key0 = t0 + 64 * wave;  // first key of this wavefront
+
+  float acc[4][4];  // column sums of keys key0 + 16 kb + 4 g + e over rows n mod 16
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[kb][e] = 0.f;
+
+  if (stages > 0) {
+    // Decode the wavefront's keys.
+    const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.bt_stride;
+    const uint32_t rec = uint32_t(p.hkv) * kRow;
+    const int gr = min(key0 + 16 * (lane & 3), len - 1) >> 4;  // lane i % 4 looks up 16-row group i
+    const int col = int((uint64_t(gr) * uint64_t(p.magic)) >> 36);
+    const int64_t blk = int64_t(bt[col]);
+    const bool there = blk >= 0 && blk < p.num_blocks && key0 + 16 * (lane & 3) < len;
+    const int64_t off_lane =
+        there ? (blk * p.block_size + 16 * (gr - col * (p.block_size >> 4))) * int64_t(rec) + int64_t(h) * kRow : int64_t(-1);
+    const uint32_t ok_groups = uint32_t(__ballot(off_lane >= 0)) & 15u;
+    typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+    lk_u32x4 raw[4][kSlices];
+    float ksc[4][4];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      const int lo = __builtin_amdgcn_readlane(int(uint64_t(off_lane)), kb);
+      const int hi = __builtin_amdgcn_readlane(int(uint64_t(off_lane) >> 32), kb);
+      const int64_t off = int64_t((uint64_t(uint32_t(hi)) << 32) | uint32_t(lo));
+      const uint8_t *kp = p.key_cache + (off < 0 ? 0 : off);
+#pragma unroll
+      for (int i = 0; i < kSlices; ++i)
+        raw[kb][i] = *reinterpret_cast<const u32x4_a4 *>(kp + uint32_t(n) * rec + 16u * g + 64 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        ksc[kb][e] = *reinterpret_cast<const float *>(kp + uint32_t(4 * g + e) * rec + kD) * p.scale_log2;
+    }
+    fill_lookup<kBf16, kThreads>(sm.table, tid);
+    lds_barrier();
+    const uint32_t lane4 = uint32_t(4 * lane);
+    lk_u32x4 kf[4][kQS];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      __builtin_amdgcn_sched_barrier(0);  // one block's lookups at a time: registers
+#pragma unroll
+      for (int i = 0; i < kQS; ++i)
+        kf[kb][i] = look8<false>(raw[kb][i >> 1][2 * (i & 1)], raw[kb][i >> 1][2 * (i & 1) + 1], lane4, table);
+    }
+    lds_barrier();  // the ring takes the table's place
+
+    // Stage s: rows r_lo + 32 s .. + 31; rows past the last repeat it.  Wavefront
+    // w brings half of the operands of row block w / 2.
+    const uint16_t *query = static_cast<const uint16_t *>(p.query);
+    auto fetch = [&](int s) {
+      const int r = min(r_lo + kStage * s + 16 * (wave >> 1) + n, r_hi - 1);
+      int tok, head;
+      row_place(p, h, r, tok, head);
+      const uint16_t *q = query + (size_t(begin + tok) * p.hq + head) * kD + 16 * g;
+      const uint32_t to = table + uint32_t((s % kRing) * kStageBytes) + uint32_t((wave >> 1) * kQS * 1024);
+#pragma unroll
+      for (int j = 0; j < kDma; ++j) {
+        const int i = (wave & 1) * kDma + j;
+        dma16(q + 64 * (i >> 1) + 8 * (i & 1), to + 1024u * uint32_t(i));
+      }
+    };
+    float2 st[2] = {};  // (M, 1 / L) of this lane's rows in the stage
+    auto load_stats = [&](int s) {
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        const int r = r_lo + kStage * s + 16 * rb + n;
+        int tok, head;
+        row_place(p, h, min(r, r_hi - 1), tok, head);
+        const float2 v = reinterpret_cast<const float2 *>(p.stat)[size_t(begin + tok) * p.hq + head];
+        st[rb] = float2{v.x, r < r_hi ? v.y : 0.f};
+      }
+    };
+    fetch(0);
+    if (stages > 1) fetch(1);
+    if constexpr (kSums) load_stats(0);
+    for (int s = 0; s < stages; ++s) {
+      if (s + 1 < stages) wait_vmcnt<kDma>();  // this stage's copies; the next one's may be in flight
+      else wait_vmcnt<0>();
+      lds_barrier();  // every wavefront's copies have landed, and it is done with the stage before
+      if constexpr (!kSums) {
+        // Join the previous stage's rows over the wavefronts.
+        if (s > 0 && tid < kStage) {
+          const int r = r_lo + kStage * (s - 1) + tid;
+          int tok, head;
+          row_place(p, h, r, tok, head);
+          float2 v = sm.ml[(s - 1) & 1][0][tid];
+#pragma unroll
+          for (int w = 1; w < 4; ++w) {
+            const float2 o = sm.ml[(s - 1) & 1][w][tid];
+            const float mx = fmaxf(v.x, o.x);
+            const float a = v.y != 0.f ? __builtin_amdgcn_exp2f(v.x - mx) * v.y : 0.f;
+            const float c = o.y != 0.f ? __builtin_amdgcn_exp2f(o.x - mx) * o.y : 0.f;
+            v = float2{mx, a + c};
+          }
+          const size_t chunk_rows = size_t(p.tok_hi - p.tok_lo) * p.hq;
+          reinterpret_cast<float2 *>(p.part)[size_t(tile) * chunk_rows + size_t(begin + tok - p.tok_lo) * p.hq + head] = v;
+        }
+      }
+      float2 cur[2] = {st[0], st[1]};
+      if (s + 2 < stages) fetch(s + 2);
+      if constexpr (kSums) {
+        if (s + 1 < stages) load_stats(s + 1);
+      }
+      const lk_u32x4 *q = reinterpret_cast<const lk_u32x4 *>(reinterpret_cast<const uint8_t *>(sm.table) +
+                                                            (s % kRing) * kStageBytes);
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int r0 = r_lo + kStage * s + 16 * rb;
+        lk_f32x4 d[4];
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) d[kb] = lk_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kQS; ++i) {
+          const lk_u32x4 qf = q[(rb * kQS + i) * kWave + lane];
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb) d[kb] = mfma_16x16x32<kBf16>(kf[kb][i], qf, d[kb]);
+        }
+        // Every row of the block sees every key of the wavefront (uniform).
+        int tok0, head0;
+        row_place(p, h, r0, tok0, head0);
+        const bool full = key0 + 64 <= len && ok_groups == 15u && (!p.causal || key0 + 63 <= shift + tok0);
+        int lim = len;
+        if (!full && p.causal) {
+          int tok, head;
+          row_place(p, h, min(r0 + n, r_hi - 1), tok, head);
+          lim = min(len, shift + tok + 1);
+        }
+        // One copy of the arithmetic per case: a test per element would branch in the loop.
+        auto block = [&](auto all) {
+          constexpr bool kAll = decltype(all)::value;
+          auto visible = [&](int kb, int e) {
+            return ((ok_groups >> kb) & 1u) && key0 + 16 * kb + 4 * g + e < lim;
+          };
+          if constexpr (kSums) {
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(d[kb][e], ksc[kb][e], -cur[rb].x));
+                const float sum = fmaf(w, cur[rb].y, acc[kb][e]);
+                acc[kb][e] = kAll || (visible(kb, e) && r0 + n < r_hi) ? sum : acc[kb][e];
+              }
+          } else {
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = d[kb][e] * ksc[kb][e];
+                d[kb][e] = kAll || visible(kb, e) ? x : -__builtin_inff();
+                mx = fmaxf(mx, d[kb][e]);
+              }
+            mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+            const float use = mx == -__builtin_inff() ? 0.f : mx;
+            float l = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) l += __builtin_amdgcn_exp2f(d[kb][e] - use);
+            l += __shfl_xor(l, 16, kWave);
+            l += __shfl_xor(l, 32, kWave);
+            if (g == 0) sm.ml[s & 1][wave][16 * rb + n] = float2{mx, l};
+          }
+        };
+        if (full) block(std::true_type{});
+        else block(std::false_type{});
+      }
+    }
+    if constexpr (!kSums) {
+      lds_barrier();
+      const int s = stages - 1;
+      const int r = r_lo + kStage * s + tid;
+      if (tid < kStage && r < r_hi) {
+        int tok, head;
+        row_place(p, h, r, tok, head);
+        float2 v = sm.ml[s & 1][0][tid];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+          const float2 o = sm.ml[s & 1][w][tid];
+          const float mx = fmaxf(v.x, o.x);
+          const float a = v.y != 0.f ? __builtin_amdgcn_exp2f(v.x - mx) * v.y : 0.f;
+          const float c = o.y != 0.f ? __builtin_amdgcn_exp2f(o.x - mx) * o.y : 0.f;
+          v = float2{mx, a + c};
+        }
+        const size_t chunk_rows = size_t(p.tok_hi - p.tok_lo) * p.hq;
+        reinterpret_cast<float2 *>(p.part)[size_t(tile) * chunk_rows + size_t(begin + tok - p.tok_lo) * p.hq + head] = v;
+      }
+    }
+  }
+  if constexpr (kSums) {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = acc[kb][e];
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, kWave);
+        const int t = key0 + 16 * kb + 4 * g + e;
+        if (n == 0 && t < len) {
+          if (p.part_w) {
+            p.part_w[((int64_t(split) * p.batch + b) * p.hkv + h) * p.w_pad + t] = v;
+          } else {
+            float *w = p.weights + (int64_t(b) * p.hkv + h) * p.w_stride + t;
+            *w = p.accumulate ? *w + v : v;
+          }
+        }
+      }
+  }
+}
+
+// (M, 1 / L) of every (query row, head) of a chunk from its key tiles.
+__global__ __launch_bounds__(kThreads) void key_stats_join(const WeightParams p) {
+  const int64_t rows = int64_t(p.tok_hi - p.tok_lo) * p.hq;
+  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  if (i >= rows) return;
+  const int row = p.tok_lo + int(i / p.hq);
+  int lo = 0, hi = p.batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (p.start_loc[mid] <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  int begin, count;
+  request_rows(p, lo, begin, count);
+  if (row < begin || row - begin >= count) return;  // a row behind the last request
+  const int end = rows_of(p, clamp_rows(p.lens[lo], p.max_len), count, row - begin);
+  const int tiles = (end + kKeys - 1) / kKeys;
+  const float2 *part = reinterpret_cast<const float2 *>(p.part) + i;
+  float m = -__builtin_inff(), l = 0.f;
+#pragma unroll 4
+  for (int t = 0; t < tiles; ++t) {
+    const float2 v = part[int64_t(t) * rows];
+    const float mx = fmaxf(m, v.x);
+    l = (l != 0.f ? __builtin_amdgcn_exp2f(m - mx) * l : 0.f) + (v.y != 0.f ? __builtin_amdgcn_exp2f(v.x - mx) * v.y : 0.f);
+    m = mx;
+  }
+  reinterpret_cast<float2 *>(p.stat)[int64_t(p.tok_lo) * p.hq + i] =
+      float2{m == -__builtin_inff() ? 0.f : m, l != 0.f ? 1.f / l : 0.f};
+}
+
+// Adds the row splits' sums, in order.
+__global__ __launch_bounds__(kThreads) void key_sums_join(const WeightParams p) {
+  const int t = int(blockIdx.x) * kThreads + threadIdx.x, h = int(blockIdx.y), b = int(blockIdx.z);
+  if (t >= clamp_rows(p.lens[b], p.max_len)) return;
+  const int64_t bh = int64_t(b) * p.hkv + h;
+  float v = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < p.row_splits; ++s) v += p.part_w[(int64_t(s) * p.batch * p.hkv + bh) * p.w_pad + t];
+  float *w = p.weights + bh * p.w_stride + t;
+  *w = p.accumulate ? *w + v : v;
+}
+
+// ------------------------------------------------------------- host side
+
+struct WeightPlan {
+  bool mfma;
+  int tiles, row_splits, split_rows;
+  int64_t chunk_tokens;  // query tokens whose partial statistics are held at once
+};
+
+constexpr int64_t kPartBytes = int64_t(64) << 20;
+
+WeightPlan plan_weights(int64_t batch, int64_t heads, int64_t hkv, int64_t d, int64_t block_size, int64_t total_q,
+                        int64_t max_query, int64_t max_len) {
+  WeightPlan pl{};
+  const int64_t group = heads / hkv;
+  pl.mfma = (d == 64 || d == 128 || d == 256) && block_size % 16 == 0 && block_size / 16 < (int64_t(1) << 20) &&
+            (max_len / 16 + 1) * (block_size / 16) < (int64_t(1) << 36) && max_query * group * group < (int64_t(1) << 31);
+  if (!pl.mfma) return pl;
+  pl.tiles = int((max_len + kKeys - 1) / kKeys);
+  const int64_t rows = max_query * group;
+  const int64_t items = batch * hkv * pl.tiles;
+  // Row splits of at least 512 rows (a workgroup's keys cost about as much to decode as
+  // 64 rows to pass) until there are about 1024 workgroups.
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>((1024 + items - 1) / items, rows / 512));
+  pl.split_rows = int(((rows + splits - 1) / splits + kStage - 1) / kStage * kStage);
+  pl.row_splits = int((rows + pl.split_rows - 1) / pl.split_rows);
+  pl.chunk_tokens = std::min<int64_t>(total_q, std::max<int64_t>(64, kPartBytes / (int64_t(pl.tiles) * heads * 8)));
+  return pl;
+}
+
+// The statistics, then the chunk's partial ones, then the row splits' sums.
+struct WeightSpace {
+  size_t stat, part, part_w;
+};
+
+WeightSpace weight_space(const WeightPlan &pl, int64_t batch, int64_t heads, int64_t hkv, int64_t total_q,
+                         int64_t max_len) {
+  WeightSpace w{};
+  w.stat = (size_t(total_q) * heads * 8 + 255) / 256 * 256;
+  if (pl.mfma) {
+    w.part = (size_t(pl.tiles) * size_t(pl.chunk_tokens) * heads * 8 + 255) / 256 * 256;
+    if (pl.row_splits > 1) w.part_w = size_t(pl.row_splits) * batch * hkv * size_t(pl.tiles) * kKeys * 4;
+  }
+  return w;
+}
+
+template <int kD, bool kBf16, typename BtT>
+void launch_weights(WeightParams p, const WeightPlan &pl, hipStream_t s) {
+  const int64_t outer = (int64_t(p.batch) * p.hkv * p.row_splits + 7) / 8 * 8;
+  const unsigned blocks = unsigned(outer * p.tiles);
+  for (int64_t lo = 0; lo < p.total_q; lo += pl.chunk_tokens) {
+    p.tok_lo = int(lo);
+    p.tok_hi = int(std::min<int64_t>(p.total_q, lo + pl.chunk_tokens));
+    key_pass_mfma<kD, kBf16, false, BtT><<<blocks, kThreads, 0, s>>>(p);
+    const int64_t rows = int64_t(p.tok_hi - p.tok_lo) * p.hq;
+    key_stats_join<<<unsigned((rows + kThreads - 1) / kThreads), kThreads, 0, s>>>(p);
+  }
+  p.tok_lo = 0;
+  p.tok_hi = p.total_q;
+  key_pass_mfma<kD, kBf16, true, BtT><<<blocks, kThreads, 0, s>>>(p);
+  if (p.part_w)
+    key_sums_join<<<dim3(unsigned((p.max_len + kThreads - 1) / kThreads), unsigned(p.hkv), unsigned(p.batch)), kThreads, 0,
+                    s>>>(p);
+}
+
+template <bool kBf16, typename BtT>
+void launch_key_weights(const WeightParams &p, const WeightPlan &pl, unsigned rows, unsigned sums, hipStream_t s) {
+  if (!pl.mfma) {
+    if (rows) key_stats_any<kBf16, BtT><<<rows, kThreads, 0, s>>>(p);
+    key_sums_any<kBf16, BtT><<<sums, kThreads, 0, s>>>(p, int((p.max_len + 63) / 64));
+  } else if (p.d == 64) {
+    launch_weights<64, kBf16, BtT>(p, pl, s);
+  } else if (p.d == 128) {
+    launch_weights<128, kBf16, BtT>(p, pl, s);
+  } else {
+    launch_weights<256, kBf16, BtT>(p, pl, s);
   }
 }
 
@@ -150,12 +563,16 @@ __global__ __launch_bounds__(kThreads) void key_sums_any(const WeightParams p, i
 using namespace hif8;
 
 extern "C" size_t hif8_key_weights_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
-                                                  int64_t head_size, int64_t total_query_tokens,
+                                                  int64_t head_size, int64_t block_size, int64_t total_query_tokens,
                                                   int64_t max_query_len, int64_t max_seq_len) {
-  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || total_query_tokens <= 0 ||
-      max_query_len <= 0 || max_seq_len <= 0 || num_heads % num_kv_heads)
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || block_size <= 0 ||
+      total_query_tokens < 0 || max_query_len < 0 || max_seq_len <= 0 || num_heads % num_kv_heads)
     return 0;
-  return size_t(total_query_tokens) * num_heads * 2 * sizeof(float);
+  // Either kernel: the query's alignment, which also decides, is not known here.
+  const WeightPlan pl = plan_weights(batch, num_heads, num_kv_heads, head_size, block_size, total_query_tokens,
+                                     std::max<int64_t>(max_query_len, 1), max_seq_len);
+  const WeightSpace w = weight_space(pl, batch, num_heads, num_kv_heads, total_query_tokens, max_seq_len);
+  return w.stat + w.part + w.part_w;
 }
 
 extern "C" int hif8_key_weights(const void *query, int q_dtype, const uint8_t *key_cache, int64_t num_blocks,
@@ -196,8 +613,8 @@ extern "C" int hif8_key_weights(const void *query, int q_dtype, const uint8_t *k
   if (!aligned(query, 2)) return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: query must be 2-byte aligned", kName);
   if (!aligned(key_weights, 4))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: key_weights must be 4-byte aligned", kName);
-  const size_t need = hif8_key_weights_workspace_size(batch, num_heads, num_kv_heads, head_size, total_query_tokens,
-                                                      max_query_len, max_seq_len);
+  const size_t need = hif8_key_weights_workspace_size(batch, num_heads, num_kv_heads, head_size, block_size,
+                                                      total_query_tokens, max_query_len, max_seq_len);
   if (need && (!workspace || workspace_bytes < need))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes required (got %zu)", kName, need,
                 workspace_bytes);
@@ -230,18 +647,29 @@ extern "C" int hif8_key_weights(const void *query, int q_dtype, const uint8_t *k
   p.causal = causal ? 1 : 0;
   p.accumulate = accumulate ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
+  WeightPlan pl = plan_weights(batch, num_heads, num_kv_heads, head_size, block_size, total_query_tokens,
+                               std::max<int64_t>(max_query_len, 1), max_seq_len);
+  if (pl.mfma) {
+    const WeightSpace w = weight_space(pl, batch, num_heads, num_kv_heads, total_query_tokens, max_seq_len);
+    p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + w.stat);
+    if (w.part_w) p.part_w = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + w.stat + w.part);
+    p.w_pad = int64_t(pl.tiles) * kKeys;
+    p.magic = ((int64_t(1) << 36) + block_size / 16 - 1) / (block_size / 16);
+    p.group_magic = ((int64_t(1) << 32) + p.group - 1) / p.group;
+    p.tiles = pl.tiles;
+    p.row_splits = pl.row_splits;
+    p.split_rows = pl.split_rows;
+    // 32-bit launch sizes, and operands that the copies into LDS can take.
+    if (!aligned(query, 16) || batch > 0xFFFF || num_kv_heads > 0xFFFF ||
+        (batch * num_kv_heads * pl.row_splits + 7) / 8 * 8 * pl.tiles > most)
+      pl.mfma = false;
+  }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool bf16 = q_dtype == HIF8_DTYPE_BF16, i64 = block_table_dtype == HIF8_INDEX_INT64;
   const unsigned rows = unsigned(total_query_tokens * num_heads), sums = unsigned(batch * num_kv_heads * tiles);
-#define HIF8_KEY_WEIGHTS(BF16, BT)                                                         \
-  do {                                                                                     \
-    if (rows) key_stats_any<BF16, BT><<<rows, kThreads, 0, s>>>(p);                        \
-    key_sums_any<BF16, BT><<<sums, kThreads, 0, s>>>(p, int(tiles));                       \
-  } while (0)
-  if (bf16 && i64) HIF8_KEY_WEIGHTS(true, int64_t);
-  else if (bf16) HIF8_KEY_WEIGHTS(true, int32_t);
-  else if (i64) HIF8_KEY_WEIGHTS(false, int64_t);
-  else HIF8_KEY_WEIGHTS(false, int32_t);
-#undef HIF8_KEY_WEIGHTS
+  if (bf16 && i64) launch_key_weights<true, int64_t>(p, pl, rows, sums, s);
+  else if (bf16) launch_key_weights<true, int32_t>(p, pl, rows, sums, s);
+  else if (i64) launch_key_weights<false, int64_t>(p, pl, rows, sums, s);
+  else launch_key_weights<false, int32_t>(p, pl, rows, sums, s);
   return check_launch(kName);
 }

@@ -362,22 +362,27 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
         }
       }
       float top = -__builtin_inff();
+      auto logits = [&](auto all) {
+        constexpr bool kAll = decltype(all)::value;
 #pragma unroll
-      for (int kb = 0; kb < kKB; ++kb) {
-        lk_f32x4 x;
+        for (int kb = 0; kb < kKB; ++kb) {
+          lk_f32x4 x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool vis = (seen[rb] >> (4 * kb + e)) & 1u;
-          x[e] = vis ? s[rb][kb][e] * ksc[kb][e] : -__builtin_inff();
-          y[rb][kb][e] = x[e] + ve[kb][e];
-          top = fmaxf(top, y[rb][kb][e]);
+          for (int e = 0; e < 4; ++e) {
+            const float z = s[rb][kb][e] * ksc[kb][e];
+            x[e] = kAll || ((seen[rb] >> (4 * kb + e)) & 1u) ? z : -__builtin_inff();
+            y[rb][kb][e] = x[e] + ve[kb][e];
+            top = fmaxf(top, y[rb][kb][e]);
+          }
+          if constexpr (kX) {
+            const int t = t0 + 16 * (wave * kKB + kb) + 4 * g;
+            if (row_ok[rb] && t < t_end)
+              *reinterpret_cast<lk_f32x4 *>(p.x + (size_t(qrow[rb]) * p.hq + head[rb]) * p.x_stride + t) = x;
+          }
         }
-        if constexpr (kX) {
-          const int t = t0 + 16 * (wave * kKB + kb) + 4 * g;
-          if (row_ok[rb] && t < t_end)
-            *reinterpret_cast<lk_f32x4 *>(p.x + (size_t(qrow[rb]) * p.hq + head[rb]) * p.x_stride + t) = x;
-        }
-      }
+      };
+      if (full) logits(std::true_type{});
+      else logits(std::false_type{});
       top = fmaxf(top, __shfl_xor(top, 16, kWave));
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
       if (g == 0) sm.top[wave][16 * rb + n] = top;
@@ -399,27 +404,28 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
         m[rb] = next;
       }
       const float ref = m[rb] == -__builtin_inff() ? 0.f : m[rb];
+      auto weights = [&](auto all) {
+        constexpr bool kAll = decltype(all)::value;
 #pragma unroll
-      for (int kb = 0; kb < kKB; ++kb) {
-        float w[4];
+        for (int kb = 0; kb < kKB; ++kb) {
+          float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float pw = __builtin_amdgcn_exp2f(y[rb][kb][e] - ref);
-          if (full) {
-            l[rb] = fmaf(pw, vi[kb][e], l[rb]);
-            w[e] = pw * vm[kb][e];
-          } else {
-            const bool vis = (seen[rb] >> (4 * kb + e)) & 1u;
-            l[rb] = vis ? fmaf(pw, vi[kb][e], l[rb]) : l[rb];
+          for (int e = 0; e < 4; ++e) {
+            const float pw = __builtin_amdgcn_exp2f(y[rb][kb][e] - ref);
+            const bool vis = kAll || ((seen[rb] >> (4 * kb + e)) & 1u);
+            const float sum = fmaf(pw, vi[kb][e], l[rb]);
+            l[rb] = vis ? sum : l[rb];
             w[e] = vis ? pw * vm[kb][e] : 0.f;
           }
+          const int j = wave * kKB + kb;
+          typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+          *reinterpret_cast<u32x2 *>(sm.pt + (16 * rb + n) * kPStride + 32 * (j >> 1) + 8 * g + 4 * (j & 1)) =
+              u32x2{uint32_t(float_to_f16_bits(w[0])) | (uint32_t(float_to_f16_bits(w[1])) << 16),
+                    uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
         }
-        const int j = wave * kKB + kb;
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        *reinterpret_cast<u32x2 *>(sm.pt + (16 * rb + n) * kPStride + 32 * (j >> 1) + 8 * g + 4 * (j & 1)) =
-            u32x2{uint32_t(float_to_f16_bits(w[0])) | (uint32_t(float_to_f16_bits(w[1])) << 16),
-                  uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
-      }
+      };
+      if (full) weights(std::true_type{});
+      else weights(std::false_type{});
     }
     lds_barrier();
     // O^T += V^T P^T: slots 8 g + e of a 32-row step are rows 4 g + e of its
