@@ -185,6 +185,16 @@ __device__ __forceinline__ void row_place(const WeightParams &p, int h, int r, i
   head = h * p.group + (r - tok * p.group);
 }
 
+// The (token, head) rows, counted within the request and KV head, of the chunk's
+// query tokens that see cached row t0 or a later one.
+__device__ __forceinline__ void rows_that_see(const WeightParams &p, int t0, int len, int begin, int count, int &first,
+                                              int &end) {
+  const int lo = max(p.causal ? max(t0 - (len - count), 0) : 0, p.tok_lo - begin);
+  const int hi = max(min(count, p.tok_hi - begin), 0);
+  first = min(max(lo, 0), hi) * p.group;
+  end = hi * p.group;
+}
+
 template <int kD, bool kBf16, bool kSums, typename BtT>
 __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams p) {
   constexpr int kRow = kD + 4;
@@ -215,13 +225,13 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
   if (t0 >= len) return;  // uniform
   int begin, count;
   request_rows(p, b, begin, count);
-  // Query rows of this split and chunk that see row t0 or later.
+  // Query rows of this chunk that see row t0 or later, and this split of them.
   const int shift = p.causal ? len - count : len;     // row i sees rows up to shift + i (causal)
-  const int first_tok = p.causal ? max(t0 - shift, 0) : 0;
-  const int lo_tok = max(first_tok, p.tok_lo - begin), hi_tok = min(count, p.tok_hi - begin);
-  const int64_t lo64 = max(int64_t(split) * p.split_rows, int64_t(max(lo_tok, 0)) * p.group);
-  const int64_t hi64 = min((int64_t(split) + 1) * p.split_rows, int64_t(max(hi_tok, 0)) * p.group);
-  const int r_lo = int(min(lo64, int64_t(0x7FFFFFFF))), r_hi = int(min(hi64, int64_t(0x7FFFFFFF)));
+  int row_first, row_end;
+  rows_that_see(p, t0, len, begin, count, row_first, row_end);
+  const int r_lo = int(min(int64_t(row_first) + int64_t(split) * p.split_rows, int64_t(row_end)));
+  const int r_hi = int(min(int64_t(r_lo) + p.split_rows, int64_t(row_end)));
+  if (split > 0 && r_lo >= r_hi) return;  // uniform: nothing is read of this split
   const int stages = r_hi > r_lo ? (r_hi - r_lo + kStage - 1) / kStage : 0;
   const int key0 = t0 + 64 * wave;  // first key of this wavefront
 
@@ -244,32 +254,44 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
     const uint32_t ok_groups = uint32_t(__ballot(off_lane >= 0)) & 15u;
     typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
     lk_u32x4 raw[4][kSlices];
-    float ksc[4][4];
+    const uint8_t *base[4];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
       const int lo = __builtin_amdgcn_readlane(int(uint64_t(off_lane)), kb);
       const int hi = __builtin_amdgcn_readlane(int(uint64_t(off_lane) >> 32), kb);
       const int64_t off = int64_t((uint64_t(uint32_t(hi)) << 32) | uint32_t(lo));
-      const uint8_t *kp = p.key_cache + (off < 0 ? 0 : off);
+      base[kb] = p.key_cache + (off < 0 ? 0 : off);
 #pragma unroll
       for (int i = 0; i < kSlices; ++i)
-        raw[kb][i] = *reinterpret_cast<const u32x4_a4 *>(kp + uint32_t(n) * rec + 16u * g + 64 * i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        ksc[kb][e] = *reinterpret_cast<const float *>(kp + uint32_t(4 * g + e) * rec + kD) * p.scale_log2;
+        raw[kb][i] = *reinterpret_cast<const u32x4_a4 *>(base[kb] + uint32_t(n) * rec + 16u * g + 64 * i);
     }
-    fill_lookup<kBf16, kThreads>(sm.table, tid);
+    fill_lookup<kBf16>(sm.table, reinterpret_cast<uint32_t *>(sm.ml), tid);
     lds_barrier();
     const uint32_t lane4 = uint32_t(4 * lane);
     lk_u32x4 kf[4][kQS];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
-      __builtin_amdgcn_sched_barrier(0);  // one block's lookups at a time: registers
 #pragma unroll
-      for (int i = 0; i < kQS; ++i)
-        kf[kb][i] = look8<false>(raw[kb][i >> 1][2 * (i & 1)], raw[kb][i >> 1][2 * (i & 1) + 1], lane4, table);
+      for (int i = 0; i < kQS; i += 2) {
+        // Sixteen lookups at a time, packed here: left alone, the compiler holds
+        // the halves apart until the loop and spills them.
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = i; j < i + 2; ++j) {
+          kf[kb][j] = look8<false>(raw[kb][i >> 1][2 * (j & 1)], raw[kb][i >> 1][2 * (j & 1) + 1], lane4, table);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(kf[kb][j][w]));
+        }
+      }
     }
     lds_barrier();  // the ring takes the table's place
+    // The row scales, only now: held over the lookups they were spilled one by one.
+    float ksc[4][4];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        ksc[kb][e] = *reinterpret_cast<const float *>(base[kb] + uint32_t(4 * g + e) * rec + kD) * p.scale_log2;
 
     // Stage s: rows r_lo + 32 s .. + 31; rows past the last repeat it.  Wavefront
     // w brings half of the operands of row block w / 2.
@@ -293,8 +315,7 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
         const int r = r_lo + kStage * s + 16 * rb + n;
         int tok, head;
         row_place(p, h, min(r, r_hi - 1), tok, head);
-        const float2 v = reinterpret_cast<const float2 *>(p.stat)[size_t(begin + tok) * p.hq + head];
-        st[rb] = float2{v.x, r < r_hi ? v.y : 0.f};
+        st[rb] = reinterpret_cast<const float2 *>(p.stat)[size_t(begin + tok) * p.hq + head];
       }
     };
     fetch(0);
@@ -323,7 +344,16 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
           reinterpret_cast<float2 *>(p.part)[size_t(tile) * chunk_rows + size_t(begin + tok - p.tok_lo) * p.hq + head] = v;
         }
       }
+      // The statistics arrive here, before newer copies are in flight: a wait for
+      // them further down would wait for those too.
       float2 cur[2] = {st[0], st[1]};
+      if constexpr (kSums) {
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+          asm volatile("" : "+v"(cur[rb].x), "+v"(cur[rb].y));
+          if (r_lo + kStage * s + 16 * rb + n >= r_hi) cur[rb].y = 0.f;
+        }
+      }
       if (s + 2 < stages) fetch(s + 2);
       if constexpr (kSums) {
         if (s + 1 < stages) load_stats(s + 1);
@@ -353,11 +383,12 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
           row_place(p, h, min(r0 + n, r_hi - 1), tok, head);
           lim = min(len, shift + tok + 1);
         }
+        if (kSums && r0 + n >= r_hi) lim = 0;  // its statistics need not be a number
         // One copy of the arithmetic per case: a test per element would branch in the loop.
         auto block = [&](auto all) {
           constexpr bool kAll = decltype(all)::value;
           auto visible = [&](int kb, int e) {
-            return ((ok_groups >> kb) & 1u) && key0 + 16 * kb + 4 * g + e < lim;
+            return bool(((ok_groups >> kb) & 1u) & uint32_t(key0 + 16 * kb + 4 * g + e < lim));
           };
           if constexpr (kSums) {
 #pragma unroll
@@ -366,7 +397,7 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
               for (int e = 0; e < 4; ++e) {
                 const float w = __builtin_amdgcn_exp2f(fmaf(d[kb][e], ksc[kb][e], -cur[rb].x));
                 const float sum = fmaf(w, cur[rb].y, acc[kb][e]);
-                acc[kb][e] = kAll || (visible(kb, e) && r0 + n < r_hi) ? sum : acc[kb][e];
+                acc[kb][e] = kAll || visible(kb, e) ? sum : acc[kb][e];
               }
           } else {
             float mx = -__builtin_inff();
@@ -378,16 +409,14 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
                 d[kb][e] = kAll || visible(kb, e) ? x : -__builtin_inff();
                 mx = fmaxf(mx, d[kb][e]);
               }
-            mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+            mx = max_over_groups(mx);
             const float use = mx == -__builtin_inff() ? 0.f : mx;
             float l = 0.f;
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
               for (int e = 0; e < 4; ++e) l += __builtin_amdgcn_exp2f(d[kb][e] - use);
-            l += __shfl_xor(l, 16, kWave);
-            l += __shfl_xor(l, 32, kWave);
+            l = sum_over_groups(l);
             if (g == 0) sm.ml[s & 1][wave][16 * rb + n] = float2{mx, l};
           }
         };
@@ -470,11 +499,16 @@ __global__ __launch_bounds__(kThreads) void key_stats_join(const WeightParams p)
 // Adds the row splits' sums, in order.
 __global__ __launch_bounds__(kThreads) void key_sums_join(const WeightParams p) {
   const int t = int(blockIdx.x) * kThreads + threadIdx.x, h = int(blockIdx.y), b = int(blockIdx.z);
-  if (t >= clamp_rows(p.lens[b], p.max_len)) return;
+  const int len = clamp_rows(p.lens[b], p.max_len);
+  if (t >= len) return;
   const int64_t bh = int64_t(b) * p.hkv + h;
+  int begin, count, first, end;
+  request_rows(p, b, begin, count);
+  rows_that_see(p, t / kKeys * kKeys, len, begin, count, first, end);
+  const int splits = max(1, int((int64_t(end) - first + p.split_rows - 1) / p.split_rows));
   float v = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < p.row_splits; ++s) v += p.part_w[(int64_t(s) * p.batch * p.hkv + bh) * p.w_pad + t];
+  for (int s = 0; s < splits; ++s) v += p.part_w[(int64_t(s) * p.batch * p.hkv + bh) * p.w_pad + t];
   float *w = p.weights + bh * p.w_stride + t;
   *w = p.accumulate ? *w + v : v;
 }
@@ -489,8 +523,36 @@ struct WeightPlan {
 
 constexpr int64_t kPartBytes = int64_t(64) << 20;
 
+// Query rows of a workgroup.  512 workgroups run at a time (two per CU); one
+// costs its rows and, for its keys' decode, about 128 more at D = 256, and the
+// last ones leave half a workgroup's time of idle CUs.  For one causal prompt
+// of 4096 tokens, 4 KV heads of 4 query heads each, both passes measured 327 us
+// with 128 rows, 244 with 256, 237 with 384, 233 with 576, 220 with 672, 223
+// with 768, 250 with 1024, 272 with 1152 (one workgroup per slot, unevenly over
+// the XCDs).
+int64_t best_split(int64_t items, int64_t tiles, int64_t d, int64_t group, int64_t max_query, int64_t max_len, bool causal) {
+  const int64_t rows = max_query * group, step = std::max<int64_t>(1, tiles / 128);
+  int64_t best = 0, best_cost = 0;
+  for (int64_t split = 128;; split += std::max<int64_t>(32, split / 16 / 32 * 32)) {
+    split = std::min<int64_t>(split, (rows + kStage - 1) / kStage * kStage);
+    int64_t groups = 0;
+    for (int64_t j = 0; j < tiles; j += step) {  // a sample of the tiles where there are many
+      const int64_t first = causal ? std::max<int64_t>(0, j * kKeys - (max_len - max_query)) * group : 0;
+      groups += std::max<int64_t>(1, (rows - std::min(first, rows) + split - 1) / split) * std::min(step, tiles - j);
+    }
+    const int64_t count = items * groups;
+    const int64_t cost = std::max<int64_t>(512, count + 256) * (split + 32 + 3 * d / 8);
+    if (!best || cost < best_cost) {
+      best = split;
+      best_cost = cost;
+    }
+    if (split >= rows || split >= 8192) break;
+  }
+  return best;
+}
+
 WeightPlan plan_weights(int64_t batch, int64_t heads, int64_t hkv, int64_t d, int64_t block_size, int64_t total_q,
-                        int64_t max_query, int64_t max_len) {
+                        int64_t max_query, int64_t max_len, bool causal) {
   WeightPlan pl{};
   const int64_t group = heads / hkv;
   pl.mfma = (d == 64 || d == 128 || d == 256) && block_size % 16 == 0 && block_size / 16 < (int64_t(1) << 20) &&
@@ -498,11 +560,7 @@ WeightPlan plan_weights(int64_t batch, int64_t heads, int64_t hkv, int64_t d, in
   if (!pl.mfma) return pl;
   pl.tiles = int((max_len + kKeys - 1) / kKeys);
   const int64_t rows = max_query * group;
-  const int64_t items = batch * hkv * pl.tiles;
-  // Row splits of at least 512 rows (a workgroup's keys cost about as much to decode as
-  // 64 rows to pass) until there are about 1024 workgroups.
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>((1024 + items - 1) / items, rows / 512));
-  pl.split_rows = int(((rows + splits - 1) / splits + kStage - 1) / kStage * kStage);
+  pl.split_rows = int(best_split(batch * hkv, pl.tiles, d, group, max_query, max_len, causal));
   pl.row_splits = int((rows + pl.split_rows - 1) / pl.split_rows);
   pl.chunk_tokens = std::min<int64_t>(total_q, std::max<int64_t>(64, kPartBytes / (int64_t(pl.tiles) * heads * 8)));
   return pl;
@@ -564,13 +622,13 @@ using namespace hif8;
 
 extern "C" size_t hif8_key_weights_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
                                                   int64_t head_size, int64_t block_size, int64_t total_query_tokens,
-                                                  int64_t max_query_len, int64_t max_seq_len) {
+                                                  int64_t max_query_len, int64_t max_seq_len, int causal) {
   if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || block_size <= 0 ||
       total_query_tokens < 0 || max_query_len < 0 || max_seq_len <= 0 || num_heads % num_kv_heads)
     return 0;
   // Either kernel: the query's alignment, which also decides, is not known here.
   const WeightPlan pl = plan_weights(batch, num_heads, num_kv_heads, head_size, block_size, total_query_tokens,
-                                     std::max<int64_t>(max_query_len, 1), max_seq_len);
+                                     std::max<int64_t>(max_query_len, 1), max_seq_len, causal != 0);
   const WeightSpace w = weight_space(pl, batch, num_heads, num_kv_heads, total_query_tokens, max_seq_len);
   return w.stat + w.part + w.part_w;
 }
@@ -614,7 +672,7 @@ extern "C" int hif8_key_weights(const void *query, int q_dtype, const uint8_t *k
   if (!aligned(key_weights, 4))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: key_weights must be 4-byte aligned", kName);
   const size_t need = hif8_key_weights_workspace_size(batch, num_heads, num_kv_heads, head_size, block_size,
-                                                      total_query_tokens, max_query_len, max_seq_len);
+                                                      total_query_tokens, max_query_len, max_seq_len, causal);
   if (need && (!workspace || workspace_bytes < need))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes required (got %zu)", kName, need,
                 workspace_bytes);
@@ -648,7 +706,7 @@ extern "C" int hif8_key_weights(const void *query, int q_dtype, const uint8_t *k
   p.accumulate = accumulate ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
   WeightPlan pl = plan_weights(batch, num_heads, num_kv_heads, head_size, block_size, total_query_tokens,
-                               std::max<int64_t>(max_query_len, 1), max_seq_len);
+                               std::max<int64_t>(max_query_len, 1), max_seq_len, causal != 0);
   if (pl.mfma) {
     const WeightSpace w = weight_space(pl, batch, num_heads, num_kv_heads, total_query_tokens, max_seq_len);
     p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + w.stat);

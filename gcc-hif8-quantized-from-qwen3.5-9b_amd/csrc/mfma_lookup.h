@@ -19,15 +19,19 @@ typedef _Float16 lk_f16x8 __attribute__((ext_vector_type(8)));
 typedef float lk_f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short lk_u16x2 __attribute__((ext_vector_type(2)));
 
-// Fills the table at LDS byte 0 of `table`; the caller synchronises.
-template <bool kBf16Low, int kThreads>
-__device__ __forceinline__ void fill_lookup(uint32_t *table, int tid) {
-#pragma unroll 4
-  for (int c = tid; c < kLookupBytes / 16; c += kThreads) {
-    const int code = c >> 4;
-    const uint32_t lo = kBf16Low ? kDeviceTables.decode_bf16[code] : kDeviceTables.decode_f16[code];
-    const uint32_t v = lo | (uint32_t(kDeviceTables.decode_f16[code]) << 16);
-    reinterpret_cast<lk_u32x4 *>(table)[c] = lk_u32x4{v, v, v, v};
+// Fills the table, with 256 words of LDS for the entries before they are spread
+// (each thread of 256 works one out: loading them took longer than a short
+// call's attention).  The caller synchronises afterwards.
+template <bool kBf16Low>
+__device__ __forceinline__ void fill_lookup(uint32_t *table, uint32_t *entries, int tid) {
+  const uint32_t f = decode_bits(uint32_t(tid));
+  const uint32_t h = float_to_f16_bits(__uint_as_float(f));  // exact
+  entries[tid] = (kBf16Low ? f >> 16 : h) | (h << 16);
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t v = entries[(tid >> 4) + 16 * i];
+    reinterpret_cast<lk_u32x4 *>(table)[tid + 256 * i] = lk_u32x4{v, v, v, v};
   }
 }
 
@@ -70,6 +74,24 @@ __device__ __forceinline__ lk_f32x4 mfma_16x16x32(lk_u32x4 a, lk_u32x4 b, lk_f32
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(lk_f16x8, a), __builtin_bit_cast(lk_f16x8, b), c,
                                                   0, 0, 0);
+}
+
+// The other lanes' values of the same column (lane % 16): the row swaps of gfx950
+// leave x of lanes 16 (or 32) apart side by side, without a trip through LDS.
+__device__ __forceinline__ float max_over_groups(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ float sum_over_groups(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 // True when some byte of w is an infinity (0x6F, 0xEF) or NaN (0x80); may also

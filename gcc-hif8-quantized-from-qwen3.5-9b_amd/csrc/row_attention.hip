@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
   constexpr int kPStride = kT + 8;        // fp16 values of a row of P in LDS
   struct Smem {
     uint32_t table[kLookupBytes / 4];     // at LDS byte 0: a lookup's address needs no addition
-    uint16_t pt[kRows * kPStride];
+    __attribute__((aligned(16))) uint16_t pt[kRows * kPStride];
     float top[4][kRows];
   };
   __shared__ __attribute__((aligned(16))) Smem sm;
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
     for (int i = 0; i < kQS; ++i)  // step 2 i + s: dims 64 i + 16 g + 8 s + [0, 8)
       qf[rb][i] = row_ok[rb] ? *reinterpret_cast<const lk_u32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1)) : lk_u32x4{0, 0, 0, 0};
   }
-  fill_lookup<kBf16, kThreads>(sm.table, tid);
+  fill_lookup<kBf16>(sm.table, reinterpret_cast<uint32_t *>(sm.pt), tid);
   lk_f32x4 oacc[kRB][4];
   float m[kRB], l[kRB];
 #pragma unroll
@@ -383,8 +383,7 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
       };
       if (full) logits(std::true_type{});
       else logits(std::false_type{});
-      top = fmaxf(top, __shfl_xor(top, 16, kWave));
-      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      top = max_over_groups(top);
       if (g == 0) sm.top[wave][16 * rb + n] = top;
     }
     lds_barrier();
@@ -508,8 +507,7 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
   lds_barrier();
 #pragma unroll
   for (int rb = 0; rb < kRB; ++rb) {
-    float lt = l[rb] + __shfl_xor(l[rb], 16, kWave);
-    lt += __shfl_xor(lt, 32, kWave);
+    const float lt = sum_over_groups(l[rb]);
     if (g == 0) sm.top[wave][16 * rb + n] = lt;
   }
   lk_f32x4 *spill = reinterpret_cast<lk_f32x4 *>(sm.table);

@@ -1428,7 +1428,7 @@ void Hif8KeyWeights(const at::Tensor &query, const at::Tensor &key_cache, const 
   if (batch == 0) return;
   const c10::OptionalDeviceGuard guard(query.device());
   const size_t bytes = hif8_key_weights_workspace_size(batch, query.size(1), o.kv_heads, o.d, o.block_size,
-                                                       query.size(0), max_query_len, max_seq_len);
+                                                       query.size(0), max_query_len, max_seq_len, causal ? 1 : 0);
   const auto ws = Workspace(bytes, query);
   CheckStatus(hif8_key_weights(query.data_ptr(), DtypeCode(query.scalar_type()), key_cache.data_ptr<uint8_t>(),
                                o.num_blocks, o.block_size, o.kv_heads, o.d, block_table.data_ptr(), o.bt_code,

@@ -447,7 +447,8 @@ int hif8_paged_decode_attention_weights(const void *query, int q_dtype, const ui
  * query rows adds (or stores) zeros.
  */
 size_t hif8_key_weights_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
-                                       int64_t block_size, int64_t total_query_tokens, int64_t max_query_len, int64_t max_seq_len);
+                                       int64_t block_size, int64_t total_query_tokens, int64_t max_query_len,
+                                       int64_t max_seq_len, int causal);
 int hif8_key_weights(const void *query, int q_dtype, const uint8_t *key_cache, int64_t num_blocks, int64_t block_size,
                      int64_t num_kv_heads, int64_t head_size, const void *block_table, int block_table_dtype,
                      int64_t max_blocks_per_seq, const int32_t *query_start_loc, const int32_t *seq_lens,

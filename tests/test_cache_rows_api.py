@@ -19,7 +19,7 @@ def lib():
     lib.hif8_last_error.restype = ctypes.c_char_p
     for name, n in (("hif8_tree_attention_workspace_size", 9), ("hif8_paged_decode_attention_weights_workspace_size", 7),
                     ("hif8_key_weights_workspace_size", 8), ("hif8_kv_evict_workspace_size", 3)):
-        getattr(lib, name).argtypes = [ctypes.c_int64] * n
+        getattr(lib, name).argtypes = [ctypes.c_int64] * n + [ctypes.c_int] * (name == "hif8_key_weights_workspace_size")
         getattr(lib, name).restype = ctypes.c_size_t
     return lib
 
@@ -191,7 +191,7 @@ def test_workspace_sizes(lib):
     assert lib.hif8_tree_attention_workspace_size(1, 16, 4, 256, 256, 128, 8, 8, 512) > 0
     # The logits of every head and cached row are kept between the two launches.
     assert lib.hif8_paged_decode_attention_weights_workspace_size(2, 16, 4, 256, 256, 128, 1000) >= 2 * 16 * 1000 * 4
-    assert lib.hif8_key_weights_workspace_size(1, 16, 4, 256, 128, 32, 32, 4096) >= 32 * 16 * 8
+    assert lib.hif8_key_weights_workspace_size(1, 16, 4, 256, 128, 32, 32, 4096, 1) >= 32 * 16 * 8
     # Two lists of at most half the rows, and a count, per KV head.
     assert lib.hif8_kv_evict_workspace_size(2, 4, 1000) == 2 * 4 * (2 * 501 + 1) * 4
 
