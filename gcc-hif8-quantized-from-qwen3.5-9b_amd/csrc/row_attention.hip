@@ -145,20 +145,11 @@ struct RowTile {
 __device__ __forceinline__ void split_scale(float s, float &e, float &mant, float &inv) {
   const uint32_t u = __float_as_uint(s);
   const int ex = int((u >> 23) & 0xFFu);
-  if (ex == 0xFF) {
-    e = 0.f;
-    mant = s;
-    inv = 1.f;
-  } else if (ex < 127 - 64) {
-    e = -64.f;
-    mant = s * 0x1p64f;
-    inv = 0x1p64f;
-  } else {
-    e = float(ex - 127);
-    mant = __uint_as_float((u & 0x807FFFFFu) | 0x3F800000u);
-    inv = __uint_as_float(uint32_t(254 - ex) << 23);
-    if (ex == 254) inv = 0x1p-127f;
-  }
+  const int at = ex == 0xFF ? 127 : max(ex, 127 - 64);  // biased exponent taken
+  e = float(at - 127);
+  inv = __uint_as_float(uint32_t(max(254 - at, 1)) << 23);  // 2^-127 for the largest: 2^-126 is as good as none
+  mant = at == ex ? __uint_as_float((u & 0x807FFFFFu) | 0x3F800000u) : s;
+  if (ex < 127 - 64) mant = s * 0x1p64f;
 }
 
 template <int kD, bool kBf16, int kRB, bool kX, typename BtT>
@@ -222,10 +213,11 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
   auto group_of = [&](int t0) { return min(t0 + 16 * (lane & (kGroups - 1)), t_end - 1) >> 4; };
   auto block_at = [&](int t0) {
     const int gr = group_of(t0);
-    return int64_t(bt[int((uint64_t(gr) * uint64_t(tile.magic)) >> 36)]);
+    return bt[int((uint64_t(gr) * uint64_t(tile.magic)) >> 36)];  // not widened here: that would wait for it
   };
   // Byte offset of the group's first row of this KV head, or -1.
-  auto offset_at = [&](int t0, int64_t blk) {
+  auto offset_at = [&](int t0, BtT entry) {
+    const int64_t blk = int64_t(entry);
     const int gr = group_of(t0);
     const int in16 = gr - int((uint64_t(gr) * uint64_t(tile.magic)) >> 36) * bs16;
     return blk >= 0 && blk < p.num_blocks && t0 + 16 * (lane & (kGroups - 1)) < t_end
@@ -277,22 +269,23 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
     }
   };
 
-  int64_t blk_next = -1;
-  if (ntiles > 0) {
-    const int64_t blk = block_at(t_begin);
-    if (ntiles > 1) blk_next = block_at(t_begin + kT);
-    off_lane = offset_at(t_begin, blk);
-    ok_groups = uint32_t(__ballot(off_lane >= 0));
-    load_k();
-    load_v();
-  }
+  // The query rows first: what is waited for last must not be issued behind the cache.
   lk_u32x4 qf[kRB][kQS];
 #pragma unroll
   for (int rb = 0; rb < kRB; ++rb) {
     const uint16_t *q = static_cast<const uint16_t *>(p.query) + (size_t(qrow[rb]) * p.hq + head[rb]) * kD + 16 * g;
 #pragma unroll
     for (int i = 0; i < kQS; ++i)  // step 2 i + s: dims 64 i + 16 g + 8 s + [0, 8)
-      qf[rb][i] = row_ok[rb] ? *reinterpret_cast<const lk_u32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1)) : lk_u32x4{0, 0, 0, 0};
+      qf[rb][i] = *reinterpret_cast<const lk_u32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1));
+  }
+  BtT blk_next = -1;
+  if (ntiles > 0) {
+    const BtT blk = block_at(t_begin);
+    blk_next = block_at(min(t_begin + kT, t_end - 1));
+    off_lane = offset_at(t_begin, blk);
+    ok_groups = uint32_t(__ballot(off_lane >= 0));
+    load_k();
+    load_v();
   }
   fill_lookup<kBf16>(sm.table, reinterpret_cast<uint32_t *>(sm.pt), tid);
   lk_f32x4 oacc[kRB][4];
@@ -305,6 +298,13 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
     for (int q = 0; q < 4; ++q) oacc[rb][q] = lk_f32x4{0.f, 0.f, 0.f, 0.f};
   }
   lds_barrier();
+  // The query rows have arrived: without this the loop would wait for them, and
+  // with them for every load behind them, in every iteration.  Columns of no
+  // row repeat the request's first row and are not written.
+#pragma unroll
+  for (int rb = 0; rb < kRB; ++rb)
+#pragma unroll
+    for (int i = 0; i < kQS; ++i) asm volatile("" : "+v"(qf[rb][i]));
 
   for (int it = 0; it < ntiles; ++it) {
     const int t0 = t_begin + it * kT;
@@ -332,14 +332,17 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
       for (int e = 0; e < 4; ++e) {
         ksc[kb][e] = ks[kb][e] * p.scale_log2;
         split_scale(vs[kb][e], ve[kb][e], vm[kb][e], vi[kb][e]);
+        // Worked out here, before the registers of ks and vs are loaded again.
+        asm volatile("" : "+v"(ksc[kb][e]), "+v"(ve[kb][e]), "+v"(vm[kb][e]), "+v"(vi[kb][e]));
       }
-    // The next tile's K, in flight from here to the next S.
-    if (it + 1 < ntiles) {
-      off_lane = offset_at(t0 + kT, blk_next);
-      ok_groups = uint32_t(__ballot(off_lane >= 0));
-      if (it + 2 < ntiles) blk_next = block_at(t0 + 2 * kT);
-      load_k();
-    }
+    // The next tile's K, in flight from here to the next S.  Past the last tile
+    // the loads go on, to the cache's first rows: loads under a condition would
+    // be copied, and so waited for, where the branches meet.
+    const BtT blk = blk_next;
+    blk_next = block_at(min(t0 + 2 * kT, t_end - 1));
+    off_lane = offset_at(t0 + kT, blk);
+    ok_groups = uint32_t(__ballot(off_lane >= 0));
+    load_k();
     // Logits (base 2), the rows each query row sees, and the tile's maxima.
     uint32_t seen[kRB];  // bit 4 kb + e: this query row sees cache row 4 g + e of block kb
     float y[kRB][kKB][4];
@@ -500,7 +503,7 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
       column(std::integral_constant<int, 2>{});
       column(std::integral_constant<int, 3>{});
     }
-    if (it + 1 < ntiles) load_v();
+    load_v();
   }
 
   // The wavefronts' shares of the softmax sum, and (D < 256) of O.
