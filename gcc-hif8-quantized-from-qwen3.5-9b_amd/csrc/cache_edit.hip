@@ -15,14 +15,27 @@ constexpr int kThreads = 256;
 
 __device__ __forceinline__ int clamp_rows(int n, int most) { return n < 0 ? 0 : (n > most ? most : n); }
 
-// First flat slot of the page of a request's row, or -1.
+// Flat slot of a request's row, or -1 where the table or the cache ends before it.
+// Rows are below 2^31, so the division is a 32-bit one (a shift for powers of two).
+struct Pages {
+  int64_t width, num_blocks;
+  int block_size, log2_block;  // log2_block -1: no power of two
+};
+
 template <typename BtT>
-__device__ __forceinline__ int64_t slot_of(const BtT *bt, int64_t row, int64_t width, int block_size,
-                                           int64_t num_blocks) {
-  const int64_t col = row / block_size;
-  if (row < 0 || col >= width) return -1;
+__device__ __forceinline__ int64_t slot_of(const BtT *bt, int64_t row, const Pages &pg) {
+  if (row < 0 || row > 0x7FFFFFFF) return -1;
+  const uint32_t r = uint32_t(row);
+  const uint32_t col = pg.log2_block >= 0 ? r >> pg.log2_block : r / uint32_t(pg.block_size);
+  if (int64_t(col) >= pg.width) return -1;
   const int64_t blk = int64_t(bt[col]);
-  return blk < 0 || blk >= num_blocks ? int64_t(-1) : blk * block_size + row % block_size;
+  return blk < 0 || blk >= pg.num_blocks ? int64_t(-1) : blk * pg.block_size + (r - col * uint32_t(pg.block_size));
+}
+
+int log2_or_none(int64_t v) {
+  int l = 0;
+  while ((int64_t(1) << l) < v) ++l;
+  return (int64_t(1) << l) == v ? l : -1;
 }
 
 // --------------------------------------------------------------- acceptance
@@ -37,8 +50,8 @@ struct AcceptParams {
   const int32_t *path;          // [batch, path_width] draft indices, rising
   const int32_t *counts;        // [batch]
   int32_t *new_lens;            // [batch]
-  int64_t bt_stride, num_blocks;
-  int block_size, path_width, caches;
+  Pages pages;
+  int path_width, caches;
 };
 
 // Row lens[b] + path[b][i] -> row lens[b] + i for i < counts[b], in every cache.
@@ -54,7 +67,7 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(const AcceptParams p) 
   if (c == 0 && blockIdx.z == 0 && threadIdx.x == 0 && p.new_lens) p.new_lens[b] = ctx + count;
   const int words = p.words[c];
   if (col >= words) return;
-  const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.bt_stride;
+  const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.pages.width;
   const int32_t *path = p.path + size_t(b) * p.path_width;
   uint32_t *cache = p.cache[c] + col;
   for (int i0 = 0; i0 < count; i0 += kAhead) {
@@ -68,9 +81,9 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(const AcceptParams p) 
       if (i < count) {
         const int a = path[i];
         const int64_t from =
-            a < 0 || a == i ? int64_t(-1) : slot_of(bt, int64_t(ctx) + a, p.bt_stride, p.block_size, p.num_blocks);
+            a < 0 || a == i ? int64_t(-1) : slot_of(bt, int64_t(ctx) + a, p.pages);
         if (from >= 0) {
-          to[j] = slot_of(bt, int64_t(ctx) + i, p.bt_stride, p.block_size, p.num_blocks);
+          to[j] = slot_of(bt, int64_t(ctx) + i, p.pages);
           w[j] = cache[from * words];
         }
       }
@@ -90,10 +103,11 @@ struct EvictParams {
   float *weights;                      // [batch, Hkv, w_stride]
   int32_t *positions;                  // [batch, Hkv, w_stride] or null
   int32_t *new_lens;                   // [batch]
-  int32_t *moves;                      // [batch * Hkv, 2, move_stride]: to, from
+  int2 *moves;                         // [batch * Hkv, move_stride]: (to, from)
   int32_t *move_counts;                // [batch * Hkv]
-  int64_t bt_stride, num_blocks, w_stride, move_stride;
-  int block_size, hkv, key_words, value_words, max_len, keep_all, sinks;
+  int64_t w_stride, move_stride;
+  Pages pages;
+  int hkv, key_words, value_words, max_len, keep_all, sinks;
 };
 
 // Larger is kept first: protected rows, then weights in falling order, NaN last.
@@ -106,112 +120,216 @@ __device__ __forceinline__ uint32_t rank_of(float w, bool safe) {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
-
-// Exclusive prefix of a flag over the workgroup, and the total.
-__device__ __forceinline__ int block_rank(bool flag, int *red, int &total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint64_t ball = __ballot(flag);
-  const int before = __popcll(ball & ((uint64_t(1) << lane) - 1));
-  __syncthreads();
-  if (lane == 0) red[wave] = __popcll(ball);
-  __syncthreads();
-  int base = 0;
-  total = 0;
-  for (int w = 0; w < kSelWaves; ++w) {
-    if (w < wave) base += red[w];
-    total += red[w];
-  }
-  return base + before;
-}
+constexpr int kBins = 2048;
 
 // One workgroup per (request, KV head): the rank of the last kept row by radix
-// selection (four 8-bit digits from the top), then in row order the dropped
-// rows before the new length and the kept rows behind it, paired one to one.
+// selection (digits of 11, 11 and 10 bits from the top), then the dropped rows
+// before the new length and the kept rows behind it, each in row order and
+// paired one to one.  Every wavefront owns a run of consecutive rows, so ranks
+// within it are ballots and only its totals cross the workgroup.  The ranks of
+// up to 64 kHeld rows per wavefront stay in registers (kHeld 0: they are read
+// again in every pass).  Bound by the latency of one read and about fifteen
+// barriers.
+template <int kHeld>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictParams p) {
-  __shared__ int hist[256];
-  __shared__ int red[kSelWaves];
-  __shared__ int pick[2];
-  const int tid = threadIdx.x;
+  __shared__ int hist[kBins];
+  __shared__ int red[kSelWaves][2];
+  __shared__ int pick[3];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bh = blockIdx.x, b = bh / p.hkv;
   const int len = clamp_rows(p.lens[b], p.max_len);
   const int keep = min(max(p.keep ? p.keep[b] : p.keep_all, 0), len);
   if (tid == 0 && bh % p.hkv == 0) p.new_lens[b] = keep;
-  if (tid == 0) p.move_counts[bh] = 0;
-  if (keep == len) return;  // uniform: nothing to drop
+  if (keep == len) {  // uniform: nothing to drop
+    if (tid == 0) p.move_counts[bh] = 0;
+    return;
+  }
   float *w = p.weights + int64_t(bh) * p.w_stride;
   int32_t *pos = p.positions ? p.positions + int64_t(bh) * p.w_stride : nullptr;
   const int from = p.protect_from ? p.protect_from[b] : 0x7FFFFFFF;
-  auto rank_at = [&](int t) {
+  const int steps = (len + kSelThreads - 1) / kSelThreads;  // 64-row steps of a wavefront
+  const int row0 = wave * steps * kWave + lane;
+  auto load = [&](int t) {
     const int at = pos ? pos[t] : t;
     return rank_of(w[t], at < p.sinks || (p.protect_from && at >= from));
   };
-  uint32_t limit = 0;  // the rank of the keep-th row, digit by digit
-  int need = keep;     // rows of the digits still open that are kept
+  uint32_t held[kHeld ? kHeld : 1];
+  if constexpr (kHeld > 0) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int t = row0 + i * kWave;
+      held[i] = i < steps && t < len ? load(t) : 0u;
+    }
+  }
+  // f(row, rank, is a row) for the wavefront's rows in order; every lane takes part.
+  auto each = [&](auto f) {
+    if constexpr (kHeld > 0) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        if (i >= steps) break;
+        f(row0 + i * kWave, held[i], row0 + i * kWave < len);
+      }
+    } else {
+      for (int i = 0; i < steps; ++i) {
+        const int t = row0 + i * kWave;
+        f(t, t < len ? load(t) : 0u, t < len);
+      }
+    }
+  };
+
+  // Rows with rank >> shift above `limit` are kept, and the first `need` of those equal to it.
+  uint32_t limit = 0xFFFFFFFFu;
+  int shift = 0, need = 0;
   if (keep > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+    need = keep;
+    limit = 0;
+    int width = 11;
+    for (shift = 21;; shift -= width) {
+      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      for (int t = tid; t < len; t += kSelThreads) {
-        const uint32_t k = rank_at(t);
-        if (shift == 24 || (k >> (shift + 8)) == (limit >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255u], 1);
+      each([&](int, uint32_t k, bool in) {
+        if (in && (shift == 21 || (k >> (shift + width)) == limit))
+          atomicAdd(&hist[(k >> shift) & ((1u << width) - 1u)], 1);
+      });
+      __syncthreads();
+      // From the top: thread i holds bins 2047 - 2 i and 2046 - 2 i.
+      const int h0 = hist[kBins - 1 - 2 * tid], h1 = hist[kBins - 2 - 2 * tid];
+      int sum = h0 + h1;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) {
+        const int up = __shfl_up(sum, o, kWave);
+        if (lane >= o) sum += up;
+      }
+      if (lane == kWave - 1) red[wave][0] = sum;
+      __syncthreads();
+      int base = 0;
+      for (int i = 0; i < wave; ++i) base += red[i][0];
+      const int before = base + sum - h0 - h1;  // rows in higher bins
+      if (before < need && need <= before + h0 + h1) {  // one thread
+        const bool first = need <= before + h0;
+        pick[0] = first ? kBins - 1 - 2 * tid : kBins - 2 - 2 * tid;
+        pick[1] = need - before - (first ? 0 : h0);
+        pick[2] = first ? h0 : h1;
       }
       __syncthreads();
-      if (tid == 0) {
-        int left = need, d = 255;
-        while (d > 0 && hist[d] < left) left -= hist[d--];
-        pick[0] = d;
-        pick[1] = left;
-      }
-      __syncthreads();
-      limit |= uint32_t(pick[0]) << shift;
+      limit = (limit << width) | uint32_t(pick[0]);
       need = pick[1];
+      if (shift == 0 || need == pick[2]) break;  // the whole bin is kept: no finer digit matters
+      if (shift == 10) width = 10;
       __syncthreads();
     }
   }
-  int32_t *to = p.moves + int64_t(bh) * 2 * p.move_stride, *src = to + p.move_stride;
-  int equal = 0, holes = 0, movers = 0;
-  for (int t0 = 0; t0 < len; t0 += kSelThreads) {
-    const int t = t0 + tid;
-    const bool in = t < len;
-    const uint32_t k = in ? rank_at(t) : 0u;
-    int total;
-    const int eq = equal + block_rank(in && k == limit, red, total);
-    equal += total;
-    const bool kept = in && keep > 0 && (k > limit || (k == limit && eq < need));
-    const int hole = holes + block_rank(in && t < keep && !kept, red, total);
-    if (in && t < keep && !kept) to[hole] = t;
-    holes += total;
-    const int mover = movers + block_rank(kept && t >= keep, red, total);
-    if (kept && t >= keep) src[mover] = t;
-    movers += total;
+  // Totals of the wavefront's rows equal to the limit, then of its dropped and moving rows.
+  int equal = 0;
+  each([&](int, uint32_t k, bool in) { equal += __popcll(__ballot(in && (k >> shift) == limit)); });
+  if (lane == 0) red[wave][0] = equal;
+  __syncthreads();
+  equal = 0;
+  for (int i = 0; i < wave; ++i) equal += red[i][0];
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  auto kept = [&](uint32_t k, bool in, int &seen) {
+    const bool same = in && (k >> shift) == limit;
+    const uint64_t ball = __ballot(same);
+    const bool yes = in && keep > 0 && ((k >> shift) > limit || (same && seen + __popcll(ball & below) < need));
+    seen += __popcll(ball);
+    return yes;
+  };
+  int seen = equal, holes = 0, movers = 0;
+  each([&](int t, uint32_t k, bool in) {
+    const bool yes = kept(k, in, seen);
+    holes += __popcll(__ballot(in && t < keep && !yes));
+    movers += __popcll(__ballot(yes && t >= keep));
+  });
+  __syncthreads();
+  if (lane == 0) {
+    red[wave][0] = holes;
+    red[wave][1] = movers;
   }
-  if (tid == 0) p.move_counts[bh] = holes;
+  __syncthreads();
+  holes = movers = 0;
+  for (int i = 0; i < wave; ++i) {
+    holes += red[i][0];
+    movers += red[i][1];
+  }
+  int count = 0;
+  for (int i = 0; i < kSelWaves; ++i) count += red[i][0];
+  int2 *moves = p.moves + int64_t(bh) * p.move_stride;
+  seen = equal;
+  each([&](int t, uint32_t k, bool in) {
+    const bool yes = kept(k, in, seen);
+    const bool hole = in && t < keep && !yes, mover = yes && t >= keep;
+    const uint64_t hb = __ballot(hole), mb = __ballot(mover);
+    if (hole) moves[holes + __popcll(hb & below)].x = t;
+    if (mover) moves[movers + __popcll(mb & below)].y = t;
+    holes += __popcll(hb);
+    movers += __popcll(mb);
+  });
+  if (tid == 0) p.move_counts[bh] = count;
   __threadfence_block();
   __syncthreads();
-  for (int i = tid; i < holes; i += kSelThreads) {
-    w[to[i]] = w[src[i]];
-    if (pos) pos[to[i]] = pos[src[i]];
+  for (int i = tid; i < count; i += kSelThreads) {
+    const int2 m = moves[i];
+    w[m.x] = w[m.y];
+    if (pos) pos[m.x] = pos[m.y];
   }
   __syncthreads();
   for (int t = keep + tid; t < len; t += kSelThreads) w[t] = 0.f;
 }
 
-// Copies the paired rows, a wavefront per row (K, then V).
+// Copies the paired rows, 16 bytes per thread: consecutive threads take the
+// pieces of a row's K, then of its V; four pieces of other rows are loaded
+// before the first is stored.
+typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
 template <typename BtT>
 __global__ __launch_bounds__(kThreads) void evict_move_kernel(const EvictParams p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int kAhead = 4;
   const int bh = blockIdx.y, b = bh / p.hkv, h = bh % p.hkv;
   const int count = p.move_counts[bh];
-  const int32_t *to = p.moves + int64_t(bh) * 2 * p.move_stride, *src = to + p.move_stride;
-  const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.bt_stride;
-  for (int i = int(blockIdx.x) * (kThreads / kWave) + wave; i < count; i += int(gridDim.x) * (kThreads / kWave)) {
-    const int64_t d = slot_of(bt, to[i], p.bt_stride, p.block_size, p.num_blocks);
-    const int64_t s = slot_of(bt, src[i], p.bt_stride, p.block_size, p.num_blocks);
-    if (d < 0 || s < 0) continue;
-    const uint32_t *ks = p.key_cache + (s * p.hkv + h) * p.key_words, *vs = p.value_cache + (s * p.hkv + h) * p.value_words;
-    uint32_t *kd = p.key_cache + (d * p.hkv + h) * p.key_words, *vd = p.value_cache + (d * p.hkv + h) * p.value_words;
-    for (int j = lane; j < p.key_words; j += kWave) kd[j] = ks[j];
-    for (int j = lane; j < p.value_words; j += kWave) vd[j] = vs[j];
+  const int2 *moves = p.moves + int64_t(bh) * p.move_stride;
+  const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.pages.width;
+  const uint32_t kc = uint32_t(p.key_words + 3) / 4, per_row = kc + uint32_t(p.value_words + 3) / 4;
+  const uint64_t pieces = uint64_t(count) * per_row, stride = uint64_t(gridDim.x) * kThreads;
+  for (uint64_t i0 = uint64_t(blockIdx.x) * kThreads + threadIdx.x; i0 < pieces; i0 += kAhead * stride) {
+    u32x4_a4 v[kAhead];
+    uint32_t *to[kAhead];
+    int words[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const uint64_t i = i0 + j * stride;
+      words[j] = 0;
+      if (i >= pieces) continue;
+      const uint32_t row = uint32_t(i / per_row);
+      uint32_t c = uint32_t(i - uint64_t(row) * per_row);
+      const int2 m = moves[row];
+      const int64_t d = slot_of(bt, m.x, p.pages), s = slot_of(bt, m.y, p.pages);
+      if (d < 0 || s < 0) continue;
+      const bool is_v = c >= kc;
+      if (is_v) c -= kc;
+      const int width = is_v ? p.value_words : p.key_words;
+      uint32_t *cache = is_v ? p.value_cache : p.key_cache;
+      const uint32_t *src = cache + (s * p.hkv + h) * width + 4 * c;
+      to[j] = cache + (d * p.hkv + h) * width + 4 * c;
+      words[j] = min(4, width - int(4 * c));
+      if (words[j] == 4) {
+        v[j] = *reinterpret_cast<const u32x4_a4 *>(src);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < words[j]) v[j][e] = src[e];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (words[j] == 4) {
+        *reinterpret_cast<u32x4_a4 *>(to[j]) = v[j];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < words[j]) to[j][e] = v[j][e];
+      }
+    }
   }
 }
 
@@ -259,9 +377,7 @@ extern "C" int hif8_accept_drafts(void *const *caches, const int64_t *row_bytes,
     p.path = accepted;
     p.counts = accepted_counts;
     p.new_lens = c0 == 0 ? new_lens : nullptr;
-    p.bt_stride = max_blocks_per_seq;
-    p.num_blocks = num_blocks;
-    p.block_size = int(block_size);
+    p.pages = Pages{max_blocks_per_seq, num_blocks, int(block_size), log2_or_none(block_size)};
     p.path_width = int(accepted_width);
     const dim3 grid(unsigned(batch), unsigned(p.caches), unsigned((widest + kThreads - 1) / kThreads));
     if (block_table_dtype == HIF8_INDEX_INT64) accept_kernel<int64_t><<<grid, kThreads, 0, s>>>(p);
@@ -272,6 +388,7 @@ extern "C" int hif8_accept_drafts(void *const *caches, const int64_t *row_bytes,
 
 extern "C" size_t hif8_kv_evict_workspace_size(int64_t batch, int64_t num_kv_heads, int64_t max_seq_len) {
   if (batch <= 0 || num_kv_heads <= 0 || max_seq_len <= 0) return 0;
+  // The lists of pairs, then a count per (request, KV head).
   return size_t(batch) * num_kv_heads * (2 * evict_list_stride(max_seq_len) + 1) * sizeof(int32_t);
 }
 
@@ -322,13 +439,11 @@ extern "C" int hif8_kv_evict(uint8_t *key_cache, uint8_t *value_cache, int64_t n
   p.weights = key_weights;
   p.positions = positions;
   p.new_lens = new_lens;
-  p.move_counts = static_cast<int32_t *>(workspace);
-  p.moves = p.move_counts + batch * num_kv_heads;
-  p.bt_stride = max_blocks_per_seq;
-  p.num_blocks = num_blocks;
+  p.moves = static_cast<int2 *>(workspace);
+  p.move_counts = reinterpret_cast<int32_t *>(p.moves + size_t(batch) * num_kv_heads * lists);
+  p.pages = Pages{max_blocks_per_seq, num_blocks, int(block_size), log2_or_none(block_size)};
   p.w_stride = weights_stride;
   p.move_stride = int64_t(lists);
-  p.block_size = int(block_size);
   p.hkv = int(num_kv_heads);
   p.key_words = int((head_size + 4) / 4);
   p.value_words = int((head_size_v + 4) / 4);
@@ -337,8 +452,12 @@ extern "C" int hif8_kv_evict(uint8_t *key_cache, uint8_t *value_cache, int64_t n
   p.sinks = int(std::min<int64_t>(sinks, 0x7FFFFFFF));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const unsigned bh = unsigned(batch * num_kv_heads);
-  evict_select_kernel<<<bh, kSelThreads, 0, s>>>(p);
-  const unsigned movers = unsigned(std::min<size_t>((lists + 3) / 4, std::max<size_t>(1, 2048 / bh)));
+  if (max_seq_len <= 4 * kSelThreads) evict_select_kernel<4><<<bh, kSelThreads, 0, s>>>(p);
+  else if (max_seq_len <= 32 * kSelThreads) evict_select_kernel<32><<<bh, kSelThreads, 0, s>>>(p);
+  else evict_select_kernel<0><<<bh, kSelThreads, 0, s>>>(p);
+  // Four pieces per thread where there are rows for it, up to about eight workgroups per CU.
+  const int64_t most = int64_t(lists) * ((p.key_words + 3) / 4 + (p.value_words + 3) / 4);
+  const unsigned movers = unsigned(std::min<int64_t>((most + 4 * kThreads - 1) / (4 * kThreads), std::max<int64_t>(1, 2048 / bh)));
   if (block_table_dtype == HIF8_INDEX_INT64) evict_move_kernel<int64_t><<<dim3(movers, bh), kThreads, 0, s>>>(p);
   else evict_move_kernel<int32_t><<<dim3(movers, bh), kThreads, 0, s>>>(p);
   return check_launch(kName);

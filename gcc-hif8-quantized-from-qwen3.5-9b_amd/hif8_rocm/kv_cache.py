@@ -359,10 +359,17 @@ def paged_attention(
         int(max_seq_len), bool(causal))
 
 
+def _as_int32(t: torch.Tensor, device) -> torch.Tensor:
+    """``t`` as a contiguous int32 tensor on ``device``; itself where it is one (the usual call: no copy, few checks)."""
+    if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
+        return t
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
 def _device_lengths(lens, name: str, device) -> tuple[torch.Tensor, list[int] | None]:
     """Request lengths as an int32 device tensor, and as host integers where they came so."""
     if isinstance(lens, torch.Tensor):
-        return lens.to(device=device, dtype=torch.int32).contiguous(), None
+        return _as_int32(lens, device), None
     host = [int(v) for v in lens]
     if any(v < 0 for v in host):
         raise ValueError(f"{name} must be non-negative")
@@ -372,6 +379,9 @@ def _device_lengths(lens, name: str, device) -> tuple[torch.Tensor, list[int] | 
 def _device_table(block_table: torch.Tensor, batch: int, device) -> torch.Tensor:
     if block_table.ndim != 2 or block_table.shape[0] < batch:
         raise ValueError("block_table must have shape [batch, max_blocks]")
+    if block_table.shape[0] == batch and block_table.device == device and block_table.is_contiguous() and \
+            block_table.dtype in (torch.int32, torch.int64):
+        return block_table
     table = block_table[:batch]
     if table.dtype not in (torch.int32, torch.int64):
         table = table.to(torch.int64)
@@ -395,8 +405,8 @@ def _request_rows(query, query_lens, query_start_loc, max_query_len, validate: b
         return loc, len(host), int(max_query_len), host
     if query_start_loc.ndim != 1 or query_start_loc.numel() < 1:
         raise ValueError("query_start_loc must have shape [batch + 1]")
-    loc = query_start_loc.to(device=query.device, dtype=torch.int32).contiguous()
-    batch = loc.numel() - 1
+    loc = _as_int32(query_start_loc, query.device)
+    batch = loc.shape[0] - 1
     if max_query_len is None or (validate and batch):
         longest = int((loc[1:] - loc[:-1]).max().item()) if batch else 0
         if max_query_len is None:
@@ -474,7 +484,9 @@ def tree_attention(
         _check_pages(total, table, max_seq_len, key_cache.shape[1], key_cache.shape[0])
     extension = native.load_extension()
     return native._operator("hif8_tree_attention", extension)(
-        query.contiguous(), key_cache, value_cache, table, loc, lens, tree_mask.to(query.device).contiguous(),
+        query.contiguous(), key_cache, value_cache, table, loc, lens,
+        tree_mask if tree_mask.device == query.device and tree_mask.is_contiguous() else
+        tree_mask.to(query.device).contiguous(),
         float(scale), max_query_len, int(max_seq_len))
 
 
@@ -505,10 +517,11 @@ def accept_drafts(
     values = [value_caches] if isinstance(value_caches, torch.Tensor) else list(value_caches)
     if not keys or len(keys) != len(values):
         raise ValueError("accept_drafts needs a value cache for every key cache")
-    for k, v in zip(keys, values):
-        _check_caches(k, v)
-        if k.shape[:2] != keys[0].shape[:2]:
-            raise ValueError("all caches must have the same blocks")
+    if validate:  # the operator checks each cache in any case
+        for k, v in zip(keys, values):
+            _check_caches(k, v)
+            if k.shape[:2] != keys[0].shape[:2]:
+                raise ValueError("all caches must have the same blocks")
     device = keys[0].device
     if accepted.ndim != 2:
         raise ValueError("accepted must have shape [batch, width]")
@@ -521,7 +534,7 @@ def accept_drafts(
         raise ValueError("one context length is required per request")
     if counts.ndim != 1 or counts.numel() < batch:
         raise ValueError("one accepted count is required per request")
-    path = accepted.to(device=device, dtype=torch.int32).contiguous()
+    path = _as_int32(accepted, device)
     table = _device_table(block_table, batch, device)
     if validate and batch:
         live = torch.arange(width, device=device) < counts[:batch, None]
@@ -584,7 +597,8 @@ def _weighted_request(key_cache, block_table, seq_lens, key_weights, batch: int,
     lens, host = _device_lengths(seq_lens, "sequence lengths", key_cache.device)
     if lens.ndim != 1 or (lens.numel() < batch if host is None else lens.numel() != batch):
         raise ValueError("one sequence length is required per request")
-    lens = lens[:batch]
+    if lens.shape[0] != batch:
+        lens = lens[:batch]
     if max_seq_len is None:
         max_seq_len = (max(host, default=0) if host is not None else int(lens.max().item())) if batch else 0
     if max_seq_len > block_table.shape[1] * key_cache.shape[1]:
@@ -691,7 +705,7 @@ def evict_kv_rows(
     if keep_all < 0 or (validate and keep_each is not None and bool((keep_each < 0).any())):
         raise ValueError("keep must not be negative")
     if protect_from is not None:
-        protect_from = torch.as_tensor(protect_from).to(device=key_cache.device, dtype=torch.int32).contiguous()
+        protect_from = _as_int32(torch.as_tensor(protect_from), key_cache.device)
         if protect_from.ndim != 1 or protect_from.numel() < batch:
             raise ValueError("one protect_from position is required per request")
     extension = native.load_extension()
