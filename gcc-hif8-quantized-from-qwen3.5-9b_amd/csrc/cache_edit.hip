@@ -156,11 +156,21 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictPa
   };
   uint32_t held[kHeld ? kHeld : 1];
   if constexpr (kHeld > 0) {
+    // Every load is issued before the first is used; rows past the end repeat the last.
+    float wv[kHeld];
+    int at[kHeld];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int t = row0 + i * kWave;
-      held[i] = i < steps && t < len ? load(t) : 0u;
+    for (int i = 0; i < kHeld; ++i) wv[i] = w[min(row0 + i * kWave, len - 1)];
+    if (pos) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) at[i] = pos[min(row0 + i * kWave, len - 1)];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) at[i] = row0 + i * kWave;
     }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      held[i] = rank_of(wv[i], (at[i] < p.sinks) | (p.protect_from && at[i] >= from));
   }
   // f(row, rank, is a row) for the wavefront's rows in order; every lane takes part.
   auto each = [&](auto f) {
@@ -453,6 +463,7 @@ extern "C" int hif8_kv_evict(uint8_t *key_cache, uint8_t *value_cache, int64_t n
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const unsigned bh = unsigned(batch * num_kv_heads);
   if (max_seq_len <= 4 * kSelThreads) evict_select_kernel<4><<<bh, kSelThreads, 0, s>>>(p);
+  else if (max_seq_len <= 16 * kSelThreads) evict_select_kernel<16><<<bh, kSelThreads, 0, s>>>(p);
   else if (max_seq_len <= 32 * kSelThreads) evict_select_kernel<32><<<bh, kSelThreads, 0, s>>>(p);
   else evict_select_kernel<0><<<bh, kSelThreads, 0, s>>>(p);
   // Four pieces per thread where there are rows for it, up to about eight workgroups per CU.

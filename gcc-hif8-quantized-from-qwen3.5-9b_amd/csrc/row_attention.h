@@ -20,12 +20,18 @@ struct RowAttnParams {
   const int32_t *lens;         // [batch]
   const uint8_t *mask;         // [total_q, mask_stride] or null
   void *out;                   // [total_q, Hq, Dv]
-  float *part_o;               // [total_q * Hq, num_splits, Dv]
-  float *part_ml;              // [total_q * Hq, num_splits, 2]
+  // Partial outputs and (maximum, sum): any-shape kernel [total_q * Hq, num_splits],
+  // matrix cores [workers + batch, Hkv, rows_cap].
+  float *part_o;
+  float *part_ml;
+  int64_t *plan;               // matrix cores: [batch + 1] tiles before each request
   float *x;                    // [total_q * Hq, x_stride] base-2 logits, or null
   float *weights;              // [batch, Hkv, w_stride], or null
   int64_t bt_stride, num_blocks, mask_stride, x_stride, w_stride;
   int block_size, hkv, hq, group, d, dv, batch, total_q, max_len, num_splits, split_tokens, accumulate;
+  // Matrix cores: workers that share the tiles, row tiles of the longest request,
+  // query rows of all of them (a KV head's), cache rows of a tile.
+  int workers, row_tiles, rows_cap, tile_rows;
   float scale_log2;            // softmax scale * log2(e)
 };
 

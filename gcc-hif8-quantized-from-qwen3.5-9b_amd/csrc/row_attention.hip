@@ -22,7 +22,8 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kMaxSplits = 256;
+constexpr int kMaxSplits = 256;  // any-shape kernel
+constexpr int kMaxParts = 512;   // parts of a query row: splits, or workers
 
 // Any head size up to 512, group, block size and alignment: a workgroup per
 // (query row, head, split), its wavefronts taking every fourth cache row with a
@@ -117,10 +118,13 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 // ---------------------------------------------------- on the matrix cores
 //
 // Head sizes 64, 128 and 256 (K and V alike), pages of a multiple of 16 rows.
-// A workgroup of four wavefronts owns (request, KV head, 16 kRB query rows,
-// split); its query rows are the (draft, head) pairs of the KV head, so every
-// cached code is decoded once for all of them.  It walks its split in tiles of
-// kT = 16384 / D cache rows, with two barriers per tile:
+// A workgroup of four wavefronts is a worker for (KV head, 16 kRB query rows);
+// its query rows are the (draft, head) pairs of the KV head, so every
+// cached code is decoded once for all of them.  The tiles of kT = 16384 / D
+// cache rows of all requests, one after the other, are dealt out to the
+// workers in equal runs, so ragged lengths leave none idle; a run that reaches
+// into another request goes on with that one's query rows.  Per tile, with two
+// barriers:
 //   * S^T = K Q^T: every wavefront takes a quarter of the tile's rows, loaded
 //     from HBM straight into the MFMA A operand (row = lane % 16, 16 codes per
 //     lane) and decoded in registers; Q is the B operand, held all along;
@@ -133,11 +137,23 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 // sum_t P_t 2^-e_t is the softmax sum against the same maximum.
 constexpr float kLazy = 6.f;  // log2 headroom of the maximum: it moves in steps of more than 2^6
 
-struct RowTile {
-  int64_t magic;       // ceil(2^36 / (block_size / 16))
-  int rows_per_wg;     // 16 * kRB
-  int row_tiles;       // of the longest request
-};
+// Tiles of request b.
+__device__ __forceinline__ int64_t tiles_of(const RowAttnParams &p, int b) {
+  int begin, count;
+  request_rows(p, b, begin, count);
+  return (int64_t(rows_seen(p, clamp_rows(p.lens[b], p.max_len), count)) + p.tile_rows - 1) / p.tile_rows;
+}
+
+// Inclusive sum over the lanes of a wavefront.
+__device__ __forceinline__ int64_t wave_prefix(int64_t v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int64_t up = int64_t(__shfl_up(static_cast<long long>(v), o, kWave));
+    if (lane >= o) v += up;
+  }
+  return v;
+}
 
 // Exponent, signed mantissa and 2^-exponent of a V row's scale.  Scales below
 // 2^-64 keep 2^-64 as exponent (and a mantissa below one); NaN and infinity
@@ -154,7 +170,7 @@ __device__ __forceinline__ void split_scale(float s, float &e, float &mant, floa
 
 template <int kD, bool kBf16, int kRB, bool kX, typename BtT>
 __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(const RowAttnParams p,
-                                                                               const RowTile tile) {
+                                                                               const int64_t page_magic) {
   constexpr int kRow = kD + 4;
   constexpr int kT = 16384 / kD;          // cache rows of a tile
   constexpr int kKB = kT / 64;            // 16-row blocks of a wavefront in S
@@ -165,7 +181,8 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
   constexpr int kPStride = kT + 8;        // fp16 values of a row of P in LDS
   struct Smem {
     uint32_t table[kLookupBytes / 4];     // at LDS byte 0: a lookup's address needs no addition
-    __attribute__((aligned(16))) uint16_t pt[kRows * kPStride];
+    // P of a tile; at a segment's end the wavefronts' shares of O (D < 256).
+    __attribute__((aligned(16))) uint16_t pt[kSlices < 4 && kRows * kPStride < 6144 ? 6144 : kRows * kPStride];
     float top[4][kRows];
   };
   __shared__ __attribute__((aligned(16))) Smem sm;
@@ -175,23 +192,79 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   const uint32_t lane4 = uint32_t(4 * lane);
-  // The KV heads and row tiles of one (request, split) read the same cache
-  // lines: their blocks are equal modulo 8, on one XCD.
-  const int inner = p.hkv * tile.row_tiles;
+  // The KV heads and row tiles of one worker read the same cache lines: their
+  // blocks are equal modulo 8, on one XCD.
+  const int inner = p.hkv * p.row_tiles;
   const int xcd = int(blockIdx.x) & 7, slot = int(blockIdx.x) >> 3;
-  const int outer = (slot / inner) * 8 + xcd;
-  if (outer >= p.batch * p.num_splits) return;  // padding block (uniform)
-  const int rt = (slot % inner) % tile.row_tiles, h = (slot % inner) / tile.row_tiles;
-  const int b = outer / p.num_splits, split = outer % p.num_splits;
+  const int worker = (slot / inner) * 8 + xcd;
+  if (worker >= p.workers) return;  // padding block (uniform)
+  const int rt = (slot % inner) % p.row_tiles, h = (slot % inner) / p.row_tiles;
+  // This worker's run of the requests' tiles, and the running total per request
+  // (kept for the join by the first workgroup).  incl: of the first 64 requests.
+  int64_t total = 0, incl = 0;
+  for (int base = 0; base < p.batch; base += kWave) {
+    const int i = base + lane;
+    const int64_t mine = i < p.batch ? tiles_of(p, i) : 0;
+    const int64_t upto = wave_prefix(mine);
+    if (base == 0) incl = upto;
+    if (worker == 0 && rt == 0 && h == 0 && wave == 0 && i < p.batch) p.plan[i] = total + upto - mine;
+    total += int64_t(__shfl(static_cast<long long>(upto), kWave - 1, kWave));
+  }
+  if (worker == 0 && rt == 0 && h == 0 && tid == 0) p.plan[p.batch] = total;
+  const int64_t workers = min(int64_t(p.workers), total);  // a tile each at least: no part is left unwritten
+  if (worker >= workers) return;                           // uniform
+  int64_t cur = total * worker / workers;
+  const int64_t run_end = total * (worker + 1) / workers;
+  fill_lookup<kBf16>(sm.table, reinterpret_cast<uint32_t *>(sm.pt), tid);
+
+  const uint32_t rec = uint32_t(p.hkv) * kRow;
+  const int bs16 = p.block_size >> 4;
+  const int vslice = wave % kSlices, vgroup = wave / kSlices;
+  const uint32_t k_off = uint32_t(n) * rec + 16u * g;              // K: row n, codes 16 g + 64 i
+  uint32_t v_off[4], s_off[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v_off[e] = uint32_t(4 * g + e) * rec + uint32_t(64 * vslice + 4 * n);  // V: row 4 g + e, four dims
+    s_off[e] = uint32_t(4 * g + e) * rec + uint32_t(kD);                   // scale of row 4 g + e
+  }
+
+  while (cur < run_end) {
+  // The request of tile `cur` (uniform), and this segment's tiles of it.
+  int b = 0;
+  int64_t first = 0;
+  if (p.batch <= kWave) {
+    b = __builtin_ctzll(__ballot(incl > cur));
+    first = b ? int64_t(__shfl(static_cast<long long>(incl), b - 1, kWave)) : 0;
+  } else {
+    int64_t before = 0;
+    for (int base = 0; base < p.batch; base += kWave) {
+      const int i = base + lane;
+      const int64_t upto = before + wave_prefix(i < p.batch ? tiles_of(p, i) : 0);
+      const uint64_t past = __ballot(upto > cur);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        b = base + at;
+        first = at ? int64_t(__shfl(static_cast<long long>(upto), at - 1, kWave)) : before;
+        break;
+      }
+      before = int64_t(__shfl(static_cast<long long>(upto), kWave - 1, kWave));
+    }
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
   int begin, count;
   request_rows(p, b, begin, count);
   const int rows = count * p.group;
   const int ctx = clamp_rows(p.lens[b], p.max_len);
   const int len = rows_seen(p, ctx, count);
-  const int t_begin = split * p.split_tokens, t_end = min(t_begin + p.split_tokens, len);
-  if (rt * kRows >= rows) return;  // uniform
-  if (t_begin >= t_end && !(split == 0 && p.num_splits == 1)) return;
-  const int ntiles = max(t_end - t_begin + kT - 1, 0) / kT;
+  const int tile_first = __builtin_amdgcn_readfirstlane(int(cur - first));
+  const int seg_tiles = __builtin_amdgcn_readfirstlane(
+      int(min(run_end - cur, int64_t((len + kT - 1) / kT) - int64_t(tile_first))));
+  cur += seg_tiles;
+  if (rt * kRows >= rows) continue;  // uniform: the request has no query rows here
+  const int t_begin = tile_first * kT, t_end = min(t_begin + seg_tiles * kT, len);
+  const int ntiles = seg_tiles;
+  const bool whole = t_begin == 0 && t_end == len;  // this segment holds all of the request's cache rows
+  const size_t part_row = (size_t(worker) + b) * p.hkv + h;
 
   // This lane's query rows (column n of every row block).
   int qrow[kRB], head[kRB];
@@ -204,22 +277,19 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
     qrow[rb] = begin + tok;
     head[rb] = h * p.group + (row_ok[rb] ? r - tok * p.group : 0);
   }
-
   const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.bt_stride;
-  const uint32_t rec = uint32_t(p.hkv) * kRow;
-  const int bs16 = p.block_size >> 4;
   // Lane i % kGroups looks up 16-row group i of a tile; the entry is loaded a
   // tile ahead of its use.
   auto group_of = [&](int t0) { return min(t0 + 16 * (lane & (kGroups - 1)), t_end - 1) >> 4; };
   auto block_at = [&](int t0) {
     const int gr = group_of(t0);
-    return bt[int((uint64_t(gr) * uint64_t(tile.magic)) >> 36)];  // not widened here: that would wait for it
+    return bt[int((uint64_t(gr) * uint64_t(page_magic)) >> 36)];  // not widened here: that would wait for it
   };
   // Byte offset of the group's first row of this KV head, or -1.
   auto offset_at = [&](int t0, BtT entry) {
     const int64_t blk = int64_t(entry);
     const int gr = group_of(t0);
-    const int in16 = gr - int((uint64_t(gr) * uint64_t(tile.magic)) >> 36) * bs16;
+    const int in16 = gr - int((uint64_t(gr) * uint64_t(page_magic)) >> 36) * bs16;
     return blk >= 0 && blk < p.num_blocks && t0 + 16 * (lane & (kGroups - 1)) < t_end
                ? (blk * p.block_size + 16 * in16) * int64_t(rec) + int64_t(h) * kRow
                : int64_t(-1);
@@ -230,14 +300,6 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
     return int64_t((uint64_t(uint32_t(hi)) << 32) | uint32_t(lo));
   };
 
-  const int vslice = wave % kSlices, vgroup = wave / kSlices;
-  const uint32_t k_off = uint32_t(n) * rec + 16u * g;              // K: row n, codes 16 g + 64 i
-  uint32_t v_off[4], s_off[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v_off[e] = uint32_t(4 * g + e) * rec + uint32_t(64 * vslice + 4 * n);  // V: row 4 g + e, four dims
-    s_off[e] = uint32_t(4 * g + e) * rec + uint32_t(kD);                   // scale of row 4 g + e
-  }
   typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
   lk_u32x4 kraw[kKB][kSlices];
   float ks[kKB][4], vs[kKB][4];
@@ -278,16 +340,12 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
     for (int i = 0; i < kQS; ++i)  // step 2 i + s: dims 64 i + 16 g + 8 s + [0, 8)
       qf[rb][i] = *reinterpret_cast<const lk_u32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1));
   }
-  BtT blk_next = -1;
-  if (ntiles > 0) {
-    const BtT blk = block_at(t_begin);
-    blk_next = block_at(min(t_begin + kT, t_end - 1));
-    off_lane = offset_at(t_begin, blk);
-    ok_groups = uint32_t(__ballot(off_lane >= 0));
-    load_k();
-    load_v();
-  }
-  fill_lookup<kBf16>(sm.table, reinterpret_cast<uint32_t *>(sm.pt), tid);
+  const BtT blk_first = block_at(t_begin);
+  BtT blk_next = block_at(min(t_begin + kT, t_end - 1));
+  off_lane = offset_at(t_begin, blk_first);
+  ok_groups = uint32_t(__ballot(off_lane >= 0));
+  load_k();
+  load_v();
   lk_f32x4 oacc[kRB][4];
   float m[kRB], l[kRB];
 #pragma unroll
@@ -304,7 +362,10 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
 #pragma unroll
   for (int rb = 0; rb < kRB; ++rb)
 #pragma unroll
-    for (int i = 0; i < kQS; ++i) asm volatile("" : "+v"(qf[rb][i]));
+    for (int i = 0; i < kQS; ++i) {
+      if constexpr (kRB > 2) asm volatile("" : "+a"(qf[rb][i]));  // 128 registers: kept out of the way
+      else asm volatile("" : "+v"(qf[rb][i]));
+    }
 
   for (int it = 0; it < ntiles; ++it) {
     const int t0 = t_begin + it * kT;
@@ -350,16 +411,31 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
     for (int rb = 0; rb < kRB; ++rb) {
       seen[rb] = 0xFFFFFFFFu;
       if (!full) {
+        // All mask bytes are loaded before one is used (clamped into the row; what is
+        // no draft does not look at its byte).
+        uint32_t byte[kKB][4];
+        if (p.mask) {  // uniform
+          const uint8_t *mrow = p.mask + size_t(qrow[rb]) * p.mask_stride;
+          const int last = int(min(p.mask_stride, int64_t(p.max_len)) - 1);
+#pragma unroll
+          for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              byte[kb][e] = mrow[min(max(t0 + 16 * (wave * kKB + kb) + 4 * g + e - ctx, 0), last)];
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) byte[kb][e] = 1;
+        }
         seen[rb] = 0;
-        const uint8_t *mrow = p.mask + (p.mask ? size_t(qrow[rb]) * p.mask_stride : 0);
 #pragma unroll
         for (int kb = 0; kb < kKB; ++kb) {
           const bool in = (ok_now >> (wave * kKB + kb)) & 1u;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int t = t0 + 16 * (wave * kKB + kb) + 4 * g + e;
-            bool vis = in && t < t_end;
-            if (vis && t >= ctx) vis = mrow[t - ctx] != 0;
+            const bool vis = in & (t < t_end) & ((t < ctx) | (byte[kb][e] != 0));
             seen[rb] |= uint32_t(vis) << (4 * kb + e);
           }
         }
@@ -513,115 +589,177 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
     const float lt = sum_over_groups(l[rb]);
     if (g == 0) sm.top[wave][16 * rb + n] = lt;
   }
-  lk_f32x4 *spill = reinterpret_cast<lk_f32x4 *>(sm.table);
   if constexpr (kSlices < 4) {
-    if (vgroup > 0) {
+    lk_f32x4 *spill = reinterpret_cast<lk_f32x4 *>(sm.pt);
 #pragma unroll
-      for (int rb = 0; rb < kRB; ++rb)
+    for (int rb = 0; rb < kRB; ++rb) {
+      if (rb > 0) lds_barrier();
+      if (vgroup > 0) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          spill[(((vgroup - 1) * kSlices + vslice) * kRB * 4 + rb * 4 + q) * kWave + lane] = oacc[rb][q];
+        for (int q = 0; q < 4; ++q) spill[(((vgroup - 1) * kSlices + vslice) * 4 + q) * kWave + lane] = oacc[rb][q];
+      }
+      lds_barrier();
+      if (vgroup == 0) {
+#pragma unroll
+        for (int og = 0; og < 4 / kSlices - 1; ++og)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) oacc[rb][q] += spill[((og * kSlices + vslice) * 4 + q) * kWave + lane];
+      }
+    }
+  } else {
+    lds_barrier();
+  }
+  if (vgroup == 0) {
+#pragma unroll
+    for (int rb = 0; rb < kRB; ++rb) {
+      if (!row_ok[rb]) continue;
+      const float sum = sm.top[0][16 * rb + n] + sm.top[1][16 * rb + n] + sm.top[2][16 * rb + n] + sm.top[3][16 * rb + n];
+      const size_t r = part_row * p.rows_cap + size_t(rt * kRows + 16 * rb + n);
+      const int dim = 64 * vslice + 16 * g;  // element e of accumulator q: dim + 4 e + q
+      if (whole) {
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          w[i] = uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i) & 3][i >> 1] * inv)) |
+                 (uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i + 1) & 3][i >> 1] * inv)) << 16);
+        lk_u32x4 *o = reinterpret_cast<lk_u32x4 *>(static_cast<uint16_t *>(p.out) +
+                                                   (size_t(qrow[rb]) * p.hq + head[rb]) * kD + dim);
+        o[0] = lk_u32x4{w[0], w[1], w[2], w[3]};
+        o[1] = lk_u32x4{w[4], w[5], w[6], w[7]};
+      } else {
+        lk_f32x4 *po = reinterpret_cast<lk_f32x4 *>(p.part_o + r * kD + dim);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) po[e] = lk_f32x4{oacc[rb][0][e], oacc[rb][1][e], oacc[rb][2][e], oacc[rb][3][e]};
+      }
+      if (g == 0 && vslice == 0) {
+        p.part_ml[2 * r] = m[rb];
+        p.part_ml[2 * r + 1] = sum;
+      }
     }
   }
-  lds_barrier();
-  if constexpr (kSlices < 4) {
-    if (vgroup > 0) return;
-#pragma unroll
-    for (int og = 0; og < 4 / kSlices - 1; ++og)
-#pragma unroll
-      for (int rb = 0; rb < kRB; ++rb)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) oacc[rb][q] += spill[((og * kSlices + vslice) * kRB * 4 + rb * 4 + q) * kWave + lane];
-  }
-#pragma unroll
-  for (int rb = 0; rb < kRB; ++rb) {
-    if (!row_ok[rb]) continue;
-    const float total = sm.top[0][16 * rb + n] + sm.top[1][16 * rb + n] + sm.top[2][16 * rb + n] + sm.top[3][16 * rb + n];
-    const size_t r = size_t(qrow[rb]) * p.hq + head[rb];
-    const int dim = 64 * vslice + 16 * g;  // element e of accumulator q: dim + 4 e + q
-    if (p.num_splits == 1) {
-      const float inv = total != 0.f ? 1.f / total : 0.f;
-      uint32_t w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        w[i] = uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i) & 3][i >> 1] * inv)) |
-               (uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i + 1) & 3][i >> 1] * inv)) << 16);
-      lk_u32x4 *o = reinterpret_cast<lk_u32x4 *>(static_cast<uint16_t *>(p.out) + r * kD + dim);
-      o[0] = lk_u32x4{w[0], w[1], w[2], w[3]};
-      o[1] = lk_u32x4{w[4], w[5], w[6], w[7]};
-    } else {
-      lk_f32x4 *po = reinterpret_cast<lk_f32x4 *>(p.part_o + (r * p.num_splits + split) * kD + dim);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) po[e] = lk_f32x4{oacc[rb][0][e], oacc[rb][1][e], oacc[rb][2][e], oacc[rb][3][e]};
-    }
-    if (g == 0 && vslice == 0) {
-      p.part_ml[2 * (r * p.num_splits + split)] = m[rb];
-      p.part_ml[2 * (r * p.num_splits + split) + 1] = total;
-    }
+  lds_barrier();  // the next segment writes sm.top and sm.pt
   }
 }
 
-// Joins the splits of every query row and, where the call asks for them, adds
+// Joins the parts of every query row and, where the call asks for them, adds
 // the heads' weights onto the cached rows:
 //   M = max_s m_s, L = sum_s 2^(m_s - M) l_s, out = sum_s 2^(m_s - M) O_s / L,
 //   weights[b, h, t] (+)= sum over the heads of h of 2^(x_t - M) / L.
-// Blocks below p.total_q * Hq * dim_slices take a (row, head, 64 dims) each:
-// 16 threads of four dims by 16 groups of splits; the rest take 1024 cached
-// rows of a (request, KV head) each.  Every sum has one order.
+// The first blocks take outputs.  kWide false (few query rows, each with many
+// parts): a (row, head, 64 dims) per block, 16 threads of four dims by 16
+// groups of parts; kWide true: a (row, head) per wavefront, four dims per lane.
+// The rest take 1024 cached rows of a (request, KV head) each.  Every sum has
+// one order.
 constexpr int kSliceDims = 64;
 constexpr int kWeightKeys = 4 * kThreads;
 
-// (M, 1 / L) of (row, head) `r` over the splits that hold keys; every lane of
-// the calling wavefront gets them.
-__device__ __forceinline__ void join_stats(const RowAttnParams &p, size_t r, int ns, float &m, float &inv) {
+// Where the partial results of query row `row` (request b, its row `tok`) and
+// `head` lie: `count` of them, `stride` apart.  None: it saw nothing.
+struct Parts {
+  size_t first, stride;
+  int count;
+};
+
+__device__ __forceinline__ Parts parts_of(const RowAttnParams &p, int b, int row, int tok, int head) {
+  if (p.workers == 0) {
+    int begin, count;
+    request_rows(p, b, begin, count);
+    const int len = rows_seen(p, clamp_rows(p.lens[b], p.max_len), count);
+    return Parts{(size_t(row) * p.hq + head) * p.num_splits, 1, (len + p.split_tokens - 1) / p.split_tokens};
+  }
+  // Tiles lo .. hi - 1 are the request's; worker w of them has floor(total w / workers) on.
+  const int64_t total = p.plan[p.batch], lo = p.plan[b], hi = p.plan[b + 1];
+  const int64_t in_request = int64_t(tok) * p.group + head % p.group;
+  if (lo == hi || in_request >= p.rows_cap) return Parts{0, 1, 0};  // nothing seen, or past the longest request told
+  const int64_t workers = min(int64_t(p.workers), total);
+  int w0, w1;
+  if (total < (int64_t(1) << 22)) {  // workers is at most 512: the division has 32 bits
+    w0 = int((uint32_t(lo + 1) * uint32_t(workers) - 1) / uint32_t(total));
+    w1 = int((uint32_t(hi) * uint32_t(workers) - 1) / uint32_t(total));
+  } else {
+    w0 = int(((lo + 1) * workers - 1) / total);
+    w1 = int((hi * workers - 1) / total);
+  }
+  return Parts{((size_t(w0) + b) * p.hkv + head / p.group) * p.rows_cap + size_t(in_request), size_t(p.hkv) * p.rows_cap, w1 - w0 + 1};
+}
+
+// (M, 1 / L) over the parts; every lane of the calling wavefront gets them.
+__device__ __forceinline__ void join_stats(const RowAttnParams &p, const Parts &parts, float &m, float &inv) {
   const int lane = threadIdx.x & 63;
-  const float *ml = p.part_ml + 2 * r * p.num_splits;
   float mx = -__builtin_inff();
-  for (int s = lane; s < ns; s += kWave) mx = fmaxf(mx, ml[2 * s]);
+  for (int s = lane; s < parts.count; s += kWave) mx = fmaxf(mx, p.part_ml[2 * (parts.first + s * parts.stride)]);
   mx = wave_max(mx);
   float total = 0.f;
-  for (int s = lane; s < ns; s += kWave) {
-    // A split that saw nothing has l = 0; one with a NaN logit has l = NaN, whatever its maximum.
-    const float ls = ml[2 * s + 1];
-    if (ls != 0.f) total += __builtin_amdgcn_exp2f(ml[2 * s] - mx) * ls;
+  for (int s = lane; s < parts.count; s += kWave) {
+    // A part that saw nothing has l = 0; one with a NaN logit has l = NaN, whatever its maximum.
+    const float *ml = p.part_ml + 2 * (parts.first + s * parts.stride);
+    if (ml[1] != 0.f) total += __builtin_amdgcn_exp2f(ml[0] - mx) * ml[1];
   }
   total = wave_sum(total);
   m = mx == -__builtin_inff() ? 0.f : mx;
   inv = total != 0.f ? 1.f / total : 0.f;
 }
 
-// dim_slices 0: the outputs are written already.
-template <bool kBf16>
+template <bool kBf16, bool kWide>
 __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnParams p, int dim_slices) {
   __shared__ float red[kThreads / 16][kSliceDims + 4];
-  __shared__ float fac[kMaxSplits];
+  __shared__ float fac[kMaxParts];
   __shared__ float stat[kWave][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t out_blocks = int64_t(p.total_q) * p.hq * dim_slices;
-  if (int64_t(blockIdx.x) < out_blocks) {
-    const int slice = int(blockIdx.x) % dim_slices;
-    const int r = int(blockIdx.x) / dim_slices;
-    const int b = request_of_row(p, r / p.hq);
+  const int64_t out_rows = int64_t(p.total_q) * p.hq;
+  const int64_t out_blocks = kWide ? (out_rows + kWaves - 1) / kWaves : out_rows * dim_slices;
+  if (kWide && int64_t(blockIdx.x) < out_blocks) {
+    const int64_t r = int64_t(blockIdx.x) * kWaves + wave;
+    if (r >= out_rows) return;
+    const int row = int(r / p.hq);
+    const int b = request_of_row(p, row);
     if (b < 0) return;
     int begin, count;
     request_rows(p, b, begin, count);
-    const int ctx = clamp_rows(p.lens[b], p.max_len);
-    const int len = rows_seen(p, ctx, count);
-    const int ns = (len + p.split_tokens - 1) / p.split_tokens;
+    const Parts parts = parts_of(p, b, row, row - begin, int(r) - row * p.hq);
+    if (p.workers > 0 && parts.count == 1) return;  // written already
     float m, inv;
-    join_stats(p, r, ns, m, inv);
+    join_stats(p, parts, m, inv);
+    for (int d4 = 4 * lane; d4 < p.dv; d4 += 4 * kWave) {
+      const float *po = p.part_o + parts.first * p.dv + d4;
+      f32x4_t acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int s = 0; s < parts.count; ++s) {
+        const float *ml = p.part_ml + 2 * (parts.first + s * parts.stride);
+        const f32x4_t v = *reinterpret_cast<const f32x4_t *>(po + size_t(s) * parts.stride * p.dv);
+        // A part that saw nothing was not written (any-shape kernel): its rubbish may be no number.
+        if (ml[1] != 0.f) acc += __builtin_amdgcn_exp2f(ml[0] - m) * v;
+      }
+      uint16_t *o = static_cast<uint16_t *>(p.out) + size_t(r) * p.dv + d4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = float_to_half_bits<kBf16>(acc[e] * inv);
+    }
+    return;
+  }
+  if (int64_t(blockIdx.x) < out_blocks) {
+    const int slice = int(blockIdx.x) % dim_slices;
+    const int r = int(blockIdx.x) / dim_slices, row = r / p.hq;
+    const int b = request_of_row(p, row);
+    if (b < 0) return;
+    int begin, count;
+    request_rows(p, b, begin, count);
+    const Parts parts = parts_of(p, b, row, row - begin, r - row * p.hq);
+    if (p.workers > 0 && parts.count == 1) return;  // uniform: written already
+    float m, inv;
+    join_stats(p, parts, m, inv);
     if (wave == 0)
-      for (int s = lane; s < ns; s += kWave) {
-        const float *ml = p.part_ml + 2 * (size_t(r) * p.num_splits + s);
+      for (int s = lane; s < parts.count; s += kWave) {
+        const float *ml = p.part_ml + 2 * (parts.first + s * parts.stride);
         fac[s] = ml[1] != 0.f ? __builtin_amdgcn_exp2f(ml[0] - m) : 0.f;
       }
     __syncthreads();
     const int d4 = slice * kSliceDims + 4 * (tid & 15), g = tid >> 4;
     f32x4_t acc{0.f, 0.f, 0.f, 0.f};
     if (d4 < p.dv) {
-      const float *po = p.part_o + size_t(r) * p.num_splits * p.dv + d4;
-      for (int s = g; s < ns; s += kThreads / 16)
-        if (fac[s] != 0.f) acc += fac[s] * *reinterpret_cast<const f32x4_t *>(po + size_t(s) * p.dv);
+      const float *po = p.part_o + parts.first * p.dv + d4;
+      for (int s = g; s < parts.count; s += kThreads / 16)
+        if (fac[s] != 0.f) acc += fac[s] * *reinterpret_cast<const f32x4_t *>(po + size_t(s) * parts.stride * p.dv);
     }
     *reinterpret_cast<f32x4_t *>(&red[g][4 * (tid & 15)]) = acc;
     __syncthreads();
@@ -641,7 +779,6 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
   const int len = clamp_rows(p.lens[b], p.max_len);
   const int t = chunk * kWeightKeys + 4 * tid;
   if (chunk * kWeightKeys >= len) return;  // uniform
-  const int ns = (len + p.split_tokens - 1) / p.split_tokens;
   const size_t r0 = size_t(b) * p.hq + size_t(h) * p.group;
   f32x4_t acc{0.f, 0.f, 0.f, 0.f};
   for (int g0 = 0; g0 < p.group; g0 += kWave) {
@@ -649,7 +786,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     __syncthreads();
     for (int j = wave; j < here; j += kWaves) {
       float m, inv;
-      join_stats(p, r0 + g0 + j, ns, m, inv);
+      join_stats(p, parts_of(p, b, b, 0, h * p.group + g0 + j), m, inv);
       if (lane == 0) {
         stat[j][0] = m;
         stat[j][1] = inv;
@@ -673,9 +810,9 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
 // ------------------------------------------------------------- host side
 
 struct RowPlan {
-  int split_tokens, num_splits;
-  int row_blocks;  // 16-row blocks of a workgroup on the matrix cores; 0: any-shape kernel
-  int row_tiles;
+  int split_tokens, num_splits;              // any-shape kernel
+  int row_blocks, row_tiles, workers;        // matrix cores: 16-row blocks of a workgroup (0: any-shape kernel)
+  int64_t parts;                             // partial results: rows of part_o and part_ml
   int64_t magic;
 };
 
@@ -696,42 +833,57 @@ RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int6
     splits = std::min<int64_t>(splits, kMaxSplits);
     pl.split_tokens = int((len + splits - 1) / splits);
     pl.num_splits = int((len + pl.split_tokens - 1) / pl.split_tokens);
+    pl.parts = total_q * heads * pl.num_splits;
     return pl;
   }
   const int64_t rows = std::max<int64_t>(max_query, 1) * (heads / hkv);
   pl.row_blocks = rows <= 16 ? 1 : rows <= 32 || d == 64 ? 2 : 4;
   pl.row_tiles = int((rows + 16 * pl.row_blocks - 1) / (16 * pl.row_blocks));
   pl.magic = ((int64_t(1) << 36) + block_size / 16 - 1) / (block_size / 16);
-  const int64_t tile = 16384 / d, tiles = (len + tile - 1) / tile;
-  // About 512 workgroups (two per CU), whole tiles each.
-  const int64_t items = batch * hkv * pl.row_tiles;
-  const int64_t splits = std::min<int64_t>(std::max<int64_t>(1, (512 + items - 1) / items), kMaxSplits);
-  const int64_t per = std::max<int64_t>((tiles + splits - 1) / splits, 1);
-  pl.split_tokens = int(per * tile);
-  pl.num_splits = int((tiles + per - 1) / per);
+  // A workgroup for each slot that the GPU has: two per CU, one with 64 query rows (registers).
+  const int64_t tile = 16384 / d, tiles = batch * ((len + tile - 1) / tile);
+  const int64_t slots = (pl.row_blocks > 2 ? 256 : 512) / (hkv * pl.row_tiles);
+  pl.workers = int(std::min<int64_t>(std::max<int64_t>(slots, 1), tiles));
+  pl.parts = (pl.workers + batch) * hkv * pl.row_tiles * 16 * pl.row_blocks;
   return pl;
 }
 
 int64_t x_stride_of(int64_t max_len) { return (std::max<int64_t>(max_len, 1) + 63) / 64 * 64; }
 
+// The partial results, the logits (weights), the plan.
+struct RowSpace {
+  size_t o, ml, x, plan;
+  size_t total() const { return o + ml + x + plan; }
+};
+
+RowSpace row_space(const RowPlan &pl, int64_t batch, int64_t total_q, int64_t heads, int64_t dv, int64_t max_len,
+                   bool weights) {
+  auto round = [](size_t v) { return (v + 255) / 256 * 256; };
+  RowSpace w{};
+  w.o = round(size_t(pl.parts) * dv * sizeof(float));
+  w.ml = round(size_t(pl.parts) * 2 * sizeof(float));
+  if (weights) w.x = round(size_t(total_q) * heads * size_t(x_stride_of(max_len)) * sizeof(float));
+  if (pl.row_blocks) w.plan = round(size_t(batch + 1) * sizeof(int64_t));
+  return w;
+}
+
 // Bytes for either kernel: the query's alignment, which also decides, is not known here.
 size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv, int64_t d, int64_t dv,
                      int64_t block_size, int64_t max_query, int64_t max_len, bool weights) {
-  int64_t splits = plan_rows(false, batch, total_q, heads, hkv, d, block_size, max_query, max_len).num_splits;
-  if (mfma_rows(d, dv, block_size, max_len))
-    splits = std::max<int64_t>(splits, plan_rows(true, batch, total_q, heads, hkv, d, block_size, max_query, max_len).num_splits);
-  size_t floats = size_t(total_q) * heads * splits * size_t(dv + 2);
-  floats = (floats + 3) / 4 * 4;
-  if (weights) floats += size_t(total_q) * heads * size_t(x_stride_of(max_len));
-  return floats * sizeof(float);
+  size_t need = 0;
+  for (const bool mfma : {false, true}) {
+    if (mfma && !mfma_rows(d, dv, block_size, max_len)) continue;
+    const RowPlan pl = plan_rows(mfma, batch, total_q, heads, hkv, d, block_size, max_query, max_len);
+    need = std::max(need, row_space(pl, batch, total_q, heads, dv, max_len, weights).total());
+  }
+  return need;
 }
 
 template <int kD, bool kBf16, int kRB, typename BtT>
-void launch_rows(const RowAttnParams &p, const RowTile &tile, hipStream_t s) {
-  const int64_t outer = (int64_t(p.batch) * p.num_splits + 7) / 8 * 8;
-  const unsigned blocks = unsigned(outer * p.hkv * tile.row_tiles);
-  if (p.x) row_attention_mfma<kD, kBf16, kRB, true, BtT><<<blocks, kThreads, 0, s>>>(p, tile);
-  else row_attention_mfma<kD, kBf16, kRB, false, BtT><<<blocks, kThreads, 0, s>>>(p, tile);
+void launch_rows(const RowAttnParams &p, int64_t magic, hipStream_t s) {
+  const unsigned blocks = unsigned((int64_t(p.workers) + 7) / 8 * 8 * p.hkv * p.row_tiles);
+  if (p.x) row_attention_mfma<kD, kBf16, kRB, true, BtT><<<blocks, kThreads, 0, s>>>(p, magic);
+  else row_attention_mfma<kD, kBf16, kRB, false, BtT><<<blocks, kThreads, 0, s>>>(p, magic);
 }
 
 template <bool kBf16, typename BtT>
@@ -740,12 +892,11 @@ void launch_row_attention(const RowAttnParams &p, const RowPlan &pl, hipStream_t
     row_attention_any<kBf16, BtT><<<dim3(unsigned(p.total_q) * unsigned(p.hq), unsigned(p.num_splits)), kThreads, 0, s>>>(p);
     return;
   }
-  const RowTile tile{pl.magic, 16 * pl.row_blocks, pl.row_tiles};
   const auto with_dim = [&](auto dim) {
     constexpr int kD = decltype(dim)::value;
-    if (pl.row_blocks == 1) launch_rows<kD, kBf16, 1, BtT>(p, tile, s);
-    else if (kD == 64 || pl.row_blocks == 2) launch_rows<kD, kBf16, 2, BtT>(p, tile, s);
-    else launch_rows<kD, kBf16, kD == 64 ? 2 : 4, BtT>(p, tile, s);
+    if (pl.row_blocks == 1) launch_rows<kD, kBf16, 1, BtT>(p, pl.magic, s);
+    else if (kD == 64 || pl.row_blocks == 2) launch_rows<kD, kBf16, 2, BtT>(p, pl.magic, s);
+    else launch_rows<kD, kBf16, kD == 64 ? 2 : 4, BtT>(p, pl.magic, s);
   };
   if (p.d == 64) with_dim(std::integral_constant<int, 64>{});
   else if (p.d == 128) with_dim(std::integral_constant<int, 128>{});
@@ -834,20 +985,30 @@ int row_attention(const char *name, const RowArgs &a) {
   p.accumulate = a.accumulate ? 1 : 0;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   const size_t rows = size_t(a.total_q) * a.heads;
-  p.part_o = static_cast<float *>(a.workspace);
-  p.part_ml = p.part_o + rows * pl.num_splits * a.dv;
+  const RowSpace space = row_space(pl, a.batch, a.total_q, a.heads, a.dv, a.max_len, a.weights != nullptr);
+  uint8_t *ws = static_cast<uint8_t *>(a.workspace);
+  p.part_o = reinterpret_cast<float *>(ws);
+  p.part_ml = reinterpret_cast<float *>(ws + space.o);
   if (a.weights) {
-    p.x = p.part_o + (rows * pl.num_splits * size_t(a.dv + 2) + 3) / 4 * 4;
+    p.x = reinterpret_cast<float *>(ws + space.o + space.ml);
     p.x_stride = x_stride_of(a.max_len);
     p.weights = a.weights;
     p.w_stride = a.w_stride;
   }
-  // One split of the matrix-core kernel writes the outputs itself.
-  const int dim_slices = mfma && pl.num_splits == 1 ? 0 : int((a.dv + kSliceDims - 1) / kSliceDims);
-  const int64_t join_blocks = int64_t(rows) * dim_slices +
+  if (mfma) {
+    p.plan = reinterpret_cast<int64_t *>(ws + space.o + space.ml + space.x);
+    p.workers = pl.workers;
+    p.row_tiles = pl.row_tiles;
+    p.rows_cap = pl.row_tiles * 16 * pl.row_blocks;
+    p.tile_rows = int(16384 / a.d);
+  }
+  const int dim_slices = int((a.dv + kSliceDims - 1) / kSliceDims);
+  // From 1024 (row, head) pairs on, a wavefront each fills the GPU (192 rows of 16
+  // heads, about four parts each: 37 us in slices).
+  const bool wide = int64_t(rows) >= 1024;
+  const int64_t join_blocks = (wide ? (int64_t(rows) + kWaves - 1) / kWaves : int64_t(rows) * dim_slices) +
                               (a.weights ? a.batch * a.hkv * ((a.max_len + kWeightKeys - 1) / kWeightKeys) : 0);
-  const int64_t attn_blocks =
-      mfma ? (a.batch * pl.num_splits + 7) / 8 * 8 * a.hkv * pl.row_tiles : int64_t(rows);
+  const int64_t attn_blocks = mfma ? (int64_t(pl.workers) + 7) / 8 * 8 * a.hkv * pl.row_tiles : int64_t(rows);
   if (std::max(join_blocks, attn_blocks) > 0xFFFFFFFFll / kThreads)  // threads of one launch
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
   hipStream_t s = reinterpret_cast<hipStream_t>(a.stream);
@@ -856,10 +1017,11 @@ int row_attention(const char *name, const RowArgs &a) {
   else if (bf16) launch_row_attention<true, int32_t>(p, pl, s);
   else if (i64) launch_row_attention<false, int64_t>(p, pl, s);
   else launch_row_attention<false, int32_t>(p, pl, s);
-  if (join_blocks > 0) {
-    if (bf16) row_attention_join<true><<<unsigned(join_blocks), kThreads, 0, s>>>(p, dim_slices);
-    else row_attention_join<false><<<unsigned(join_blocks), kThreads, 0, s>>>(p, dim_slices);
-  }
+  const unsigned blocks = unsigned(join_blocks);
+  if (bf16 && wide) row_attention_join<true, true><<<blocks, kThreads, 0, s>>>(p, dim_slices);
+  else if (bf16) row_attention_join<true, false><<<blocks, kThreads, 0, s>>>(p, dim_slices);
+  else if (wide) row_attention_join<false, true><<<blocks, kThreads, 0, s>>>(p, dim_slices);
+  else row_attention_join<false, false><<<blocks, kThreads, 0, s>>>(p, dim_slices);
   return check_launch(name);
 }
 
