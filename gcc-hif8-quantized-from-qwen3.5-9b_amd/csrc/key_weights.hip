@@ -265,7 +265,7 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
       for (int i = 0; i < kSlices; ++i)
         raw[kb][i] = *reinterpret_cast<const u32x4_a4 *>(base[kb] + uint32_t(n) * rec + 16u * g + 64 * i);
     }
-    fill_lookup<kBf16>(sm.table, reinterpret_cast<uint32_t *>(sm.ml), tid);
+    fill_lookup<kBf16, kThreads>(sm.table, reinterpret_cast<uint32_t *>(sm.ml), tid);
     lds_barrier();
     const uint32_t lane4 = uint32_t(4 * lane);
     lk_u32x4 kf[4][kQS];

@@ -20,18 +20,20 @@ typedef float lk_f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short lk_u16x2 __attribute__((ext_vector_type(2)));
 
 // Fills the table, with 256 words of LDS for the entries before they are spread
-// (each thread of 256 works one out: loading them took longer than a short
-// call's attention).  The caller synchronises afterwards.
-template <bool kBf16Low>
+// (256 threads work one out each: loading them took longer than a short call's
+// attention).  The caller synchronises afterwards.
+template <bool kBf16Low, int kThreads>
 __device__ __forceinline__ void fill_lookup(uint32_t *table, uint32_t *entries, int tid) {
-  const uint32_t f = decode_bits(uint32_t(tid));
-  const uint32_t h = float_to_f16_bits(__uint_as_float(f));  // exact
-  entries[tid] = (kBf16Low ? f >> 16 : h) | (h << 16);
+  if (tid < 256) {
+    const uint32_t f = decode_bits(uint32_t(tid));
+    const uint32_t h = float_to_f16_bits(__uint_as_float(f));  // exact
+    entries[tid] = (kBf16Low ? f >> 16 : h) | (h << 16);
+  }
   lds_barrier();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t v = entries[(tid >> 4) + 16 * i];
-    reinterpret_cast<lk_u32x4 *>(table)[tid + 256 * i] = lk_u32x4{v, v, v, v};
+  for (int i = 0; i < 4096 / kThreads; ++i) {
+    const uint32_t v = entries[(tid >> 4) + kThreads / 16 * i];
+    reinterpret_cast<lk_u32x4 *>(table)[tid + kThreads * i] = lk_u32x4{v, v, v, v};
   }
 }
 

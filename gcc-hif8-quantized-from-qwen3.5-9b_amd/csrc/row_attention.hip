@@ -137,6 +137,12 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 // sum_t P_t 2^-e_t is the softmax sum against the same maximum.
 constexpr float kLazy = 6.f;  // log2 headroom of the maximum: it moves in steps of more than 2^6
 
+// Wavefronts of a workgroup: four, two workgroups to a CU; with 64 query rows
+// eight, one workgroup, since the table and the query rows in LDS leave no room
+// for two and the registers of four none for the rows.
+constexpr int waves_of(int row_blocks) { return row_blocks > 2 ? 8 : 4; }
+constexpr int max_of(int a, int b) { return a > b ? a : b; }
+
 // Tiles of request b.
 __device__ __forceinline__ int64_t tiles_of(const RowAttnParams &p, int b) {
   int begin, count;
@@ -169,21 +175,26 @@ __device__ __forceinline__ void split_scale(float s, float &e, float &mant, floa
 }
 
 template <int kD, bool kBf16, int kRB, bool kX, typename BtT>
-__global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(const RowAttnParams p,
-                                                                               const int64_t page_magic) {
+__global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(const RowAttnParams p,
+                                                                            const int64_t page_magic) {
+  constexpr int kW = waves_of(kRB);       // wavefronts
+  constexpr bool kQLds = kRB > 2;         // the query rows lie in LDS, in operand order, instead of registers
   constexpr int kRow = kD + 4;
-  constexpr int kT = 16384 / kD;          // cache rows of a tile
-  constexpr int kKB = kT / 64;            // 16-row blocks of a wavefront in S
+  constexpr int kT = 4096 / kD * kW;      // cache rows of a tile
+  constexpr int kKB = 256 / kD;           // 16-row blocks of a wavefront in S
   constexpr int kQS = kD / 32;            // MFMA steps over the head dims
   constexpr int kSlices = kD / 64;        // 64-dim slices of V
+  constexpr int kVG = kW / kSlices;       // wavefronts that share a slice, 64 rows of the tile each
   constexpr int kGroups = kT / 16;        // 16-row groups of a tile
+  static_assert(kGroups < 32 && kVG * 64 == kT, "a bit per group, 64 rows per wavefront of a slice");
   constexpr int kRows = 16 * kRB;
   constexpr int kPStride = kT + 8;        // fp16 values of a row of P in LDS
   struct Smem {
     uint32_t table[kLookupBytes / 4];     // at LDS byte 0: a lookup's address needs no addition
-    // P of a tile; at a segment's end the wavefronts' shares of O (D < 256).
-    __attribute__((aligned(16))) uint16_t pt[kSlices < 4 && kRows * kPStride < 6144 ? 6144 : kRows * kPStride];
-    float top[4][kRows];
+    // P of a tile; at a segment's end the shares of O of wavefronts of one slice.
+    __attribute__((aligned(16))) uint16_t pt[max_of(kRows * kPStride, (kVG - 1) * kSlices * 2048)];
+    lk_u32x4 q[kQLds ? kRB * kQS * kWave : 1];
+    float top[kW][kRows];
   };
   __shared__ __attribute__((aligned(16))) Smem sm;
   const uint32_t table = lds_address(sm.table);
@@ -215,7 +226,7 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
   if (worker >= workers) return;                           // uniform
   int64_t cur = total * worker / workers;
   const int64_t run_end = total * (worker + 1) / workers;
-  fill_lookup<kBf16>(sm.table, reinterpret_cast<uint32_t *>(sm.pt), tid);
+  fill_lookup<kBf16, 64 * kW>(sm.table, reinterpret_cast<uint32_t *>(sm.pt), tid);
 
   const uint32_t rec = uint32_t(p.hkv) * kRow;
   const int bs16 = p.block_size >> 4;
@@ -332,13 +343,24 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
   };
 
   // The query rows first: what is waited for last must not be issued behind the cache.
-  lk_u32x4 qf[kRB][kQS];
+  // Step 2 i + s of a row block: dims 64 i + 16 g + 8 s + [0, 8).
+  lk_u32x4 qf[kQLds ? 1 : kRB][kQLds ? kRB * kQS / kW : kQS];
+  if constexpr (kQLds) {
 #pragma unroll
-  for (int rb = 0; rb < kRB; ++rb) {
-    const uint16_t *q = static_cast<const uint16_t *>(p.query) + (size_t(qrow[rb]) * p.hq + head[rb]) * kD + 16 * g;
+    for (int j = 0; j < kRB * kQS / kW; ++j) {
+      const int f = wave * (kRB * kQS / kW) + j, i = f % kQS;
+      const int r = min(rt * kRows + 16 * (f / kQS) + n, rows - 1), tok = r / p.group;
+      const uint16_t *q = static_cast<const uint16_t *>(p.query) +
+                          (size_t(begin + tok) * p.hq + h * p.group + (r - tok * p.group)) * kD + 16 * g;
+      qf[0][j] = *reinterpret_cast<const lk_u32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1));
+    }
+  } else {
 #pragma unroll
-    for (int i = 0; i < kQS; ++i)  // step 2 i + s: dims 64 i + 16 g + 8 s + [0, 8)
-      qf[rb][i] = *reinterpret_cast<const lk_u32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1));
+    for (int rb = 0; rb < kRB; ++rb) {
+      const uint16_t *q = static_cast<const uint16_t *>(p.query) + (size_t(qrow[rb]) * p.hq + head[rb]) * kD + 16 * g;
+#pragma unroll
+      for (int i = 0; i < kQS; ++i) qf[rb][i] = *reinterpret_cast<const lk_u32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1));
+    }
   }
   const BtT blk_first = block_at(t_begin);
   BtT blk_next = block_at(min(t_begin + kT, t_end - 1));
@@ -355,17 +377,20 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
 #pragma unroll
     for (int q = 0; q < 4; ++q) oacc[rb][q] = lk_f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  if constexpr (kQLds) {
+#pragma unroll
+    for (int j = 0; j < kRB * kQS / kW; ++j) sm.q[(wave * (kRB * kQS / kW) + j) * kWave + lane] = qf[0][j];
+  }
   lds_barrier();
   // The query rows have arrived: without this the loop would wait for them, and
   // with them for every load behind them, in every iteration.  Columns of no
-  // row repeat the request's first row and are not written.
+  // row repeat a row of the request and are not written.
+  if constexpr (!kQLds) {
 #pragma unroll
-  for (int rb = 0; rb < kRB; ++rb)
+    for (int rb = 0; rb < kRB; ++rb)
 #pragma unroll
-    for (int i = 0; i < kQS; ++i) {
-      if constexpr (kRB > 2) asm volatile("" : "+a"(qf[rb][i]));  // 128 registers: kept out of the way
-      else asm volatile("" : "+v"(qf[rb][i]));
-    }
+      for (int i = 0; i < kQS; ++i) asm volatile("" : "+v"(qf[rb][i]));
+  }
 
   for (int it = 0; it < ntiles; ++it) {
     const int t0 = t_begin + it * kT;
@@ -383,7 +408,10 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
         const lk_u32x4 w = kraw[kb][i >> 1];
         const lk_u32x4 a = look8<false>(w[2 * (i & 1)], w[2 * (i & 1) + 1], lane4, table);
 #pragma unroll
-        for (int rb = 0; rb < kRB; ++rb) s[rb][kb] = mfma_16x16x32<kBf16>(a, qf[rb][i], s[rb][kb]);
+        for (int rb = 0; rb < kRB; ++rb) {
+          const lk_u32x4 q = kQLds ? sm.q[(rb * kQS + i) * kWave + lane] : qf[kQLds ? 0 : rb][kQLds ? 0 : i];
+          s[rb][kb] = mfma_16x16x32<kBf16>(a, q, s[rb][kb]);
+        }
       }
     }
     float ksc[kKB][4], ve[kKB][4], vm[kKB][4], vi[kKB][4];
@@ -468,8 +496,9 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
     lds_barrier();
 #pragma unroll
     for (int rb = 0; rb < kRB; ++rb) {
-      const float top = fmaxf(fmaxf(sm.top[0][16 * rb + n], sm.top[1][16 * rb + n]),
-                              fmaxf(sm.top[2][16 * rb + n], sm.top[3][16 * rb + n]));
+      float top = sm.top[0][16 * rb + n];
+#pragma unroll
+      for (int w = 1; w < kW; ++w) top = fmaxf(top, sm.top[w][16 * rb + n]);
       const bool grow = top > m[rb] + kLazy;
       if (__any(grow)) {
         const float next = grow ? top : m[rb];
@@ -582,14 +611,14 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
     load_v();
   }
 
-  // The wavefronts' shares of the softmax sum, and (D < 256) of O.
+  // The wavefronts' shares of the softmax sum, and of O where some share a slice.
   lds_barrier();
 #pragma unroll
   for (int rb = 0; rb < kRB; ++rb) {
     const float lt = sum_over_groups(l[rb]);
     if (g == 0) sm.top[wave][16 * rb + n] = lt;
   }
-  if constexpr (kSlices < 4) {
+  if constexpr (kVG > 1) {
     lk_f32x4 *spill = reinterpret_cast<lk_f32x4 *>(sm.pt);
 #pragma unroll
     for (int rb = 0; rb < kRB; ++rb) {
@@ -601,7 +630,7 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
       lds_barrier();
       if (vgroup == 0) {
 #pragma unroll
-        for (int og = 0; og < 4 / kSlices - 1; ++og)
+        for (int og = 0; og < kVG - 1; ++og)
 #pragma unroll
           for (int q = 0; q < 4; ++q) oacc[rb][q] += spill[((og * kSlices + vslice) * 4 + q) * kWave + lane];
       }
@@ -613,7 +642,9 @@ __global__ __launch_bounds__(kThreads, kRB > 3 ? 1 : 2) void row_attention_mfma(
 #pragma unroll
     for (int rb = 0; rb < kRB; ++rb) {
       if (!row_ok[rb]) continue;
-      const float sum = sm.top[0][16 * rb + n] + sm.top[1][16 * rb + n] + sm.top[2][16 * rb + n] + sm.top[3][16 * rb + n];
+      float sum = sm.top[0][16 * rb + n];
+#pragma unroll
+      for (int w = 1; w < kW; ++w) sum += sm.top[w][16 * rb + n];
       const size_t r = part_row * p.rows_cap + size_t(rt * kRows + 16 * rb + n);
       const int dim = 64 * vslice + 16 * g;  // element e of accumulator q: dim + 4 e + q
       if (whole) {
@@ -811,7 +842,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
 
 struct RowPlan {
   int split_tokens, num_splits;              // any-shape kernel
-  int row_blocks, row_tiles, workers;        // matrix cores: 16-row blocks of a workgroup (0: any-shape kernel)
+  int row_blocks, row_tiles, workers, tile_rows;  // matrix cores: 16-row blocks of a workgroup (0: any-shape kernel)
   int64_t parts;                             // partial results: rows of part_o and part_ml
   int64_t magic;
 };
@@ -840,9 +871,10 @@ RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int6
   pl.row_blocks = rows <= 16 ? 1 : rows <= 32 || d == 64 ? 2 : 4;
   pl.row_tiles = int((rows + 16 * pl.row_blocks - 1) / (16 * pl.row_blocks));
   pl.magic = ((int64_t(1) << 36) + block_size / 16 - 1) / (block_size / 16);
-  // A workgroup for each slot that the GPU has: two per CU, one with 64 query rows (registers).
-  const int64_t tile = 16384 / d, tiles = batch * ((len + tile - 1) / tile);
-  const int64_t slots = (pl.row_blocks > 2 ? 256 : 512) / (hkv * pl.row_tiles);
+  // A workgroup for each slot that the GPU has: eight wavefronts per CU.
+  pl.tile_rows = int(4096 / d * waves_of(pl.row_blocks));
+  const int64_t tiles = batch * ((len + pl.tile_rows - 1) / pl.tile_rows);
+  const int64_t slots = 2048 / waves_of(pl.row_blocks) / (hkv * pl.row_tiles);
   pl.workers = int(std::min<int64_t>(std::max<int64_t>(slots, 1), tiles));
   pl.parts = (pl.workers + batch) * hkv * pl.row_tiles * 16 * pl.row_blocks;
   return pl;
@@ -881,9 +913,9 @@ size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv,
 
 template <int kD, bool kBf16, int kRB, typename BtT>
 void launch_rows(const RowAttnParams &p, int64_t magic, hipStream_t s) {
-  const unsigned blocks = unsigned((int64_t(p.workers) + 7) / 8 * 8 * p.hkv * p.row_tiles);
-  if (p.x) row_attention_mfma<kD, kBf16, kRB, true, BtT><<<blocks, kThreads, 0, s>>>(p, magic);
-  else row_attention_mfma<kD, kBf16, kRB, false, BtT><<<blocks, kThreads, 0, s>>>(p, magic);
+  const unsigned blocks = unsigned((int64_t(p.workers) + 7) / 8 * 8 * p.hkv * p.row_tiles), threads = 64 * waves_of(kRB);
+  if (p.x) row_attention_mfma<kD, kBf16, kRB, true, BtT><<<blocks, threads, 0, s>>>(p, magic);
+  else row_attention_mfma<kD, kBf16, kRB, false, BtT><<<blocks, threads, 0, s>>>(p, magic);
 }
 
 template <bool kBf16, typename BtT>
@@ -1000,7 +1032,7 @@ int row_attention(const char *name, const RowArgs &a) {
     p.workers = pl.workers;
     p.row_tiles = pl.row_tiles;
     p.rows_cap = pl.row_tiles * 16 * pl.row_blocks;
-    p.tile_rows = int(16384 / a.d);
+    p.tile_rows = pl.tile_rows;
   }
   const int dim_slices = int((a.dv + kSliceDims - 1) / kSliceDims);
   // From 1024 (row, head) pairs on, a wavefront each fills the GPU (192 rows of 16
