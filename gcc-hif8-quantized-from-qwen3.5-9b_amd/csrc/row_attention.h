@@ -24,14 +24,14 @@ struct RowAttnParams {
   // matrix cores [workers + batch, Hkv, rows_cap].
   float *part_o;
   float *part_ml;
-  int64_t *plan;               // matrix cores: [batch + 1] tiles before each request
+  int32_t *plan;               // matrix cores: [batch + 1] tiles before each request
   float *x;                    // [total_q * Hq, x_stride] base-2 logits, or null
   float *weights;              // [batch, Hkv, w_stride], or null
   int64_t bt_stride, num_blocks, mask_stride, x_stride, w_stride;
   int block_size, hkv, hq, group, d, dv, batch, total_q, max_len, num_splits, split_tokens, accumulate;
   // Matrix cores: workers that share the tiles, row tiles of the longest request,
   // query rows of all of them (a KV head's), cache rows of a tile.
-  int workers, row_tiles, rows_cap, tile_rows;
+  int workers, row_tiles, rows_cap, tile_rows, log2_tile_rows, heads_together;
   float scale_log2;            // softmax scale * log2(e)
 };
 

@@ -144,18 +144,19 @@ constexpr int waves_of(int row_blocks) { return row_blocks > 2 ? 8 : 4; }
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
 
 // Tiles of request b.
-__device__ __forceinline__ int64_t tiles_of(const RowAttnParams &p, int b) {
+__device__ __forceinline__ int tiles_of(const RowAttnParams &p, int b) {
   int begin, count;
   request_rows(p, b, begin, count);
-  return (int64_t(rows_seen(p, clamp_rows(p.lens[b], p.max_len), count)) + p.tile_rows - 1) / p.tile_rows;
+  return int((uint32_t(rows_seen(p, clamp_rows(p.lens[b], p.max_len), count)) + uint32_t(p.tile_rows) - 1) >>
+             p.log2_tile_rows);
 }
 
 // Inclusive sum over the lanes of a wavefront.
-__device__ __forceinline__ int64_t wave_prefix(int64_t v) {
+__device__ __forceinline__ int wave_prefix(int v) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) {
-    const int64_t up = int64_t(__shfl_up(static_cast<long long>(v), o, kWave));
+    const int up = __shfl_up(v, o, kWave);
     if (lane >= o) v += up;
   }
   return v;
@@ -203,30 +204,32 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   const uint32_t lane4 = uint32_t(4 * lane);
-  // The KV heads and row tiles of one worker read the same cache lines: their
-  // blocks are equal modulo 8, on one XCD.
-  const int inner = p.hkv * p.row_tiles;
+  // The row tiles of one (worker, KV head) read the same cache rows: their blocks
+  // are equal modulo 8, on one XCD.  So are all of a worker's KV heads, whose rows
+  // share cache lines, where that spreads the workers evenly.
+  const int inner = p.heads_together ? p.hkv * p.row_tiles : p.row_tiles;
   const int xcd = int(blockIdx.x) & 7, slot = int(blockIdx.x) >> 3;
-  const int worker = (slot / inner) * 8 + xcd;
+  const int outer = (slot / inner) * 8 + xcd, rest = slot % inner;
+  const int worker = p.heads_together ? outer : outer / p.hkv;
   if (worker >= p.workers) return;  // padding block (uniform)
-  const int rt = (slot % inner) % p.row_tiles, h = (slot % inner) / p.row_tiles;
+  const int rt = rest % p.row_tiles, h = p.heads_together ? rest / p.row_tiles : outer % p.hkv;
   // This worker's run of the requests' tiles, and the running total per request
   // (kept for the join by the first workgroup).  incl: of the first 64 requests.
-  int64_t total = 0, incl = 0;
+  int total = 0, incl = 0;
   for (int base = 0; base < p.batch; base += kWave) {
     const int i = base + lane;
-    const int64_t mine = i < p.batch ? tiles_of(p, i) : 0;
-    const int64_t upto = wave_prefix(mine);
+    const int mine = i < p.batch ? tiles_of(p, i) : 0;
+    const int upto = wave_prefix(mine);
     if (base == 0) incl = upto;
     if (worker == 0 && rt == 0 && h == 0 && wave == 0 && i < p.batch) p.plan[i] = total + upto - mine;
-    total += int64_t(__shfl(static_cast<long long>(upto), kWave - 1, kWave));
+    total += __builtin_amdgcn_readlane(upto, kWave - 1);
   }
   if (worker == 0 && rt == 0 && h == 0 && tid == 0) p.plan[p.batch] = total;
-  const int64_t workers = min(int64_t(p.workers), total);  // a tile each at least: no part is left unwritten
-  if (worker >= workers) return;                           // uniform
-  int64_t cur = total * worker / workers;
-  const int64_t run_end = total * (worker + 1) / workers;
-  fill_lookup<kBf16, 64 * kW>(sm.table, reinterpret_cast<uint32_t *>(sm.pt), tid);
+  const int workers = min(p.workers, total);  // a tile each at least: no part is left unwritten
+  if (worker >= workers) return;              // uniform
+  int cur = int(int64_t(total) * worker / workers);
+  const int run_end = int(int64_t(total) * (worker + 1) / workers);
+  bool filled = false;
 
   const uint32_t rec = uint32_t(p.hkv) * kRow;
   const int bs16 = p.block_size >> 4;
@@ -241,24 +244,23 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
 
   while (cur < run_end) {
   // The request of tile `cur` (uniform), and this segment's tiles of it.
-  int b = 0;
-  int64_t first = 0;
+  int b = 0, first = 0;
   if (p.batch <= kWave) {
     b = __builtin_ctzll(__ballot(incl > cur));
-    first = b ? int64_t(__shfl(static_cast<long long>(incl), b - 1, kWave)) : 0;
+    first = b ? __builtin_amdgcn_readlane(incl, b - 1) : 0;
   } else {
-    int64_t before = 0;
+    int before = 0;
     for (int base = 0; base < p.batch; base += kWave) {
       const int i = base + lane;
-      const int64_t upto = before + wave_prefix(i < p.batch ? tiles_of(p, i) : 0);
+      const int upto = before + wave_prefix(i < p.batch ? tiles_of(p, i) : 0);
       const uint64_t past = __ballot(upto > cur);
       if (past) {
         const int at = __builtin_ctzll(past);
         b = base + at;
-        first = at ? int64_t(__shfl(static_cast<long long>(upto), at - 1, kWave)) : before;
+        first = at ? __builtin_amdgcn_readlane(upto, at - 1) : before;
         break;
       }
-      before = int64_t(__shfl(static_cast<long long>(upto), kWave - 1, kWave));
+      before = __builtin_amdgcn_readlane(upto, kWave - 1);
     }
   }
   b = __builtin_amdgcn_readfirstlane(b);
@@ -267,9 +269,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   const int rows = count * p.group;
   const int ctx = clamp_rows(p.lens[b], p.max_len);
   const int len = rows_seen(p, ctx, count);
-  const int tile_first = __builtin_amdgcn_readfirstlane(int(cur - first));
-  const int seg_tiles = __builtin_amdgcn_readfirstlane(
-      int(min(run_end - cur, int64_t((len + kT - 1) / kT) - int64_t(tile_first))));
+  const int tile_first = cur - first;
+  const int seg_tiles = min(run_end - cur, int((uint32_t(len) + kT - 1) / kT) - tile_first);
   cur += seg_tiles;
   if (rt * kRows >= rows) continue;  // uniform: the request has no query rows here
   const int t_begin = tile_first * kT, t_end = min(t_begin + seg_tiles * kT, len);
@@ -277,17 +278,20 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   const bool whole = t_begin == 0 && t_end == len;  // this segment holds all of the request's cache rows
   const size_t part_row = (size_t(worker) + b) * p.hkv + h;
 
-  // This lane's query rows (column n of every row block).
-  int qrow[kRB], head[kRB];
-  bool row_ok[kRB];
-#pragma unroll
-  for (int rb = 0; rb < kRB; ++rb) {
-    const int r = rt * kRows + 16 * rb + n;
-    row_ok[rb] = r < rows;
-    const int tok = row_ok[rb] ? r / p.group : 0;
-    qrow[rb] = begin + tok;
-    head[rb] = h * p.group + (row_ok[rb] ? r - tok * p.group : 0);
-  }
+  // This lane's query row in row block rb (column n): whether there is one, its
+  // row of the query and its head (of the request's first row where there is none).
+  // Worked out where it is needed: held over the loop they cost registers.
+  struct Row {
+    bool ok;
+    int query, head;
+  };
+  auto row_at = [&](int rb) {
+    int r = rt * kRows + 16 * rb + n;
+    asm volatile("" : "+v"(r));
+    const bool ok = r < rows;
+    const int tok = ok ? r / p.group : 0;
+    return Row{ok, begin + tok, h * p.group + (ok ? r - tok * p.group : 0)};
+  };
   const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.bt_stride;
   // Lane i % kGroups looks up 16-row group i of a tile; the entry is loaded a
   // tile ahead of its use.
@@ -311,34 +315,39 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     return int64_t((uint64_t(uint32_t(hi)) << 32) | uint32_t(lo));
   };
 
-  typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
   lk_u32x4 kraw[kKB][kSlices];
   float ks[kKB][4], vs[kKB][4];
   uint32_t vraw[2][8];
   int64_t off_lane = -1;   // group offsets of the tile whose K is in flight
   uint32_t ok_groups = 0;  // its groups that lie in the cache, a bit each
+  // Buffer loads: the 16-row group's address in scalar registers, a 32-bit offset
+  // per lane (64-bit addresses per load were spilled), nothing past the group.
+  const int span = int(15 * rec + uint32_t(kRow));
+  auto group_rows = [&](const uint8_t *cache, int group) {
+    const int64_t off = uniform_offset(off_lane, group);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(cache + (off < 0 ? 0 : off)), 0, span, 0x00027000);
+  };
   auto load_k = [&]() {
 #pragma unroll
     for (int kb = 0; kb < kKB; ++kb) {
-      const int64_t off = uniform_offset(off_lane, wave * kKB + kb);
-      const uint8_t *kp = p.key_cache + (off < 0 ? 0 : off), *vp = p.value_cache + (off < 0 ? 0 : off);
+      const auto kp = group_rows(p.key_cache, wave * kKB + kb), vp = group_rows(p.value_cache, wave * kKB + kb);
 #pragma unroll
-      for (int i = 0; i < kSlices; ++i) kraw[kb][i] = *reinterpret_cast<const u32x4_a4 *>(kp + k_off + 64 * i);
+      for (int i = 0; i < kSlices; ++i)
+        kraw[kb][i] = __builtin_bit_cast(lk_u32x4, __builtin_amdgcn_raw_buffer_load_b128(kp, k_off + 64 * i, 0, 0));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        ks[kb][e] = *reinterpret_cast<const float *>(kp + s_off[e]);
-        vs[kb][e] = *reinterpret_cast<const float *>(vp + s_off[e]);
+        ks[kb][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(kp, s_off[e], 0, 0));
+        vs[kb][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(vp, s_off[e], 0, 0));
       }
     }
   };
   auto load_v = [&]() {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t off = uniform_offset(off_lane, 4 * vgroup + j);
-      const uint8_t *vp = p.value_cache + (off < 0 ? 0 : off);
+      const auto vp = group_rows(p.value_cache, 4 * vgroup + j);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        vraw[j >> 1][4 * (j & 1) + e] = *reinterpret_cast<const uint32_t *>(vp + v_off[e]);
+        vraw[j >> 1][4 * (j & 1) + e] = __builtin_amdgcn_raw_buffer_load_b32(vp, v_off[e], 0, 0);
     }
   };
 
@@ -357,7 +366,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   } else {
 #pragma unroll
     for (int rb = 0; rb < kRB; ++rb) {
-      const uint16_t *q = static_cast<const uint16_t *>(p.query) + (size_t(qrow[rb]) * p.hq + head[rb]) * kD + 16 * g;
+      const Row row = row_at(rb);
+      const uint16_t *q = static_cast<const uint16_t *>(p.query) + (size_t(row.query) * p.hq + row.head) * kD + 16 * g;
 #pragma unroll
       for (int i = 0; i < kQS; ++i) qf[rb][i] = *reinterpret_cast<const lk_u32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1));
     }
@@ -368,6 +378,18 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   ok_groups = uint32_t(__ballot(off_lane >= 0));
   load_k();
   load_v();
+  if (!filled) {  // while the first loads are on their way
+    fill_lookup<kBf16, 64 * kW>(sm.table, reinterpret_cast<uint32_t *>(sm.pt), tid);
+    filled = true;
+  }
+  int64_t xrow[kX ? kRB : 1];  // rows of p.x, or -1
+  if constexpr (kX) {
+#pragma unroll
+    for (int rb = 0; rb < kRB; ++rb) {
+      const Row row = row_at(rb);
+      xrow[rb] = row.ok ? int64_t(row.query) * p.hq + row.head : -1;
+    }
+  }
   lk_f32x4 oacc[kRB][4];
   float m[kRB], l[kRB];
 #pragma unroll
@@ -397,6 +419,47 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     const uint32_t ok_now = ok_groups;
     // Every row of the tile lies in the cache and every query row sees it (uniform).
     const bool full = t0 + kT <= min(ctx, t_end) && (ok_now & ((1u << kGroups) - 1u)) == (1u << kGroups) - 1u;
+    // The rows each query row sees: bit 4 kb + e for cache row 4 g + e of block kb.  All
+    // mask bytes are loaded before one is used (clamped into the row; what is no
+    // draft does not look at its byte).
+    uint32_t seen[kRB];
+#pragma unroll
+    for (int rb = 0; rb < kRB; ++rb) seen[rb] = 0xFFFFFFFFu;
+    if (!full) {
+      const int base = t0 + 16 * wave * kKB + 4 * g;
+      uint32_t byte[kRB][kKB][4];
+      if (p.mask) {  // uniform
+        const int last = int(min(p.mask_stride, int64_t(p.max_len)) - 1);
+#pragma unroll
+        for (int rb = 0; rb < kRB; ++rb) {
+          const uint8_t *mrow = p.mask + size_t(row_at(rb).query) * p.mask_stride;
+#pragma unroll
+          for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) byte[rb][kb][e] = mrow[min(max(base + 16 * kb + e - ctx, 0), last)];
+        }
+      } else {
+#pragma unroll
+        for (int rb = 0; rb < kRB; ++rb)
+#pragma unroll
+          for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) byte[rb][kb][e] = 1;
+      }
+#pragma unroll
+      for (int rb = 0; rb < kRB; ++rb) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = base + 16 * kb + e;
+            const bool vis = bool((ok_now >> (wave * kKB + kb)) & 1u) & (t < t_end) & ((t < ctx) | (byte[rb][kb][e] != 0));
+            bits |= uint32_t(vis) << (4 * kb + e);
+          }
+        seen[rb] = bits;
+      }
+    }
     // S^T of this wavefront's rows.
     lk_f32x4 s[kRB][kKB];
 #pragma unroll
@@ -405,6 +468,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
       for (int rb = 0; rb < kRB; ++rb) s[rb][kb] = lk_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kQS; ++i) {
+        // The lookups of two steps at a time: of all of them at once they would spill.
+        if (!(i & 1)) __builtin_amdgcn_sched_barrier(0);
         const lk_u32x4 w = kraw[kb][i >> 1];
         const lk_u32x4 a = look8<false>(w[2 * (i & 1)], w[2 * (i & 1) + 1], lane4, table);
 #pragma unroll
@@ -432,42 +497,10 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     off_lane = offset_at(t0 + kT, blk);
     ok_groups = uint32_t(__ballot(off_lane >= 0));
     load_k();
-    // Logits (base 2), the rows each query row sees, and the tile's maxima.
-    uint32_t seen[kRB];  // bit 4 kb + e: this query row sees cache row 4 g + e of block kb
+    // Logits (base 2) and the tile's maxima.
     float y[kRB][kKB][4];
 #pragma unroll
     for (int rb = 0; rb < kRB; ++rb) {
-      seen[rb] = 0xFFFFFFFFu;
-      if (!full) {
-        // All mask bytes are loaded before one is used (clamped into the row; what is
-        // no draft does not look at its byte).
-        uint32_t byte[kKB][4];
-        if (p.mask) {  // uniform
-          const uint8_t *mrow = p.mask + size_t(qrow[rb]) * p.mask_stride;
-          const int last = int(min(p.mask_stride, int64_t(p.max_len)) - 1);
-#pragma unroll
-          for (int kb = 0; kb < kKB; ++kb)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              byte[kb][e] = mrow[min(max(t0 + 16 * (wave * kKB + kb) + 4 * g + e - ctx, 0), last)];
-        } else {
-#pragma unroll
-          for (int kb = 0; kb < kKB; ++kb)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) byte[kb][e] = 1;
-        }
-        seen[rb] = 0;
-#pragma unroll
-        for (int kb = 0; kb < kKB; ++kb) {
-          const bool in = (ok_now >> (wave * kKB + kb)) & 1u;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int t = t0 + 16 * (wave * kKB + kb) + 4 * g + e;
-            const bool vis = in & (t < t_end) & ((t < ctx) | (byte[kb][e] != 0));
-            seen[rb] |= uint32_t(vis) << (4 * kb + e);
-          }
-        }
-      }
       float top = -__builtin_inff();
       auto logits = [&](auto all) {
         constexpr bool kAll = decltype(all)::value;
@@ -483,8 +516,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
           }
           if constexpr (kX) {
             const int t = t0 + 16 * (wave * kKB + kb) + 4 * g;
-            if (row_ok[rb] && t < t_end)
-              *reinterpret_cast<lk_f32x4 *>(p.x + (size_t(qrow[rb]) * p.hq + head[rb]) * p.x_stride + t) = x;
+            if (xrow[rb] >= 0 && t < t_end) *reinterpret_cast<lk_f32x4 *>(p.x + xrow[rb] * p.x_stride + t) = x;
           }
         }
       };
@@ -547,8 +579,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
         for (int e = 0; e < 4; ++e) {
           uint32_t &w = vraw[j >> 1][4 * (j & 1) + e];
           const int t = t0 + 64 * vgroup + 16 * j + 4 * g + e;
-          if (!((ok_now >> (4 * vgroup + j)) & 1u) || t >= t_end) w = 0;
-          odd |= t >= ctx && some_not_finite(w);
+          w = bool((ok_now >> (4 * vgroup + j)) & 1u) & (t < t_end) ? w : 0u;
+          odd |= (t >= ctx) & some_not_finite(w);
         }
       if (__any(odd)) {
 #pragma unroll 1
@@ -574,7 +606,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
 #pragma unroll
               for (int rb = 0; rb < kRB; ++rb) {
                 // (t, dim) is element sn % 4 of accumulator `byte` in the lanes of group sn / 4.
-                const bool vis = g == (sn >> 2) && row_ok[rb] && p.mask[size_t(qrow[rb]) * p.mask_stride + (t - ctx)] != 0;
+                const Row row = row_at(rb);
+                const bool vis = g == (sn >> 2) && row.ok && p.mask[size_t(row.query) * p.mask_stride + (t - ctx)] != 0;
                 const uint16_t pb = sm.pt[(16 * rb + n) * kPStride + at];
                 const float add = vis ? ((pb & 0x8000u) ? -v : v) : 0.f;
 #pragma unroll
@@ -599,6 +632,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
         pf[rb] = *reinterpret_cast<const lk_u32x4 *>(sm.pt + (16 * rb + n) * kPStride + 64 * vgroup + 32 * hf + 8 * g);
       auto column = [&](auto byte) {
         constexpr int q = decltype(byte)::value;
+        if (!(q & 1)) __builtin_amdgcn_sched_barrier(0);
         const lk_u32x4 a = look_column<q, true>(vraw[hf], lane4, table);
 #pragma unroll
         for (int rb = 0; rb < kRB; ++rb) oacc[rb][q] = mfma_16x16x32<false>(a, pf[rb], oacc[rb][q]);
@@ -641,7 +675,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   if (vgroup == 0) {
 #pragma unroll
     for (int rb = 0; rb < kRB; ++rb) {
-      if (!row_ok[rb]) continue;
+      const Row row = row_at(rb);
+      if (!row.ok) continue;
       float sum = sm.top[0][16 * rb + n];
 #pragma unroll
       for (int w = 1; w < kW; ++w) sum += sm.top[w][16 * rb + n];
@@ -655,7 +690,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
           w[i] = uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i) & 3][i >> 1] * inv)) |
                  (uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i + 1) & 3][i >> 1] * inv)) << 16);
         lk_u32x4 *o = reinterpret_cast<lk_u32x4 *>(static_cast<uint16_t *>(p.out) +
-                                                   (size_t(qrow[rb]) * p.hq + head[rb]) * kD + dim);
+                                                   (size_t(row.query) * p.hq + row.head) * kD + dim);
         o[0] = lk_u32x4{w[0], w[1], w[2], w[3]};
         o[1] = lk_u32x4{w[4], w[5], w[6], w[7]};
       } else {
@@ -700,17 +735,17 @@ __device__ __forceinline__ Parts parts_of(const RowAttnParams &p, int b, int row
     return Parts{(size_t(row) * p.hq + head) * p.num_splits, 1, (len + p.split_tokens - 1) / p.split_tokens};
   }
   // Tiles lo .. hi - 1 are the request's; worker w of them has floor(total w / workers) on.
-  const int64_t total = p.plan[p.batch], lo = p.plan[b], hi = p.plan[b + 1];
+  const int total = p.plan[p.batch], lo = p.plan[b], hi = p.plan[b + 1];
   const int64_t in_request = int64_t(tok) * p.group + head % p.group;
   if (lo == hi || in_request >= p.rows_cap) return Parts{0, 1, 0};  // nothing seen, or past the longest request told
-  const int64_t workers = min(int64_t(p.workers), total);
+  const int workers = min(p.workers, total);
   int w0, w1;
-  if (total < (int64_t(1) << 22)) {  // workers is at most 512: the division has 32 bits
+  if (total < 1 << 22) {  // workers is at most 512: the division has 32 bits
     w0 = int((uint32_t(lo + 1) * uint32_t(workers) - 1) / uint32_t(total));
     w1 = int((uint32_t(hi) * uint32_t(workers) - 1) / uint32_t(total));
   } else {
-    w0 = int(((lo + 1) * workers - 1) / total);
-    w1 = int((hi * workers - 1) / total);
+    w0 = int((int64_t(lo + 1) * workers - 1) / total);
+    w1 = int((int64_t(hi) * workers - 1) / total);
   }
   return Parts{((size_t(w0) + b) * p.hkv + head / p.group) * p.rows_cap + size_t(in_request), size_t(p.hkv) * p.rows_cap, w1 - w0 + 1};
 }
@@ -868,7 +903,7 @@ RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int6
     return pl;
   }
   const int64_t rows = std::max<int64_t>(max_query, 1) * (heads / hkv);
-  pl.row_blocks = rows <= 16 ? 1 : rows <= 32 || d == 64 ? 2 : 4;
+  pl.row_blocks = rows <= 16 ? 1 : rows <= 32 || d < 256 ? 2 : 4;
   pl.row_tiles = int((rows + 16 * pl.row_blocks - 1) / (16 * pl.row_blocks));
   pl.magic = ((int64_t(1) << 36) + block_size / 16 - 1) / (block_size / 16);
   // A workgroup for each slot that the GPU has: eight wavefronts per CU.
@@ -895,7 +930,7 @@ RowSpace row_space(const RowPlan &pl, int64_t batch, int64_t total_q, int64_t he
   w.o = round(size_t(pl.parts) * dv * sizeof(float));
   w.ml = round(size_t(pl.parts) * 2 * sizeof(float));
   if (weights) w.x = round(size_t(total_q) * heads * size_t(x_stride_of(max_len)) * sizeof(float));
-  if (pl.row_blocks) w.plan = round(size_t(batch + 1) * sizeof(int64_t));
+  if (pl.row_blocks) w.plan = round(size_t(batch + 1) * sizeof(int32_t));
   return w;
 }
 
@@ -911,9 +946,14 @@ size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv,
   return need;
 }
 
+int64_t row_blocks_of(const RowAttnParams &p) {
+  const int64_t outer = p.heads_together ? p.workers : int64_t(p.workers) * p.hkv;
+  return (outer + 7) / 8 * 8 * p.row_tiles * (p.heads_together ? p.hkv : 1);
+}
+
 template <int kD, bool kBf16, int kRB, typename BtT>
 void launch_rows(const RowAttnParams &p, int64_t magic, hipStream_t s) {
-  const unsigned blocks = unsigned((int64_t(p.workers) + 7) / 8 * 8 * p.hkv * p.row_tiles), threads = 64 * waves_of(kRB);
+  const unsigned blocks = unsigned(row_blocks_of(p)), threads = 64 * waves_of(kRB);
   if (p.x) row_attention_mfma<kD, kBf16, kRB, true, BtT><<<blocks, threads, 0, s>>>(p, magic);
   else row_attention_mfma<kD, kBf16, kRB, false, BtT><<<blocks, threads, 0, s>>>(p, magic);
 }
@@ -927,8 +967,8 @@ void launch_row_attention(const RowAttnParams &p, const RowPlan &pl, hipStream_t
   const auto with_dim = [&](auto dim) {
     constexpr int kD = decltype(dim)::value;
     if (pl.row_blocks == 1) launch_rows<kD, kBf16, 1, BtT>(p, pl.magic, s);
-    else if (kD == 64 || pl.row_blocks == 2) launch_rows<kD, kBf16, 2, BtT>(p, pl.magic, s);
-    else launch_rows<kD, kBf16, kD == 64 ? 2 : 4, BtT>(p, pl.magic, s);
+    else if (kD < 256 || pl.row_blocks == 2) launch_rows<kD, kBf16, 2, BtT>(p, pl.magic, s);
+    else launch_rows<kD, kBf16, kD < 256 ? 2 : 4, BtT>(p, pl.magic, s);
   };
   if (p.d == 64) with_dim(std::integral_constant<int, 64>{});
   else if (p.d == 128) with_dim(std::integral_constant<int, 128>{});
@@ -990,6 +1030,8 @@ int row_attention(const char *name, const RowArgs &a) {
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", name);
 
   const bool mfma = mfma_rows(a.d, a.dv, a.block_size, a.max_len) && aligned(a.query, 16) && aligned(a.out, 16);
+  if (mfma && a.batch * (a.max_len / 64 + 1) > 0x7FFFFFFFll / 2)
+    return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
   const RowPlan pl = plan_rows(mfma, a.batch, a.total_q, a.heads, a.hkv, a.d, a.block_size, a.max_query, a.max_len);
   RowAttnParams p{};
   p.query = a.query;
@@ -1028,11 +1070,13 @@ int row_attention(const char *name, const RowArgs &a) {
     p.w_stride = a.w_stride;
   }
   if (mfma) {
-    p.plan = reinterpret_cast<int64_t *>(ws + space.o + space.ml + space.x);
+    p.plan = reinterpret_cast<int32_t *>(ws + space.o + space.ml + space.x);
     p.workers = pl.workers;
+    p.heads_together = pl.workers % 8 == 0;
     p.row_tiles = pl.row_tiles;
     p.rows_cap = pl.row_tiles * 16 * pl.row_blocks;
     p.tile_rows = pl.tile_rows;
+    p.log2_tile_rows = __builtin_ctz(unsigned(pl.tile_rows));
   }
   const int dim_slices = int((a.dv + kSliceDims - 1) / kSliceDims);
   // From 1024 (row, head) pairs on, a wavefront each fills the GPU (192 rows of 16
@@ -1040,7 +1084,7 @@ int row_attention(const char *name, const RowArgs &a) {
   const bool wide = int64_t(rows) >= 1024;
   const int64_t join_blocks = (wide ? (int64_t(rows) + kWaves - 1) / kWaves : int64_t(rows) * dim_slices) +
                               (a.weights ? a.batch * a.hkv * ((a.max_len + kWeightKeys - 1) / kWeightKeys) : 0);
-  const int64_t attn_blocks = mfma ? (int64_t(pl.workers) + 7) / 8 * 8 * a.hkv * pl.row_tiles : int64_t(rows);
+  const int64_t attn_blocks = mfma ? row_blocks_of(p) : int64_t(rows);
   if (std::max(join_blocks, attn_blocks) > 0xFFFFFFFFll / kThreads)  // threads of one launch
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
   hipStream_t s = reinterpret_cast<hipStream_t>(a.stream);
