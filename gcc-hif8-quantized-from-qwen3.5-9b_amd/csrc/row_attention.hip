@@ -123,19 +123,20 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 // cached code is decoded once for all of them.  The tiles of kT = 16384 / D
 // cache rows of all requests, one after the other, are dealt out to the
 // workers in equal runs, so ragged lengths leave none idle; a run that reaches
-// into another request goes on with that one's query rows.  Per tile, with two
-// barriers:
+// into another request goes on with that one's query rows.  Per tile:
 //   * S^T = K Q^T: every wavefront takes a quarter of the tile's rows, loaded
 //     from HBM straight into the MFMA A operand (row = lane % 16, 16 codes per
 //     lane) and decoded in registers; Q is the B operand, held all along;
-//   * the row maxima meet in LDS; P = 2^(x + e - m) in fp16 goes to LDS, where e
+//   * P = 2^(x + e - m) in fp16 goes to LDS, against a maximum m that moves only
+//     when some row outgrows it by 2^6 (then the wavefronts' maxima meet in LDS
+//     and P is written again), so most tiles have one barrier; e
 //     is the exponent of the row's V scale and its mantissa is multiplied in,
 //     so V itself stays the exact dec(code) and no scale is rounded;
 //   * O^T += V^T P^T: every wavefront takes 64 dims of 64 rows (all of the
 //     tile's at D = 256), 4 bytes of 16 rows per lane.
 // The next tile's K loads are issued as soon as S is done, its V loads after O.
 // sum_t P_t 2^-e_t is the softmax sum against the same maximum.
-constexpr float kLazy = 6.f;  // log2 headroom of the maximum: it moves in steps of more than 2^6
+constexpr float kLazy = 6.f;  // log2 headroom of the maximum: P' stays below 2^7, in fp16's range
 
 // Wavefronts of a workgroup: four, two workgroups to a CU; with 64 query rows
 // eight, one workgroup, since the table and the query rows in LDS leave no room
@@ -190,12 +191,15 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   static_assert(kGroups < 32 && kVG * 64 == kT, "a bit per group, 64 rows per wavefront of a slice");
   constexpr int kRows = 16 * kRB;
   constexpr int kPStride = kT + 8;        // fp16 values of a row of P in LDS
+  // Two buffers of P where that leaves room for two workgroups of four wavefronts.
+  constexpr int kBuffers = kW == 8 || kLookupBytes + 4 * kRows * kPStride + 32 * kRows <= 81920 - 1024 ? 2 : 1;
   struct Smem {
     uint32_t table[kLookupBytes / 4];     // at LDS byte 0: a lookup's address needs no addition
-    // P of a tile; at a segment's end the shares of O of wavefronts of one slice.
-    __attribute__((aligned(16))) uint16_t pt[max_of(kRows * kPStride, (kVG - 1) * kSlices * 2048)];
+    // P of a tile and of the next; at a segment's end the shares of O of wavefronts of one slice.
+    __attribute__((aligned(16))) uint16_t pt[max_of(kBuffers * kRows * kPStride, (kVG - 1) * kSlices * 2048)];
     lk_u32x4 q[kQLds ? kRB * kQS * kWave : 1];
     float top[kW][kRows];
+    int grow[2];                          // the last tile (counted from 1) whose maximum moved, by parity
   };
   __shared__ __attribute__((aligned(16))) Smem sm;
   const uint32_t table = lds_address(sm.table);
@@ -230,6 +234,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   int cur = int(int64_t(total) * worker / workers);
   const int run_end = int(int64_t(total) * (worker + 1) / workers);
   bool filled = false;
+  int tile_no = 0;  // tiles done, over all segments
+  if (tid < 2) sm.grow[tid] = 0;
 
   const uint32_t rec = uint32_t(p.hkv) * kRow;
   const int bs16 = p.block_size >> 4;
@@ -497,11 +503,12 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     off_lane = offset_at(t0 + kT, blk);
     ok_groups = uint32_t(__ballot(off_lane >= 0));
     load_k();
-    // Logits (base 2) and the tile's maxima.
-    float y[kRB][kKB][4];
+    // Logits (base 2), each with its V scale's exponent.
+    float y[kRB][kKB][4], top[kRB];
+    bool grow = false;
 #pragma unroll
     for (int rb = 0; rb < kRB; ++rb) {
-      float top = -__builtin_inff();
+      top[rb] = -__builtin_inff();
       auto logits = [&](auto all) {
         constexpr bool kAll = decltype(all)::value;
 #pragma unroll
@@ -512,7 +519,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
             const float z = s[rb][kb][e] * ksc[kb][e];
             x[e] = kAll || ((seen[rb] >> (4 * kb + e)) & 1u) ? z : -__builtin_inff();
             y[rb][kb][e] = x[e] + ve[kb][e];
-            top = fmaxf(top, y[rb][kb][e]);
+            top[rb] = fmaxf(top[rb], y[rb][kb][e]);
           }
           if constexpr (kX) {
             const int t = t0 + 16 * (wave * kKB + kb) + 4 * g;
@@ -522,51 +529,74 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
       };
       if (full) logits(std::true_type{});
       else logits(std::false_type{});
-      top = max_over_groups(top);
-      if (g == 0) sm.top[wave][16 * rb + n] = top;
+      grow |= top[rb] > m[rb] + kLazy;
+    }
+    // P against the maximum as it stands, which it does in most tiles: one barrier.
+    // Where some wavefront's rows outgrew it, all of them meet once more for the
+    // new one and write P again.
+    ++tile_no;
+    uint16_t *pt = sm.pt + (kBuffers == 2 ? (tile_no & 1) * kRows * kPStride : 0);
+    float psum[kRB];
+    auto put = [&]() {
+#pragma unroll
+      for (int rb = 0; rb < kRB; ++rb) {
+        const float ref = m[rb] == -__builtin_inff() ? 0.f : m[rb];
+        psum[rb] = 0.f;
+        auto weights = [&](auto all) {
+          constexpr bool kAll = decltype(all)::value;
+#pragma unroll
+          for (int kb = 0; kb < kKB; ++kb) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float pw = __builtin_amdgcn_exp2f(y[rb][kb][e] - ref);
+              const bool vis = kAll || ((seen[rb] >> (4 * kb + e)) & 1u);
+              const float sum = fmaf(pw, vi[kb][e], psum[rb]);
+              psum[rb] = vis ? sum : psum[rb];
+              w[e] = vis ? pw * vm[kb][e] : 0.f;
+            }
+            const int j = wave * kKB + kb;
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            *reinterpret_cast<u32x2 *>(pt + (16 * rb + n) * kPStride + 32 * (j >> 1) + 8 * g + 4 * (j & 1)) =
+                u32x2{uint32_t(float_to_f16_bits(w[0])) | (uint32_t(float_to_f16_bits(w[1])) << 16),
+                      uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
+          }
+        };
+        if (full) weights(std::true_type{});
+        else weights(std::false_type{});
+      }
+    };
+    if (__any(grow)) {
+      if (lane == 0) sm.grow[tile_no & 1] = tile_no;
+    } else {
+      put();
     }
     lds_barrier();
+    if (sm.grow[tile_no & 1] == tile_no) {  // uniform
 #pragma unroll
-    for (int rb = 0; rb < kRB; ++rb) {
-      float top = sm.top[0][16 * rb + n];
+      for (int rb = 0; rb < kRB; ++rb) {
+        const float t = max_over_groups(top[rb]);
+        if (g == 0) sm.top[wave][16 * rb + n] = t;
+      }
+      lds_barrier();
 #pragma unroll
-      for (int w = 1; w < kW; ++w) top = fmaxf(top, sm.top[w][16 * rb + n]);
-      const bool grow = top > m[rb] + kLazy;
-      if (__any(grow)) {
-        const float next = grow ? top : m[rb];
-        if (!__all(!grow || m[rb] == -__builtin_inff())) {
-          const float alpha = grow ? __builtin_amdgcn_exp2f(m[rb] - next) : 1.f;
+      for (int rb = 0; rb < kRB; ++rb) {
+        float t = sm.top[0][16 * rb + n];
+#pragma unroll
+        for (int w = 1; w < kW; ++w) t = fmaxf(t, sm.top[w][16 * rb + n]);
+        if (t > m[rb] + kLazy) {
+          const float alpha = m[rb] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[rb] - t);
           l[rb] *= alpha;
 #pragma unroll
           for (int q = 0; q < 4; ++q) oacc[rb][q] *= alpha;
+          m[rb] = t;
         }
-        m[rb] = next;
       }
-      const float ref = m[rb] == -__builtin_inff() ? 0.f : m[rb];
-      auto weights = [&](auto all) {
-        constexpr bool kAll = decltype(all)::value;
-#pragma unroll
-        for (int kb = 0; kb < kKB; ++kb) {
-          float w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float pw = __builtin_amdgcn_exp2f(y[rb][kb][e] - ref);
-            const bool vis = kAll || ((seen[rb] >> (4 * kb + e)) & 1u);
-            const float sum = fmaf(pw, vi[kb][e], l[rb]);
-            l[rb] = vis ? sum : l[rb];
-            w[e] = vis ? pw * vm[kb][e] : 0.f;
-          }
-          const int j = wave * kKB + kb;
-          typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-          *reinterpret_cast<u32x2 *>(sm.pt + (16 * rb + n) * kPStride + 32 * (j >> 1) + 8 * g + 4 * (j & 1)) =
-              u32x2{uint32_t(float_to_f16_bits(w[0])) | (uint32_t(float_to_f16_bits(w[1])) << 16),
-                    uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
-        }
-      };
-      if (full) weights(std::true_type{});
-      else weights(std::false_type{});
+      put();
+      lds_barrier();
     }
-    lds_barrier();
+#pragma unroll
+    for (int rb = 0; rb < kRB; ++rb) l[rb] += psum[rb];
     // O^T += V^T P^T: slots 8 g + e of a 32-row step are rows 4 g + e of its
     // first 16, then of its second 16, as P lies in LDS.
     if (!full) {
@@ -608,7 +638,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
                 // (t, dim) is element sn % 4 of accumulator `byte` in the lanes of group sn / 4.
                 const Row row = row_at(rb);
                 const bool vis = g == (sn >> 2) && row.ok && p.mask[size_t(row.query) * p.mask_stride + (t - ctx)] != 0;
-                const uint16_t pb = sm.pt[(16 * rb + n) * kPStride + at];
+                const uint16_t pb = pt[(16 * rb + n) * kPStride + at];
                 const float add = vis ? ((pb & 0x8000u) ? -v : v) : 0.f;
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
@@ -629,7 +659,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
       lk_u32x4 pf[kRB];
 #pragma unroll
       for (int rb = 0; rb < kRB; ++rb)
-        pf[rb] = *reinterpret_cast<const lk_u32x4 *>(sm.pt + (16 * rb + n) * kPStride + 64 * vgroup + 32 * hf + 8 * g);
+        pf[rb] = *reinterpret_cast<const lk_u32x4 *>(pt + (16 * rb + n) * kPStride + 64 * vgroup + 32 * hf + 8 * g);
       auto column = [&](auto byte) {
         constexpr int q = decltype(byte)::value;
         if (!(q & 1)) __builtin_amdgcn_sched_barrier(0);
@@ -643,6 +673,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
       column(std::integral_constant<int, 3>{});
     }
     load_v();
+    if constexpr (kBuffers == 1) lds_barrier();  // the next tile writes P where this one is read
   }
 
   // The wavefronts' shares of the softmax sum, and of O where some share a slice.
