@@ -472,17 +472,25 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     for (int kb = 0; kb < kKB; ++kb) {
 #pragma unroll
       for (int rb = 0; rb < kRB; ++rb) s[rb][kb] = lk_f32x4{0.f, 0.f, 0.f, 0.f};
+      // The lookups (and the query rows) of a step are on their way while the
+      // step before multiplies.  Further ahead they would spill.
+      auto codes = [&](int i) { return look8<false>(kraw[kb][i >> 1][2 * (i & 1)], kraw[kb][i >> 1][2 * (i & 1) + 1], lane4, table); };
+      auto query = [&](int rb, int i) { return kQLds ? sm.q[(rb * kQS + i) * kWave + lane] : qf[kQLds ? 0 : rb][kQLds ? 0 : i]; };
+      lk_u32x4 a = codes(0), q[kRB];
+#pragma unroll
+      for (int rb = 0; rb < kRB; ++rb) q[rb] = query(rb, 0);
 #pragma unroll
       for (int i = 0; i < kQS; ++i) {
-        // The lookups of two steps at a time: of all of them at once they would spill.
-        if (!(i & 1)) __builtin_amdgcn_sched_barrier(0);
-        const lk_u32x4 w = kraw[kb][i >> 1];
-        const lk_u32x4 a = look8<false>(w[2 * (i & 1)], w[2 * (i & 1) + 1], lane4, table);
+        __builtin_amdgcn_sched_barrier(0);
+        lk_u32x4 a_next = a, q_next[kRB];
+        if (i + 1 < kQS) a_next = codes(i + 1);
 #pragma unroll
-        for (int rb = 0; rb < kRB; ++rb) {
-          const lk_u32x4 q = kQLds ? sm.q[(rb * kQS + i) * kWave + lane] : qf[kQLds ? 0 : rb][kQLds ? 0 : i];
-          s[rb][kb] = mfma_16x16x32<kBf16>(a, q, s[rb][kb]);
-        }
+        for (int rb = 0; rb < kRB; ++rb) q_next[rb] = i + 1 < kQS ? query(rb, i + 1) : q[rb];
+#pragma unroll
+        for (int rb = 0; rb < kRB; ++rb) s[rb][kb] = mfma_16x16x32<kBf16>(a, q[rb], s[rb][kb]);
+        a = a_next;
+#pragma unroll
+        for (int rb = 0; rb < kRB; ++rb) q[rb] = q_next[rb];
       }
     }
     float ksc[kKB][4], ve[kKB][4], vm[kKB][4], vi[kKB][4];
@@ -660,12 +668,16 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
 #pragma unroll
       for (int rb = 0; rb < kRB; ++rb)
         pf[rb] = *reinterpret_cast<const lk_u32x4 *>(pt + (16 * rb + n) * kPStride + 64 * vgroup + 32 * hf + 8 * g);
+      // As above: the next byte's lookups are on their way while one multiplies.
+      lk_u32x4 a = look_column<0, true>(vraw[hf], lane4, table);
       auto column = [&](auto byte) {
         constexpr int q = decltype(byte)::value;
-        if (!(q & 1)) __builtin_amdgcn_sched_barrier(0);
-        const lk_u32x4 a = look_column<q, true>(vraw[hf], lane4, table);
+        __builtin_amdgcn_sched_barrier(0);
+        lk_u32x4 next = a;
+        if constexpr (q < 3) next = look_column<q + 1, true>(vraw[hf], lane4, table);
 #pragma unroll
         for (int rb = 0; rb < kRB; ++rb) oacc[rb][q] = mfma_16x16x32<false>(a, pf[rb], oacc[rb][q]);
+        a = next;
       };
       column(std::integral_constant<int, 0>{});
       column(std::integral_constant<int, 1>{});
