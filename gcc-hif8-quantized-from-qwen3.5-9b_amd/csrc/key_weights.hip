@@ -37,13 +37,15 @@ struct WeightParams {
   int64_t w_pad;
   int tok_lo, tok_hi;          // query tokens of this chunk
   int tiles, row_splits, split_rows;
+  int max_query;               // query rows of a request that the launches are sized for
 };
 
 __device__ __forceinline__ int clamp_rows(int n, int most) { return n < 0 ? 0 : (n > most ? most : n); }
 
+// Query rows of request b, clipped to the query tensor and to the longest request told (start_loc is caller data).
 __device__ __forceinline__ void request_rows(const WeightParams &p, int b, int &begin, int &count) {
   begin = max(p.start_loc[b], 0);
-  count = max(min(p.start_loc[b + 1], p.total_q) - begin, 0);
+  count = min(max(min(p.start_loc[b + 1], p.total_q) - begin, 0), p.max_query);
 }
 
 // Rows that query row i of a request with `len` cached rows sees.
@@ -702,6 +704,7 @@ extern "C" int hif8_key_weights(const void *query, int q_dtype, const uint8_t *k
   p.batch = int(batch);
   p.total_q = int(total_query_tokens);
   p.max_len = int(max_seq_len);
+  p.max_query = int(std::min<int64_t>(max_query_len, total_query_tokens));
   p.causal = causal ? 1 : 0;
   p.accumulate = accumulate ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;

@@ -1375,7 +1375,7 @@ at::Tensor Hif8TreeAttention(const at::Tensor &query, const at::Tensor &key_cach
   CheckSameDevice(tree_mask, key_cache.device(), "tree_mask");
   const c10::OptionalDeviceGuard guard(query.device());
   auto out = at::empty({query.size(0), query.size(1), o.dv}, query.options());
-  if (batch == 0 || query.size(0) == 0 || max_query_len == 0) return out;
+  if (batch == 0 || query.size(0) == 0 || max_query_len == 0) return out.zero_();  // rows of no request, if any
   const size_t bytes = hif8_tree_attention_workspace_size(batch, query.size(1), o.kv_heads, o.d, o.dv, o.block_size,
                                                           query.size(0), max_query_len, max_seq_len);
   const auto ws = Workspace(bytes, query);

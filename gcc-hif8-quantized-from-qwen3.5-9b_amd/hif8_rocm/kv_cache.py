@@ -363,6 +363,8 @@ def _as_int32(t: torch.Tensor, device) -> torch.Tensor:
     """``t`` as a contiguous int32 tensor on ``device``; itself where it is one (the usual call: no copy, few checks)."""
     if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
         return t
+    if t.dtype is torch.int64:   # a count past int32 ("all of them") must not wrap
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 

@@ -254,3 +254,8 @@ def test_c_entries_refuse_bad_arguments(lib):
     for kw, text in [({"q": None}, b"null pointer"), ({"w": None}, b"null pointer"), ({"w": _p(2)}, b"4-byte aligned"),
                      ({"hq": 15}, b"divisible"), ({"mq": 0}, b"max_query_len"), ({"stride": 400}, b"shorter"), ({}, b"workspace of")]:
         assert add(**kw) == 1 and text in lib.hif8_last_error(), (kw, lib.hif8_last_error())
+
+
+def test_counts_past_int32_do_not_wrap():
+    t = kv_cache._as_int32(torch.tensor([1 << 40, (1 << 32) + 5, -(1 << 40), 7]), torch.device("cpu"))
+    assert t.dtype == torch.int32 and t.tolist() == [(1 << 31) - 1, (1 << 31) - 1, -(1 << 31), 7]

@@ -629,3 +629,137 @@ def test_prompt_evict_draft_accept_decode(native_ops, device):
     half = 2.0 ** -8 * out[11:12].double().abs() + 2 * torch.from_numpy(e[11:12]).to(device)
     assert ((last.double() - out[11:12].double()).abs() <= half).all()
     assert (w[:, :, keep:keep + 5] > 0).all() and not w[:, :, keep + 5:].any()
+
+
+# ---------------------------------------- many requests, loose bounds, misuse
+
+def _many(count, seed, most=40):
+    g = np.random.default_rng(seed)
+    return [int(x) for x in g.integers(0, most, count)]
+
+
+@pytest.mark.parametrize("hq, hkv, d, drafts", [(16, 4, 256, 4), (8, 8, 64, 3), (16, 4, 256, 17), (6, 2, 20, 2)])
+def test_tree_of_more_requests_than_workers(native_ops, device, hq, hkv, d, drafts):
+    """150 short requests, some of them empty: workers go from one request into the next."""
+    ctx = _many(150, 70)
+    qlens = [min(n, drafts) for n in _many(150, 71, drafts + 2)]
+    ctx[3], qlens[3], ctx[149] = 0, 0, 200
+    _tree(device, ctx, qlens, hq, hkv, d, 16 if d != 20 else 5, seed=72, mask="any")
+
+
+@pytest.mark.parametrize("hq, hkv, d", [(16, 4, 256), (8, 8, 64)])
+def test_decode_weights_of_more_requests_than_workers(native_ops, device, hq, hkv, d):
+    _weighted(device, _many(150, 73), [1] * 150, hq, hkv, d, 16, seed=74)
+
+
+@pytest.mark.parametrize("hq, hkv, d", [(40, 1, 256), (140, 2, 256), (80, 1, 128)])
+def test_decode_weights_of_many_heads_per_kv_head(native_ops, device, hq, hkv, d):
+    _weighted(device, [300, 1, 0, 77], [1] * 4, hq, hkv, d, 32, seed=hq)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_key_weights_of_many_requests(native_ops, device, causal):
+    lens = _many(90, 75)
+    _weighted(device, lens, [min(n, 1 + i % 5) for i, n in enumerate(lens)], 8, 2, 64, 16, causal=causal, seed=76)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_key_weights_under_loose_bounds(native_ops, device, causal):
+    """max_seq_len far above every length: the rows' partial sums are held for 64 query tokens at a time."""
+    from hif8_rocm import kv_cache
+
+    lens, qlens, hq, d, bs, most = [300, 90], [150, 37], 64, 64, 16, 1 << 19
+    kc, _, table = build_cache(device, lens, 1, d, bs, 77)
+    wide = torch.full((2, most // bs), -1, dtype=I32)
+    wide[:, :table.shape[1]] = table
+    q = randn((sum(qlens), hq, d), 78)
+    w = torch.full((2, 1, most), 3.0, device=device)
+    loc = torch.tensor([0, 150, 187], dtype=I32, device=device)
+    for accumulate in (False, True):
+        kv_cache.accumulate_key_weights(q.to(device), kc, wide.to(device), torch.tensor(lens, dtype=I32, device=device), w,
+                                        scale=0.125, query_start_loc=loc, max_query_len=150, max_seq_len=most, causal=causal,
+                                        accumulate=accumulate, validate=False)
+    want, bound = weights_reference(q.double().numpy(), kc.cpu().numpy(), table.numpy(), lens, qlens, 0.125, causal)
+    for b, n in enumerate(lens):
+        _near(w[b, :, :n], 2 * want[b, :, :n], 2 * bound[b, :, :n] + 2.0 ** -23 * want[b, :, :n])
+        assert (w[b, :, n:] == 3).all()
+
+
+@pytest.mark.parametrize("lens, keep", [([16384, 100], 9000), ([20000], 19999), ([32768, 4097, 5], 4096)])
+def test_evict_at_the_edges_of_what_registers_hold(native_ops, device, lens, keep):
+    _evict(device, lens, keep, 1, 20, 64, positions=True, sinks=4, seed=79)
+
+
+def test_evict_keeps_all_rows_for_counts_past_int32(native_ops, device):
+    from hif8_rocm import kv_cache
+
+    kc, vc, table = build_cache(device, [90, 40], 2, 64, 16, 80)
+    w = torch.rand(2, 2, 90, device=device)
+    was = [t.clone() for t in (kc, vc, w)]
+    for keep in (torch.tensor([1 << 40, (1 << 32) + 5]), 1 << 40):
+        new = kv_cache.evict_kv_rows(kc, vc, table.to(device), [90, 40], w, keep)
+        assert new.tolist() == [90, 40] and all(torch.equal(a, b) for a, b in zip(was, (kc, vc, w)))
+
+
+def test_requests_without_rows(native_ops, device):
+    """Nothing but empty requests: outputs of rows that no request has are zeros, stored sums become zero."""
+    from hif8_rocm import kv_cache
+
+    kc, vc, table = build_cache(device, [50, 20], 2, 64, 16, 81)
+    q = randn((3, 4, 64), 82).to(device)
+    loc = torch.zeros(3, dtype=I32, device=device)
+    mask = torch.ones(3, 4, dtype=torch.bool, device=device)
+    out = kv_cache.tree_attention(q, kc, vc, table.to(device), [50, 20], mask, scale=0.1, query_start_loc=loc)
+    assert not out.any()
+    assert kv_cache.tree_attention(q[:0], kc, vc, table.to(device), [50, 20], mask[:0], scale=0.1,
+                                   query_lens=[0, 0]).shape == (0, 4, 64)
+    w = torch.ones(2, 2, 64, device=device)
+    kv_cache.accumulate_key_weights(q[:0], kc, table.to(device), [50, 20], w, scale=0.1, query_lens=[0, 0])
+    assert (w == 1).all()
+    kv_cache.accumulate_key_weights(q[:0], kc, table.to(device), [50, 20], w, scale=0.1, query_lens=[0, 0], accumulate=False)
+    assert not w[0, :, :50].any() and not w[1, :, :20].any() and (w[0, :, 50:] == 1).all() and (w[1, :, 20:] == 1).all()
+
+
+def test_a_longest_request_told_too_short_stays_in_bounds(native_ops, device):
+    """Without validation: a request longer than max_query_len leaves the other one's results as they are."""
+    from hif8_rocm import kv_cache
+
+    for hq, hkv, d, bs in ((16, 4, 256, 128), (6, 2, 20, 12)):
+        lens, qlens = [330, 400], [5, 200]
+        kc, vc, table = build_cache(device, lens, hkv, d, bs, 83)
+        q = randn((205, hq, d), 84).to(device)
+        mask = torch.from_numpy(_tree_mask([205], 85)[:, :6].copy()).to(device)
+        loc = torch.tensor([0, 5, 205], dtype=I32, device=device)
+        dt = table.to(device)
+        args = dict(scale=0.1, query_start_loc=loc, max_query_len=5, max_seq_len=400, validate=False)
+        ctx = torch.tensor([325, 200], dtype=I32, device=device)
+        out = kv_cache.tree_attention(q, kc, vc, dt, ctx, mask, **args)
+        alone = kv_cache.tree_attention(q[:5], kc, vc, dt[:1], [325], mask[:5], scale=0.1, query_lens=[5])
+        # Each is rounded once (2^-8) and its weights once (2^-11 of sum p |V|, below two here).
+        assert torch.allclose(out[:5].float(), alone.float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+        w = torch.zeros(2, hkv, 400, device=device)
+        kv_cache.accumulate_key_weights(q, kc, dt, torch.tensor(lens, dtype=I32, device=device), w, **args)
+        want, bound = weights_reference(q[:5].double().cpu().numpy(), kc.cpu().numpy(), table.numpy()[:1], lens[:1], [5], 0.1)
+        _near(w[:1, :, :330], want, bound)
+        assert not w[0, :, 330:].any()
+
+
+def test_two_calls_at_once(native_ops, device):
+    """The same operators on two streams at a time, each on its own outputs."""
+    states = [_step_buffers(device, 90), _step_buffers(device, 91)]
+    want = []
+    for i in (0, 1):
+        s = _step_buffers(device, 90 + i)
+        want.append((_step(s), s))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for i in (0, 1):
+        with torch.cuda.stream(streams[i]):
+            got[i] = _step(states[i])
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for a, b in zip(got[i], want[i][0]):
+            assert torch.equal(a, b)
+        for k in ("kc", "vc", "w", "pos"):
+            assert torch.equal(states[i][k], want[i][1][k]), k
