@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 //     tile's at D = 256), 4 bytes of 16 rows per lane.
 // The next tile's K loads are issued as soon as S is done, its V loads after O.
 // sum_t P_t 2^-e_t is the softmax sum against the same maximum.
-constexpr float kLazy = 6.f;  // log2 headroom of the maximum: P' stays below 2^7, in fp16's range
+constexpr float kLazy = 14.f;  // log2 headroom of the maximum: P' stays below 2^15, in fp16's range
 
 // Wavefronts of a workgroup: four, two workgroups to a CU; with 64 query rows
 // eight, one workgroup, since the table and the query rows in LDS leave no room
@@ -178,7 +178,7 @@ __device__ __forceinline__ void split_scale(float s, float &e, float &mant, floa
 
 template <int kD, bool kBf16, int kRB, bool kX, typename BtT>
 __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(const RowAttnParams p,
-                                                                            const int64_t page_magic) {
+                                                                            const uint32_t page_magic) {
   constexpr int kW = waves_of(kRB);       // wavefronts
   constexpr bool kQLds = kRB > 2;         // the query rows lie in LDS, in operand order, instead of registers
   constexpr int kRow = kD + 4;
@@ -304,15 +304,16 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   auto group_of = [&](int t0) { return min(t0 + 16 * (lane & (kGroups - 1)), t_end - 1) >> 4; };
   auto block_at = [&](int t0) {
     const int gr = group_of(t0);
-    return bt[int((uint64_t(gr) * uint64_t(page_magic)) >> 36)];  // not widened here: that would wait for it
+    return bt[__umulhi(2u * uint32_t(gr), page_magic)];  // not widened here: that would wait for it
   };
   // Byte offset of the group's first row of this KV head, or -1.
+  const uint32_t page_bytes = uint32_t(p.block_size) * rec;
   auto offset_at = [&](int t0, BtT entry) {
     const int64_t blk = int64_t(entry);
-    const int gr = group_of(t0);
-    const int in16 = gr - int((uint64_t(gr) * uint64_t(page_magic)) >> 36) * bs16;
+    const uint32_t gr = uint32_t(group_of(t0));
+    const uint32_t in16 = gr - __umulhi(2u * gr, page_magic) * uint32_t(bs16);
     return blk >= 0 && blk < p.num_blocks && t0 + 16 * (lane & (kGroups - 1)) < t_end
-               ? (blk * p.block_size + 16 * in16) * int64_t(rec) + int64_t(h) * kRow
+               ? int64_t(uint64_t(uint32_t(blk)) * page_bytes + (16u * in16 * rec + uint32_t(h * kRow)))
                : int64_t(-1);
   };
   auto uniform_offset = [&](int64_t off, int group) {
@@ -420,6 +421,22 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
       for (int i = 0; i < kQS; ++i) asm volatile("" : "+v"(qf[rb][i]));
   }
 
+  // f(no row is masked, row block) for every row block: one copy for all of them,
+  // whose latencies overlap, where the registers last for it.
+  auto rows_with = [](bool full, auto f) __attribute__((always_inline)) {
+    constexpr bool kTogether = kRB * kKB * (kX ? 2 : 1) <= 4;
+    if (kTogether && full) {
+#pragma unroll
+      for (int rb = 0; rb < kRB; ++rb) f(std::true_type{}, rb);
+      return;
+    }
+#pragma unroll
+    for (int rb = 0; rb < kRB; ++rb) {
+      if (!kTogether && full) f(std::true_type{}, rb);
+      else f(std::false_type{}, rb);
+    }
+  };
+
   for (int it = 0; it < ntiles; ++it) {
     const int t0 = t_begin + it * kT;
     const uint32_t ok_now = ok_groups;
@@ -514,66 +531,56 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     // Logits (base 2), each with its V scale's exponent.
     float y[kRB][kKB][4], top[kRB];
     bool grow = false;
-#pragma unroll
-    for (int rb = 0; rb < kRB; ++rb) {
+    auto logits = [&](auto all, int rb) __attribute__((always_inline)) {
+      constexpr bool kAll = decltype(all)::value;
       top[rb] = -__builtin_inff();
-      auto logits = [&](auto all) {
-        constexpr bool kAll = decltype(all)::value;
 #pragma unroll
-        for (int kb = 0; kb < kKB; ++kb) {
-          lk_f32x4 x;
+      for (int kb = 0; kb < kKB; ++kb) {
+        lk_f32x4 x;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float z = s[rb][kb][e] * ksc[kb][e];
-            x[e] = kAll || ((seen[rb] >> (4 * kb + e)) & 1u) ? z : -__builtin_inff();
-            y[rb][kb][e] = x[e] + ve[kb][e];
-            top[rb] = fmaxf(top[rb], y[rb][kb][e]);
-          }
-          if constexpr (kX) {
-            const int t = t0 + 16 * (wave * kKB + kb) + 4 * g;
-            if (xrow[rb] >= 0 && t < t_end) *reinterpret_cast<lk_f32x4 *>(p.x + xrow[rb] * p.x_stride + t) = x;
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float z = s[rb][kb][e] * ksc[kb][e];
+          x[e] = kAll || ((seen[rb] >> (4 * kb + e)) & 1u) ? z : -__builtin_inff();
+          y[rb][kb][e] = x[e] + ve[kb][e];
+          top[rb] = fmaxf(top[rb], y[rb][kb][e]);
         }
-      };
-      if (full) logits(std::true_type{});
-      else logits(std::false_type{});
+        if constexpr (kX) {
+          const int t = t0 + 16 * (wave * kKB + kb) + 4 * g;
+          if (xrow[rb] >= 0 && t < t_end) *reinterpret_cast<lk_f32x4 *>(p.x + xrow[rb] * p.x_stride + t) = x;
+        }
+      }
       grow |= top[rb] > m[rb] + kLazy;
-    }
+    };
+    rows_with(full, logits);
     // P against the maximum as it stands, which it does in most tiles: one barrier.
     // Where some wavefront's rows outgrew it, all of them meet once more for the
     // new one and write P again.
     ++tile_no;
     uint16_t *pt = sm.pt + (kBuffers == 2 ? (tile_no & 1) * kRows * kPStride : 0);
     float psum[kRB];
-    auto put = [&]() {
+    auto weights = [&](auto all, int rb) __attribute__((always_inline)) {
+      constexpr bool kAll = decltype(all)::value;
+      const float ref = m[rb] == -__builtin_inff() ? 0.f : m[rb];
+      psum[rb] = 0.f;
 #pragma unroll
-      for (int rb = 0; rb < kRB; ++rb) {
-        const float ref = m[rb] == -__builtin_inff() ? 0.f : m[rb];
-        psum[rb] = 0.f;
-        auto weights = [&](auto all) {
-          constexpr bool kAll = decltype(all)::value;
+      for (int kb = 0; kb < kKB; ++kb) {
+        float w[4];
 #pragma unroll
-          for (int kb = 0; kb < kKB; ++kb) {
-            float w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float pw = __builtin_amdgcn_exp2f(y[rb][kb][e] - ref);
-              const bool vis = kAll || ((seen[rb] >> (4 * kb + e)) & 1u);
-              const float sum = fmaf(pw, vi[kb][e], psum[rb]);
-              psum[rb] = vis ? sum : psum[rb];
-              w[e] = vis ? pw * vm[kb][e] : 0.f;
-            }
-            const int j = wave * kKB + kb;
-            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-            *reinterpret_cast<u32x2 *>(pt + (16 * rb + n) * kPStride + 32 * (j >> 1) + 8 * g + 4 * (j & 1)) =
-                u32x2{uint32_t(float_to_f16_bits(w[0])) | (uint32_t(float_to_f16_bits(w[1])) << 16),
-                      uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
-          }
-        };
-        if (full) weights(std::true_type{});
-        else weights(std::false_type{});
+        for (int e = 0; e < 4; ++e) {
+          const float pw = __builtin_amdgcn_exp2f(y[rb][kb][e] - ref);
+          const bool vis = kAll || ((seen[rb] >> (4 * kb + e)) & 1u);
+          const float sum = fmaf(pw, vi[kb][e], psum[rb]);
+          psum[rb] = vis ? sum : psum[rb];
+          w[e] = vis ? pw * vm[kb][e] : 0.f;
+        }
+        const int j = wave * kKB + kb;
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        *reinterpret_cast<u32x2 *>(pt + (16 * rb + n) * kPStride + 32 * (j >> 1) + 8 * g + 4 * (j & 1)) =
+            u32x2{uint32_t(float_to_f16_bits(w[0])) | (uint32_t(float_to_f16_bits(w[1])) << 16),
+                  uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
       }
     };
+    auto put = [&]() __attribute__((always_inline)) { rows_with(full, weights); };
     if (__any(grow)) {
       if (lane == 0) sm.grow[tile_no & 1] = tile_no;
     } else {
@@ -922,13 +929,15 @@ struct RowPlan {
   int split_tokens, num_splits;              // any-shape kernel
   int row_blocks, row_tiles, workers, tile_rows;  // matrix cores: 16-row blocks of a workgroup (0: any-shape kernel)
   int64_t parts;                             // partial results: rows of part_o and part_ml
-  int64_t magic;
+  uint32_t magic;                            // ceil(2^31 / 16-row groups of a page)
 };
 
 // The matrix-core kernel's shapes; the query's and output's alignment comes on top.
-bool mfma_rows(int64_t d, int64_t dv, int64_t block_size, int64_t max_len) {
-  return (d == 64 || d == 128 || d == 256) && dv == d && block_size % 16 == 0 &&
-         (max_len / 16 + 1) * (block_size / 16) < (int64_t(1) << 36) && block_size / 16 < (int64_t(1) << 20);
+// Row groups and the bytes of a page have 31 bits there (a page of 2 GiB goes to the other kernel).
+bool mfma_rows(int64_t d, int64_t dv, int64_t hkv, int64_t block_size, int64_t max_len) {
+  return (d == 64 || d == 128 || d == 256) && dv == d && block_size % 16 == 0 && block_size / 16 < (int64_t(1) << 20) &&
+         (max_len / 16 + 1) * (block_size / 16) < (int64_t(1) << 31) &&
+         block_size * hkv * (d + 4) < (int64_t(1) << 31);
 }
 
 RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int64_t hkv, int64_t d, int64_t block_size,
@@ -948,7 +957,7 @@ RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int6
   const int64_t rows = std::max<int64_t>(max_query, 1) * (heads / hkv);
   pl.row_blocks = rows <= 16 ? 1 : rows <= 32 || d < 256 ? 2 : 4;
   pl.row_tiles = int((rows + 16 * pl.row_blocks - 1) / (16 * pl.row_blocks));
-  pl.magic = ((int64_t(1) << 36) + block_size / 16 - 1) / (block_size / 16);
+  pl.magic = uint32_t(((int64_t(1) << 31) + block_size / 16 - 1) / (block_size / 16));
   // A workgroup for each slot that the GPU has: eight wavefronts per CU.
   pl.tile_rows = int(4096 / d * waves_of(pl.row_blocks));
   const int64_t tiles = batch * ((len + pl.tile_rows - 1) / pl.tile_rows);
@@ -982,7 +991,7 @@ size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv,
                      int64_t block_size, int64_t max_query, int64_t max_len, bool weights) {
   size_t need = 0;
   for (const bool mfma : {false, true}) {
-    if (mfma && !mfma_rows(d, dv, block_size, max_len)) continue;
+    if (mfma && !mfma_rows(d, dv, hkv, block_size, max_len)) continue;
     const RowPlan pl = plan_rows(mfma, batch, total_q, heads, hkv, d, block_size, max_query, max_len);
     need = std::max(need, row_space(pl, batch, total_q, heads, dv, max_len, weights).total());
   }
@@ -995,7 +1004,7 @@ int64_t row_blocks_of(const RowAttnParams &p) {
 }
 
 template <int kD, bool kBf16, int kRB, typename BtT>
-void launch_rows(const RowAttnParams &p, int64_t magic, hipStream_t s) {
+void launch_rows(const RowAttnParams &p, uint32_t magic, hipStream_t s) {
   const unsigned blocks = unsigned(row_blocks_of(p)), threads = 64 * waves_of(kRB);
   if (p.x) row_attention_mfma<kD, kBf16, kRB, true, BtT><<<blocks, threads, 0, s>>>(p, magic);
   else row_attention_mfma<kD, kBf16, kRB, false, BtT><<<blocks, threads, 0, s>>>(p, magic);
@@ -1072,7 +1081,7 @@ int row_attention(const char *name, const RowArgs &a) {
   if (!aligned(a.workspace, 16))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", name);
 
-  const bool mfma = mfma_rows(a.d, a.dv, a.block_size, a.max_len) && aligned(a.query, 16) && aligned(a.out, 16);
+  const bool mfma = mfma_rows(a.d, a.dv, a.hkv, a.block_size, a.max_len) && aligned(a.query, 16) && aligned(a.out, 16);
   if (mfma && a.batch * (a.max_len / 64 + 1) > 0x7FFFFFFFll / 2)
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
   const RowPlan pl = plan_rows(mfma, a.batch, a.total_q, a.heads, a.hkv, a.d, a.block_size, a.max_query, a.max_len);
