@@ -30,8 +30,9 @@ struct RowAttnParams {
   int64_t bt_stride, num_blocks, mask_stride, x_stride, w_stride;
   int block_size, hkv, hq, group, d, dv, batch, total_q, max_len, num_splits, split_tokens, accumulate;
   // Matrix cores: workers that share the tiles, row tiles of the longest request,
-  // query rows of all of them (a KV head's), cache rows of a tile.
-  int workers, row_tiles, rows_cap, tile_rows, log2_tile_rows, heads_together;
+  // query rows of all of them (a KV head's), ceil(2^31 / group).
+  int workers, row_tiles, rows_cap, heads_together;
+  uint32_t group_magic;
   float scale_log2;            // softmax scale * log2(e)
 };
 

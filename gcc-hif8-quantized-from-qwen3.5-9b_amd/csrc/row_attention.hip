@@ -144,14 +144,6 @@ constexpr float kLazy = 14.f;  // log2 headroom of the maximum: P' stays below 2
 constexpr int waves_of(int row_blocks) { return row_blocks > 2 ? 8 : 4; }
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
 
-// Tiles of request b.
-__device__ __forceinline__ int tiles_of(const RowAttnParams &p, int b) {
-  int begin, count;
-  request_rows(p, b, begin, count);
-  return int((uint32_t(rows_seen(p, clamp_rows(p.lens[b], p.max_len), count)) + uint32_t(p.tile_rows) - 1) >>
-             p.log2_tile_rows);
-}
-
 // Inclusive sum over the lanes of a wavefront.
 __device__ __forceinline__ int wave_prefix(int v) {
   const int lane = threadIdx.x & 63;
@@ -209,30 +201,70 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   const int n = lane & 15, g = lane >> 4;
   const uint32_t lane4 = uint32_t(4 * lane);
   // The row tiles of one (worker, KV head) read the same cache rows: their blocks
-  // are equal modulo 8, on one XCD.  So are all of a worker's KV heads, whose rows
-  // share cache lines, where that spreads the workers evenly.
-  const int inner = p.heads_together ? p.hkv * p.row_tiles : p.row_tiles;
-  const int xcd = int(blockIdx.x) & 7, slot = int(blockIdx.x) >> 3;
-  const int outer = (slot / inner) * 8 + xcd, rest = slot % inner;
-  const int worker = p.heads_together ? outer : outer / p.hkv;
+  // are equal modulo 8 (the grid's x), on one XCD.  So are all of a worker's KV
+  // heads, whose rows share cache lines, where that spreads the workers evenly.
+  const int outer = int(blockIdx.z) * 8 + int(blockIdx.x), rest = int(blockIdx.y);
+  int worker = outer, rt = rest, h = 0;
+  if (p.heads_together) {
+    if (p.row_tiles == 1) rt = 0, h = rest;
+    else h = rest / p.row_tiles, rt = rest - h * p.row_tiles;
+  } else {
+    worker = outer / p.hkv;
+    h = outer - worker * p.hkv;
+  }
   if (worker >= p.workers) return;  // padding block (uniform)
-  const int rt = rest % p.row_tiles, h = p.heads_together ? rest / p.row_tiles : outer % p.hkv;
   // This worker's run of the requests' tiles, and the running total per request
   // (kept for the join by the first workgroup).  incl: of the first 64 requests.
+  struct Request {
+    int begin, count, ctx;
+  };
+  auto request = [&](int i) {
+    Request r;
+    request_rows(p, i, r.begin, r.count);
+    r.ctx = clamp_rows(p.lens[i], p.max_len);
+    return r;
+  };
+  auto tiles_of = [&](const Request &r) {
+    return int((uint32_t(rows_seen(p, r.ctx, r.count)) + uint32_t(kT) - 1) / kT);
+  };
   int total = 0, incl = 0;
+  Request early{};  // lane i: request i
   for (int base = 0; base < p.batch; base += kWave) {
     const int i = base + lane;
-    const int mine = i < p.batch ? tiles_of(p, i) : 0;
+    const Request r = request(min(i, p.batch - 1));
+    const int mine = i < p.batch ? tiles_of(r) : 0;
     const int upto = wave_prefix(mine);
-    if (base == 0) incl = upto;
+    if (base == 0) {
+      incl = upto;
+      early = r;
+    }
     if (worker == 0 && rt == 0 && h == 0 && wave == 0 && i < p.batch) p.plan[i] = total + upto - mine;
     total += __builtin_amdgcn_readlane(upto, kWave - 1);
   }
   if (worker == 0 && rt == 0 && h == 0 && tid == 0) p.plan[p.batch] = total;
   const int workers = min(p.workers, total);  // a tile each at least: no part is left unwritten
   if (worker >= workers) return;              // uniform
-  int cur = int(int64_t(total) * worker / workers);
-  const int run_end = int(int64_t(total) * (worker + 1) / workers);
+  int cur, run_end;
+  if (total < 1 << 22) {  // workers is at most 512: the divisions have 32 bits
+    cur = int(uint32_t(total) * uint32_t(worker) / uint32_t(workers));
+    run_end = int(uint32_t(total) * uint32_t(worker + 1) / uint32_t(workers));
+  } else {
+    cur = int(int64_t(total) * worker / workers);
+    run_end = int(int64_t(total) * (worker + 1) / workers);
+  }
+  // The request of tile `cur`.  The first one's numbers are in some lane already.
+  int b = 0, first = 0;
+  auto among_early = [&]() {
+    b = __builtin_ctzll(__ballot(incl > cur));
+    first = b ? __builtin_amdgcn_readlane(incl, b - 1) : 0;
+  };
+  Request now{};
+  bool known = p.batch <= kWave;
+  if (known) {
+    among_early();
+    now = Request{__builtin_amdgcn_readlane(early.begin, b), __builtin_amdgcn_readlane(early.count, b),
+                  __builtin_amdgcn_readlane(early.ctx, b)};
+  }
   bool filled = false;
   int tile_no = 0;  // tiles done, over all segments
   if (tid < 2) sm.grow[tid] = 0;
@@ -249,31 +281,32 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   }
 
   while (cur < run_end) {
-  // The request of tile `cur` (uniform), and this segment's tiles of it.
-  int b = 0, first = 0;
-  if (p.batch <= kWave) {
-    b = __builtin_ctzll(__ballot(incl > cur));
-    first = b ? __builtin_amdgcn_readlane(incl, b - 1) : 0;
-  } else {
-    int before = 0;
-    for (int base = 0; base < p.batch; base += kWave) {
-      const int i = base + lane;
-      const int upto = before + wave_prefix(i < p.batch ? tiles_of(p, i) : 0);
-      const uint64_t past = __ballot(upto > cur);
-      if (past) {
-        const int at = __builtin_ctzll(past);
-        b = base + at;
-        first = at ? __builtin_amdgcn_readlane(upto, at - 1) : before;
-        break;
+  // This segment: the run's tiles of one request (uniform).
+  if (!known) {
+    if (p.batch <= kWave) {
+      among_early();
+    } else {
+      int before = 0;
+      for (int base = 0; base < p.batch; base += kWave) {
+        const int i = base + lane;
+        const int upto = before + wave_prefix(i < p.batch ? tiles_of(request(i)) : 0);
+        const uint64_t past = __ballot(upto > cur);
+        if (past) {
+          const int at = __builtin_ctzll(past);
+          b = base + at;
+          first = at ? __builtin_amdgcn_readlane(upto, at - 1) : before;
+          break;
+        }
+        before = __builtin_amdgcn_readlane(upto, kWave - 1);
       }
-      before = __builtin_amdgcn_readlane(upto, kWave - 1);
     }
+    b = __builtin_amdgcn_readfirstlane(b);
+    now = request(b);
   }
-  b = __builtin_amdgcn_readfirstlane(b);
-  int begin, count;
-  request_rows(p, b, begin, count);
+  known = false;
+  const int begin = now.begin, count = now.count;
   const int rows = count * p.group;
-  const int ctx = clamp_rows(p.lens[b], p.max_len);
+  const int ctx = now.ctx;
   const int len = rows_seen(p, ctx, count);
   const int tile_first = cur - first;
   const int seg_tiles = min(run_end - cur, int((uint32_t(len) + kT - 1) / kT) - tile_first);
@@ -284,6 +317,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   const bool whole = t_begin == 0 && t_end == len;  // this segment holds all of the request's cache rows
   const size_t part_row = (size_t(worker) + b) * p.hkv + h;
 
+  // The query token of row r: r / group.
+  auto token_of = [&](int r) { return int(__umulhi(2u * uint32_t(r), p.group_magic)); };
   // This lane's query row in row block rb (column n): whether there is one, its
   // row of the query and its head (of the request's first row where there is none).
   // Worked out where it is needed: held over the loop they cost registers.
@@ -295,7 +330,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     int r = rt * kRows + 16 * rb + n;
     asm volatile("" : "+v"(r));
     const bool ok = r < rows;
-    const int tok = ok ? r / p.group : 0;
+    const int tok = ok ? token_of(r) : 0;
     return Row{ok, begin + tok, h * p.group + (ok ? r - tok * p.group : 0)};
   };
   const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.bt_stride;
@@ -365,7 +400,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
 #pragma unroll
     for (int j = 0; j < kRB * kQS / kW; ++j) {
       const int f = wave * (kRB * kQS / kW) + j, i = f % kQS;
-      const int r = min(rt * kRows + 16 * (f / kQS) + n, rows - 1), tok = r / p.group;
+      const int r = min(rt * kRows + 16 * (f / kQS) + n, rows - 1), tok = token_of(r);
       const uint16_t *q = static_cast<const uint16_t *>(p.query) +
                           (size_t(begin + tok) * p.hq + h * p.group + (r - tok * p.group)) * kD + 16 * g;
       qf[0][j] = *reinterpret_cast<const lk_u32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1));
@@ -998,14 +1033,16 @@ size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv,
   return need;
 }
 
-int64_t row_blocks_of(const RowAttnParams &p) {
-  const int64_t outer = p.heads_together ? p.workers : int64_t(p.workers) * p.hkv;
-  return (outer + 7) / 8 * 8 * p.row_tiles * (p.heads_together ? p.hkv : 1);
+// x: XCDs; y: blocks that share a worker's cache rows; z: the workers (by KV head) in eights.
+dim3 row_grid(const RowAttnParams &p) {
+  const int outer = p.heads_together ? p.workers : p.workers * p.hkv;
+  return dim3(8, unsigned(p.row_tiles * (p.heads_together ? p.hkv : 1)), unsigned((outer + 7) / 8));
 }
 
 template <int kD, bool kBf16, int kRB, typename BtT>
 void launch_rows(const RowAttnParams &p, uint32_t magic, hipStream_t s) {
-  const unsigned blocks = unsigned(row_blocks_of(p)), threads = 64 * waves_of(kRB);
+  const unsigned threads = 64 * waves_of(kRB);
+  const dim3 blocks = row_grid(p);
   if (p.x) row_attention_mfma<kD, kBf16, kRB, true, BtT><<<blocks, threads, 0, s>>>(p, magic);
   else row_attention_mfma<kD, kBf16, kRB, false, BtT><<<blocks, threads, 0, s>>>(p, magic);
 }
@@ -1081,7 +1118,9 @@ int row_attention(const char *name, const RowArgs &a) {
   if (!aligned(a.workspace, 16))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", name);
 
-  const bool mfma = mfma_rows(a.d, a.dv, a.hkv, a.block_size, a.max_len) && aligned(a.query, 16) && aligned(a.out, 16);
+  const int64_t group = a.heads / a.hkv, longest = std::max<int64_t>(a.max_query, 1);
+  const bool mfma = mfma_rows(a.d, a.dv, a.hkv, a.block_size, a.max_len) && aligned(a.query, 16) && aligned(a.out, 16) &&
+                    longest * group < 0xFFFF * 16 && (longest * group + 64) * group < (int64_t(1) << 31);  // the grid's y, token_of
   if (mfma && a.batch * (a.max_len / 64 + 1) > 0x7FFFFFFFll / 2)
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
   const RowPlan pl = plan_rows(mfma, a.batch, a.total_q, a.heads, a.hkv, a.d, a.block_size, a.max_query, a.max_len);
@@ -1127,8 +1166,7 @@ int row_attention(const char *name, const RowArgs &a) {
     p.heads_together = pl.workers % 8 == 0;
     p.row_tiles = pl.row_tiles;
     p.rows_cap = pl.row_tiles * 16 * pl.row_blocks;
-    p.tile_rows = pl.tile_rows;
-    p.log2_tile_rows = __builtin_ctz(unsigned(pl.tile_rows));
+    p.group_magic = uint32_t(((int64_t(1) << 31) + p.group - 1) / p.group);
   }
   const int dim_slices = int((a.dv + kSliceDims - 1) / kSliceDims);
   // From 1024 (row, head) pairs on, a wavefront each fills the GPU (192 rows of 16
@@ -1136,8 +1174,7 @@ int row_attention(const char *name, const RowArgs &a) {
   const bool wide = int64_t(rows) >= 1024;
   const int64_t join_blocks = (wide ? (int64_t(rows) + kWaves - 1) / kWaves : int64_t(rows) * dim_slices) +
                               (a.weights ? a.batch * a.hkv * ((a.max_len + kWeightKeys - 1) / kWeightKeys) : 0);
-  const int64_t attn_blocks = mfma ? row_blocks_of(p) : int64_t(rows);
-  if (std::max(join_blocks, attn_blocks) > 0xFFFFFFFFll / kThreads)  // threads of one launch
+  if (std::max(join_blocks, int64_t(rows)) > 0xFFFFFFFFll / kThreads)  // threads of one launch
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
   hipStream_t s = reinterpret_cast<hipStream_t>(a.stream);
   const bool bf16 = a.q_dtype == HIF8_DTYPE_BF16, i64 = a.bt_dtype == HIF8_INDEX_INT64;
