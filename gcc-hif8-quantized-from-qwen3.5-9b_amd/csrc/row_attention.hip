@@ -143,6 +143,8 @@ constexpr float kLazy = 14.f;  // log2 headroom of the maximum: P' stays below 2
 // for two and the registers of four none for the rows.
 constexpr int waves_of(int row_blocks) { return row_blocks > 2 ? 8 : 4; }
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
+// Cache rows of a tile.
+constexpr int tile_rows_of(int d, int row_blocks) { return row_blocks > 2 ? 128 : 16384 / d; }
 
 // Inclusive sum over the lanes of a wavefront.
 __device__ __forceinline__ int wave_prefix(int v) {
@@ -174,13 +176,14 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   constexpr int kW = waves_of(kRB);       // wavefronts
   constexpr bool kQLds = kRB > 2;         // the query rows lie in LDS, in operand order, instead of registers
   constexpr int kRow = kD + 4;
-  constexpr int kT = 4096 / kD * kW;      // cache rows of a tile
-  constexpr int kKB = 256 / kD;           // 16-row blocks of a wavefront in S
+  constexpr int kT = tile_rows_of(kD, kRB);  // cache rows of a tile
+  constexpr int kKB = kT / 16 / kW;       // 16-row blocks of a wavefront in S
   constexpr int kQS = kD / 32;            // MFMA steps over the head dims
   constexpr int kSlices = kD / 64;        // 64-dim slices of V
-  constexpr int kVG = kW / kSlices;       // wavefronts that share a slice, 64 rows of the tile each
+  constexpr int kVG = kW / kSlices;       // wavefronts that share a slice, kVR rows of the tile each
+  constexpr int kVR = kT / kVG;
   constexpr int kGroups = kT / 16;        // 16-row groups of a tile
-  static_assert(kGroups < 32 && kVG * 64 == kT, "a bit per group, 64 rows per wavefront of a slice");
+  static_assert(kGroups < 32 && kVR % 32 == 0 && kKB * kW * 16 == kT, "a bit per group, whole MFMA steps");
   constexpr int kRows = 16 * kRB;
   constexpr int kPStride = kT + 8;        // fp16 values of a row of P in LDS
   // Two buffers of P where that leaves room for two workgroups of four wavefronts.
@@ -359,7 +362,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
 
   lk_u32x4 kraw[kKB][kSlices];
   float ks[kKB][4], vs[kKB][4];
-  uint32_t vraw[2][8];
+  uint32_t vraw[kVR / 32][8];
   int64_t off_lane = -1;   // group offsets of the tile whose K is in flight
   uint32_t ok_groups = 0;  // its groups that lie in the cache, a bit each
   // Buffer loads: the 16-row group's address in scalar registers, a 32-bit offset
@@ -385,8 +388,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   };
   auto load_v = [&]() {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const auto vp = group_rows(p.value_cache, 4 * vgroup + j);
+    for (int j = 0; j < kVR / 16; ++j) {
+      const auto vp = group_rows(p.value_cache, kVR / 16 * vgroup + j);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         vraw[j >> 1][4 * (j & 1) + e] = __builtin_amdgcn_raw_buffer_load_b32(vp, v_off[e], 0, 0);
@@ -654,22 +657,22 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
       // query row that does not see one must not meet it in the product.
       bool odd = false;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < kVR / 16; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint32_t &w = vraw[j >> 1][4 * (j & 1) + e];
-          const int t = t0 + 64 * vgroup + 16 * j + 4 * g + e;
-          w = bool((ok_now >> (4 * vgroup + j)) & 1u) & (t < t_end) ? w : 0u;
+          const int t = t0 + kVR * vgroup + 16 * j + 4 * g + e;
+          w = bool((ok_now >> (kVR / 16 * vgroup + j)) & 1u) & (t < t_end) ? w : 0u;
           odd |= (t >= ctx) & some_not_finite(w);
         }
       if (__any(odd)) {
 #pragma unroll 1
-        for (int k = 0; k < 16; ++k) {
+        for (int k = 0; k < kVR / 4; ++k) {
           const int j = k >> 2, e = k & 3;
           uint32_t w = 0;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w = i == k ? vraw[i >> 3][i & 7] : w;
-          const int t_lane = t0 + 64 * vgroup + 16 * j + 4 * g + e;
+          for (int i = 0; i < kVR / 4; ++i) w = i == k ? vraw[i >> 3][i & 7] : w;
+          const int t_lane = t0 + kVR * vgroup + 16 * j + 4 * g + e;
 #pragma unroll 1
           for (int byte = 0; byte < 4; ++byte) {
             const uint32_t c = (w >> (8 * byte)) & 0xFFu;
@@ -681,8 +684,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
               left &= left - 1;
               const float v = __uint_as_float(decode_bits(uint32_t(__builtin_amdgcn_readlane(int(c), src))));
               const int sg = src >> 4, sn = src & 15;       // row 4 sg + e, dims 64 vslice + 4 sn + byte
-              const int t = t0 + 64 * vgroup + 16 * j + 4 * sg + e;
-              const int at = 64 * vgroup + 32 * (j >> 1) + 8 * sg + 4 * (j & 1) + e;
+              const int t = t0 + kVR * vgroup + 16 * j + 4 * sg + e;
+              const int at = kVR * vgroup + 32 * (j >> 1) + 8 * sg + 4 * (j & 1) + e;
 #pragma unroll
               for (int rb = 0; rb < kRB; ++rb) {
                 // (t, dim) is element sn % 4 of accumulator `byte` in the lanes of group sn / 4.
@@ -699,17 +702,17 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
             }
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
+          for (int i = 0; i < kVR / 4; ++i)
             if (i == k) vraw[i >> 3][i & 7] = w;
         }
       }
     }
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
+    for (int hf = 0; hf < kVR / 32; ++hf) {
       lk_u32x4 pf[kRB];
 #pragma unroll
       for (int rb = 0; rb < kRB; ++rb)
-        pf[rb] = *reinterpret_cast<const lk_u32x4 *>(pt + (16 * rb + n) * kPStride + 64 * vgroup + 32 * hf + 8 * g);
+        pf[rb] = *reinterpret_cast<const lk_u32x4 *>(pt + (16 * rb + n) * kPStride + kVR * vgroup + 32 * hf + 8 * g);
       // As above: the next byte's lookups are on their way while one multiplies.
       lk_u32x4 a = look_column<0, true>(vraw[hf], lane4, table);
       auto column = [&](auto byte) {
@@ -990,11 +993,11 @@ RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int6
     return pl;
   }
   const int64_t rows = std::max<int64_t>(max_query, 1) * (heads / hkv);
-  pl.row_blocks = rows <= 16 ? 1 : rows <= 32 || d < 256 ? 2 : 4;
+  pl.row_blocks = rows <= 16 ? 1 : rows <= 32 || d < 128 ? 2 : 4;
   pl.row_tiles = int((rows + 16 * pl.row_blocks - 1) / (16 * pl.row_blocks));
   pl.magic = uint32_t(((int64_t(1) << 31) + block_size / 16 - 1) / (block_size / 16));
   // A workgroup for each slot that the GPU has: eight wavefronts per CU.
-  pl.tile_rows = int(4096 / d * waves_of(pl.row_blocks));
+  pl.tile_rows = tile_rows_of(int(d), pl.row_blocks);
   const int64_t tiles = batch * ((len + pl.tile_rows - 1) / pl.tile_rows);
   const int64_t slots = 2048 / waves_of(pl.row_blocks) / (hkv * pl.row_tiles);
   pl.workers = int(std::min<int64_t>(std::max<int64_t>(slots, 1), tiles));
@@ -1056,8 +1059,8 @@ void launch_row_attention(const RowAttnParams &p, const RowPlan &pl, hipStream_t
   const auto with_dim = [&](auto dim) {
     constexpr int kD = decltype(dim)::value;
     if (pl.row_blocks == 1) launch_rows<kD, kBf16, 1, BtT>(p, pl.magic, s);
-    else if (kD < 256 || pl.row_blocks == 2) launch_rows<kD, kBf16, 2, BtT>(p, pl.magic, s);
-    else launch_rows<kD, kBf16, kD < 256 ? 2 : 4, BtT>(p, pl.magic, s);
+    else if (kD < 128 || pl.row_blocks == 2) launch_rows<kD, kBf16, 2, BtT>(p, pl.magic, s);
+    else launch_rows<kD, kBf16, kD < 128 ? 2 : 4, BtT>(p, pl.magic, s);
   };
   if (p.d == 64) with_dim(std::integral_constant<int, 64>{});
   else if (p.d == 128) with_dim(std::integral_constant<int, 128>{});
