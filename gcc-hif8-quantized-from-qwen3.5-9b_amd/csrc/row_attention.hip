@@ -144,7 +144,7 @@ constexpr float kLazy = 14.f;  // log2 headroom of the maximum: P' stays below 2
 constexpr int waves_of(int row_blocks) { return row_blocks > 2 ? 8 : 4; }
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
 // Cache rows of a tile.
-constexpr int tile_rows_of(int d, int row_blocks) { return row_blocks > 2 ? 128 : 16384 / d; }
+constexpr int tile_rows_of(int d, int row_blocks) { return d == 256 && row_blocks <= 2 ? 64 : 128; }
 
 // Inclusive sum over the lanes of a wavefront.
 __device__ __forceinline__ int wave_prefix(int v) {
