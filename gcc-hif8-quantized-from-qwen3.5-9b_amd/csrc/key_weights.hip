@@ -216,12 +216,11 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
   const int n = lane & 15, g = lane >> 4;
 
   // The key tiles of one (request, KV head, row split) read the same queries:
-  // their blocks are equal modulo 8, on one XCD.
-  const int xcd = int(blockIdx.x) & 7, slot = int(blockIdx.x) >> 3;
-  const int outer = (slot / p.tiles) * 8 + xcd;
-  if (outer >= p.batch * p.hkv * p.row_splits) return;  // padding block (uniform)
-  const int tile = slot % p.tiles;
-  const int h = outer % p.hkv, split = (outer / p.hkv) % p.row_splits, b = outer / (p.hkv * p.row_splits);
+  // their blocks are equal modulo 8 (the grid's x), on one XCD.
+  const int outer = int(blockIdx.z) * 8 + int(blockIdx.x), tile = int(blockIdx.y);
+  const int bs = outer / p.hkv, h = outer - bs * p.hkv;
+  const int b = p.row_splits == 1 ? bs : bs / p.row_splits, split = bs - b * p.row_splits;
+  if (b >= p.batch) return;  // padding block (uniform)
   const int len = clamp_rows(p.lens[b], p.max_len);
   const int t0 = tile * kKeys;
   if (t0 >= len) return;  // uniform
@@ -362,68 +361,84 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
       }
       const lk_u32x4 *q = reinterpret_cast<const lk_u32x4 *>(reinterpret_cast<const uint8_t *>(sm.table) +
                                                             (s % kRing) * kStageBytes);
+      const int r0 = r_lo + kStage * s;
+      lk_f32x4 d[2][4];
+      auto product = [&](int rb) __attribute__((always_inline)) {
 #pragma unroll
-      for (int rb = 0; rb < 2; ++rb) {
-        __builtin_amdgcn_sched_barrier(0);
-        const int r0 = r_lo + kStage * s + 16 * rb;
-        lk_f32x4 d[4];
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) d[kb] = lk_f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int kb = 0; kb < 4; ++kb) d[rb][kb] = lk_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < kQS; ++i) {
           const lk_u32x4 qf = q[(rb * kQS + i) * kWave + lane];
 #pragma unroll
-          for (int kb = 0; kb < 4; ++kb) d[kb] = mfma_16x16x32<kBf16>(kf[kb][i], qf, d[kb]);
+          for (int kb = 0; kb < 4; ++kb) d[rb][kb] = mfma_16x16x32<kBf16>(kf[kb][i], qf, d[rb][kb]);
         }
-        // Every row of the block sees every key of the wavefront (uniform).
-        int tok0, head0;
-        row_place(p, h, r0, tok0, head0);
-        const bool full = key0 + 64 <= len && ok_groups == 15u && (!p.causal || key0 + 63 <= shift + tok0);
-        int lim = len;
-        if (!full && p.causal) {
-          int tok, head;
-          row_place(p, h, min(r0 + n, r_hi - 1), tok, head);
-          lim = min(len, shift + tok + 1);
-        }
-        if (kSums && r0 + n >= r_hi) lim = 0;  // its statistics need not be a number
-        // One copy of the arithmetic per case: a test per element would branch in the loop.
-        auto block = [&](auto all) {
-          constexpr bool kAll = decltype(all)::value;
-          auto visible = [&](int kb, int e) {
-            return bool(((ok_groups >> kb) & 1u) & uint32_t(key0 + 16 * kb + 4 * g + e < lim));
-          };
-          if constexpr (kSums) {
-#pragma unroll
-            for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(d[kb][e], ksc[kb][e], -cur[rb].x));
-                const float sum = fmaf(w, cur[rb].y, acc[kb][e]);
-                acc[kb][e] = kAll || visible(kb, e) ? sum : acc[kb][e];
-              }
-          } else {
-            float mx = -__builtin_inff();
-#pragma unroll
-            for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float x = d[kb][e] * ksc[kb][e];
-                d[kb][e] = kAll || visible(kb, e) ? x : -__builtin_inff();
-                mx = fmaxf(mx, d[kb][e]);
-              }
-            mx = max_over_groups(mx);
-            const float use = mx == -__builtin_inff() ? 0.f : mx;
-            float l = 0.f;
-#pragma unroll
-            for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) l += __builtin_amdgcn_exp2f(d[kb][e] - use);
-            l = sum_over_groups(l);
-            if (g == 0) sm.ml[s & 1][wave][16 * rb + n] = float2{mx, l};
-          }
+      };
+      // The rows of block rb: whether they see key kb, e, unless all of them see all.
+      auto finish = [&](auto all, int rb, int lim) __attribute__((always_inline)) {
+        constexpr bool kAll = decltype(all)::value;
+        auto visible = [&](int kb, int e) {
+          return bool(((ok_groups >> kb) & 1u) & uint32_t(key0 + 16 * kb + 4 * g + e < lim));
         };
-        if (full) block(std::true_type{});
-        else block(std::false_type{});
+        if constexpr (kSums) {
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float w = __builtin_amdgcn_exp2f(fmaf(d[rb][kb][e], ksc[kb][e], -cur[rb].x));
+              const float sum = fmaf(w, cur[rb].y, acc[kb][e]);
+              acc[kb][e] = kAll || visible(kb, e) ? sum : acc[kb][e];
+            }
+        } else {
+          float mx = -__builtin_inff();
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = d[rb][kb][e] * ksc[kb][e];
+              d[rb][kb][e] = kAll || visible(kb, e) ? x : -__builtin_inff();
+              mx = fmaxf(mx, d[rb][kb][e]);
+            }
+          mx = max_over_groups(mx);
+          const float use = mx == -__builtin_inff() ? 0.f : mx;
+          float l = 0.f;
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) l += __builtin_amdgcn_exp2f(d[rb][kb][e] - use);
+          l = sum_over_groups(l);
+          if (g == 0) sm.ml[s & 1][wave][16 * rb + n] = float2{mx, l};
+        }
+      };
+      // Every row of the stage sees every key of the wavefront (uniform).
+      int tok0, head0;
+      row_place(p, h, r0, tok0, head0);
+      const bool full = key0 + 64 <= len && ok_groups == 15u && (!p.causal || key0 + 63 <= shift + tok0) &&
+                        (!kSums || r0 + kStage <= r_hi);
+      product(0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (full) {
+        // The second block's products and the first one's exponentials in turn: the
+        // wavefronts of a SIMD take their stages in step, so that neither unit was
+        // busy half of the time when each wavefront did one thing after the other.
+        product(1);
+        finish(std::true_type{}, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4 * kQS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+          __builtin_amdgcn_sched_group_barrier(0x002, 128 / (4 * kQS) > 4 ? 8 : 4, 0);  // vector instructions
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        finish(std::true_type{}, 1, 0);
+      } else {
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+          int tok, head;
+          row_place(p, h, min(r0 + 16 * rb + n, r_hi - 1), tok, head);
+          int lim = p.causal ? min(len, shift + tok + 1) : len;
+          if (kSums && r0 + 16 * rb + n >= r_hi) lim = 0;  // its statistics need not be a number
+          finish(std::false_type{}, rb, lim);
+          if (rb == 0) product(1);
+        }
       }
     }
     if constexpr (!kSums) {
@@ -448,23 +463,24 @@ __global__ __launch_bounds__(kThreads, 2) void key_pass_mfma(const WeightParams 
     }
   }
   if constexpr (kSums) {
+    // Every lane of a group has the group's 16 sums; lane n keeps that of its own key.
+    float v = 0.f;
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float v = acc[kb][e];
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, kWave);
-        const int t = key0 + 16 * kb + 4 * g + e;
-        if (n == 0 && t < len) {
-          if (p.part_w) {
-            p.part_w[((int64_t(split) * p.batch + b) * p.hkv + h) * p.w_pad + t] = v;
-          } else {
-            float *w = p.weights + (int64_t(b) * p.hkv + h) * p.w_stride + t;
-            *w = p.accumulate ? *w + v : v;
-          }
-        }
+        const float sum = sum_over_columns(acc[kb][e]);
+        v = n == 4 * kb + e ? sum : v;
       }
+    const int t = key0 + 16 * (n >> 2) + 4 * g + (n & 3);
+    if (t < len) {
+      if (p.part_w) {
+        p.part_w[((int64_t(split) * p.batch + b) * p.hkv + h) * p.w_pad + t] = v;
+      } else {
+        float *w = p.weights + (int64_t(b) * p.hkv + h) * p.w_stride + t;
+        *w = p.accumulate ? *w + v : v;
+      }
+    }
   }
 }
 
@@ -586,8 +602,7 @@ WeightSpace weight_space(const WeightPlan &pl, int64_t batch, int64_t heads, int
 
 template <int kD, bool kBf16, typename BtT>
 void launch_weights(WeightParams p, const WeightPlan &pl, hipStream_t s) {
-  const int64_t outer = (int64_t(p.batch) * p.hkv * p.row_splits + 7) / 8 * 8;
-  const unsigned blocks = unsigned(outer * p.tiles);
+  const dim3 blocks(8, unsigned(p.tiles), unsigned((int64_t(p.batch) * p.hkv * p.row_splits + 7) / 8));
   for (int64_t lo = 0; lo < p.total_q; lo += pl.chunk_tokens) {
     p.tok_lo = int(lo);
     p.tok_hi = int(std::min<int64_t>(p.total_q, lo + pl.chunk_tokens));
@@ -722,7 +737,7 @@ extern "C" int hif8_key_weights(const void *query, int q_dtype, const uint8_t *k
     p.split_rows = pl.split_rows;
     // 32-bit launch sizes, and operands that the copies into LDS can take.
     if (!aligned(query, 16) || batch > 0xFFFF || num_kv_heads > 0xFFFF ||
-        (batch * num_kv_heads * pl.row_splits + 7) / 8 * 8 * pl.tiles > most)
+        pl.tiles > 0xFFFF || (batch * num_kv_heads * pl.row_splits + 7) / 8 > 0xFFFF)
       pl.mfma = false;
   }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -96,6 +96,30 @@ __device__ __forceinline__ float sum_over_groups(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Sum over the 16 lanes of a group (lane / 16), in all of them: rotations within
+// the row of 16, which cost an addition each (shuffles through LDS took 30 times as long).
+template <int kBy>
+__device__ __forceinline__ float rotated(float x) {
+  return __uint_as_float(uint32_t(__builtin_amdgcn_update_dpp(0, int(__float_as_uint(x)), 0x120 + kBy, 0xF, 0xF, false)));
+}
+__device__ __forceinline__ float sum_over_columns(float x) {
+  x += rotated<8>(x);
+  x += rotated<4>(x);
+  x += rotated<2>(x);
+  return x + rotated<1>(x);
+}
+
+// Inclusive sum over the lanes of a wavefront: shifts within rows of 16, then the
+// rows' last lanes handed on to the rows behind.
+__device__ __forceinline__ int wave_prefix(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+}
+
 // True when some byte of w is an infinity (0x6F, 0xEF) or NaN (0x80); may also
 // be true next to such a byte, never false on one.
 __device__ __forceinline__ bool some_not_finite(uint32_t w) {

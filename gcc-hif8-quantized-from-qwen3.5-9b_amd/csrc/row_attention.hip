@@ -146,17 +146,6 @@ constexpr int max_of(int a, int b) { return a > b ? a : b; }
 // Cache rows of a tile.
 constexpr int tile_rows_of(int d, int row_blocks) { return d == 256 && row_blocks <= 2 ? 64 : 128; }
 
-// Inclusive sum over the lanes of a wavefront.
-__device__ __forceinline__ int wave_prefix(int v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int up = __shfl_up(v, o, kWave);
-    if (lane >= o) v += up;
-  }
-  return v;
-}
-
 // Exponent, signed mantissa and 2^-exponent of a V row's scale.  Scales below
 // 2^-64 keep 2^-64 as exponent (and a mantissa below one); NaN and infinity
 // become the mantissa.
