@@ -57,7 +57,9 @@ struct AcceptParams {
 // Row lens[b] + path[b][i] -> row lens[b] + i for i < counts[b], in every cache.
 // A thread owns one 4-byte column of the rows and moves them in order, eight
 // loads ahead of eight stores.  path rises, so path[j] >= j and a row that is
-// written is never read later: the move is in place and needs no barrier.
+// written is never read later: the move is in place and needs no barrier.  Bound
+// by latency (table, path, row: three round trips): 32 requests' paths of up to
+// eight drafts in eight layers' caches take 7.6 us in one launch.
 template <typename BtT>
 __global__ __launch_bounds__(kThreads) void accept_kernel(const AcceptParams p) {
   constexpr int kAhead = 8;
@@ -129,7 +131,10 @@ constexpr int kBins = 2048;
 // within it are ballots and only its totals cross the workgroup.  The ranks of
 // up to 64 kHeld rows per wavefront stay in registers (kHeld 0: they are read
 // again in every pass).  Bound by the latency of one read and about fifteen
-// barriers.
+// barriers: 7 us for 600 rows, 22 us for 32 pairs of 16384 rows each (one
+// workgroup per pair leaves most of the GPU idle; the rows that move afterwards
+// take longer than that).  With ranks read again in every pass, digits of eight
+// bits and 4-byte moves, the whole calls took 41 and 117 us; now 18 and 56.
 template <int kHeld>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictParams p) {
   __shared__ int hist[kBins];
@@ -289,7 +294,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictPa
 
 // Copies the paired rows, 16 bytes per thread: consecutive threads take the
 // pieces of a row's K, then of its V; four pieces of other rows are loaded
-// before the first is stored.
+// before the first is stored.  Bound by HBM: 102 MB (read and written) of 32
+// pairs cut from 16384 to 4096 rows take 29 us, 3.5 TB/s in pieces of 260 bytes.
 typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 template <typename BtT>

@@ -97,7 +97,7 @@ __device__ __forceinline__ float sum_over_groups(float x) {
 }
 
 // Sum over the 16 lanes of a group (lane / 16), in all of them: rotations within
-// the row of 16, which cost an addition each (shuffles through LDS took 30 times as long).
+// the row of 16, an addition each, where shuffles go through LDS.
 template <int kBy>
 __device__ __forceinline__ float rotated(float x) {
   return __uint_as_float(uint32_t(__builtin_amdgcn_update_dpp(0, int(__float_as_uint(x)), 0x120 + kBy, 0xF, 0xF, false)));

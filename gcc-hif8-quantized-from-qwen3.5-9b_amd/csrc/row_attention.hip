@@ -118,32 +118,47 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 // ---------------------------------------------------- on the matrix cores
 //
 // Head sizes 64, 128 and 256 (K and V alike), pages of a multiple of 16 rows.
-// A workgroup of four wavefronts is a worker for (KV head, 16 kRB query rows);
-// its query rows are the (draft, head) pairs of the KV head, so every
-// cached code is decoded once for all of them.  The tiles of kT = 16384 / D
-// cache rows of all requests, one after the other, are dealt out to the
-// workers in equal runs, so ragged lengths leave none idle; a run that reaches
-// into another request goes on with that one's query rows.  Per tile:
-//   * S^T = K Q^T: every wavefront takes a quarter of the tile's rows, loaded
-//     from HBM straight into the MFMA A operand (row = lane % 16, 16 codes per
-//     lane) and decoded in registers; Q is the B operand, held all along;
+// A workgroup is a worker for (KV head, 16 kRB query rows); its query rows are
+// the (draft, head) pairs of the KV head, so every cached code is decoded once
+// for all of them.  The tiles of kT cache rows of all requests, one after the
+// other, are dealt out to the workers in equal runs (one worker for each
+// workgroup that fits on the GPU), so ragged lengths leave none idle; a run that
+// reaches into another request goes on with that one's query rows.  Per tile:
+//   * S^T = K Q^T: the wavefronts share the tile's rows, loaded from HBM straight
+//     into the MFMA A operand (row = lane % 16, 16 codes per lane) and decoded
+//     there by the table of mfma_lookup.h; Q is the B operand, in registers (up
+//     to 32 rows) or in LDS in operand order (64);
 //   * P = 2^(x + e - m) in fp16 goes to LDS, against a maximum m that moves only
-//     when some row outgrows it by 2^6 (then the wavefronts' maxima meet in LDS
-//     and P is written again), so most tiles have one barrier; e
-//     is the exponent of the row's V scale and its mantissa is multiplied in,
-//     so V itself stays the exact dec(code) and no scale is rounded;
-//   * O^T += V^T P^T: every wavefront takes 64 dims of 64 rows (all of the
-//     tile's at D = 256), 4 bytes of 16 rows per lane.
+//     when some row outgrows it by 2^14 (then the wavefronts' maxima meet in LDS
+//     and P is written again), so nearly all tiles have one barrier; e is the
+//     exponent of the row's V scale and its mantissa is multiplied in, so V
+//     itself stays the exact dec(code), no scale is rounded, and P is rounded
+//     once (2^-11, as in any product of 16-bit weights);
+//   * O^T += V^T P^T: every wavefront takes 64 dims of 32 or 64 rows, 4 bytes of
+//     each row per lane, transposed by the lookup itself (byte q of eight words).
 // The next tile's K loads are issued as soon as S is done, its V loads after O.
 // sum_t P_t 2^-e_t is the softmax sum against the same maximum.
+//
+// What bounds it (16 query and 4 KV heads of 256, 8 x 16384 cached rows, 171 MB):
+// one token per request runs at 3.9 TB/s (43 us), what the card's plain reads
+// reach; 32 tokens each take 106 us, where the LDS lookups (128 per lane and
+// tile), the query operands from LDS and the vector instructions around them
+// add up, as the eight wavefronts go through a tile's phases together.  In
+// cycles per tile there: S 2100 to 2800, loads 1300 + 700, logits 600, P 1200,
+// O 2400 to 2900.  Two workgroups of 16 query rows per row tile, each decoding
+// the cache for itself, took 195 us.  Short calls (512 rows) are latency: 10 us
+// and 4.5 for the join, of which the dependent reads of lengths, table and rows
+// are three round trips to HBM.
 constexpr float kLazy = 14.f;  // log2 headroom of the maximum: P' stays below 2^15, in fp16's range
 
 // Wavefronts of a workgroup: four, two workgroups to a CU; with 64 query rows
 // eight, one workgroup, since the table and the query rows in LDS leave no room
-// for two and the registers of four none for the rows.
+// for two and the registers of four none for the rows (24 heads of 128 under 61
+// drafts each: 44 us against 50 in row tiles of 32).
 constexpr int waves_of(int row_blocks) { return row_blocks > 2 ? 8 : 4; }
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
-// Cache rows of a tile.
+// Cache rows of a tile.  256 of them at D = 64 left one workgroup to a CU (32
+// drafts of 16 heads over 8 x 16k: 111 us against 73).
 constexpr int tile_rows_of(int d, int row_blocks) { return d == 256 && row_blocks <= 2 ? 64 : 128; }
 
 // Exponent, signed mantissa and 2^-exponent of a V row's scale.  Scales below
