@@ -131,10 +131,10 @@ constexpr int kBins = 2048;
 // within it are ballots and only its totals cross the workgroup.  The ranks of
 // up to 64 kHeld rows per wavefront stay in registers (kHeld 0: they are read
 // again in every pass).  Bound by the latency of one read and about fifteen
-// barriers: 7 us for 600 rows, 22 us for 32 pairs of 16384 rows each (one
+// barriers: 7 us for 600 rows, 20 us for 32 pairs of 16384 rows each (one
 // workgroup per pair leaves most of the GPU idle; the rows that move afterwards
 // take longer than that).  With ranks read again in every pass, digits of eight
-// bits and 4-byte moves, the whole calls took 41 and 117 us; now 18 and 56.
+// bits and 4-byte moves, the whole calls took 41 and 117 us; now 18 and 53.
 template <int kHeld>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictParams p) {
   __shared__ int hist[kBins];
@@ -235,15 +235,21 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictPa
       __syncthreads();
     }
   }
-  // Totals of the wavefront's rows equal to the limit, then of its dropped and moving rows.
+  // Totals of the wavefront's rows equal to the limit where not all of those are
+  // kept, then of its dropped and moving rows.
+  const bool ties = keep == 0 || need < pick[2];  // uniform
+  const uint32_t least = limit << shift;
   int equal = 0;
-  each([&](int, uint32_t k, bool in) { equal += __popcll(__ballot(in && (k >> shift) == limit)); });
-  if (lane == 0) red[wave][0] = equal;
-  __syncthreads();
-  equal = 0;
-  for (int i = 0; i < wave; ++i) equal += red[i][0];
+  if (ties) {
+    each([&](int, uint32_t k, bool in) { equal += __popcll(__ballot(in && (k >> shift) == limit)); });
+    if (lane == 0) red[wave][0] = equal;
+    __syncthreads();
+    equal = 0;
+    for (int i = 0; i < wave; ++i) equal += red[i][0];
+  }
   const uint64_t below = (uint64_t(1) << lane) - 1;
   auto kept = [&](uint32_t k, bool in, int &seen) {
+    if (!ties) return in && k >= least;
     const bool same = in && (k >> shift) == limit;
     const uint64_t ball = __ballot(same);
     const bool yes = in && keep > 0 && ((k >> shift) > limit || (same && seen + __popcll(ball & below) < need));
