@@ -5,6 +5,8 @@
 #include <stddef.h>
 
 #include <algorithm>
+#include <memory>
+#include <new>
 
 #include "hif8_common.h"
 
@@ -386,6 +388,19 @@ extern "C" int hif8_accept_drafts(void *const *caches, const int64_t *row_bytes,
       return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: a token's rows must be a multiple of four bytes", kName);
     widest = std::max(widest, row_bytes[i] / 4);
   }
+  // Two threads would move the same rows, one of them onto rows that the other has yet to read.
+  struct Span {
+    uintptr_t first;
+    uint64_t bytes;
+  };
+  const std::unique_ptr<Span[]> spans(new (std::nothrow) Span[size_t(num_caches)]);
+  if (!spans) return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: too many caches", kName);
+  for (int64_t i = 0; i < num_caches; ++i)
+    spans[i] = {reinterpret_cast<uintptr_t>(caches[i]), uint64_t(num_blocks) * uint64_t(block_size) * uint64_t(row_bytes[i])};
+  std::sort(spans.get(), spans.get() + num_caches, [](const Span &a, const Span &b) { return a.first < b.first; });
+  for (int64_t i = 1; i < num_caches; ++i)
+    if (spans[i].first - spans[i - 1].first < spans[i - 1].bytes)
+      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: caches must not overlap", kName);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   for (int64_t c0 = 0; c0 < num_caches; c0 += kMaxCaches) {
     AcceptParams p{};

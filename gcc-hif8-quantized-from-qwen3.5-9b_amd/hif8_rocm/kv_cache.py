@@ -509,8 +509,8 @@ def accept_drafts(
     ``context_lens[b] + i`` for ``i < accepted_counts[b]``.  ``accepted``
     (int32, ``[B, width]``) lists draft indices in strictly rising order, the
     path from the root (every parent precedes its children).  The caches are
-    one layer's pair or the pairs of all layers, which share ``block_table``;
-    all move in one launch.  Returns the new lengths, int32 ``[B]``, on the
+    one layer's pair or the pairs of all layers, which share ``block_table``
+    and no memory; all move in one launch.  Returns the new lengths, int32 ``[B]``, on the
     device.  The pages must belong to one request each.
 
     ``validate`` checks counts, order and pages on the host.

@@ -460,7 +460,8 @@ int hif8_key_weights(const void *query, int q_dtype, const uint8_t *key_cache, i
  * Moves the rows of accepted drafts to the end of the context, in place, in any number of
  * caches that share a block table (K and V of every layer), in one launch per 128 caches:
  *   row context_lens[b] + accepted[b][i]  ->  row context_lens[b] + i,  i < accepted_counts[b]
- *   caches [num_caches]  host array of device pointers; row_bytes[i] = Hkv * (D + 4) of cache i
+ *   caches [num_caches]  host array of device pointers; row_bytes[i] = Hkv * (D + 4) of cache i;
+ *     no two may overlap
  *   accepted [batch, accepted_width] int32: draft indices in strictly rising order (a path
  *     from the root: parents come before children); not rising, the rows' contents are
  *     unspecified, the accesses stay inside the cache

@@ -243,6 +243,8 @@ def test_c_entries_refuse_bad_arguments(lib):
     for kw, text in [({"ptrs": (256, 0)}, b"null pointer"), ({"ptrs": (256, 258)}, b"4-byte aligned"),
                      ({"row": 1042}, b"multiple of four"), ({"path": None}, b"null pointer"), ({"n": -1}, b"positive")]:
         assert take(**kw) == 1 and text in lib.hif8_last_error(), (kw, lib.hif8_last_error())
+    for ptrs in ((256, 256), (256 + 1040 * 8 * 128 - 4, 256)):   # the same cache twice, or one that ends inside another
+        assert take(ptrs=ptrs) == 1 and b"must not overlap" in lib.hif8_last_error()
     assert take(batch=0) == 0 and take(n=0) == 0
 
     weights = lib.hif8_key_weights
