@@ -570,7 +570,7 @@ constexpr int64_t kPartBytes = int64_t(64) << 20;
 // with 768, 250 with 1024, 272 with 1152 (one workgroup per slot, unevenly over
 // the XCDs).
 int64_t best_split(int64_t items, int64_t tiles, int64_t d, int64_t group, int64_t max_query, int64_t max_len, bool causal) {
-  const int64_t rows = max_query * group, step = std::max<int64_t>(1, tiles / 128);
+  const int64_t rows = max_query * group, step = std::max<int64_t>(1, tiles / 32);
   int64_t best = 0, best_cost = 0;
   for (int64_t split = 128;; split += std::max<int64_t>(32, split / 16 / 32 * 32)) {
     split = std::min<int64_t>(split, (rows + kStage - 1) / kStage * kStage);
@@ -709,8 +709,10 @@ extern "C" int hif8_key_weights(const void *query, int q_dtype, const uint8_t *k
   if (!aligned(query, 2)) return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: query must be 2-byte aligned", kName);
   if (!aligned(key_weights, 4))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: key_weights must be 4-byte aligned", kName);
-  const size_t need = hif8_key_weights_workspace_size(batch, num_heads, num_kv_heads, head_size, block_size,
-                                                      total_query_tokens, max_query_len, max_seq_len, causal);
+  WeightPlan pl = plan_weights(batch, num_heads, num_kv_heads, head_size, block_size, total_query_tokens,
+                               std::max<int64_t>(max_query_len, 1), max_seq_len, causal != 0);
+  const WeightSpace w = weight_space(pl, batch, num_heads, num_kv_heads, total_query_tokens, max_seq_len);
+  const size_t need = w.stat + w.part + w.part_w;
   if (need && (!workspace || workspace_bytes < need))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes required (got %zu)", kName, need,
                 workspace_bytes);
@@ -744,10 +746,7 @@ extern "C" int hif8_key_weights(const void *query, int q_dtype, const uint8_t *k
   p.causal = causal ? 1 : 0;
   p.accumulate = accumulate ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
-  WeightPlan pl = plan_weights(batch, num_heads, num_kv_heads, head_size, block_size, total_query_tokens,
-                               std::max<int64_t>(max_query_len, 1), max_seq_len, causal != 0);
   if (pl.mfma) {
-    const WeightSpace w = weight_space(pl, batch, num_heads, num_kv_heads, total_query_tokens, max_seq_len);
     p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + w.stat);
     if (w.part_w) p.part_w = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + w.stat + w.part);
     p.w_pad = int64_t(pl.tiles) * kKeys;
