@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void key_sums_any(const WeightParams p, i
 // the row splits; all orders of summation are fixed.
 //
 // What bounds it: a causal prompt of 4096 tokens (16 query, 4 KV heads of 256:
-// 2 x 68.7 GFLOP at the visible half) takes 103 to 112 us a pass, 0.64 PFLOP/s.  A
+// 2 x 68.7 GFLOP at the visible half) takes 103 to 115 us a pass, 0.6 PFLOP/s.  A
 // stage costs a wavefront 1024 cycles of matrix instructions and about as many
 // of vector ones (an exponential per logit among them, at a quarter of the rate),
 // and the two wavefronts of a SIMD overlap these in part.  Decoding the keys (256

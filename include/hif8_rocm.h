@@ -396,7 +396,8 @@ int hif8_paged_prefill_attention(const void *query, int q_dtype, const uint8_t *
  *     context rows and the drafts j < min(n_b, mask_width) with a byte other than zero
  *     in column j of its row (its ancestors and, usually, itself)
  *   max_query_len >= every n_b, <= mask_width; max_seq_len >= every context_lens[b] + n_b
- *     (lengths are clamped to it), <= max_blocks_per_seq * block_size
+ *     (lengths are clamped to it), <= max_blocks_per_seq * block_size; a request's drafts past
+ *     max_query_len get zeros or their attention, nothing out of bounds is touched
  *   out [total_query_tokens, num_heads, Dv] in the query dtype: softmax(scale * q . K) V over
  *     the rows seen, K and V dec(code) * row scale; a row that sees nothing gets zeros,
  *     and what is not seen has no influence, whatever it holds.  Cache rows whose block id
@@ -444,7 +445,8 @@ int hif8_paged_decode_attention_weights(const void *query, int q_dtype, const ui
  *                             head h of softmax_t(scale * q_i . K_t), t < seq_lens[b]
  * query, query_start_loc, seq_lens, max_query_len, max_seq_len and causal as in
  * hif8_paged_prefill_attention; key_weights and accumulate as above.  A request without
- * query rows adds (or stores) zeros.
+ * query rows adds (or stores) zeros; one with more than max_query_len gets sums that mean
+ * nothing, without an access out of bounds.
  */
 size_t hif8_key_weights_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
                                        int64_t block_size, int64_t total_query_tokens, int64_t max_query_len,
