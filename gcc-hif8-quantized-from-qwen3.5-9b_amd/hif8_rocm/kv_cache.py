@@ -458,6 +458,8 @@ def tree_attention(
     (bool or uint8, ``[T, at least max_query_len]``) is set: its ancestors and,
     usually, itself.  A draft that sees nothing gets zeros; what is not seen
     has no influence, NaN and infinities included.
+    Weights have 16 bits beside V, so an infinite V whose weight is below 2^-25
+    of the row's largest gives NaN, as zero times infinity.
 
     The request split is given as for :func:`paged_attention`.  ``max_seq_len``
     bounds ``context_lens[b] + query_lens[b]``; with device tensors pass it and

@@ -763,3 +763,20 @@ def test_two_calls_at_once(native_ops, device):
             assert torch.equal(a, b)
         for k in ("kc", "vc", "w", "pos"):
             assert torch.equal(states[i][k], want[i][1][k]), k
+
+
+@pytest.mark.parametrize("ctx, qlens, hq, hkv, d, bs", [
+    ([40, 30], [150, 30], 6, 2, 20, 12),       # any-shape kernel, a wavefront per output row
+    ([25], [130], 8, 4, 512, 16),
+    ([2000, 5], [40, 3], 16, 4, 64, 16),
+    ([1500, 0, 300], [61, 2, 30], 24, 8, 128, 16),
+    ([1100], [16], 16, 16, 128, 48),
+])
+def test_tree_of_many_rows(native_ops, device, ctx, qlens, hq, hkv, d, bs):
+    for mask in ("tree", "any"):
+        _tree(device, ctx, qlens, hq, hkv, d, bs, seed=95 + d, mask=mask, dtype=torch.float16, mixed=True)
+
+
+def test_weights_of_many_heads_and_long_rows(native_ops, device):
+    """Decode form where outputs take a wavefront each, and rows over several chunks of the join."""
+    _weighted(device, [2100, 1025, 1024, 1] + [33] * 12, [1] * 16, 64, 4, 64, 16, seed=96, dtype=torch.float16)
