@@ -118,6 +118,63 @@ struct EvictParams {
   int hkv, key_words, value_words, max_len, keep_all, sinks;
 };
 
+typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Copies the paired rows, 16 bytes per thread: consecutive threads take the
+// pieces of a row's K, then of its V; four pieces of other rows are loaded
+// before the first is stored.  Bound by HBM: 102 MB (read and written) of 32
+// pairs cut from 16384 to 4096 rows take 29 us, 3.5 TB/s in pieces of 260 bytes.
+template <typename BtT>
+__device__ __forceinline__ void move_rows(const EvictParams &p, int bh, int count, uint64_t thread, uint64_t stride) {
+  constexpr int kAhead = 4;
+  const int b = bh / p.hkv, h = bh % p.hkv;
+  const int2 *moves = p.moves + int64_t(bh) * p.move_stride;
+  const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.pages.width;
+  const uint32_t kc = uint32_t(p.key_words + 3) / 4, per_row = kc + uint32_t(p.value_words + 3) / 4;
+  const uint64_t pieces = uint64_t(count) * per_row;
+  const bool few = pieces >> 32 == 0;  // uniform: 32-bit divisions
+  for (uint64_t i0 = thread; i0 < pieces; i0 += kAhead * stride) {
+    u32x4_a4 v[kAhead];
+    uint32_t *to[kAhead];
+    int words[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const uint64_t i = i0 + j * stride;
+      words[j] = 0;
+      if (i >= pieces) continue;
+      const uint32_t row = few ? uint32_t(i) / per_row : uint32_t(i / per_row);
+      uint32_t c = uint32_t(i - uint64_t(row) * per_row);
+      const int2 m = moves[row];
+      const int64_t d = slot_of(bt, m.x, p.pages), s = slot_of(bt, m.y, p.pages);
+      if (d < 0 || s < 0) continue;
+      const bool is_v = c >= kc;
+      if (is_v) c -= kc;
+      const int width = is_v ? p.value_words : p.key_words;
+      uint32_t *cache = is_v ? p.value_cache : p.key_cache;
+      const uint32_t *src = cache + (s * p.hkv + h) * width + 4 * c;
+      to[j] = cache + (d * p.hkv + h) * width + 4 * c;
+      words[j] = min(4, width - int(4 * c));
+      if (words[j] == 4) {
+        v[j] = *reinterpret_cast<const u32x4_a4 *>(src);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < words[j]) v[j][e] = src[e];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (words[j] == 4) {
+        *reinterpret_cast<u32x4_a4 *>(to[j]) = v[j];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < words[j]) to[j][e] = v[j][e];
+      }
+    }
+  }
+}
+
 // Larger is kept first: protected rows, then weights in falling order, NaN last.
 __device__ __forceinline__ uint32_t rank_of(float w, bool safe) {
   if (safe) return 0xFFFFFFFFu;
@@ -137,11 +194,11 @@ constexpr int kBins = 2048;
 // within it are ballots and only its totals cross the workgroup.  The ranks of
 // up to 64 kHeld rows per wavefront stay in registers (kHeld 0: they are read
 // again in every pass).  Bound by the latency of one read and about fifteen
-// barriers: 7 us for 600 rows, 20 us for 32 pairs of 16384 rows each (one
+// barriers: 7 us for 600 rows (11 with the move of 88 of them), 20 us for 32 pairs of 16384 rows each (one
 // workgroup per pair leaves most of the GPU idle; the rows that move afterwards
 // take longer than that).  With ranks read again in every pass, digits of eight
-// bits and 4-byte moves, the whole calls took 41 and 117 us; now 18 and 53.
-template <int kHeld>
+// bits and 4-byte moves, the whole calls took 41 and 117 us; now 16 and 53.
+template <int kHeld, typename Mover>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictParams p) {
   __shared__ int hist[kBins];
   __shared__ int red[kSelWaves][2];
@@ -302,63 +359,13 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictPa
   }
   __syncthreads();
   for (int t = keep + tid; t < len; t += kSelThreads) w[t] = 0.f;
+  if constexpr (!std::is_void_v<Mover>) move_rows<Mover>(p, bh, count, uint64_t(tid), kSelThreads);
 }
-
-// Copies the paired rows, 16 bytes per thread: consecutive threads take the
-// pieces of a row's K, then of its V; four pieces of other rows are loaded
-// before the first is stored.  Bound by HBM: 102 MB (read and written) of 32
-// pairs cut from 16384 to 4096 rows take 29 us, 3.5 TB/s in pieces of 260 bytes.
-typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 template <typename BtT>
 __global__ __launch_bounds__(kThreads) void evict_move_kernel(const EvictParams p) {
-  constexpr int kAhead = 4;
-  const int bh = blockIdx.y, b = bh / p.hkv, h = bh % p.hkv;
-  const int count = p.move_counts[bh];
-  const int2 *moves = p.moves + int64_t(bh) * p.move_stride;
-  const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.pages.width;
-  const uint32_t kc = uint32_t(p.key_words + 3) / 4, per_row = kc + uint32_t(p.value_words + 3) / 4;
-  const uint64_t pieces = uint64_t(count) * per_row, stride = uint64_t(gridDim.x) * kThreads;
-  for (uint64_t i0 = uint64_t(blockIdx.x) * kThreads + threadIdx.x; i0 < pieces; i0 += kAhead * stride) {
-    u32x4_a4 v[kAhead];
-    uint32_t *to[kAhead];
-    int words[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const uint64_t i = i0 + j * stride;
-      words[j] = 0;
-      if (i >= pieces) continue;
-      const uint32_t row = uint32_t(i / per_row);
-      uint32_t c = uint32_t(i - uint64_t(row) * per_row);
-      const int2 m = moves[row];
-      const int64_t d = slot_of(bt, m.x, p.pages), s = slot_of(bt, m.y, p.pages);
-      if (d < 0 || s < 0) continue;
-      const bool is_v = c >= kc;
-      if (is_v) c -= kc;
-      const int width = is_v ? p.value_words : p.key_words;
-      uint32_t *cache = is_v ? p.value_cache : p.key_cache;
-      const uint32_t *src = cache + (s * p.hkv + h) * width + 4 * c;
-      to[j] = cache + (d * p.hkv + h) * width + 4 * c;
-      words[j] = min(4, width - int(4 * c));
-      if (words[j] == 4) {
-        v[j] = *reinterpret_cast<const u32x4_a4 *>(src);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (e < words[j]) v[j][e] = src[e];
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      if (words[j] == 4) {
-        *reinterpret_cast<u32x4_a4 *>(to[j]) = v[j];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (e < words[j]) to[j][e] = v[j][e];
-      }
-    }
-  }
+  move_rows<BtT>(p, int(blockIdx.y), p.move_counts[blockIdx.y], uint64_t(blockIdx.x) * kThreads + threadIdx.x,
+                 uint64_t(gridDim.x) * kThreads);
 }
 
 size_t evict_list_stride(int64_t max_len) { return size_t(std::max<int64_t>(max_len, 2) / 2 + 1); }
@@ -498,14 +505,26 @@ extern "C" int hif8_kv_evict(uint8_t *key_cache, uint8_t *value_cache, int64_t n
   p.sinks = int(std::min<int64_t>(sinks, 0x7FFFFFFF));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const unsigned bh = unsigned(batch * num_kv_heads);
-  if (max_seq_len <= 4 * kSelThreads) evict_select_kernel<4><<<bh, kSelThreads, 0, s>>>(p);
-  else if (max_seq_len <= 16 * kSelThreads) evict_select_kernel<16><<<bh, kSelThreads, 0, s>>>(p);
-  else if (max_seq_len <= 32 * kSelThreads) evict_select_kernel<32><<<bh, kSelThreads, 0, s>>>(p);
-  else evict_select_kernel<0><<<bh, kSelThreads, 0, s>>>(p);
+  const bool i64 = block_table_dtype == HIF8_INDEX_INT64;
+  const int64_t per_row = (p.key_words + 3) / 4 + (p.value_words + 3) / 4;
+  const int64_t kept = std::min<int64_t>(p.keep_all, max_seq_len);
+  const int64_t most_moves = keep ? max_seq_len / 2 : std::min(kept, max_seq_len - kept);
+  if (max_seq_len <= kSelThreads && most_moves * per_row <= 5 * kSelThreads) {
+    // The workgroup that selects rows moves them too where that is at most five
+    // pieces per thread: 88 rows of 600 (D = 256) take 15.7 us against 18.2 with a
+    // launch for the move, 256 of 1024 would take 21.8 against 18.7.
+    if (i64) evict_select_kernel<1, int64_t><<<bh, kSelThreads, 0, s>>>(p);
+    else evict_select_kernel<1, int32_t><<<bh, kSelThreads, 0, s>>>(p);
+    return check_launch(kName);
+  }
+  if (max_seq_len <= 4 * kSelThreads) evict_select_kernel<4, void><<<bh, kSelThreads, 0, s>>>(p);
+  else if (max_seq_len <= 16 * kSelThreads) evict_select_kernel<16, void><<<bh, kSelThreads, 0, s>>>(p);
+  else if (max_seq_len <= 32 * kSelThreads) evict_select_kernel<32, void><<<bh, kSelThreads, 0, s>>>(p);
+  else evict_select_kernel<0, void><<<bh, kSelThreads, 0, s>>>(p);
   // Four pieces per thread where there are rows for it, up to about eight workgroups per CU.
-  const int64_t most = int64_t(lists) * ((p.key_words + 3) / 4 + (p.value_words + 3) / 4);
+  const int64_t most = int64_t(lists) * per_row;
   const unsigned movers = unsigned(std::min<int64_t>((most + 4 * kThreads - 1) / (4 * kThreads), std::max<int64_t>(1, 2048 / bh)));
-  if (block_table_dtype == HIF8_INDEX_INT64) evict_move_kernel<int64_t><<<dim3(movers, bh), kThreads, 0, s>>>(p);
+  if (i64) evict_move_kernel<int64_t><<<dim3(movers, bh), kThreads, 0, s>>>(p);
   else evict_move_kernel<int32_t><<<dim3(movers, bh), kThreads, 0, s>>>(p);
   return check_launch(kName);
 }
