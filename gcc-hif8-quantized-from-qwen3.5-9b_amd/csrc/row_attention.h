@@ -29,6 +29,7 @@ struct RowAttnParams {
   float *weights;              // [batch, Hkv, w_stride], or null
   int64_t bt_stride, num_blocks, mask_stride, x_stride, w_stride;
   int block_size, hkv, hq, group, d, dv, batch, total_q, max_len, num_splits, split_tokens, accumulate;
+  int zero_rest;               // query rows of no request get zeros (else they are left as they were)
   // Matrix cores: workers that share the tiles, row tiles of the longest request,
   // query rows of all of them (a KV head's), ceil(2^31 / group).
   int workers, row_tiles, rows_cap, heads_together;

@@ -872,7 +872,12 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     if (r >= out_rows) return;
     const int row = int(r / p.hq);
     const int b = request_of_row(p, row);
-    if (b < 0) return;
+    uint16_t *o_row = static_cast<uint16_t *>(p.out) + size_t(r) * p.dv;
+    if (b < 0) {
+      if (p.zero_rest)
+        for (int dim = lane; dim < p.dv; dim += kWave) o_row[dim] = 0;
+      return;
+    }
     int begin, count;
     request_rows(p, b, begin, count);
     const Parts parts = parts_of(p, b, row, row - begin, int(r) - row * p.hq);
@@ -889,9 +894,8 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
         // A part that saw nothing was not written (any-shape kernel): its rubbish may be no number.
         if (ml[1] != 0.f) acc += __builtin_amdgcn_exp2f(ml[0] - m) * v;
       }
-      uint16_t *o = static_cast<uint16_t *>(p.out) + size_t(r) * p.dv + d4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = float_to_half_bits<kBf16>(acc[e] * inv);
+      for (int e = 0; e < 4; ++e) o_row[d4 + e] = float_to_half_bits<kBf16>(acc[e] * inv);
     }
     return;
   }
@@ -899,7 +903,11 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     const int slice = int(blockIdx.x) % dim_slices;
     const int r = int(blockIdx.x) / dim_slices, row = r / p.hq;
     const int b = request_of_row(p, row);
-    if (b < 0) return;
+    const int dim = slice * kSliceDims + tid;
+    if (b < 0) {  // uniform
+      if (p.zero_rest && tid < kSliceDims && dim < p.dv) static_cast<uint16_t *>(p.out)[size_t(r) * p.dv + dim] = 0;
+      return;
+    }
     int begin, count;
     request_rows(p, b, begin, count);
     const Parts parts = parts_of(p, b, row, row - begin, r - row * p.hq);
@@ -921,7 +929,6 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     }
     *reinterpret_cast<f32x4_t *>(&red[g][4 * (tid & 15)]) = acc;
     __syncthreads();
-    const int dim = slice * kSliceDims + tid;
     if (tid >= kSliceDims || dim >= p.dv) return;
     float y = 0.f;
 #pragma unroll
@@ -1087,6 +1094,7 @@ struct RowArgs {
   float *weights;
   int64_t w_stride;
   int accumulate;
+  int zero_rest;
   void *workspace;
   size_t workspace_bytes;
   hif8_stream_t stream;
@@ -1155,6 +1163,7 @@ int row_attention(const char *name, const RowArgs &a) {
   p.num_splits = pl.num_splits;
   p.split_tokens = pl.split_tokens;
   p.accumulate = a.accumulate ? 1 : 0;
+  p.zero_rest = a.zero_rest;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   const size_t rows = size_t(a.total_q) * a.heads;
   const RowSpace space = row_space(pl, a.batch, a.total_q, a.heads, a.dv, a.max_len, a.weights != nullptr);
@@ -1213,6 +1222,24 @@ extern "C" size_t hif8_tree_attention_workspace_size(int64_t batch, int64_t num_
                        max_query_len, max_seq_len, false);
 }
 
+namespace {
+
+int tree_attention(const char *name, const RowArgs &a) {
+  clear_error();
+  if (a.max_query < 0 || a.mask_stride < 0)
+    return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions must be positive", name);
+  if (a.batch > 0 && a.total_q > 0) {
+    if (a.max_query == 0)
+      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: max_query_len must cover the query rows", name);
+    if (a.mask_stride < a.max_query)
+      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: tree_mask rows are shorter than max_query_len", name);
+    if (!a.mask || !a.start_loc) return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: null pointer argument", name);
+  }
+  return row_attention(name, a);
+}
+
+}  // namespace
+
 extern "C" int hif8_tree_attention(const void *query, int q_dtype, const uint8_t *key_cache,
                                    const uint8_t *value_cache, int64_t num_blocks, int64_t block_size,
                                    int64_t num_kv_heads, int64_t head_size, int64_t head_size_v,
@@ -1222,23 +1249,27 @@ extern "C" int hif8_tree_attention(const void *query, int q_dtype, const uint8_t
                                    int64_t total_query_tokens, int64_t max_query_len, int64_t max_seq_len,
                                    float scale, void *out, void *workspace, size_t workspace_bytes,
                                    hif8_stream_t stream) {
-  static const char *kName = "hif8_tree_attention";
-  clear_error();
-  if (max_query_len < 0 || mask_width < 0)
-    return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions must be positive", kName);
-  if (batch > 0 && total_query_tokens > 0) {
-    if (max_query_len == 0)
-      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: max_query_len must cover the query rows", kName);
-    if (mask_width < max_query_len)
-      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: tree_mask rows are shorter than max_query_len", kName);
-    if (!tree_mask || !query_start_loc)
-      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: null pointer argument", kName);
-  }
-  return row_attention(kName, RowArgs{query, q_dtype, key_cache, value_cache, num_blocks, block_size, num_kv_heads,
-                                      head_size, head_size_v, block_table, block_table_dtype, max_blocks_per_seq,
-                                      query_start_loc, context_lens, tree_mask, mask_width, batch, num_heads,
-                                      total_query_tokens, max_query_len, max_seq_len, scale, out, nullptr, 0, 0, workspace,
-                                      workspace_bytes, stream});
+  return tree_attention("hif8_tree_attention",
+                        RowArgs{query, q_dtype, key_cache, value_cache, num_blocks, block_size, num_kv_heads, head_size,
+                                head_size_v, block_table, block_table_dtype, max_blocks_per_seq, query_start_loc,
+                                context_lens, tree_mask, mask_width, batch, num_heads, total_query_tokens, max_query_len,
+                                max_seq_len, scale, out, nullptr, 0, 0, 0, workspace, workspace_bytes, stream});
+}
+
+extern "C" int hif8_tree_attention_padded(const void *query, int q_dtype, const uint8_t *key_cache,
+                                          const uint8_t *value_cache, int64_t num_blocks, int64_t block_size,
+                                          int64_t num_kv_heads, int64_t head_size, int64_t head_size_v,
+                                          const void *block_table, int block_table_dtype, int64_t max_blocks_per_seq,
+                                          const int32_t *query_start_loc, const int32_t *context_lens,
+                                          const uint8_t *tree_mask, int64_t mask_width, int64_t batch, int64_t num_heads,
+                                          int64_t total_query_tokens, int64_t max_query_len, int64_t max_seq_len,
+                                          float scale, void *out, void *workspace, size_t workspace_bytes,
+                                          hif8_stream_t stream) {
+  return tree_attention("hif8_tree_attention_padded",
+                        RowArgs{query, q_dtype, key_cache, value_cache, num_blocks, block_size, num_kv_heads, head_size,
+                                head_size_v, block_table, block_table_dtype, max_blocks_per_seq, query_start_loc,
+                                context_lens, tree_mask, mask_width, batch, num_heads, total_query_tokens, max_query_len,
+                                max_seq_len, scale, out, nullptr, 0, 0, 1, workspace, workspace_bytes, stream});
 }
 
 extern "C" size_t hif8_paged_decode_attention_weights_workspace_size(int64_t batch, int64_t num_heads,
@@ -1268,5 +1299,5 @@ extern "C" int hif8_paged_decode_attention_weights(const void *query, int q_dtyp
   return row_attention(kName, RowArgs{query, q_dtype, key_cache, value_cache, num_blocks, block_size, num_kv_heads,
                                       head_size, head_size_v, block_table, block_table_dtype, max_blocks_per_seq,
                                       nullptr, seq_lens, nullptr, 0, batch, num_heads, batch, 1, max_seq_len, scale, out,
-                                      key_weights, weights_stride, accumulate, workspace, workspace_bytes, stream});
+                                      key_weights, weights_stride, accumulate, 0, workspace, workspace_bytes, stream});
 }

@@ -1379,12 +1379,13 @@ at::Tensor Hif8TreeAttention(const at::Tensor &query, const at::Tensor &key_cach
   const size_t bytes = hif8_tree_attention_workspace_size(batch, query.size(1), o.kv_heads, o.d, o.dv, o.block_size,
                                                           query.size(0), max_query_len, max_seq_len);
   const auto ws = Workspace(bytes, query);
-  CheckStatus(hif8_tree_attention(query.data_ptr(), DtypeCode(query.scalar_type()), key_cache.data_ptr<uint8_t>(),
-                                  value_cache.data_ptr<uint8_t>(), o.num_blocks, o.block_size, o.kv_heads, o.d, o.dv,
-                                  block_table.data_ptr(), o.bt_code, o.max_blocks, query_start_loc.data_ptr<int32_t>(),
-                                  context_lens.data_ptr<int32_t>(), static_cast<const uint8_t *>(tree_mask.data_ptr()),
-                                  tree_mask.size(1), batch, query.size(1), query.size(0), max_query_len, max_seq_len,
-                                  float(scale), out.data_ptr(), WorkspacePtr(ws), bytes, CurrentStream(query.device())),
+  CheckStatus(hif8_tree_attention_padded(
+                  query.data_ptr(), DtypeCode(query.scalar_type()), key_cache.data_ptr<uint8_t>(),
+                  value_cache.data_ptr<uint8_t>(), o.num_blocks, o.block_size, o.kv_heads, o.d, o.dv,
+                  block_table.data_ptr(), o.bt_code, o.max_blocks, query_start_loc.data_ptr<int32_t>(),
+                  context_lens.data_ptr<int32_t>(), static_cast<const uint8_t *>(tree_mask.data_ptr()),
+                  tree_mask.size(1), batch, query.size(1), query.size(0), max_query_len, max_seq_len, float(scale),
+                  out.data_ptr(), WorkspacePtr(ws), bytes, CurrentStream(query.device())),
               "hif8_tree_attention");
   return out;
 }

@@ -456,7 +456,8 @@ def tree_attention(
     behind them, at cache rows ``context_lens[b] + j``.  Draft i sees every
     context row and the drafts j of its request where ``tree_mask[row, j]``
     (bool or uint8, ``[T, at least max_query_len]``) is set: its ancestors and,
-    usually, itself.  A draft that sees nothing gets zeros; what is not seen
+    usually, itself.  A draft that sees nothing gets zeros, and so do rows that
+    ``query_start_loc`` gives to no request (a padded batch); what is not seen
     has no influence, NaN and infinities included.
     Weights have 16 bits beside V, so an infinite V whose weight is below 2^-25
     of the row's largest gives NaN, as zero times infinity.

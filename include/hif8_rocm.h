@@ -402,7 +402,8 @@ int hif8_paged_prefill_attention(const void *query, int q_dtype, const uint8_t *
  *     the rows seen, K and V dec(code) * row scale; a row that sees nothing gets zeros,
  *     and what is not seen has no influence, whatever it holds.  Cache rows whose block id
  *     lies outside [0, num_blocks) are left out.  Rows before query_start_loc[0] or from
- *     query_start_loc[batch] on are not written.
+ *     query_start_loc[batch] on are not written; hif8_tree_attention_padded, which is the
+ *     same call otherwise, gives them zeros (batch > 0), for an `out` that nobody has filled.
  *   workspace  at least hif8_tree_attention_workspace_size(...) bytes, 16-byte aligned; its
  *              size depends on these arguments alone
  */
@@ -416,6 +417,13 @@ int hif8_tree_attention(const void *query, int q_dtype, const uint8_t *key_cache
                         const uint8_t *tree_mask, int64_t mask_width, int64_t batch, int64_t num_heads,
                         int64_t total_query_tokens, int64_t max_query_len, int64_t max_seq_len, float scale,
                         void *out, void *workspace, size_t workspace_bytes, hif8_stream_t stream);
+int hif8_tree_attention_padded(const void *query, int q_dtype, const uint8_t *key_cache, const uint8_t *value_cache,
+                               int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_size,
+                               int64_t head_size_v, const void *block_table, int block_table_dtype,
+                               int64_t max_blocks_per_seq, const int32_t *query_start_loc, const int32_t *context_lens,
+                               const uint8_t *tree_mask, int64_t mask_width, int64_t batch, int64_t num_heads,
+                               int64_t total_query_tokens, int64_t max_query_len, int64_t max_seq_len, float scale,
+                               void *out, void *workspace, size_t workspace_bytes, hif8_stream_t stream);
 
 /*
  * hif8_paged_decode_attention that also accumulates the weight each cached row got (no

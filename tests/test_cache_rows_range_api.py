@@ -1,0 +1,36 @@
+"""Refusals and workspaces of the operators on rows of the KV cache at the edges
+of their ranges (CPU)."""
+
+import ctypes
+
+import pytest
+
+from conftest import PKG_ROOT
+
+
+@pytest.fixture(scope="module")
+def lib():
+    lib = ctypes.CDLL(str(PKG_ROOT / "hif8_rocm" / "libhif8_rocm.so"))
+    lib.hif8_last_error.restype = ctypes.c_char_p
+    return lib
+
+
+def _p(v=256):
+    return ctypes.c_void_p(v)
+
+
+def test_the_padded_tree_entry_refuses_what_the_other_does(lib):
+    i64, ptr, i32 = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int
+    tree = lib.hif8_tree_attention_padded
+    tree.argtypes = [ptr, i32, ptr, ptr] + [i64] * 5 + [ptr, i32, i64, ptr, ptr, ptr] + [i64] * 6 + \
+        [ctypes.c_float, ptr, ptr, ctypes.c_size_t, ptr]
+
+    def call(q=_p(), d=256, mask=_p(), mask_w=8, batch=1, total=8, mq=8, ml=500):
+        return tree(q, 1, _p(), _p(), 8, 128, 4, d, 256, _p(), 0, 4, _p(), _p(), mask, mask_w, batch, 16, total, mq, ml, 0.1,
+                    _p(), None, 0, None)
+
+    for kw, code, text in [({"q": None}, 1, b"null pointer"), ({"mask": None}, 1, b"null pointer"), ({"d": 516}, 2, b"above 512"),
+                           ({"ml": 513}, 1, b"block table capacity"), ({"mask_w": 7}, 1, b"tree_mask rows"),
+                           ({"mq": 0}, 1, b"max_query_len"), ({"mq": -1}, 1, b"positive"), ({}, 1, b"workspace of")]:
+        assert call(**kw) == code and text in lib.hif8_last_error(), (kw, lib.hif8_last_error())
+    assert call(batch=0) == 0 and call(total=0) == 0
