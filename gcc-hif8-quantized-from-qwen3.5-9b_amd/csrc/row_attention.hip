@@ -6,7 +6,10 @@
 //
 // o_i = sum_t p_it V_t with p_i = softmax over the rows t that query row i sees
 // of scale * q_i . K_t; a query row that sees nothing gets zeros.  K_t and V_t
-// are dec(code) * row scale, in FP32 without a rounding in between.
+// are dec(code) * row scale.  Logits, maxima, weights, their sums and the scales
+// are FP32 numbers (a weight below 2^-126 of its row's largest is zero); the
+// any-shape kernel multiplies FP32 throughout, the matrix cores take codes and
+// query as they are and the weights with V's scale in 16 bits, see below.
 #include <stddef.h>
 
 #include <algorithm>
@@ -106,12 +109,13 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
     p.part_ml[2 * part + 1] = total;
   }
   if (!(total != 0.f)) return;  // nothing seen: this split's outputs are not read
+  const float inv = 1.f / total;
   for (int dim = threadIdx.x; dim < p.dv; dim += kThreads) {
     float y = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
       if (f[w] != 0.f) y += f[w] * red_o[w][dim];
-    p.part_o[part * p.dv + dim] = y;
+    p.part_o[part * p.dv + dim] = y * inv;
   }
 }
 
@@ -128,16 +132,19 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 //     into the MFMA A operand (row = lane % 16, 16 codes per lane) and decoded
 //     there by the table of mfma_lookup.h; Q is the B operand, in registers (up
 //     to 32 rows) or in LDS in operand order (64);
-//   * P = 2^(x + e - m) in fp16 goes to LDS, against a maximum m that moves only
-//     when some row outgrows it by 2^14 (then the wavefronts' maxima meet in LDS
-//     and P is written again), so nearly all tiles have one barrier; e is the
-//     exponent of the row's V scale and its mantissa is multiplied in, so V
-//     itself stays the exact dec(code), no scale is rounded, and P is rounded
-//     once (2^-11, as in any product of 16-bit weights);
+//   * w = 2^(x - m) is the weight, summed in FP32, and P = w s f in fp16 goes to
+//     LDS: s is V's row scale, so that V itself stays the exact dec(code), and f a
+//     power of two per query row that puts the largest |P| in (1/4, 1] 2^kTop.
+//     m and f stand until some |P| passes 2^15 (or the sum of w 2^40); then the
+//     wavefronts' largest x and x + log2 |s| meet in LDS, O and the sum are scaled
+//     and P is written again, so nearly all tiles have one barrier.  m follows
+//     the logits alone and f what is multiplied with V: with one reference for
+//     both, rows whose scales lie 2^126 apart fell out of the sum.  P is rounded
+//     once: 2^-11 of it, or 2^-25 where it is subnormal (below 2^-14);
 //   * O^T += V^T P^T: every wavefront takes 64 dims of 32 or 64 rows, 4 bytes of
 //     each row per lane, transposed by the lookup itself (byte q of eight words).
 // The next tile's K loads are issued as soon as S is done, its V loads after O.
-// sum_t P_t 2^-e_t is the softmax sum against the same maximum.
+// Where there are several parts of a row, each is divided by its own sum and f.
 //
 // What bounds it (16 query and 4 KV heads of 256, 8 x 16384 cached rows, 171 MB):
 // one token per request runs at 3.9 TB/s (43 us), what the card's plain reads
@@ -149,7 +156,10 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 // the cache for itself, took 195 us.  Short calls (512 rows) are latency: 10 us
 // and 4.5 for the join, of which the dependent reads of lengths, table and rows
 // are three round trips to HBM.
-constexpr float kLazy = 14.f;  // log2 headroom of the maximum: P' stays below 2^15, in fp16's range
+constexpr float kTop = 2.f;          // log2 of what P stays below where its power of two is chosen
+constexpr float kMost = 15.f;        // and of what makes the wavefronts choose again: fp16 ends at 2^16
+constexpr float kLazy = 14.f;        // log2 of what a weight may reach before a new choice moves the maximum too
+constexpr float kMostSum = 0x1p40f;  // weights that add up to more are chosen again without a large P (V scales near zero)
 
 // Wavefronts of a workgroup: four, two workgroups to a CU; with 64 query rows
 // eight, one workgroup, since the table and the query rows in LDS leave no room
@@ -160,19 +170,6 @@ constexpr int max_of(int a, int b) { return a > b ? a : b; }
 // Cache rows of a tile.  256 of them at D = 64 left one workgroup to a CU (32
 // drafts of 16 heads over 8 x 16k: 111 us against 73).
 constexpr int tile_rows_of(int d, int row_blocks) { return d == 256 && row_blocks <= 2 ? 64 : 128; }
-
-// Exponent, signed mantissa and 2^-exponent of a V row's scale.  Scales below
-// 2^-64 keep 2^-64 as exponent (and a mantissa below one); NaN and infinity
-// become the mantissa.
-__device__ __forceinline__ void split_scale(float s, float &e, float &mant, float &inv) {
-  const uint32_t u = __float_as_uint(s);
-  const int ex = int((u >> 23) & 0xFFu);
-  const int at = ex == 0xFF ? 127 : max(ex, 127 - 64);  // biased exponent taken
-  e = float(at - 127);
-  inv = __uint_as_float(uint32_t(max(254 - at, 1)) << 23);  // 2^-127 for the largest: 2^-126 is as good as none
-  mant = at == ex ? __uint_as_float((u & 0x807FFFFFu) | 0x3F800000u) : s;
-  if (ex < 127 - 64) mant = s * 0x1p64f;
-}
 
 template <int kD, bool kBf16, int kRB, bool kX, typename BtT>
 __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(const RowAttnParams p,
@@ -191,14 +188,14 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   constexpr int kRows = 16 * kRB;
   constexpr int kPStride = kT + 8;        // fp16 values of a row of P in LDS
   // Two buffers of P where that leaves room for two workgroups of four wavefronts.
-  constexpr int kBuffers = kW == 8 || kLookupBytes + 4 * kRows * kPStride + 32 * kRows <= 81920 - 1024 ? 2 : 1;
+  constexpr int kBuffers = kW == 8 || kLookupBytes + 4 * kRows * kPStride + 32 * kRows + 64 <= 81920 - 1024 ? 2 : 1;
   struct Smem {
     uint32_t table[kLookupBytes / 4];     // at LDS byte 0: a lookup's address needs no addition
     // P of a tile and of the next; at a segment's end the shares of O of wavefronts of one slice.
     __attribute__((aligned(16))) uint16_t pt[max_of(kBuffers * kRows * kPStride, (kVG - 1) * kSlices * 2048)];
     lk_u32x4 q[kQLds ? kRB * kQS * kWave : 1];
-    float top[kW][kRows];
-    int grow[2];                          // the last tile (counted from 1) whose maximum moved, by parity
+    float top[2][kW][kRows];              // a wavefront's largest logit, and logit + log2 of V's scale, per query row
+    int grow[2];                          // the last tile (counted from 1) whose P grew too large, by parity
   };
   __shared__ __attribute__((aligned(16))) Smem sm;
   const uint32_t table = lds_address(sm.table);
@@ -440,10 +437,11 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     }
   }
   lk_f32x4 oacc[kRB][4];
-  float m[kRB], l[kRB];
+  float m[kRB], f[kRB], l[kRB];
 #pragma unroll
   for (int rb = 0; rb < kRB; ++rb) {
     m[rb] = -__builtin_inff();
+    f[rb] = 0x1p126f;
     l[rb] = 0.f;
 #pragma unroll
     for (int q = 0; q < 4; ++q) oacc[rb][q] = lk_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -552,15 +550,15 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
         for (int rb = 0; rb < kRB; ++rb) q[rb] = q_next[rb];
       }
     }
-    float ksc[kKB][4], ve[kKB][4], vm[kKB][4], vi[kKB][4];
+    float ksc[kKB][4], vsc[kKB][4];
 #pragma unroll
     for (int kb = 0; kb < kKB; ++kb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         ksc[kb][e] = ks[kb][e] * p.scale_log2;
-        split_scale(vs[kb][e], ve[kb][e], vm[kb][e], vi[kb][e]);
-        // Worked out here, before the registers of ks and vs are loaded again.
-        asm volatile("" : "+v"(ksc[kb][e]), "+v"(ve[kb][e]), "+v"(vm[kb][e]), "+v"(vi[kb][e]));
+        vsc[kb][e] = vs[kb][e];
+        // Taken here, before the registers of ks and vs are loaded again.
+        asm volatile("" : "+v"(ksc[kb][e]), "+v"(vsc[kb][e]));
       }
     // The next tile's K, in flight from here to the next S.  Past the last tile
     // the loads go on, to the cache's first rows: loads under a condition would
@@ -570,50 +568,49 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     off_lane = offset_at(t0 + kT, blk);
     ok_groups = uint32_t(__ballot(off_lane >= 0));
     load_k();
-    // Logits (base 2), each with its V scale's exponent.
-    float y[kRB][kKB][4], top[kRB];
-    bool grow = false;
+    // Logits (base 2).
+    float x[kRB][kKB][4];
     auto logits = [&](auto all, int rb) __attribute__((always_inline)) {
       constexpr bool kAll = decltype(all)::value;
-      top[rb] = -__builtin_inff();
 #pragma unroll
       for (int kb = 0; kb < kKB; ++kb) {
-        lk_f32x4 x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float z = s[rb][kb][e] * ksc[kb][e];
-          x[e] = kAll || ((seen[rb] >> (4 * kb + e)) & 1u) ? z : -__builtin_inff();
-          y[rb][kb][e] = x[e] + ve[kb][e];
-          top[rb] = fmaxf(top[rb], y[rb][kb][e]);
+          x[rb][kb][e] = kAll || ((seen[rb] >> (4 * kb + e)) & 1u) ? z : -__builtin_inff();
         }
         if constexpr (kX) {
           const int t = t0 + 16 * (wave * kKB + kb) + 4 * g;
-          if (xrow[rb] >= 0 && t < t_end) *reinterpret_cast<lk_f32x4 *>(p.x + xrow[rb] * p.x_stride + t) = x;
+          if (xrow[rb] >= 0 && t < t_end)
+            *reinterpret_cast<lk_f32x4 *>(p.x + xrow[rb] * p.x_stride + t) =
+                lk_f32x4{x[rb][kb][0], x[rb][kb][1], x[rb][kb][2], x[rb][kb][3]};
         }
       }
-      grow |= top[rb] > m[rb] + kLazy;
     };
     rows_with(full, logits);
-    // P against the maximum as it stands, which it does in most tiles: one barrier.
-    // Where some wavefront's rows outgrew it, all of them meet once more for the
-    // new one and write P again.
+    // P against the maximum and the power of two as they stand, which they do in
+    // most tiles: one barrier.  Where some wavefront's rows outgrew them (and in a
+    // segment's first tile), all of them meet once more for new ones and write P again.
     ++tile_no;
     uint16_t *pt = sm.pt + (kBuffers == 2 ? (tile_no & 1) * kRows * kPStride : 0);
     float psum[kRB];
+    bool grow = false;
     auto weights = [&](auto all, int rb) __attribute__((always_inline)) {
       constexpr bool kAll = decltype(all)::value;
       const float ref = m[rb] == -__builtin_inff() ? 0.f : m[rb];
+      float most = 0.f;
       psum[rb] = 0.f;
 #pragma unroll
       for (int kb = 0; kb < kKB; ++kb) {
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float pw = __builtin_amdgcn_exp2f(y[rb][kb][e] - ref);
+          const float pw = __builtin_amdgcn_exp2f(x[rb][kb][e] - ref);
           const bool vis = kAll || ((seen[rb] >> (4 * kb + e)) & 1u);
-          const float sum = fmaf(pw, vi[kb][e], psum[rb]);
+          const float sum = psum[rb] + pw;
           psum[rb] = vis ? sum : psum[rb];
-          w[e] = vis ? pw * vm[kb][e] : 0.f;
+          w[e] = vis ? pw * vsc[kb][e] * f[rb] : 0.f;
+          most = fmaxf(most, fabsf(w[e]));
         }
         const int j = wave * kKB + kb;
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -621,32 +618,57 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
             u32x2{uint32_t(float_to_f16_bits(w[0])) | (uint32_t(float_to_f16_bits(w[1])) << 16),
                   uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
       }
+      // A row that has seen nothing yet has no maximum: what it sees first sets one.
+      grow |= (most > 0x1p15f) | (psum[rb] > kMostSum) | ((m[rb] == -__builtin_inff()) & (kAll | (seen[rb] != 0)));
     };
     auto put = [&]() __attribute__((always_inline)) { rows_with(full, weights); };
-    if (__any(grow)) {
-      if (lane == 0) sm.grow[tile_no & 1] = tile_no;
-    } else {
+    if (it > 0) {
       put();
+      if (__any(grow) && lane == 0) sm.grow[tile_no & 1] = tile_no;
+      lds_barrier();
     }
-    lds_barrier();
-    if (sm.grow[tile_no & 1] == tile_no) {  // uniform
+    if (it == 0 || sm.grow[tile_no & 1] == tile_no) {  // uniform
 #pragma unroll
       for (int rb = 0; rb < kRB; ++rb) {
-        const float t = max_over_groups(top[rb]);
-        if (g == 0) sm.top[wave][16 * rb + n] = t;
+        float tx = -__builtin_inff(), ty = tx;
+#pragma unroll
+        for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            tx = fmaxf(tx, x[rb][kb][e]);  // what is not seen is -infinity, whatever its scale
+            if (vsc[kb][e] != 0.f) ty = fmaxf(ty, x[rb][kb][e] + float(__builtin_amdgcn_frexp_expf(vsc[kb][e])));
+          }
+        tx = max_over_groups(tx);
+        ty = max_over_groups(ty);
+        if (g == 0) {
+          sm.top[0][wave][16 * rb + n] = tx;
+          sm.top[1][wave][16 * rb + n] = ty;
+        }
       }
       lds_barrier();
 #pragma unroll
       for (int rb = 0; rb < kRB; ++rb) {
-        float t = sm.top[0][16 * rb + n];
+        float tx = sm.top[0][0][16 * rb + n], ty = sm.top[1][0][16 * rb + n];
 #pragma unroll
-        for (int w = 1; w < kW; ++w) t = fmaxf(t, sm.top[w][16 * rb + n]);
-        if (t > m[rb] + kLazy) {
-          const float alpha = m[rb] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[rb] - t);
-          l[rb] *= alpha;
+        for (int w = 1; w < kW; ++w) {
+          tx = fmaxf(tx, sm.top[0][w][16 * rb + n]);
+          ty = fmaxf(ty, sm.top[1][w][16 * rb + n]);
+        }
+        // True where there is no maximum yet; also where a weight above one could take its V scale past float32.
+        const bool rise = tx > m[rb] + kLazy || (tx > m[rb] && ty - m[rb] > 127.f);
+        const float m_new = rise ? tx : m[rb];
+        const float lf = float(__builtin_amdgcn_frexp_expf(f[rb]) - 1);  // f = 2^lf; P < 2^(ty - m + lf)
+        if (rise || ty - m_new + lf > kMost) {
+          // O is in units of 2^(m - lf), which only grows: what it holds stays in range.
+          const bool none = m[rb] == -__builtin_inff();
+          const float lf_new = fminf(fmaxf(floorf(m_new - fmaxf(none ? m[rb] : m[rb] - lf, ty - kTop)), -126.f), 126.f);
+          const float of_l = none ? 0.f : __builtin_amdgcn_exp2f(m[rb] - m_new);
+          const float of_o = none ? 0.f : __builtin_amdgcn_exp2f((m[rb] - m_new) + (lf_new - lf));
+          l[rb] *= of_l;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) oacc[rb][q] *= alpha;
-          m[rb] = t;
+          for (int q = 0; q < 4; ++q) oacc[rb][q] *= of_o;
+          m[rb] = m_new;
+          f[rb] = __uint_as_float(uint32_t(int(lf_new) + 127) << 23);
         }
       }
       put();
@@ -742,7 +764,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
 #pragma unroll
   for (int rb = 0; rb < kRB; ++rb) {
     const float lt = sum_over_groups(l[rb]);
-    if (g == 0) sm.top[wave][16 * rb + n] = lt;
+    if (g == 0) sm.top[0][wave][16 * rb + n] = lt;
   }
   if constexpr (kVG > 1) {
     lk_f32x4 *spill = reinterpret_cast<lk_f32x4 *>(sm.pt);
@@ -769,18 +791,19 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     for (int rb = 0; rb < kRB; ++rb) {
       const Row row = row_at(rb);
       if (!row.ok) continue;
-      float sum = sm.top[0][16 * rb + n];
+      float sum = sm.top[0][0][16 * rb + n];
 #pragma unroll
-      for (int w = 1; w < kW; ++w) sum += sm.top[w][16 * rb + n];
+      for (int w = 1; w < kW; ++w) sum += sm.top[0][w][16 * rb + n];
+      // O / (l f): l first, f is a power of two that may be far from one.
+      const float inv = sum != 0.f ? 1.f / sum : 0.f, inv_f = 1.f / f[rb];
       const size_t r = part_row * p.rows_cap + size_t(rt * kRows + 16 * rb + n);
       const int dim = 64 * vslice + 16 * g;  // element e of accumulator q: dim + 4 e + q
       if (whole) {
-        const float inv = sum != 0.f ? 1.f / sum : 0.f;
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          w[i] = uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i) & 3][i >> 1] * inv)) |
-                 (uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i + 1) & 3][i >> 1] * inv)) << 16);
+          w[i] = uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i) & 3][i >> 1] * inv * inv_f)) |
+                 (uint32_t(float_to_half_bits<kBf16>(oacc[rb][(2 * i + 1) & 3][i >> 1] * inv * inv_f)) << 16);
         lk_u32x4 *o = reinterpret_cast<lk_u32x4 *>(static_cast<uint16_t *>(p.out) +
                                                    (size_t(row.query) * p.hq + row.head) * kD + dim);
         o[0] = lk_u32x4{w[0], w[1], w[2], w[3]};
@@ -788,7 +811,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
       } else {
         lk_f32x4 *po = reinterpret_cast<lk_f32x4 *>(p.part_o + r * kD + dim);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) po[e] = lk_f32x4{oacc[rb][0][e], oacc[rb][1][e], oacc[rb][2][e], oacc[rb][3][e]};
+        for (int e = 0; e < 4; ++e)
+          po[e] = lk_f32x4{oacc[rb][0][e], oacc[rb][1][e], oacc[rb][2][e], oacc[rb][3][e]} * inv * inv_f;
       }
       if (g == 0 && vslice == 0) {
         p.part_ml[2 * r] = m[rb];
@@ -802,7 +826,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
 
 // Joins the parts of every query row and, where the call asks for them, adds
 // the heads' weights onto the cached rows:
-//   M = max_s m_s, L = sum_s 2^(m_s - M) l_s, out = sum_s 2^(m_s - M) O_s / L,
+//   M = max_s m_s, L = sum_s 2^(m_s - M) l_s, out = sum_s 2^(m_s - M) l_s / L o_s,
+// o_s the part's own attention (so that nothing in it is larger than a V row),
 //   weights[b, h, t] (+)= sum over the heads of h of 2^(x_t - M) / L.
 // The first blocks take outputs.  kWide false (few query rows, each with many
 // parts): a (row, head, 64 dims) per block, 16 threads of four dims by 16
@@ -892,10 +917,10 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
         const float *ml = p.part_ml + 2 * (parts.first + s * parts.stride);
         const f32x4_t v = *reinterpret_cast<const f32x4_t *>(po + size_t(s) * parts.stride * p.dv);
         // A part that saw nothing was not written (any-shape kernel): its rubbish may be no number.
-        if (ml[1] != 0.f) acc += __builtin_amdgcn_exp2f(ml[0] - m) * v;
+        if (ml[1] != 0.f) acc += __builtin_amdgcn_exp2f(ml[0] - m) * ml[1] * inv * v;
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o_row[d4 + e] = float_to_half_bits<kBf16>(acc[e] * inv);
+      for (int e = 0; e < 4; ++e) o_row[d4 + e] = float_to_half_bits<kBf16>(acc[e]);
     }
     return;
   }
@@ -917,7 +942,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     if (wave == 0)
       for (int s = lane; s < parts.count; s += kWave) {
         const float *ml = p.part_ml + 2 * (parts.first + s * parts.stride);
-        fac[s] = ml[1] != 0.f ? __builtin_amdgcn_exp2f(ml[0] - m) : 0.f;
+        fac[s] = ml[1] != 0.f ? __builtin_amdgcn_exp2f(ml[0] - m) * ml[1] * inv : 0.f;
       }
     __syncthreads();
     const int d4 = slice * kSliceDims + 4 * (tid & 15), g = tid >> 4;
@@ -933,7 +958,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     float y = 0.f;
 #pragma unroll
     for (int j = 0; j < kThreads / 16; ++j) y += red[j][tid];
-    static_cast<uint16_t *>(p.out)[size_t(r) * p.dv + dim] = float_to_half_bits<kBf16>(y * inv);
+    static_cast<uint16_t *>(p.out)[size_t(r) * p.dv + dim] = float_to_half_bits<kBf16>(y);
     return;
   }
   // Weights: one query row per request (row b), so (row, head) index b * Hq + head.

@@ -9,10 +9,11 @@ import pytest
 import torch
 
 from _kv import build_cache, randn
-from _rows import tree_reference
+from _rows import DECODE, Softmax, tree_reference
 
 pytestmark = pytest.mark.gpu
 I32 = torch.int32
+TOP = 2
 
 
 def _stale(shape, dtype, device):
@@ -47,3 +48,129 @@ def test_query_rows_of_no_request_are_zeros(native_ops, device, d, dv, bs, total
     want, bound = tree_reference(q[loc[0]:loc[2]].double().numpy(), kc.cpu().numpy(), vc.cpu().numpy(), table.numpy(), ctx,
                                  qlens, mask[loc[0]:loc[2]], 1 / math.sqrt(d), torch.bfloat16)
     assert (np.abs(got[loc[0]:loc[2]] - want) <= bound).all()
+
+
+def _rows(cache, table, b, n):
+    """float64 codes [n, Hkv, D] and row scales [n, Hkv] of request b's first n rows (all in the cache)."""
+    raw = cache.cpu().numpy()
+    bs = raw.shape[1]
+    t = np.arange(n)
+    raw = raw[table.numpy()[b, t // bs], t % bs]
+    return DECODE[raw[..., :-4]], np.ascontiguousarray(raw[..., -4:]).view(np.float32)[..., 0].astype(np.float64)
+
+
+def _attention(q, kc, vc, table, lens, rows, sees, scale, dtype):
+    """(out, bound, weights, weights' bound) of `rows[b]` query rows per request over lens[b] cached rows.
+
+    P = p s 2^k (s: the V row's scale) has 11 significant bits (2^-11 of p |V|), or 2^-25 absolutely where it is
+    subnormal; k puts the largest p |s| at 2^TOP / 4 at least, so that is 2^-(23 + TOP) max(p |s|) |code|."""
+    hq, hkv, group = q.shape[1], kc.shape[2], q.shape[1] // kc.shape[2]
+    half, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    out = np.zeros((sum(rows), hq, vc.shape[3] - 4))
+    bound, sums = np.zeros_like(out), np.zeros((len(lens), hkv, max(lens)))
+    sums_bound = np.zeros_like(sums)
+    at = 0
+    for b, (n, m) in enumerate(zip(lens, rows)):
+        (k, ks), (v, vs) = _rows(kc, table, b, n), _rows(vc, table, b, n)
+        for h in range(hq):
+            g = h // group
+            sm = Softmax(q[at:at + m, h], k[:, g] * ks[:, g, None], sees(b, n, m), scale)
+            value = v[:, g] * vs[:, g, None]
+            mag = sm.p @ np.abs(value)
+            y = sm.p @ value
+            most = (sm.p * np.abs(vs[:, g])).max(axis=1, initial=0.0)
+            out[at:at + m, h] = y
+            bound[at:at + m, h] = half * np.abs(y) + (2.0 ** -11 + sm.rel) * mag + tiny + \
+                2.0 ** -(23 + TOP) * most[:, None] * np.abs(v[:, g]).sum(axis=0)
+            sums[b, g, :n] += sm.p.sum(axis=0)
+            sums_bound[b, g, :n] += (sm.rel + 2.0 ** -24 * group) * sm.p.sum(axis=0) + 2.0 ** -126
+        at += m
+    return out, bound, sums, sums_bound
+
+
+def _near(got, want, bound):
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    over = np.abs(got - want) / np.maximum(bound, 1e-300)
+    print(f"  worst error / bound {over.max(initial=0.0):.3f}", flush=True)
+    assert (over <= 1.0).all(), float(over.max())
+
+
+def _put_scales(cache, scales):
+    cache.view(-1, cache.shape[-1])[:, -4:] = scales.reshape(-1, 1).view(torch.uint8).to(cache.device)
+
+
+def _tree_and_decode(device, kc, vc, table, lens, drafts, q, scale, dtype):
+    """Both operators over the same rows against the formula: drafts that see all of the request, one row that
+    keeps its weights."""
+    from hif8_rocm import kv_cache
+
+    batch, hkv = len(lens), kc.shape[2]
+    everything = lambda b, n, m: np.ones((m, n), dtype=bool)  # noqa: E731
+    args = dict(scale=scale)
+    mask = torch.ones(batch * drafts, drafts, dtype=torch.bool, device=device)
+    out = kv_cache.tree_attention(q.to(device), kc, vc, table.to(device), [n - drafts for n in lens], mask,
+                                  query_lens=[drafts] * batch, **args)
+    qn = q.double().numpy()
+    want, bound, _, _ = _attention(qn, kc, vc, table, lens, [drafts] * batch, everything, scale, dtype)
+    _near(out, want, bound)
+    w = torch.zeros(batch, hkv, max(lens), device=device)
+    q1 = q[::drafts].contiguous()
+    out = kv_cache.paged_decode_attention_weights(q1.to(device), kc, vc, table.to(device), lens, w, **args)
+    want, bound, sums, sums_bound = _attention(q1.double().numpy(), kc, vc, table, lens, [1] * batch, everything, scale, dtype)
+    _near(out, want, bound)
+    _near(w, sums, sums_bound)
+
+
+@pytest.mark.parametrize("d, hq, hkv, bs, drafts", [(256, 16, 4, 128, 3), (256, 16, 4, 128, 9), (128, 24, 8, 16, 31),
+                                                    (64, 4, 4, 32, 5), (96, 4, 2, 20, 3)])
+def test_v_scales_far_apart(native_ops, device, d, hq, hkv, bs, drafts):
+    """Row scales of V from 2^-100 to 2^100, of both signs, zeros among them: every row counts in the softmax sum."""
+    g = torch.Generator().manual_seed(d)
+    lens = [40, 333]
+    kc, vc, table = build_cache(device, lens, hkv, d, bs, d + 1, scales=([0.9] * hkv, [0.4] * hkv))
+    n = vc.shape[0] * vc.shape[1] * hkv
+    s = (2.0 ** (200 * torch.rand(n, generator=g) - 100)) * torch.randint(-1, 2, (n,), generator=g).float()
+    _put_scales(vc, s)
+    print(f"scales d={d} hq={hq} drafts={drafts}", flush=True)
+    _tree_and_decode(device, kc, vc, table, lens, drafts, randn((len(lens) * drafts, hq, d), d + 2), 1 / math.sqrt(d),
+                     torch.bfloat16)
+
+
+@pytest.mark.parametrize("small", [0.0, 2.0 ** -120, -2.0 ** -64, 1.0])
+@pytest.mark.parametrize("large", [2.0 ** 63, -2.0 ** 100, 2.0 ** 116])
+@pytest.mark.parametrize("d", [64, 128, 256, 96])
+def test_two_rows_of_one_weight_and_distant_scales(native_ops, device, d, small, large):
+    """Two rows with the same logit: the output is half of the large one (and of the small one)."""
+    kc, vc, table = build_cache(device, [2], 2, d, 16, d, scales=([0.9] * 2, [0.4] * 2))
+    kc.view(-1, d + 4)[:, :d] = 0
+    for t, s in ((0, small), (1, large)):
+        _put_scales(vc[int(table[0, 0]), t], torch.full((2,), s))
+    print(f"two rows d={d} scales {small:g} {large:g}", flush=True)
+    _tree_and_decode(device, kc, vc, table, [2], 1, randn((1, 4, d), 5), 1 / math.sqrt(d), torch.bfloat16)
+    _put_scales(vc[int(table[0, 0]), 0], torch.full((2,), large))
+    _put_scales(vc[int(table[0, 0]), 1], torch.full((2,), small))
+    _tree_and_decode(device, kc, vc, table, [2], 1, randn((1, 4, d), 6), 1 / math.sqrt(d), torch.bfloat16)
+
+
+@pytest.mark.parametrize("d", [64, 256])
+def test_scales_that_grow_along_the_rows(native_ops, device, d):
+    """Weights fall while scales rise, tile by tile: what was summed first keeps its part."""
+    lens, hkv = [900], 2
+    kc, vc, table = build_cache(device, lens, hkv, d, 64, d, scales=([0.9] * hkv, [0.4] * hkv))
+    at = torch.full((vc.shape[0] * vc.shape[1],), 0)
+    at[(table[0, :15, None].long() * 64 + torch.arange(64)).flatten()] = torch.arange(960)
+    for rise in (0.2, -0.2):
+        _put_scales(vc, (2.0 ** (rise * (at - 450).float()))[:, None].expand(-1, hkv).contiguous())
+        _tree_and_decode(device, kc, vc, table, lens, 5, randn((5, 4, d), 7), 1 / math.sqrt(d), torch.bfloat16)
+    # Weights that fall as the scales rise, over 2^108 (a weight below 2^-126 of the largest is zero in float32).
+    kc.view(-1, hkv, d + 4)[:, :, :d] = 0
+    kc.view(-1, hkv, d + 4)[:, :, 0] = 8
+    assert DECODE[8] == 1.0
+    q = torch.zeros(5, 4, d, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    for rise in (0.12, -0.12):
+        by = rise * (at - 450).float()
+        _put_scales(vc, (2.0 ** by)[:, None].expand(-1, hkv).contiguous())
+        _put_scales(kc, (-math.log(2) * by)[:, None].expand(-1, hkv).contiguous())
+        _tree_and_decode(device, kc, vc, table, lens, 5, q, 1.0, torch.bfloat16)
