@@ -135,12 +135,13 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 //   * w = 2^(x - m) is the weight, summed in FP32, and P = w s f in fp16 goes to
 //     LDS: s is V's row scale, so that V itself stays the exact dec(code), and f a
 //     power of two per query row that puts the largest |P| in (1/4, 1] 2^kTop.
-//     m and f stand until some |P| passes 2^15 (or the sum of w 2^40); then the
+//     m and f stand until some |P| passes fp16's range (or the sum of w 2^40); then the
 //     wavefronts' largest x and x + log2 |s| meet in LDS, O and the sum are scaled
 //     and P is written again, so nearly all tiles have one barrier.  m follows
 //     the logits alone and f what is multiplied with V: with one reference for
 //     both, rows whose scales lie 2^126 apart fell out of the sum.  P is rounded
-//     once: 2^-11 of it, or 2^-25 where it is subnormal (below 2^-14);
+//     once: 2^-11 of it, or 2^-25 where it is subnormal (below 2^-14), which is at
+//     most 2^-31 of the row's largest;
 //   * O^T += V^T P^T: every wavefront takes 64 dims of 32 or 64 rows, 4 bytes of
 //     each row per lane, transposed by the lookup itself (byte q of eight words).
 // The next tile's K loads are issued as soon as S is done, its V loads after O.
@@ -156,8 +157,15 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 // the cache for itself, took 195 us.  Short calls (512 rows) are latency: 10 us
 // and 4.5 for the join, of which the dependent reads of lengths, table and rows
 // are three round trips to HBM.
-constexpr float kTop = 2.f;          // log2 of what P stays below where its power of two is chosen
-constexpr float kMost = 15.f;        // and of what makes the wavefronts choose again: fp16 ends at 2^16
+// log2 of what P stays below where its power of two is chosen.  Below 2^-14 P is
+// subnormal, so the higher it starts the smaller the weights that keep their bits
+// beside a large one of a V near zero (a first token that draws all attention);
+// the lower, the seldomer rows outgrow fp16.  At 8 a weight of 2^-24 keeps 2^-7 of
+// itself.  8 x 16k, 32 drafts: 109.6 us with 2, 111.7 with 6, 114.3 with 8, 121.5
+// with 10; ragged trees 45.4, 46.8, 48.7, 51.6; decode 59.8, 59.9, 60.1, 60.2.
+// Rows that have grown past it move back whenever the wavefronts meet (only those
+// about to overflow: 123 us with 8).
+constexpr float kTop = 8.f;
 constexpr float kLazy = 14.f;        // log2 of what a weight may reach before a new choice moves the maximum too
 constexpr float kMostSum = 0x1p40f;  // weights that add up to more are chosen again without a large P (V scales near zero)
 
@@ -619,7 +627,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
                   uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
       }
       // A row that has seen nothing yet has no maximum: what it sees first sets one.
-      grow |= (most > 0x1p15f) | (psum[rb] > kMostSum) | ((m[rb] == -__builtin_inff()) & (kAll | (seen[rb] != 0)));
+      grow |= (most > 65504.f) | (psum[rb] > kMostSum) | ((m[rb] == -__builtin_inff()) & (kAll | (seen[rb] != 0)));
     };
     auto put = [&]() __attribute__((always_inline)) { rows_with(full, weights); };
     if (it > 0) {
@@ -658,7 +666,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
         const bool rise = tx > m[rb] + kLazy || (tx > m[rb] && ty - m[rb] > 127.f);
         const float m_new = rise ? tx : m[rb];
         const float lf = float(__builtin_amdgcn_frexp_expf(f[rb]) - 1);  // f = 2^lf; P < 2^(ty - m + lf)
-        if (rise || ty - m_new + lf > kMost) {
+        if (rise || ty - m_new + lf > kTop) {
           // O is in units of 2^(m - lf), which only grows: what it holds stays in range.
           const bool none = m[rb] == -__builtin_inff();
           const float lf_new = fminf(fmaxf(floorf(m_new - fmaxf(none ? m[rb] : m[rb] - lf, ty - kTop)), -126.f), 126.f);

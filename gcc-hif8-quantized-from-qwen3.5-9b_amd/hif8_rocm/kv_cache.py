@@ -459,8 +459,8 @@ def tree_attention(
     usually, itself.  A draft that sees nothing gets zeros, and so do rows that
     ``query_start_loc`` gives to no request (a padded batch); what is not seen
     has no influence, NaN and infinities included.
-    Weights have 16 bits beside V, so an infinite V whose weight is below 2^-25
-    of the row's largest gives NaN, as zero times infinity.
+    Weights have 16 bits beside V, so an infinite V whose weight is below 2^-31
+    of the row's largest may give NaN, as zero times infinity.
 
     The request split is given as for :func:`paged_attention`.  ``max_seq_len``
     bounds ``context_lens[b] + query_lens[b]``; with device tensors pass it and

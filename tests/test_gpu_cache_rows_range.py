@@ -13,7 +13,7 @@ from _rows import DECODE, Softmax, tree_reference
 
 pytestmark = pytest.mark.gpu
 I32 = torch.int32
-TOP = 2
+TOP = 8
 
 
 def _stale(shape, dtype, device):
@@ -174,3 +174,24 @@ def test_scales_that_grow_along_the_rows(native_ops, device, d):
         _put_scales(vc, (2.0 ** by)[:, None].expand(-1, hkv).contiguous())
         _put_scales(kc, (-math.log(2) * by)[:, None].expand(-1, hkv).contiguous())
         _tree_and_decode(device, kc, vc, table, lens, 5, q, 1.0, torch.bfloat16)
+
+
+@pytest.mark.parametrize("d, hq, hkv, drafts", [(256, 4, 4, 1), (256, 16, 4, 5), (256, 16, 2, 4), (128, 16, 2, 8), (64, 8, 4, 3)])
+def test_small_weights_beside_a_large_one_of_an_empty_v(native_ops, device, d, hq, hkv, drafts):
+    """A first row that draws nearly all attention and whose V is zero: the output is what the others, at 2^-27
+    to 2^-25 each, add up to."""
+    lens = [300] * 130                            # more requests than workers: a request's rows lie in one part
+    kc, vc, table = build_cache(device, lens, hkv, d, 16, d + hq, scales=([0.9] * hkv, [0.4] * hkv))
+    g = torch.Generator().manual_seed(d)
+    kc.view(-1, hkv, d + 4)[:, :, :d] = 0
+    kc.view(-1, hkv, d + 4)[:, :, 0] = 8
+    assert DECODE[8] == 1.0
+    first = table[:, 0].long().to(device)
+    logit = -math.log(2) * (25 + 2 * torch.rand(kc.shape[0] * 16, hkv, generator=g))
+    _put_scales(kc, logit)
+    kc[first, 0, :, 0] = 0                        # logit 0
+    vc[first, 0, :, :d] = 0
+    q = torch.zeros(len(lens) * drafts, hq, d, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    print(f"sink d={d} hq={hq} drafts={drafts}", flush=True)
+    _tree_and_decode(device, kc, vc, table, lens, drafts, q, 1.0, torch.bfloat16)
