@@ -459,8 +459,10 @@ def tree_attention(
     usually, itself.  A draft that sees nothing gets zeros, and so do rows that
     ``query_start_loc`` gives to no request (a padded batch); what is not seen
     has no influence, NaN and infinities included.
-    Weights have 16 bits beside V, so an infinite V whose weight is below 2^-31
-    of the row's largest may give NaN, as zero times infinity.
+    Weights are float32 numbers and have 16 bits beside V: a weight below 2^-31
+    of its row's largest (2^-126 for other head sizes than 64, 128 and 256) may
+    count as zero, and an infinite V under it then gives NaN instead of an
+    infinity.
 
     The request split is given as for :func:`paged_attention`.  ``max_seq_len``
     bounds ``context_lens[b] + query_lens[b]``; with device tensors pass it and
@@ -577,7 +579,8 @@ def paged_decode_attention_weights(
     ``key_weights`` (float32 ``[B, Hkv, at least max_seq_len]``, contiguous)
     receives, in place, the sum of the row's softmax weights over the query
     heads of each KV head: added, or stored with ``accumulate=False``.  Entries
-    from ``seq_lens[b]`` on are left as they were.
+    from ``seq_lens[b]`` on are left as they were.  What :func:`tree_attention` says of
+    small weights beside an infinite V holds here too.
     """
     _check_caches(key_cache, value_cache)
     if query.ndim != 3:

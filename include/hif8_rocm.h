@@ -401,7 +401,9 @@ int hif8_paged_prefill_attention(const void *query, int q_dtype, const uint8_t *
  *   out [total_query_tokens, num_heads, Dv] in the query dtype: softmax(scale * q . K) V over
  *     the rows seen, K and V dec(code) * row scale; a row that sees nothing gets zeros,
  *     and what is not seen has no influence, whatever it holds.  Cache rows whose block id
- *     lies outside [0, num_blocks) are left out.  Rows before query_start_loc[0] or from
+ *     lies outside [0, num_blocks) are left out.  Weights are FP32 numbers and meet V in 16
+ *     bits (head sizes 64, 128, 256): one below 2^-31 of its row's largest may count as zero,
+ *     and an infinite V under it then gives NaN instead of an infinity.  Rows before query_start_loc[0] or from
  *     query_start_loc[batch] on are not written; hif8_tree_attention_padded, which is the
  *     same call otherwise, gives them zeros (batch > 0), for an `out` that nobody has filled.
  *   workspace  at least hif8_tree_attention_workspace_size(...) bytes, 16-byte aligned; its
@@ -432,7 +434,8 @@ int hif8_tree_attention_padded(const void *query, int q_dtype, const uint8_t *ke
  * for t < seq_lens[b]; later entries are left as they were.
  *   key_weights [batch, num_kv_heads, weights_stride] float32, weights_stride >= max_seq_len
  *   accumulate  0 stores the sums instead of adding them
- * The other arguments are those of hif8_paged_decode_attention.
+ * The other arguments are those of hif8_paged_decode_attention; small weights beside an
+ * infinite V as in hif8_tree_attention.
  */
 size_t hif8_paged_decode_attention_weights_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
                                                           int64_t head_size, int64_t head_size_v,

@@ -195,3 +195,38 @@ def test_small_weights_beside_a_large_one_of_an_empty_v(native_ops, device, d, h
     q[..., 0] = 1.0
     print(f"sink d={d} hq={hq} drafts={drafts}", flush=True)
     _tree_and_decode(device, kc, vc, table, lens, drafts, q, 1.0, torch.bfloat16)
+
+
+@pytest.mark.parametrize("d, hq, hkv, bs", [(256, 16, 4, 128), (128, 24, 8, 16), (64, 8, 2, 16), (96, 4, 2, 20)])
+def test_infinite_v_under_small_weights(native_ops, device, d, hq, hkv, bs):
+    """Infinite codes in context rows: an infinity of their sign where the weight is above 2^-31 of the row's
+    largest, no finite number where it is below, and the other dims as if the codes were finite."""
+    from hif8_rocm import kv_cache
+
+    lens, drafts = [200], 3
+    kc, vc, table = build_cache(device, lens, hkv, d, bs, d, scales=([0.9] * hkv, [0.4] * hkv))
+    kc.view(-1, hkv, d + 4)[:, :, :d] = 0
+    kc.view(-1, hkv, d + 4)[:, :, 0] = 8
+    q = torch.zeros(drafts, hq, d, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    at = {0: 0.0, 3: -20.0, 9: -29.0, 150: -60.0}     # base-2 logits; every other row 2^-40
+    _put_scales(kc, torch.full((kc.shape[0] * bs, hkv), -40 * math.log(2)))
+    plain = vc.clone()
+    for t, x in at.items():
+        blk, row = int(table[0, t // bs]), t % bs
+        _put_scales(kc[blk, row], torch.full((hkv,), x * math.log(2)))
+        if t:
+            vc[blk, row, :, t // 3] = 0xEF if t == 9 else 0x6F
+    mask = torch.ones(drafts, drafts, dtype=torch.bool, device=device)
+    w = torch.zeros(1, hkv, 200, device=device)
+    print(f"infinite V d={d}", flush=True)
+    for call in (lambda v: kv_cache.tree_attention(q.to(device), kc, v, table.to(device), [197], mask, scale=1.0,
+                                                   query_lens=[drafts]),
+                 lambda v: kv_cache.paged_decode_attention_weights(q[:1].to(device), kc, v, table.to(device), lens, w,
+                                                                   scale=1.0)):
+        got, want = call(vc), call(plain)
+        dims = torch.ones(d, dtype=torch.bool)
+        dims[[1, 3, 50]] = False
+        assert torch.equal(got[..., dims.to(device)], want[..., dims.to(device)]) and torch.isfinite(want).all()
+        assert (got[..., 1] == math.inf).all() and (got[..., 3] == -math.inf).all()
+        assert not torch.isfinite(got[..., 50]).any()
