@@ -20,8 +20,8 @@ struct RowAttnParams {
   const int32_t *lens;         // [batch]
   const uint8_t *mask;         // [total_q, mask_stride] or null
   void *out;                   // [total_q, Hq, Dv]
-  // Partial outputs and (maximum, sum): any-shape kernel [total_q * Hq, num_splits],
-  // matrix cores [workers + batch, Hkv, rows_cap].
+  // Partial outputs and (maximum, sum): any-shape kernel [total_q * Hq, num_splits] (outputs: two splits or more),
+  // matrix cores [2 workers, Hkv, rows_cap] and [workers + batch, Hkv, rows_cap].
   float *part_o;
   float *part_ml;
   int32_t *plan;               // matrix cores: [batch + 1] tiles before each request

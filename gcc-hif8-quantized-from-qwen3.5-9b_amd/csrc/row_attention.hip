@@ -108,14 +108,16 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
     p.part_ml[2 * part] = mx;
     p.part_ml[2 * part + 1] = total;
   }
-  if (!(total != 0.f)) return;  // nothing seen: this split's outputs are not read
-  const float inv = 1.f / total;
+  const bool whole = p.num_splits == 1;      // the join leaves the output to this workgroup
+  if (!whole && !(total != 0.f)) return;     // nothing seen: this split's outputs are not read
+  const float inv = total != 0.f ? 1.f / total : 0.f;
   for (int dim = threadIdx.x; dim < p.dv; dim += kThreads) {
     float y = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
       if (f[w] != 0.f) y += f[w] * red_o[w][dim];
-    p.part_o[part * p.dv + dim] = y * inv;
+    if (whole) static_cast<uint16_t *>(p.out)[size_t(blockIdx.x) * p.dv + dim] = float_to_half_bits<kBf16>(y * inv);
+    else p.part_o[part * p.dv + dim] = y * inv;
   }
 }
 
@@ -323,11 +325,15 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   const int tile_first = cur - first;
   const int seg_tiles = min(run_end - cur, int((uint32_t(len) + kT - 1) / kT) - tile_first);
   cur += seg_tiles;
+  const bool last_of_run = cur >= run_end;
   if (rt * kRows >= rows) continue;  // uniform: the request has no query rows here
   const int t_begin = tile_first * kT, t_end = min(t_begin + seg_tiles * kT, len);
   const int ntiles = seg_tiles;
   const bool whole = t_begin == 0 && t_end == len;  // this segment holds all of the request's cache rows
+  // Rows of part_ml and part_o.  Only the first and the last segment of a run can hold
+  // a part of a request: two places per worker, however many requests there are.
   const size_t part_row = (size_t(worker) + b) * p.hkv + h;
+  const size_t part_out = (size_t(2 * worker) + (last_of_run ? 1 : 0)) * p.hkv + h;
 
   // The query token of row r: r / group.
   auto token_of = [&](int r) { return int(__umulhi(2u * uint32_t(r), p.group_magic)); };
@@ -804,7 +810,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
       for (int w = 1; w < kW; ++w) sum += sm.top[0][w][16 * rb + n];
       // O / (l f): l first, f is a power of two that may be far from one.
       const float inv = sum != 0.f ? 1.f / sum : 0.f, inv_f = 1.f / f[rb];
-      const size_t r = part_row * p.rows_cap + size_t(rt * kRows + 16 * rb + n);
+      const size_t in_part = size_t(rt * kRows + 16 * rb + n);
       const int dim = 64 * vslice + 16 * g;  // element e of accumulator q: dim + 4 e + q
       if (whole) {
         uint32_t w[8];
@@ -817,12 +823,13 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
         o[0] = lk_u32x4{w[0], w[1], w[2], w[3]};
         o[1] = lk_u32x4{w[4], w[5], w[6], w[7]};
       } else {
-        lk_f32x4 *po = reinterpret_cast<lk_f32x4 *>(p.part_o + r * kD + dim);
+        lk_f32x4 *po = reinterpret_cast<lk_f32x4 *>(p.part_o + (part_out * p.rows_cap + in_part) * kD + dim);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           po[e] = lk_f32x4{oacc[rb][0][e], oacc[rb][1][e], oacc[rb][2][e], oacc[rb][3][e]} * inv * inv_f;
       }
       if (g == 0 && vslice == 0) {
+        const size_t r = part_row * p.rows_cap + in_part;
         p.part_ml[2 * r] = m[rb];
         p.part_ml[2 * r + 1] = sum;
       }
@@ -846,10 +853,14 @@ constexpr int kSliceDims = 64;
 constexpr int kWeightKeys = 4 * kThreads;
 
 // Where the partial results of query row `row` (request b, its row `tok`) and
-// `head` lie: `count` of them, `stride` apart.  None: it saw nothing.
+// `head` lie: `count` of them, (maximum, sum) `stride` rows apart from `first` on,
+// outputs o_stride apart from o_first on, the last of them o_back rows before.
+// None: it saw nothing.
 struct Parts {
   size_t first, stride;
   int count;
+  size_t o_first, o_stride, o_back;
+  __device__ size_t output(int s) const { return o_first + s * o_stride - (s == count - 1 ? o_back : 0); }
 };
 
 __device__ __forceinline__ Parts parts_of(const RowAttnParams &p, int b, int row, int tok, int head) {
@@ -857,22 +868,34 @@ __device__ __forceinline__ Parts parts_of(const RowAttnParams &p, int b, int row
     int begin, count;
     request_rows(p, b, begin, count);
     const int len = rows_seen(p, clamp_rows(p.lens[b], p.max_len), count);
-    return Parts{(size_t(row) * p.hq + head) * p.num_splits, 1, (len + p.split_tokens - 1) / p.split_tokens};
+    const size_t first = (size_t(row) * p.hq + head) * p.num_splits;
+    return Parts{first, 1, (len + p.split_tokens - 1) / p.split_tokens, first, 1, 0};
   }
   // Tiles lo .. hi - 1 are the request's; worker w of them has floor(total w / workers) on.
   const int total = p.plan[p.batch], lo = p.plan[b], hi = p.plan[b + 1];
   const int64_t in_request = int64_t(tok) * p.group + head % p.group;
-  if (lo == hi || in_request >= p.rows_cap) return Parts{0, 1, 0};  // nothing seen, or past the longest request told
+  if (lo == hi || in_request >= p.rows_cap) return Parts{0, 1, 0, 0, 1, 0};  // nothing seen, or past the longest request told
   const int workers = min(p.workers, total);
-  int w0, w1;
+  int w0, w1, w1_end;
   if (total < 1 << 22) {  // workers is at most 512: the division has 32 bits
     w0 = int((uint32_t(lo + 1) * uint32_t(workers) - 1) / uint32_t(total));
     w1 = int((uint32_t(hi) * uint32_t(workers) - 1) / uint32_t(total));
+    w1_end = int(uint32_t(total) * uint32_t(w1 + 1) / uint32_t(workers));
   } else {
     w0 = int((int64_t(lo + 1) * workers - 1) / total);
     w1 = int((int64_t(hi) * workers - 1) / total);
+    w1_end = int(int64_t(total) * (w1 + 1) / workers);
   }
-  return Parts{((size_t(w0) + b) * p.hkv + head / p.group) * p.rows_cap + size_t(in_request), size_t(p.hkv) * p.rows_cap, w1 - w0 + 1};
+  // The request's segment is the last of every worker's run but w1's, which goes on
+  // with other requests unless it ends with this one.
+  const size_t step = size_t(p.hkv) * p.rows_cap, within = size_t(head / p.group) * p.rows_cap + size_t(in_request);
+  return Parts{(size_t(w0) + b) * step + within, step, w1 - w0 + 1, size_t(2 * w0 + 1) * step + within, 2 * step,
+               w1_end > hi ? step : 0};
+}
+
+// Whether the attention kernel has written this query row's output itself.
+__device__ __forceinline__ bool written(const RowAttnParams &p, const Parts &parts) {
+  return p.workers > 0 ? parts.count == 1 : p.num_splits == 1;
 }
 
 // (M, 1 / L) over the parts; every lane of the calling wavefront gets them.
@@ -914,16 +937,15 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     int begin, count;
     request_rows(p, b, begin, count);
     const Parts parts = parts_of(p, b, row, row - begin, int(r) - row * p.hq);
-    if (p.workers > 0 && parts.count == 1) return;  // written already
+    if (written(p, parts)) return;
     float m, inv;
     join_stats(p, parts, m, inv);
     for (int d4 = 4 * lane; d4 < p.dv; d4 += 4 * kWave) {
-      const float *po = p.part_o + parts.first * p.dv + d4;
       f32x4_t acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
       for (int s = 0; s < parts.count; ++s) {
         const float *ml = p.part_ml + 2 * (parts.first + s * parts.stride);
-        const f32x4_t v = *reinterpret_cast<const f32x4_t *>(po + size_t(s) * parts.stride * p.dv);
+        const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p.part_o + parts.output(s) * p.dv + d4);
         // A part that saw nothing was not written (any-shape kernel): its rubbish may be no number.
         if (ml[1] != 0.f) acc += __builtin_amdgcn_exp2f(ml[0] - m) * ml[1] * inv * v;
       }
@@ -944,7 +966,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     int begin, count;
     request_rows(p, b, begin, count);
     const Parts parts = parts_of(p, b, row, row - begin, r - row * p.hq);
-    if (p.workers > 0 && parts.count == 1) return;  // uniform: written already
+    if (written(p, parts)) return;  // uniform
     float m, inv;
     join_stats(p, parts, m, inv);
     if (wave == 0)
@@ -956,9 +978,8 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     const int d4 = slice * kSliceDims + 4 * (tid & 15), g = tid >> 4;
     f32x4_t acc{0.f, 0.f, 0.f, 0.f};
     if (d4 < p.dv) {
-      const float *po = p.part_o + parts.first * p.dv + d4;
       for (int s = g; s < parts.count; s += kThreads / 16)
-        if (fac[s] != 0.f) acc += fac[s] * *reinterpret_cast<const f32x4_t *>(po + size_t(s) * parts.stride * p.dv);
+        if (fac[s] != 0.f) acc += fac[s] * *reinterpret_cast<const f32x4_t *>(p.part_o + parts.output(s) * p.dv + d4);
     }
     *reinterpret_cast<f32x4_t *>(&red[g][4 * (tid & 15)]) = acc;
     __syncthreads();
@@ -1010,7 +1031,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
 struct RowPlan {
   int split_tokens, num_splits;              // any-shape kernel
   int row_blocks, row_tiles, workers, tile_rows;  // matrix cores: 16-row blocks of a workgroup (0: any-shape kernel)
-  int64_t parts;                             // partial results: rows of part_o and part_ml
+  int64_t parts, outputs;                    // partial results: rows of part_ml and of part_o
   uint32_t magic;                            // ceil(2^31 / 16-row groups of a page)
 };
 
@@ -1034,6 +1055,7 @@ RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int6
     pl.split_tokens = int((len + splits - 1) / splits);
     pl.num_splits = int((len + pl.split_tokens - 1) / pl.split_tokens);
     pl.parts = total_q * heads * pl.num_splits;
+    pl.outputs = pl.num_splits > 1 ? pl.parts : 0;
     return pl;
   }
   const int64_t rows = std::max<int64_t>(max_query, 1) * (heads / hkv);
@@ -1046,6 +1068,7 @@ RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int6
   const int64_t slots = 2048 / waves_of(pl.row_blocks) / (hkv * pl.row_tiles);
   pl.workers = int(std::min<int64_t>(std::max<int64_t>(slots, 1), tiles));
   pl.parts = (pl.workers + batch) * hkv * pl.row_tiles * 16 * pl.row_blocks;
+  pl.outputs = 2 * pl.workers * hkv * pl.row_tiles * 16 * pl.row_blocks;
   return pl;
 }
 
@@ -1061,7 +1084,7 @@ RowSpace row_space(const RowPlan &pl, int64_t batch, int64_t total_q, int64_t he
                    bool weights) {
   auto round = [](size_t v) { return (v + 255) / 256 * 256; };
   RowSpace w{};
-  w.o = round(size_t(pl.parts) * dv * sizeof(float));
+  w.o = round(size_t(pl.outputs) * dv * sizeof(float));
   w.ml = round(size_t(pl.parts) * 2 * sizeof(float));
   if (weights) w.x = round(size_t(total_q) * heads * size_t(x_stride_of(max_len)) * sizeof(float));
   if (pl.row_blocks) w.plan = round(size_t(batch + 1) * sizeof(int32_t));

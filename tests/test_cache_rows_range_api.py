@@ -34,3 +34,17 @@ def test_the_padded_tree_entry_refuses_what_the_other_does(lib):
                            ({"mq": 0}, 1, b"max_query_len"), ({"mq": -1}, 1, b"positive"), ({}, 1, b"workspace of")]:
         assert call(**kw) == code and text in lib.hif8_last_error(), (kw, lib.hif8_last_error())
     assert call(batch=0) == 0 and call(total=0) == 0
+
+
+def test_workspaces_hold_no_output_per_request(lib):
+    """Partial outputs are those of the workers, of which there are as many as the GPU runs at a time: more requests
+    add their statistics (8 bytes per query row) and, in the decode form, their logits."""
+    tree = lib.hif8_tree_attention_workspace_size
+    tree.argtypes, tree.restype = [ctypes.c_int64] * 9, ctypes.c_size_t
+    few, many = (tree(b, 16, 4, 256, 256, 128, 64 * b, 64, 4096) for b in (16, 256))
+    assert many <= 64 << 20
+    assert many - few <= 240 * (64 * 16 * 8 + 4) + 1024
+    decode = lib.hif8_paged_decode_attention_weights_workspace_size
+    decode.argtypes, decode.restype = [ctypes.c_int64] * 7, ctypes.c_size_t
+    few, many = (decode(b, 16, 4, 256, 256, 128, 4096) for b in (256, 1024))
+    assert many - few <= 768 * (16 * 4096 * 4 + 4 * 16 * 8 + 4) + 1024

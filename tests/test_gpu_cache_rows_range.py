@@ -105,6 +105,7 @@ def _tree_and_decode(device, kc, vc, table, lens, drafts, q, scale, dtype):
     keeps its weights."""
     from hif8_rocm import kv_cache
 
+    assert q.dtype == dtype   # the output's type, whose rounding the bound counts
     batch, hkv = len(lens), kc.shape[2]
     everything = lambda b, n, m: np.ones((m, n), dtype=bool)  # noqa: E731
     args = dict(scale=scale)
@@ -230,3 +231,12 @@ def test_infinite_v_under_small_weights(native_ops, device, d, hq, hkv, bs):
         assert torch.equal(got[..., dims.to(device)], want[..., dims.to(device)]) and torch.isfinite(want).all()
         assert (got[..., 1] == math.inf).all() and (got[..., 3] == -math.inf).all()
         assert not torch.isfinite(got[..., 50]).any()
+
+
+@pytest.mark.parametrize("lens", [[512] * 4, [1024, 1024], [640, 1408], [128] * 5 + [1280, 300], [2048], [100] * 40 + [4000]])
+def test_runs_that_end_with_or_within_a_request(native_ops, device, lens):
+    """16 workers over 16 tiles or more: parts that end where a worker's run ends, and parts that do not."""
+    kc, vc, table = build_cache(device, lens, 32, 64, 16, len(lens))
+    print(f"runs lens={lens[:8]}", flush=True)
+    for dtype in (torch.bfloat16, torch.float16):
+        _tree_and_decode(device, kc, vc, table, lens, 3, randn((len(lens) * 3, 32, 64), 5, 1.0, dtype), 0.125, dtype)
