@@ -480,7 +480,8 @@ int hif8_key_weights(const void *query, int q_dtype, const uint8_t *key_cache, i
  *     unspecified, the accesses stay inside the cache
  *   new_lens [batch] int32 (may be NULL): context_lens[b] + accepted_counts[b]
  * Rows outside the table or in a block outside [0, num_blocks) are skipped.  The pages
- * that are written must belong to one request.
+ * that are written must belong to one request.  Without caches or requests nothing is
+ * done: the call succeeds and new_lens is left as it was.
  */
 int hif8_accept_drafts(void *const *caches, const int64_t *row_bytes, int64_t num_caches, int64_t num_blocks,
                        int64_t block_size, const void *block_table, int block_table_dtype,

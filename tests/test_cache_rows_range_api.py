@@ -48,3 +48,15 @@ def test_workspaces_hold_no_output_per_request(lib):
     decode.argtypes, decode.restype = [ctypes.c_int64] * 7, ctypes.c_size_t
     few, many = (decode(b, 16, 4, 256, 256, 128, 4096) for b in (256, 1024))
     assert many - few <= 768 * (16 * 4096 * 4 + 4 * 16 * 8 + 4) + 1024
+
+
+def test_acceptance_without_caches_or_requests_writes_nothing(lib):
+    i64, ptr, i32 = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int
+    accept = lib.hif8_accept_drafts
+    accept.argtypes = [ptr, ptr, i64, i64, i64, ptr, i32, i64, ptr, ptr, i64, ptr, i64, ptr, ptr]
+    lens = (ctypes.c_int32 * 2)(7, 9)
+    for caches, batch in ((0, 2), (1, 0)):
+        arr, rows = (ctypes.c_void_p * 1)(256), (i64 * 1)(1040)
+        assert accept(arr, rows, caches, 8, 128, _p(), 0, 4, _p(), _p(), 4, _p(), batch,
+                      ctypes.cast(lens, ctypes.c_void_p), None) == 0
+        assert list(lens) == [7, 9]
