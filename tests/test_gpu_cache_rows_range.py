@@ -240,3 +240,75 @@ def test_runs_that_end_with_or_within_a_request(native_ops, device, lens):
     print(f"runs lens={lens[:8]}", flush=True)
     for dtype in (torch.bfloat16, torch.float16):
         _tree_and_decode(device, kc, vc, table, lens, 3, randn((len(lens) * 3, 32, 64), 5, 1.0, dtype), 0.125, dtype)
+
+
+@pytest.mark.parametrize("hq, hkv, d, bs", [(16, 4, 256, 128), (24, 8, 128, 16), (8, 8, 64, 32), (6, 2, 20, 12)])
+def test_requests_of_a_batch_are_what_they_are_alone(native_ops, device, hq, hkv, d, bs):
+    """A batch against float64, and every request of it against a call of its own."""
+    from hif8_rocm import kv_cache
+
+    ctx, qlens = [3000, 40, 0, 517], [30, 6, 3, 1]
+    lens = [c + n for c, n in zip(ctx, qlens)]
+    kc, vc, table = build_cache(device, lens, hkv, d, bs, 11)
+    q = randn((sum(qlens), hq, d), 12)
+    mask = np.random.default_rng(13).random((sum(qlens), max(qlens))) < 0.4
+    starts = np.cumsum([0] + qlens)
+
+    def sees(b, n, m):
+        return np.concatenate([np.ones((m, ctx[b]), dtype=bool), mask[starts[b]:starts[b + 1], :m]], axis=1)
+
+    def call(rows, which):
+        return kv_cache.tree_attention(q[rows].to(device), kc, vc, table[which].to(device), [ctx[b] for b in which],
+                                       torch.from_numpy(mask[rows]).to(device), scale=1 / math.sqrt(d),
+                                       query_lens=[qlens[b] for b in which])
+
+    print(f"batch and alone d={d}", flush=True)
+    want, bound, _, _ = _attention(q.double().numpy(), kc, vc, table, lens, qlens, sees, 1 / math.sqrt(d), q.dtype)
+    out = call(slice(0, sum(qlens)), [0, 1, 2, 3])
+    _near(out, want, bound)
+    for b in range(4):
+        rows = slice(int(starts[b]), int(starts[b + 1]))
+        alone = call(rows, [b])
+        _near(alone, want[rows], bound[rows])
+        assert torch.equal(alone, call(rows, [b]))
+        _near(alone, out[rows].double().cpu().numpy(), 2 * bound[rows])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_key_weights_of_an_unaligned_query(native_ops, device, d):
+    """A query that does not start at 16 bytes: the any-shape kernels, in the workspace of the others."""
+    from hif8_rocm import kv_cache
+
+    hq, hkv, lens = 8, 2, [333, 90]
+    kc, vc, table = build_cache(device, lens, hkv, d, 32, d)
+    w = torch.zeros(2, hkv, 340, device=device)
+    for rows in ([1, 1], [70, 33]):
+        n = sum(rows)
+        flat = randn((1 + n * hq * d,), 3).to(device)
+        q = flat[1:].view(n, hq, d)
+        assert q.data_ptr() % 16 and q.is_contiguous()
+        print(f"unaligned query d={d} rows={rows}", flush=True)
+        sees = lambda b, n, m: np.arange(n) <= n - m + np.arange(m)[:, None]  # noqa: E731
+        want, bound, sums, sums_bound = _attention(q.double().cpu().numpy(), kc, vc, table, lens, rows, sees, 0.1, q.dtype)
+        kv_cache.accumulate_key_weights(q, kc, table.to(device), lens, w, scale=0.1, query_lens=rows, accumulate=False)
+        most = 2.0 ** -24 * max(rows) * (hq // hkv) * sums    # the rows' sum in float32
+        _near(w[..., :333], sums, sums_bound + most)
+        if n == 2:
+            w.zero_()
+            out = kv_cache.paged_decode_attention_weights(q, kc, vc, table.to(device), lens, w, scale=0.1)
+            _near(out, want, bound)
+            _near(w[..., :333], sums, sums_bound)
+
+
+@pytest.mark.parametrize("small", [0.0, 2.0 ** -126, 1.0])
+@pytest.mark.parametrize("d", [64, 128, 256, 96])
+def test_a_v_scale_of_the_largest_exponent(native_ops, device, d, small):
+    """A row scale of -1.75 x 2^127 over codes of +-0.5, beside one of the same weight."""
+    kc, vc, table = build_cache(device, [2], 2, d, 16, d, scales=([0.9] * 2, [0.4] * 2))
+    kc.view(-1, d + 4)[:, :d] = 0
+    assert DECODE[24] == 0.5 and DECODE[24 + 128] == -0.5
+    vc.view(-1, d + 4)[:, :d] = 24 + 128 * torch.randint(0, 2, (vc.numel() // (d + 4), d), device=device).to(torch.uint8)
+    for at, s in ((0, small), (1, -1.75 * 2.0 ** 127)):
+        _put_scales(vc[int(table[0, 0]), at], torch.full((2,), s))
+    print(f"largest scale d={d} beside {small:g}", flush=True)
+    _tree_and_decode(device, kc, vc, table, [2], 1, randn((1, 4, d), 5), 1 / math.sqrt(d), torch.bfloat16)
