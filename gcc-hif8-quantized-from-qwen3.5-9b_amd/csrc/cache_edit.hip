@@ -194,10 +194,10 @@ constexpr int kBins = 2048;
 // within it are ballots and only its totals cross the workgroup.  The ranks of
 // up to 64 kHeld rows per wavefront stay in registers (kHeld 0: they are read
 // again in every pass).  Bound by the latency of one read and about fifteen
-// barriers: 7 us for 600 rows (11 with the move of 88 of them), 20 us for 32 pairs of 16384 rows each (one
-// workgroup per pair leaves most of the GPU idle; the rows that move afterwards
-// take longer than that).  With ranks read again in every pass, digits of eight
-// bits and 4-byte moves, the whole calls took 41 and 117 us; now 16 and 53.
+// barriers: 7 us for 600 rows (11 with the move of 88 of them), 19 us for 32 pairs
+// of 16384 rows each (one workgroup per pair leaves most of the GPU idle), 29 more
+// for the rows that move afterwards.  With ranks read again in every pass, digits of
+// eight bits and 4-byte moves the whole calls took 41 and 117 us.
 template <int kHeld, typename Mover>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(const EvictParams p) {
   __shared__ int hist[kBins];

@@ -38,7 +38,8 @@ __device__ __forceinline__ void fill_lookup(uint32_t *table, uint32_t *entries, 
 }
 
 // One 16-bit table value: code = byte kByte of w; kHigh picks the entry's upper
-// half.  lane_base = LDS address of the table + 4 * lane, below 256 + 4 * 64.
+// half.  lane4 = 4 * lane, the low byte of the offset (the code is the high one);
+// table = the table's LDS address.
 template <int kByte, bool kHigh>
 __device__ __forceinline__ uint16_t look(uint32_t w, uint32_t lane4, uint32_t table) {
   typedef const __attribute__((address_space(3))) uint16_t lds_u16;

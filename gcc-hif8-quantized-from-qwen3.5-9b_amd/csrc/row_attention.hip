@@ -30,7 +30,10 @@ constexpr int kMaxParts = 512;   // parts of a query row: splits, or workers
 
 // Any head size up to 512, group, block size and alignment: a workgroup per
 // (query row, head, split), its wavefronts taking every fourth cache row with a
-// running maximum and sum each, joined through LDS.
+// running maximum and sum each, joined through LDS.  Bound by its lookups in a
+// global table and a reduction over the lanes for every (query head, cached row):
+// 8 x 16 drafts of 16 heads of 96 over 4096 rows take 1.8 ms, where heads of 256
+// take 50 us on the matrix cores.
 template <bool kBf16, typename BtT>
 __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParams p) {
   constexpr int kPerLane = 8;  // head sizes up to 512
@@ -150,21 +153,22 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 // Where there are several parts of a row, each is divided by its own sum and f.
 //
 // What bounds it (16 query and 4 KV heads of 256, 8 x 16384 cached rows, 171 MB):
-// one token per request runs at 3.9 TB/s (43 us), what the card's plain reads
-// reach; 32 tokens each take 106 us, where the LDS lookups (128 per lane and
-// tile), the query operands from LDS and the vector instructions around them
-// add up, as the eight wavefronts go through a tile's phases together.  In
-// cycles per tile there: S 2100 to 2800, loads 1300 + 700, logits 600, P 1200,
+// one token per request runs at 3.9 TB/s (43 us; reads of one head's rows reach 4.4
+// on this layout, a plain stream 6.1); 32 tokens each take 111 us, where the LDS
+// lookups (128 per lane and tile), the query operands from LDS and the vector
+// instructions around them add up, as the eight wavefronts go through a tile's
+// phases together.  In cycles per tile there: S 2100 to 2800, loads 1300 + 700, logits 600, P 1200,
 // O 2400 to 2900.  Two workgroups of 16 query rows per row tile, each decoding
-// the cache for itself, took 195 us.  Short calls (512 rows) are latency: 10 us
-// and 4.5 for the join, of which the dependent reads of lengths, table and rows
+// the cache for itself, took 195 us.  Short calls (512 rows) are latency: 10 to 13
+// us and 5 for the join, of which the dependent reads of lengths, table and rows
 // are three round trips to HBM.
+
 // log2 of what P stays below where its power of two is chosen.  Below 2^-14 P is
 // subnormal, so the higher it starts the smaller the weights that keep their bits
 // beside a large one of a V near zero (a first token that draws all attention);
-// the lower, the seldomer rows outgrow fp16.  At 8 a weight of 2^-24 keeps 2^-7 of
-// itself.  8 x 16k, 32 drafts: 109.6 us with 2, 111.7 with 6, 114.3 with 8, 121.5
-// with 10; ragged trees 45.4, 46.8, 48.7, 51.6; decode 59.8, 59.9, 60.1, 60.2.
+// the lower, the seldomer rows outgrow fp16.  At 8 a weight of 2^-24 is off by at
+// most 2^-7 of itself.  With 2, 6, 8 and 10: 8 x 16k under 32 drafts 109.6, 111.7,
+// 114.3 and 121.5 us, ragged trees 45.4, 46.8, 48.7 and 51.6, decode 59.8 to 60.2.
 // Rows that have grown past it move back whenever the wavefronts meet (only those
 // about to overflow: 123 us with 8).
 constexpr float kTop = 8.f;
@@ -174,7 +178,7 @@ constexpr float kMostSum = 0x1p40f;  // weights that add up to more are chosen a
 // Wavefronts of a workgroup: four, two workgroups to a CU; with 64 query rows
 // eight, one workgroup, since the table and the query rows in LDS leave no room
 // for two and the registers of four none for the rows (24 heads of 128 under 61
-// drafts each: 44 us against 50 in row tiles of 32).
+// drafts each: 44 us against 50 in row tiles of 32; 48 now).
 constexpr int waves_of(int row_blocks) { return row_blocks > 2 ? 8 : 4; }
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
 // Cache rows of a tile.  256 of them at D = 64 left one workgroup to a CU (32

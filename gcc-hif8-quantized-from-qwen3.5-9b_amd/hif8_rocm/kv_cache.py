@@ -460,9 +460,14 @@ def tree_attention(
     ``query_start_loc`` gives to no request (a padded batch); what is not seen
     has no influence, NaN and infinities included.
     Weights are float32 numbers and have 16 bits beside V: a weight below 2^-31
-    of its row's largest (2^-126 for other head sizes than 64, 128 and 256) may
-    count as zero, and an infinite V under it then gives NaN instead of an
-    infinity.
+    of its row's largest may count as zero, and an infinite V under it then gives
+    NaN instead of an infinity.
+
+    Head sizes 64, 128 and 256 (K and V alike) over pages of a multiple of 16
+    rows, with a query that starts at a multiple of 16 bytes, run on the matrix
+    cores.  Every other call takes a kernel for any shape (float32 throughout),
+    which is many times slower: 8 requests of 16 drafts over 4096 rows take
+    50 us with heads of 256 and 1.8 ms with heads of 96.
 
     The request split is given as for :func:`paged_attention`.  ``max_seq_len``
     bounds ``context_lens[b] + query_lens[b]``; with device tensors pass it and
@@ -580,7 +585,8 @@ def paged_decode_attention_weights(
     receives, in place, the sum of the row's softmax weights over the query
     heads of each KV head: added, or stored with ``accumulate=False``.  Entries
     from ``seq_lens[b]`` on are left as they were.  What :func:`tree_attention` says of
-    small weights beside an infinite V holds here too.
+    small weights beside an infinite V, and of the shapes that are fast, holds
+    here too.
     """
     _check_caches(key_cache, value_cache)
     if query.ndim != 3:
@@ -643,7 +649,9 @@ def accumulate_key_weights(
     cache alone and returns nothing.  Request b's query rows are the last
     positions of its ``seq_lens[b]`` cached tokens, given and masked as in
     :func:`paged_attention`.  ``key_weights`` as there; with
-    ``accumulate=False`` the sums are stored instead of added.
+    ``accumulate=False`` the sums are stored instead of added.  Shapes that are
+    fast as in :func:`tree_attention` (of K alone): a prompt of 1024 takes 46 us with
+    heads of 256 and 33 ms with heads of 96.
     """
     if key_cache.dtype != torch.uint8 or key_cache.ndim != 4:
         raise TypeError("key_cache must be a 4-D uint8 tensor")

@@ -408,6 +408,9 @@ int hif8_paged_prefill_attention(const void *query, int q_dtype, const uint8_t *
  *     same call otherwise, gives them zeros (batch > 0), for an `out` that nobody has filled.
  *   workspace  at least hif8_tree_attention_workspace_size(...) bytes, 16-byte aligned; its
  *              size depends on these arguments alone
+ * D = Dv of 64, 128 or 256 over pages of a multiple of 16 rows, with 16-byte aligned query and
+ * out, runs on the matrix cores; any other shape takes a kernel that is many times slower.
+ * The same holds for the two operators below (hif8_key_weights: of D and the query).
  */
 size_t hif8_tree_attention_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
                                           int64_t head_size_v, int64_t block_size, int64_t total_query_tokens,
