@@ -1,6 +1,7 @@
-// Shared by the two operators that run a few query rows per request over the
-// whole HiF8 paged cache: attention of drafted tokens under a tree mask, and
-// decode attention that also accumulates every cached row's softmax weight.
+// Shared by the operators that run a few query rows per request over the HiF8
+// paged cache: attention of drafted tokens under a tree mask, decode attention
+// that also accumulates every cached row's softmax weight, and attention within a
+// sliding window.
 #pragma once
 
 #include "hif8_common.h"
@@ -11,6 +12,9 @@ namespace hif8 {
 // null: row b alone).  It has lens[b] rows that every query row sees; under a
 // tree mask the rows behind them, one per query row of the request, are its
 // drafts, and query row i sees draft j where mask[row of i][j] is not zero.
+// With a window (no mask) lens[b] counts the request's query rows too: they are its
+// last positions, and the one at position P sees the rows t <= P with t > P - window
+// or t < sinks.
 struct RowAttnParams {
   const void *query;           // [total_q, Hq, D]
   const uint8_t *key_cache;    // [num_blocks, block_size, Hkv, D + 4]
@@ -34,6 +38,7 @@ struct RowAttnParams {
   // query rows of all of them (a KV head's), ceil(2^31 / group).
   int workers, row_tiles, rows_cap, heads_together;
   uint32_t group_magic;
+  int window, sinks, most_rows;  // window 0: none; most_rows: bound of WindowRows::rows
   float scale_log2;            // softmax scale * log2(e)
 };
 
@@ -43,6 +48,26 @@ __device__ __forceinline__ int clamp_rows(int n, int most) { return n < 0 ? 0 : 
 // drafts as it has query rows (and the mask columns).
 __device__ __forceinline__ int rows_seen(const RowAttnParams &p, int ctx, int count) {
   return p.mask ? clamp_rows(ctx + int(min(int64_t(count), p.mask_stride)), p.max_len) : ctx;
+}
+
+// The cache rows that the query rows of a request see under a window, pushed
+// together in groups of 16: `head` rows from the first on, then those behind the
+// `skip` rows that no query row sees.  `rows` of them.
+struct WindowRows {
+  int head, skip, rows;
+  // The cache row of pushed-together row t (of its group of 16, where t starts one).
+  __device__ int real(int t) const { return t < head ? t : t + skip; }
+};
+
+__device__ __forceinline__ WindowRows window_rows(const RowAttnParams &p, int len, int count) {
+  const int low = int(max(int64_t(len) - count + 1 - p.window, int64_t(0))) & ~15;  // of the first query row
+  const int head = int(min((int64_t(p.sinks) + 15) & ~int64_t(15), int64_t(low)));
+  return WindowRows{head, low - head, min(len - (low - head), p.most_rows)};
+}
+
+// Whether the query row at position `at` sees cache row t.
+__device__ __forceinline__ bool window_sees(const RowAttnParams &p, int at, int t) {
+  return t <= at && (int64_t(t) > int64_t(at) - p.window || t < p.sinks);
 }
 
 // Query rows of request b, clipped to the query tensor (start_loc is caller data).

@@ -3,6 +3,7 @@
 //   hif8_tree_attention                  drafted tokens under a tree mask
 //   hif8_paged_decode_attention_weights  one token per request, and the sum of
 //                                        its heads' softmax weights per cached row
+//   hif8_window_attention                new tokens within a sliding window
 //
 // o_i = sum_t p_it V_t with p_i = softmax over the rows t that query row i sees
 // of scale * q_i . K_t; a query row that sees nothing gets zeros.  K_t and V_t
@@ -46,7 +47,9 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
   int begin, count;
   request_rows(p, b, begin, count);
   const int ctx = clamp_rows(p.lens[b], p.max_len);
-  const int len = rows_seen(p, ctx, count);
+  const WindowRows win = p.window ? window_rows(p, ctx, count) : WindowRows{ctx, 0, 0};
+  const int at = ctx - count + (row - begin);  // window: this query row's position
+  const int len = p.window ? win.rows : rows_seen(p, ctx, count);
   const int t0 = split * p.split_tokens, t1 = min(t0 + p.split_tokens, len);
   const int h = head / p.group;
   const uint16_t *q = static_cast<const uint16_t *>(p.query) + (size_t(row) * p.hq + head) * p.d;
@@ -62,11 +65,13 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
   }
   float m = -__builtin_inff(), l = 0.f;
   for (int t = t0 + wave; t < t1; t += kWaves) {
-    const int64_t blk = int64_t(bt[t / p.block_size]);
-    const bool seen = blk >= 0 && blk < p.num_blocks && (t < ctx || mask[t - ctx] != 0);
+    const int real = p.window ? win.real(t) : t;
+    const int64_t blk = int64_t(bt[real / p.block_size]);
+    const bool seen = blk >= 0 && blk < p.num_blocks &&
+                      (p.window ? window_sees(p, at, real) : t < ctx || mask[t - ctx] != 0);
     float x = -__builtin_inff();
     if (seen) {
-      const int64_t slot = blk * p.block_size + t % p.block_size;
+      const int64_t slot = blk * p.block_size + real % p.block_size;
       const uint8_t *kr = p.key_cache + (slot * p.hkv + h) * (p.d + 4);
       const uint8_t *vr = p.value_cache + (slot * p.hkv + h) * (p.dv + 4);
       const float ksc = *reinterpret_cast<const float *>(kr + p.d);
@@ -871,7 +876,8 @@ __device__ __forceinline__ Parts parts_of(const RowAttnParams &p, int b, int row
   if (p.workers == 0) {
     int begin, count;
     request_rows(p, b, begin, count);
-    const int len = rows_seen(p, clamp_rows(p.lens[b], p.max_len), count);
+    const int ctx = clamp_rows(p.lens[b], p.max_len);
+    const int len = p.window ? window_rows(p, ctx, count).rows : rows_seen(p, ctx, count);
     const size_t first = (size_t(row) * p.hq + head) * p.num_splits;
     return Parts{first, 1, (len + p.split_tokens - 1) / p.split_tokens, first, 1, 0};
   }
@@ -1095,6 +1101,12 @@ RowSpace row_space(const RowPlan &pl, int64_t batch, int64_t total_q, int64_t he
   return w;
 }
 
+// Cache rows of a request that its query rows can see: all of them, or the window's
+// (WindowRows: whole groups of 16).
+int64_t rows_bound(int64_t max_len, int64_t max_query, int64_t window, int64_t sinks) {
+  return window ? std::min(max_len, (sinks + 15) / 16 * 16 + window + max_query + 15) : max_len;
+}
+
 // Bytes for either kernel: the query's alignment, which also decides, is not known here.
 size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv, int64_t d, int64_t dv,
                      int64_t block_size, int64_t max_query, int64_t max_len, bool weights) {
@@ -1158,6 +1170,7 @@ struct RowArgs {
   void *workspace;
   size_t workspace_bytes;
   hif8_stream_t stream;
+  int64_t window, sinks;
 };
 
 int row_attention(const char *name, const RowArgs &a) {
@@ -1185,7 +1198,8 @@ int row_attention(const char *name, const RowArgs &a) {
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: caches must be 4-byte aligned", name);
   if (!aligned(a.query, 2) || !aligned(a.out, 2))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: query/out must be 2-byte aligned", name);
-  const size_t need = row_workspace(a.batch, a.total_q, a.heads, a.hkv, a.d, a.dv, a.block_size, a.max_query, a.max_len,
+  const int64_t most_rows = rows_bound(a.max_len, a.max_query, a.window, a.sinks);
+  const size_t need = row_workspace(a.batch, a.total_q, a.heads, a.hkv, a.d, a.dv, a.block_size, a.max_query, most_rows,
                                     a.weights != nullptr);
   if (!a.workspace || a.workspace_bytes < need)
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes required (got %zu)", name, need,
@@ -1194,11 +1208,11 @@ int row_attention(const char *name, const RowArgs &a) {
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", name);
 
   const int64_t group = a.heads / a.hkv, longest = std::max<int64_t>(a.max_query, 1);
-  const bool mfma = mfma_rows(a.d, a.dv, a.hkv, a.block_size, a.max_len) && aligned(a.query, 16) && aligned(a.out, 16) &&
+  const bool mfma = !a.window && mfma_rows(a.d, a.dv, a.hkv, a.block_size, a.max_len) && aligned(a.query, 16) && aligned(a.out, 16) &&
                     longest * group < 0xFFFF * 16 && (longest * group + 64) * group < (int64_t(1) << 31);  // the grid's y, token_of
   if (mfma && a.batch * (a.max_len / 64 + 1) > 0x7FFFFFFFll / 2)
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
-  const RowPlan pl = plan_rows(mfma, a.batch, a.total_q, a.heads, a.hkv, a.d, a.block_size, a.max_query, a.max_len);
+  const RowPlan pl = plan_rows(mfma, a.batch, a.total_q, a.heads, a.hkv, a.d, a.block_size, a.max_query, most_rows);
   RowAttnParams p{};
   p.query = a.query;
   p.key_cache = a.key_cache;
@@ -1224,9 +1238,12 @@ int row_attention(const char *name, const RowArgs &a) {
   p.split_tokens = pl.split_tokens;
   p.accumulate = a.accumulate ? 1 : 0;
   p.zero_rest = a.zero_rest;
+  p.window = int(a.window);
+  p.sinks = int(a.sinks);
+  p.most_rows = int(most_rows);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   const size_t rows = size_t(a.total_q) * a.heads;
-  const RowSpace space = row_space(pl, a.batch, a.total_q, a.heads, a.dv, a.max_len, a.weights != nullptr);
+  const RowSpace space = row_space(pl, a.batch, a.total_q, a.heads, a.dv, most_rows, a.weights != nullptr);
   uint8_t *ws = static_cast<uint8_t *>(a.workspace);
   p.part_o = reinterpret_cast<float *>(ws);
   p.part_ml = reinterpret_cast<float *>(ws + space.o);
@@ -1360,4 +1377,47 @@ extern "C" int hif8_paged_decode_attention_weights(const void *query, int q_dtyp
                                       head_size, head_size_v, block_table, block_table_dtype, max_blocks_per_seq,
                                       nullptr, seq_lens, nullptr, 0, batch, num_heads, batch, 1, max_seq_len, scale, out,
                                       key_weights, weights_stride, accumulate, 0, workspace, workspace_bytes, stream});
+}
+
+extern "C" size_t hif8_window_attention_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                                                       int64_t head_size, int64_t head_size_v, int64_t block_size,
+                                                       int64_t total_query_tokens, int64_t max_query_len,
+                                                       int64_t max_seq_len, int64_t window, int64_t sinks) {
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || head_size_v <= 0 || block_size <= 0 ||
+      total_query_tokens <= 0 || max_query_len <= 0 || max_seq_len < 0 || window <= 0 || sinks < 0 ||
+      num_heads % num_kv_heads)
+    return 0;
+  window = std::min<int64_t>(window, 0x7FFFFFFF), sinks = std::min<int64_t>(sinks, 0x7FFFFFFF);
+  return row_workspace(batch, total_query_tokens, num_heads, num_kv_heads, head_size, head_size_v, block_size,
+                       max_query_len, rows_bound(max_seq_len, max_query_len, window, sinks), false);
+}
+
+extern "C" int hif8_window_attention(const void *query, int q_dtype, const uint8_t *key_cache,
+                                     const uint8_t *value_cache, int64_t num_blocks, int64_t block_size,
+                                     int64_t num_kv_heads, int64_t head_size, int64_t head_size_v,
+                                     const void *block_table, int block_table_dtype, int64_t max_blocks_per_seq,
+                                     const int32_t *query_start_loc, const int32_t *seq_lens, int64_t batch,
+                                     int64_t num_heads, int64_t total_query_tokens, int64_t max_query_len,
+                                     int64_t max_seq_len, int64_t window, int64_t sinks, float scale, void *out,
+                                     void *workspace, size_t workspace_bytes, hif8_stream_t stream) {
+  static const char *kName = "hif8_window_attention";
+  clear_error();
+  if (window <= 0 || sinks < 0)
+    return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: window must be positive and sinks not negative", kName);
+  if (max_query_len < 0) return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions must be positive", kName);
+  if (batch > 0 && total_query_tokens > 0) {
+    if (max_query_len == 0)
+      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: max_query_len must cover the query rows", kName);
+    if (!query_start_loc && (max_query_len != 1 || total_query_tokens != batch))
+      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: without query_start_loc every request has one query row", kName);
+    if (max_query_len > 0x7FFFFFFF)
+      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", kName);
+  }
+  // Past the lengths' range a window or a count of first rows means the same.
+  window = std::min<int64_t>(window, 0x7FFFFFFF), sinks = std::min<int64_t>(sinks, 0x7FFFFFFF);
+  return row_attention(kName, RowArgs{query, q_dtype, key_cache, value_cache, num_blocks, block_size, num_kv_heads,
+                                      head_size, head_size_v, block_table, block_table_dtype, max_blocks_per_seq,
+                                      query_start_loc, seq_lens, nullptr, 0, batch, num_heads, total_query_tokens,
+                                      max_query_len, max_seq_len, scale, out, nullptr, 0, 0, 1, workspace,
+                                      workspace_bytes, stream, window, sinks});
 }

@@ -1628,6 +1628,192 @@ at::Tensor Hif8GdnDecodeTokenMeta(const at::Tensor &mixed, const at::Tensor &, c
   return at::empty({mixed.size(0), v_heads * v_dim}, mixed.options());
 }
 
+// ------------------------------------------- around a decoding step
+// Attention within a sliding window, verification of drafts, pages taken and given back.
+
+at::Tensor Hif8WindowAttention(const at::Tensor &query, const at::Tensor &key_cache, const at::Tensor &value_cache,
+                               const at::Tensor &block_table, const c10::optional<at::Tensor> &query_start_loc,
+                               const at::Tensor &seq_lens, double scale, int64_t window, int64_t sinks,
+                               int64_t max_query_len, int64_t max_seq_len) {
+  TORCH_CHECK(query.dim() == 3, "query must have shape [tokens, num_heads, head_size]");
+  const int64_t tokens = query.size(0);
+  const int64_t batch = query_start_loc.has_value() ? CheckStartLoc(*query_start_loc, key_cache.device()) : tokens;
+  const auto o = CheckPaged(key_cache, &value_cache, block_table, seq_lens, "seq_lens", batch, max_seq_len);
+  CheckQuery(query, o, key_cache.device());
+  TORCH_CHECK(window > 0, "window must be positive");
+  TORCH_CHECK(sinks >= 0, "sinks must not be negative");
+  TORCH_CHECK(max_query_len >= 0, "max_query_len must be non-negative");
+  TORCH_CHECK(query_start_loc.has_value() || max_query_len == 1, "without query_start_loc max_query_len is 1");
+  const c10::OptionalDeviceGuard guard(query.device());
+  auto out = at::empty({tokens, query.size(1), o.dv}, query.options());
+  if (batch == 0 || tokens == 0 || max_query_len == 0) return out.zero_();  // rows of no request, if any
+  const size_t bytes = hif8_window_attention_workspace_size(batch, query.size(1), o.kv_heads, o.d, o.dv, o.block_size,
+                                                            tokens, max_query_len, max_seq_len, window, sinks);
+  const auto ws = Workspace(bytes, query);
+  CheckStatus(hif8_window_attention(
+                  query.data_ptr(), DtypeCode(query.scalar_type()), key_cache.data_ptr<uint8_t>(),
+                  value_cache.data_ptr<uint8_t>(), o.num_blocks, o.block_size, o.kv_heads, o.d, o.dv,
+                  block_table.data_ptr(), o.bt_code, o.max_blocks,
+                  query_start_loc.has_value() ? query_start_loc->data_ptr<int32_t>() : nullptr,
+                  seq_lens.data_ptr<int32_t>(), batch, query.size(1), tokens, max_query_len, max_seq_len, window, sinks,
+                  float(scale), out.data_ptr(), WorkspacePtr(ws), bytes, CurrentStream(query.device())),
+              "hif8_window_attention");
+  return out;
+}
+
+// Rows of probabilities: float32 [tokens, vocab], any row stride.
+void CheckProbs(const at::Tensor &t, const char *name, int64_t tokens, int64_t vocab, const at::Device &device) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a HIP device tensor, got ", t.device());
+  TORCH_CHECK(t.scalar_type() == at::ScalarType::Float, name, " must have dtype torch.float32");
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == tokens && t.size(1) == vocab, name, " must have shape [tokens, vocab]");
+  TORCH_CHECK(tokens == 0 || (t.stride(1) == 1 && t.stride(0) >= vocab), name, " must have contiguous rows");
+  CheckSameDevice(t, device, name);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> Hif8VerifyDrafts(
+    const at::Tensor &target_probs, const at::Tensor &draft_tokens, const at::Tensor &uniforms,
+    const at::Tensor &query_start_loc, const c10::optional<at::Tensor> &draft_probs,
+    const c10::optional<at::Tensor> &parents, int64_t max_query_len) {
+  const auto device = target_probs.device();
+  TORCH_CHECK(target_probs.dim() == 2 && target_probs.size(1) > 0, "target_probs must have shape [tokens, vocab]");
+  const int64_t tokens = target_probs.size(0), vocab = target_probs.size(1);
+  CheckProbs(target_probs, "target_probs", tokens, vocab, device);
+  const int64_t batch = CheckStartLoc(query_start_loc, device);
+  CheckContiguousDevice(draft_tokens, "draft_tokens");
+  const int code = IndexCode(draft_tokens, "draft_tokens");
+  TORCH_CHECK(draft_tokens.dim() == 1 && draft_tokens.numel() == tokens, "draft_tokens must hold one id per row");
+  CheckSameDevice(draft_tokens, device, "draft_tokens");
+  CheckContiguousDevice(uniforms, "uniforms");
+  TORCH_CHECK(uniforms.scalar_type() == at::ScalarType::Float && uniforms.dim() == 1 && uniforms.numel() == tokens,
+              "uniforms must hold one float32 number per row");
+  CheckSameDevice(uniforms, device, "uniforms");
+  TORCH_CHECK(!draft_probs.has_value() || !parents.has_value(),
+              "draft_probs go with a chain of drafts, not with parents");
+  if (draft_probs.has_value()) CheckProbs(*draft_probs, "draft_probs", tokens, vocab, device);
+  if (parents.has_value()) {
+    CheckContiguousDevice(*parents, "parents");
+    TORCH_CHECK(parents->scalar_type() == at::ScalarType::Int && parents->dim() == 1 && parents->numel() == tokens,
+                "parents must hold one int32 index per row");
+    CheckSameDevice(*parents, device, "parents");
+  }
+  TORCH_CHECK(max_query_len >= 0, "max_query_len must be non-negative");
+  const c10::OptionalDeviceGuard guard(device);
+  auto accepted = at::empty({batch, max_query_len}, query_start_loc.options());
+  auto counts = at::empty({batch}, query_start_loc.options());
+  auto next = at::empty({batch}, query_start_loc.options().dtype(at::ScalarType::Long));
+  if (batch == 0) return {accepted, counts, next};
+  const size_t bytes = hif8_verify_drafts_workspace_size(batch, vocab);
+  const auto ws = Workspace(bytes, target_probs);
+  CheckStatus(hif8_verify_drafts(
+                  target_probs.data_ptr<float>(), tokens > 1 ? target_probs.stride(0) : vocab,
+                  draft_probs.has_value() ? draft_probs->data_ptr<float>() : nullptr,
+                  draft_probs.has_value() && tokens > 1 ? draft_probs->stride(0) : vocab, vocab, draft_tokens.data_ptr(),
+                  code, parents.has_value() ? parents->data_ptr<int32_t>() : nullptr, uniforms.data_ptr<float>(),
+                  query_start_loc.data_ptr<int32_t>(), batch, tokens, max_query_len,
+                  max_query_len ? accepted.data_ptr<int32_t>() : nullptr, counts.data_ptr<int32_t>(),
+                  next.data_ptr<int64_t>(), WorkspacePtr(ws), bytes, CurrentStream(device)),
+              "hif8_verify_drafts");
+  return {accepted, counts, next};
+}
+
+// The table and the stack of free page ids, which change in place.
+int CheckPagePool(const at::Tensor &block_table, const at::Tensor &free_blocks, const at::Tensor &free_count,
+                  const at::Tensor &lens, const char *lens_name, int64_t block_size) {
+  CheckContiguousDevice(block_table, "block_table");
+  const int code = IndexCode(block_table, "block_table");
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(1) > 0, "block_table must have shape [batch, max_blocks]");
+  const auto device = block_table.device();
+  CheckContiguousDevice(free_blocks, "free_blocks");
+  TORCH_CHECK(free_blocks.scalar_type() == at::ScalarType::Int && free_blocks.dim() == 1,
+              "free_blocks must be an int32 tensor [pages]");
+  CheckSameDevice(free_blocks, device, "free_blocks");
+  CheckContiguousDevice(free_count, "free_count");
+  TORCH_CHECK(free_count.scalar_type() == at::ScalarType::Int && free_count.numel() == 1,
+              "free_count must be an int32 tensor of one element");
+  CheckSameDevice(free_count, device, "free_count");
+  CheckContiguousDevice(lens, lens_name);
+  TORCH_CHECK(lens.scalar_type() == at::ScalarType::Int, lens_name, " must have dtype torch.int32");
+  TORCH_CHECK(lens.dim() == 1 && lens.numel() >= block_table.size(0), lens_name,
+              " must contain one length per request");
+  CheckSameDevice(lens, device, lens_name);
+  TORCH_CHECK(block_size > 0, "block_size must be positive");
+  return code;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> Hif8ExtendBlockTables(
+    const at::Tensor &block_table, const at::Tensor &free_blocks, const at::Tensor &free_count,
+    const at::Tensor &context_lens, const at::Tensor &query_start_loc, int64_t block_size, int64_t total_query_tokens) {
+  const int code = CheckPagePool(block_table, free_blocks, free_count, context_lens, "context_lens", block_size);
+  const auto device = block_table.device();
+  const int64_t batch = CheckStartLoc(query_start_loc, device);
+  TORCH_CHECK(block_table.size(0) == batch, "block_table must have a row for every request");
+  TORCH_CHECK(total_query_tokens >= 0, "total_query_tokens must be non-negative");
+  MarkChanged(block_table);
+  MarkChanged(free_count);
+  const c10::OptionalDeviceGuard guard(device);
+  const auto longs = query_start_loc.options().dtype(at::ScalarType::Long);
+  auto slots = at::empty({total_query_tokens}, longs), positions = at::empty({total_query_tokens}, longs);
+  auto lens = at::empty({batch}, query_start_loc.options()), missing = at::empty({batch}, query_start_loc.options());
+  if (batch == 0) return {slots.fill_(-1), positions.fill_(-1), lens, missing};
+  CheckStatus(hif8_extend_block_tables(block_table.data_ptr(), code, block_table.size(1),
+                                       free_blocks.numel() ? free_blocks.data_ptr<int32_t>() : nullptr,
+                                       free_blocks.numel(), free_count.data_ptr<int32_t>(),
+                                       context_lens.data_ptr<int32_t>(), query_start_loc.data_ptr<int32_t>(), batch,
+                                       total_query_tokens, block_size,
+                                       total_query_tokens ? slots.data_ptr<int64_t>() : nullptr,
+                                       total_query_tokens ? positions.data_ptr<int64_t>() : nullptr,
+                                       lens.data_ptr<int32_t>(), missing.data_ptr<int32_t>(), CurrentStream(device)),
+              "hif8_extend_block_tables");
+  return {slots, positions, lens, missing};
+}
+
+void Hif8ReleaseBlocks(const at::Tensor &block_table, const at::Tensor &free_blocks, const at::Tensor &free_count,
+                       const at::Tensor &seq_lens, int64_t block_size, int64_t window, int64_t sinks) {
+  const int code = CheckPagePool(block_table, free_blocks, free_count, seq_lens, "seq_lens", block_size);
+  TORCH_CHECK(window >= 0 && sinks >= 0, "window and sinks must not be negative");
+  MarkChanged(block_table);
+  MarkChanged(free_blocks);
+  MarkChanged(free_count);
+  const int64_t batch = block_table.size(0);
+  if (batch == 0) return;
+  const c10::OptionalDeviceGuard guard(block_table.device());
+  const size_t bytes = hif8_release_blocks_workspace_size(batch, block_table.size(1));
+  const auto ws = Workspace(bytes, block_table);
+  CheckStatus(hif8_release_blocks(block_table.data_ptr(), code, block_table.size(1),
+                                  free_blocks.numel() ? free_blocks.data_ptr<int32_t>() : nullptr, free_blocks.numel(),
+                                  free_count.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), batch, block_size, window,
+                                  sinks, WorkspacePtr(ws), bytes, CurrentStream(block_table.device())),
+              "hif8_release_blocks");
+}
+
+at::Tensor Hif8WindowAttentionMeta(const at::Tensor &query, const at::Tensor &, const at::Tensor &value_cache,
+                                   const at::Tensor &, const c10::optional<at::Tensor> &, const at::Tensor &, double,
+                                   int64_t, int64_t, int64_t, int64_t) {
+  return at::empty({query.size(0), query.size(1), value_cache.size(3) - 4}, query.options());
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> Hif8VerifyDraftsMeta(
+    const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &query_start_loc,
+    const c10::optional<at::Tensor> &, const c10::optional<at::Tensor> &, int64_t max_query_len) {
+  const int64_t batch = query_start_loc.size(0) - 1;
+  const auto ints = query_start_loc.options().dtype(at::ScalarType::Int);
+  return {at::empty({batch, max_query_len}, ints), at::empty({batch}, ints),
+          at::empty({batch}, ints.dtype(at::ScalarType::Long))};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> Hif8ExtendBlockTablesMeta(
+    const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &query_start_loc,
+    int64_t, int64_t total_query_tokens) {
+  const int64_t batch = query_start_loc.size(0) - 1;
+  const auto ints = query_start_loc.options().dtype(at::ScalarType::Int);
+  const auto longs = ints.dtype(at::ScalarType::Long);
+  return {at::empty({total_query_tokens}, longs), at::empty({total_query_tokens}, longs), at::empty({batch}, ints),
+          at::empty({batch}, ints)};
+}
+
+void Hif8ReleaseBlocksMeta(const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &, int64_t,
+                           int64_t, int64_t) {}
+
 }  // namespace
 
 TORCH_LIBRARY(vllm_ascend_hif8, m) {
@@ -1645,6 +1831,10 @@ TORCH_LIBRARY(vllm_ascend_hif8, m) {
   m.def("hif8_key_weights(Tensor query, Tensor key_cache, Tensor block_table, Tensor query_start_loc, Tensor seq_lens, Tensor(a!) key_weights, float scale, int max_query_len, int max_seq_len, bool causal=True, bool accumulate=True) -> ()");
   m.def("hif8_accept_drafts(Tensor(a!)[] caches, Tensor block_table, Tensor context_lens, Tensor accepted, Tensor accepted_counts) -> Tensor");
   m.def("hif8_kv_evict(Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor block_table, Tensor seq_lens, Tensor(c!) key_weights, Tensor(d!)? positions, Tensor? keep, int keep_all, int sinks, Tensor? protect_from, int max_seq_len) -> Tensor");
+  m.def("hif8_window_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor? query_start_loc, Tensor seq_lens, float scale, int window, int sinks, int max_query_len, int max_seq_len) -> Tensor");
+  m.def("hif8_verify_drafts(Tensor target_probs, Tensor draft_tokens, Tensor uniforms, Tensor query_start_loc, Tensor? draft_probs, Tensor? parents, int max_query_len) -> (Tensor, Tensor, Tensor)");
+  m.def("hif8_extend_block_tables(Tensor(a!) block_table, Tensor free_blocks, Tensor(b!) free_count, Tensor context_lens, Tensor query_start_loc, int block_size, int total_query_tokens) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("hif8_release_blocks(Tensor(a!) block_table, Tensor(b!) free_blocks, Tensor(c!) free_count, Tensor seq_lens, int block_size, int window, int sinks) -> ()");
   m.def("hif8_embedding_lookup(Tensor input_ids, Tensor weight, Tensor weight_scale, Tensor(a!)? invalid_ids=None) -> Tensor");
   m.def("hif8_dynamic_quant(Tensor x) -> (Tensor, Tensor)");
   m.def("soft_hif8_fused_gemm(Tensor activation, Tensor weight, Tensor channel_scale, Tensor? bias, ScalarType output_dtype) -> Tensor");
@@ -1684,6 +1874,10 @@ TORCH_LIBRARY_IMPL(vllm_ascend_hif8, CUDA, m) {
   m.impl("hif8_key_weights", &Hif8KeyWeights);
   m.impl("hif8_accept_drafts", &Hif8AcceptDrafts);
   m.impl("hif8_kv_evict", &Hif8KVEvict);
+  m.impl("hif8_window_attention", &Hif8WindowAttention);
+  m.impl("hif8_verify_drafts", &Hif8VerifyDrafts);
+  m.impl("hif8_extend_block_tables", &Hif8ExtendBlockTables);
+  m.impl("hif8_release_blocks", &Hif8ReleaseBlocks);
   m.impl("hif8_embedding_lookup", &Hif8EmbeddingLookup);
   m.impl("hif8_dynamic_quant", &Hif8DynamicQuant);
   m.impl("soft_hif8_fused_gemm", &SoftHif8FusedGemm);
@@ -1722,6 +1916,10 @@ TORCH_LIBRARY_IMPL(vllm_ascend_hif8, Meta, m) {
   m.impl("hif8_key_weights", &Hif8KeyWeightsMeta);
   m.impl("hif8_accept_drafts", &Hif8AcceptDraftsMeta);
   m.impl("hif8_kv_evict", &Hif8KVEvictMeta);
+  m.impl("hif8_window_attention", &Hif8WindowAttentionMeta);
+  m.impl("hif8_verify_drafts", &Hif8VerifyDraftsMeta);
+  m.impl("hif8_extend_block_tables", &Hif8ExtendBlockTablesMeta);
+  m.impl("hif8_release_blocks", &Hif8ReleaseBlocksMeta);
   m.impl("hif8_embedding_lookup", &Hif8EmbeddingLookupMeta);
   m.impl("hif8_dynamic_quant", &Hif8DynamicQuantMeta);
   m.impl("soft_hif8_fused_gemm", &FusedLinearMeta);

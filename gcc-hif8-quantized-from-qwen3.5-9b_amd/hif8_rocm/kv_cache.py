@@ -130,6 +130,25 @@ def _check_caches(key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
         raise ValueError("key_cache and value_cache must have the same blocks and heads")
 
 
+def _check_window(window: int | None, sinks: int) -> None:
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window")
+        return
+    if isinstance(window, bool) or not isinstance(window, int) or window < 1:
+        raise ValueError(f"window must be a positive integer, got {window}")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+        raise ValueError(f"sinks must be a non-negative integer, got {sinks}")
+
+
+def _pages_in_window(lens: torch.Tensor, query_lens, columns: int, block_size: int, window: int, sinks: int):
+    """Which table columns the query rows of each request look at, ``[B, columns]`` (lengths apart)."""
+    first = torch.arange(columns, device=lens.device)[None, :] * block_size
+    rows = torch.as_tensor(query_lens, device=lens.device).expand(lens.shape)
+    low = (lens.to(torch.int64) - rows + 1 - window)[:, None]
+    return ((first + block_size > low) | (first < sinks)) & (rows > 0)[:, None]
+
+
 def write_kv_cache(
     key: torch.Tensor,
     value: torch.Tensor,
@@ -188,6 +207,8 @@ def paged_decode_attention(
     *,
     scale: float,
     max_seq_len: int | None = None,
+    window: int | None = None,
+    sinks: int = 0,
     validate: bool = True,
 ) -> torch.Tensor:
     """Decode attention over HiF8 pages: ``query`` ``[B, Hq, D]`` -> ``[B, Hq, Dv]``.
@@ -198,8 +219,12 @@ def paged_decode_attention(
     sequence (as the reference's ``seq_lens_list``) or an int32 device tensor;
     with a tensor, pass ``max_seq_len`` to avoid a host synchronisation.
     ``validate`` checks the block ids that the lengths reach (kv_cache.py:247-249).
+
+    With ``window`` the token sees the last ``window`` cached tokens (itself among
+    them) and the first ``sinks`` alone, as in :func:`paged_attention`.
     """
     _check_caches(key_cache, value_cache)
+    _check_window(window, sinks)
     if query.ndim != 3:
         raise ValueError("query must have shape [tokens, num_heads, head_size]")
     batch = query.shape[0]
@@ -233,10 +258,16 @@ def paged_decode_attention(
             raise ValueError("max_seq_len is smaller than a sequence length")
         needed = (max_seq_len + block_size - 1) // block_size
         used = torch.arange(needed, device=query.device)[None, :] * block_size < lens_dev[:, None].to(torch.int64)
+        if window is not None:
+            used &= _pages_in_window(lens_dev, 1, needed, block_size, window, sinks)
         ids = table[:, :needed].to(torch.int64)
         if bool(((ids < 0) | (ids >= key_cache.shape[0]))[used].any()):
             raise IndexError("block_table references a block outside the cache")
     extension = native.load_extension()
+    if window is not None:
+        return native._operator("hif8_window_attention", extension)(
+            query.contiguous(), key_cache, value_cache, table, None, lens_dev, float(scale), window, sinks, 1,
+            int(max_seq_len))
     return native._operator("hif8_paged_decode_attention", extension)(
         query.contiguous(), key_cache, value_cache, table, lens_dev, float(scale), int(max_seq_len))
 
@@ -254,6 +285,8 @@ def paged_attention(
     causal: bool = True,
     max_query_len: int | None = None,
     max_seq_len: int | None = None,
+    window: int | None = None,
+    sinks: int = 0,
     validate: bool = True,
 ) -> torch.Tensor:
     """Attention over HiF8 pages for any number of query tokens per request.
@@ -274,8 +307,21 @@ def paged_attention(
     as well, since validation checks it against ``query_start_loc``).  One
     query row per request runs the decode kernel; otherwise the multi-token
     kernel.
+
+    ``window`` (no counterpart in the reference; causal calls) makes the row at
+    position P see the rows ``t <= P`` with ``t > P - window`` or ``t < sinks``
+    alone: a sliding window, and first tokens that stay visible.  Pages that no row
+    sees are not read, so :func:`release_blocks` may have taken them.  K and V are
+    then ``dec(code) * row scale`` without a rounding to the query dtype, what a
+    row does not see has no influence on it, NaN and infinities included, and a
+    row that sees nothing gets zeros, as do rows that ``query_start_loc`` gives to
+    no request.  Small weights beside an infinite V, and the shapes that are
+    fast, are those of :func:`tree_attention`.
     """
     _check_caches(key_cache, value_cache)
+    _check_window(window, sinks)
+    if window is not None and not causal:
+        raise ValueError("a window needs causal attention")
     if query.ndim != 3:
         raise ValueError("query must have shape [tokens, num_heads, head_size]")
     if query.shape[1] % key_cache.shape[2]:
@@ -300,7 +346,7 @@ def paged_attention(
         if batch == tokens and all(v == 1 for v in q_lengths):
             # The decode case: each row is its request's last position.
             return paged_decode_attention(query, key_cache, value_cache, block_table, seq_lens, scale=scale,
-                                          max_seq_len=max_seq_len, validate=validate)
+                                          max_seq_len=max_seq_len, window=window, sinks=sinks, validate=validate)
         starts = [0]
         for v in q_lengths:
             starts.append(starts[-1] + v)
@@ -350,10 +396,16 @@ def paged_attention(
         needed = (max_seq_len + block_size - 1) // block_size
         used = (torch.arange(needed, device=query.device)[None, :] * block_size
                 < lens_dev[:batch, None].to(torch.int64))
+        if window is not None:
+            used &= _pages_in_window(lens_dev[:batch], loc[1:] - loc[:-1], needed, block_size, window, sinks)
         ids = table[:, :needed].to(torch.int64)
         if bool(((ids < 0) | (ids >= key_cache.shape[0]))[used].any()):
             raise IndexError("block_table references a block outside the cache")
     extension = native.load_extension()
+    if window is not None:
+        return native._operator("hif8_window_attention", extension)(
+            query.contiguous(), key_cache, value_cache, table, loc, lens_dev, float(scale), window, sinks,
+            int(max_query_len), int(max_seq_len))
     return native._operator("hif8_paged_prefill_attention", extension)(
         query.contiguous(), key_cache, value_cache, table, loc, lens_dev, float(scale), int(max_query_len),
         int(max_seq_len), bool(causal))
@@ -731,6 +783,205 @@ def evict_kv_rows(
 
 
 
+def verify_drafts(
+    target_probs: torch.Tensor,
+    draft_tokens: torch.Tensor,
+    uniforms: torch.Tensor,
+    *,
+    draft_probs: torch.Tensor | None = None,
+    parents: torch.Tensor | None = None,
+    query_lens: Sequence[int] | None = None,
+    query_start_loc: torch.Tensor | None = None,
+    max_query_len: int | None = None,
+    validate: bool = True,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Accepts drafted tokens against the target model's probabilities and draws the next token.
+
+    No counterpart in the reference; stands between attention over the drafts and
+    :func:`accept_drafts`.  Row i of a request is a node of its drafts:
+    ``draft_tokens`` (int32 / int64 ``[T]``) its token, row i of ``target_probs``
+    (float32 ``[T, vocab]``) what the target gives for the token behind it,
+    ``uniforms`` (float32 ``[T]``, in [0, 1)) its random number.  Row 0 holds the
+    token that the step before answered with, which stands.
+
+    * Drafts drawn from a draft model, in a chain: ``draft_probs`` (float32 ``[T,
+      vocab]``), row i what token i was drawn from (row 0 is not read).  Row i + 1
+      is accepted after row i where ``u * q(x) < p(x)`` with its own u, q and x; the
+      next token comes from ``max(p - q, 0)`` at the row that is not followed, or
+      from p behind the last.
+    * Given drafts (``draft_probs`` None), in a chain or, by ``parents`` (int32
+      ``[T]``, index within the request, below the row's own), in a tree: the
+      children of the accepted row in rising order, each accepted where
+      ``u * rest < p(x)``, rest being 1 less the p of the tokens refused before it;
+      the next token comes from p without the refused tokens.
+
+    Either way the answers are distributed as the target's.  The next token is
+    the first v at which the running sum passes u of row 0 times its total; all of
+    it in float64.  Returns ``accepted`` (int32 ``[B, max_query_len]``: the path's
+    rows in rising order, then -1) and ``accepted_counts`` (int32 ``[B]``), which
+    :func:`accept_drafts` takes, and the next tokens (int64 ``[B]``).  A request
+    without rows gets 0 and -1, one whose probabilities hold no positive finite
+    number -1.
+
+    The request split is given as for :func:`paged_attention`, at most 1024 rows
+    each.  ``validate`` checks parents and numbers on the host.
+    """
+    if target_probs.ndim != 2 or target_probs.shape[1] < 1:
+        raise ValueError("target_probs must have shape [tokens, vocab]")
+    if target_probs.dtype != torch.float32:
+        raise TypeError(f"target_probs must be float32, got {target_probs.dtype}")
+    tokens, device = target_probs.shape[0], target_probs.device
+    if draft_tokens.shape != (tokens,) or draft_tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("draft_tokens must hold one int32 or int64 id per row of target_probs")
+    if uniforms.shape != (tokens,) or uniforms.dtype != torch.float32:
+        raise ValueError("uniforms must hold one float32 number per row of target_probs")
+    if draft_probs is not None:
+        if parents is not None:
+            raise ValueError("draft_probs go with a chain of drafts, not with parents")
+        if draft_probs.shape != target_probs.shape or draft_probs.dtype != torch.float32:
+            raise ValueError("draft_probs must be float32 with the shape of target_probs")
+    if parents is not None and (parents.shape != (tokens,) or parents.dtype not in (torch.int32, torch.int64)):
+        raise ValueError("parents must hold one int32 or int64 index per row of target_probs")
+    loc, batch, max_query_len, _ = _request_rows(target_probs, query_lens, query_start_loc, max_query_len, validate)
+    if max_query_len > 1024:
+        raise ValueError("verify_drafts takes at most 1024 rows per request")
+
+    def rows(probs):
+        probs = probs.to(device)
+        return probs if tokens == 0 or (probs.stride(1) == 1 and probs.stride(0) >= probs.shape[1]) else probs.contiguous()
+
+    up = None if parents is None else _as_int32(parents, device)
+    drawn = uniforms.to(device).contiguous()
+    if validate and tokens:
+        if bool(((drawn < 0) | (drawn >= 1) | drawn.isnan()).any()):
+            raise ValueError("uniforms must be in [0, 1)")
+        if up is not None and batch:
+            row = torch.arange(tokens, device=device)
+            request = torch.searchsorted(loc.contiguous(), row, right=True, out_int32=True).long() - 1
+            inside = (request >= 0) & (request < batch)
+            index = row - loc.long()[request.clamp(0, batch - 1)]
+            if bool((inside & (index > 0) & ((up < 0) | (up >= index))).any()):
+                raise ValueError("parents must be indices below the row's own")
+    extension = native.load_extension()
+    return native._operator("hif8_verify_drafts", extension)(
+        rows(target_probs), draft_tokens.to(device).contiguous(), drawn, loc,
+        None if draft_probs is None else rows(draft_probs), up, max_query_len)
+
+
+def _check_pool(block_table, free_blocks, free_count, lens, lens_name: str, block_size: int, validate: bool):
+    """The checks that the calls with a stack of free pages share: the lengths on the device."""
+    device = block_table.device
+    if block_table.ndim != 2 or block_table.shape[1] < 1:
+        raise ValueError("block_table must have shape [batch, max_blocks]")
+    if block_table.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"block_table must be int32 or int64, got {block_table.dtype}")
+    if free_blocks.ndim != 1 or free_blocks.dtype != torch.int32:
+        raise TypeError("free_blocks must be an int32 tensor [pages]")
+    if free_count.numel() != 1 or free_count.dtype != torch.int32:
+        raise TypeError("free_count must be an int32 tensor of one element")
+    for name, t in (("block_table", block_table), ("free_blocks", free_blocks), ("free_count", free_count)):
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if t.device != device:
+            raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if block_size < 1:
+        raise ValueError("block_size must be positive")
+    batch = block_table.shape[0]
+    sizes, host = _device_lengths(lens, lens_name, device)
+    if sizes.ndim != 1 or (sizes.numel() < batch if host is None else sizes.numel() != batch):
+        raise ValueError("one length is required per request")
+    if validate:
+        if not 0 <= int(free_count.item()) <= free_blocks.numel():
+            raise ValueError("free_count must be within free_blocks")
+        if bool((sizes[:batch] < 0).any()):
+            raise ValueError(f"{lens_name} must be non-negative")
+    return sizes
+
+
+def extend_block_tables(
+    block_table: torch.Tensor,
+    free_blocks: torch.Tensor,
+    free_count: torch.Tensor,
+    context_lens: Sequence[int] | torch.Tensor,
+    *,
+    block_size: int,
+    query_lens: Sequence[int] | None = None,
+    query_start_loc: torch.Tensor | None = None,
+    total_query_tokens: int | None = None,
+    validate: bool = True,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Takes pages for a step's new tokens, in place, and works out the tokens' slots on the device.
+
+    No counterpart in the reference (its scheduler builds both on the host).
+    Request b has ``context_lens[b]`` cached tokens and ``query_lens[b]`` new
+    ones.  Every column of its row of ``block_table`` (int32 / int64 ``[B,
+    max_blocks]``, an entry below zero holds no page) that the new tokens reach
+    without finding a page gets one from the end of the stack ``free_blocks[:
+    free_count]`` (int32; the count int32 of one element, on the device), in the
+    order (request, column).  Table and count change in place.
+
+    Returns ``slot_mapping`` (int64 ``[T]``, for :func:`write_kv_cache`; -1 where
+    there is no page) and ``positions`` (int64 ``[T]``), both -1 for rows that
+    ``query_start_loc`` gives to no request, the new ``seq_lens`` (int32 ``[B]``)
+    and ``missing`` (int32 ``[B]``): columns that got no page, because the stack was
+    empty or the table too narrow.
+
+    With ``query_start_loc`` pass ``total_query_tokens`` (the rows T of the step) and
+    ``validate=False`` to avoid host synchronisations.
+    """
+    context = _check_pool(block_table, free_blocks, free_count, context_lens, "context_lens", block_size, validate)
+    if (query_lens is None) == (query_start_loc is None):
+        raise ValueError("pass exactly one of query_lens and query_start_loc")
+    if query_lens is not None:
+        host = [int(v) for v in query_lens]
+        if any(v < 0 for v in host):
+            raise ValueError("query_lens must be non-negative")
+        loc = torch.tensor([0] + host, dtype=torch.int64).cumsum(0).to(torch.int32).to(block_table.device)
+        if total_query_tokens is None:
+            total_query_tokens = sum(host)
+    else:
+        if query_start_loc.ndim != 1 or query_start_loc.numel() < 1:
+            raise ValueError("query_start_loc must have shape [batch + 1]")
+        loc = _as_int32(query_start_loc, block_table.device)
+        if total_query_tokens is None:
+            total_query_tokens = int(loc[-1].item())
+    if loc.numel() - 1 != block_table.shape[0]:
+        raise ValueError("block_table must have a row for every request")
+    if total_query_tokens < 0:
+        raise ValueError("total_query_tokens must not be negative")
+    extension = native.load_extension()
+    return native._operator("hif8_extend_block_tables", extension)(
+        block_table, free_blocks, free_count, context, loc, int(block_size), int(total_query_tokens))
+
+
+def release_blocks(
+    block_table: torch.Tensor,
+    free_blocks: torch.Tensor,
+    free_count: torch.Tensor,
+    seq_lens: Sequence[int] | torch.Tensor,
+    *,
+    block_size: int,
+    window: int | None = None,
+    sinks: int = 0,
+    validate: bool = True,
+) -> None:
+    """Gives pages that no later token needs back to the stack of free pages, in place.
+
+    No counterpart in the reference; the way back of :func:`extend_block_tables`, after
+    :func:`verify_drafts` or :func:`evict_kv_rows` has shortened requests, or a
+    window has moved on.  A page stays where request b's ``seq_lens[b]`` tokens
+    reach it and, with ``window``, where it holds one of the first ``sinks`` tokens
+    or one that the next token sees.  The others leave ``block_table`` (their entries
+    become -1) for the end of ``free_blocks``, in the order (request, column);
+    length 0 gives back all of a request.  Pages must belong to one request.
+    """
+    _check_window(window, sinks)
+    lens = _check_pool(block_table, free_blocks, free_count, seq_lens, "seq_lens", block_size, validate)
+    extension = native.load_extension()
+    native._operator("hif8_release_blocks", extension)(
+        block_table, free_blocks, free_count, lens, int(block_size), 0 if window is None else window, int(sinks))
+
+
 __all__ = [
     "HIF8_CACHE_DTYPE",
     "HIF8_SCALE_BYTES",
@@ -738,11 +989,14 @@ __all__ = [
     "accept_drafts",
     "accumulate_key_weights",
     "evict_kv_rows",
+    "extend_block_tables",
     "pack_kv_rows",
     "paged_attention",
     "paged_decode_attention",
     "paged_decode_attention_weights",
+    "release_blocks",
     "tree_attention",
     "unpack_kv_rows",
+    "verify_drafts",
     "write_kv_cache",
 ]

@@ -514,6 +514,101 @@ int hif8_kv_evict(uint8_t *key_cache, uint8_t *value_cache, int64_t num_blocks, 
                   int32_t *new_lens, void *workspace, size_t workspace_bytes, hif8_stream_t stream);
 
 /*
+ * Attention within a sliding window over the paged HiF8 cache (no counterpart in the
+ * reference): the query row at position P of its request sees the cached rows t <= P with
+ * t > P - window or t < sinks (the first rows, which stay visible).
+ *   query [total_query_tokens, num_heads, D] fp16/bf16; request b owns the rows from
+ *     query_start_loc[b] on, which are the last positions of its seq_lens[b] cached rows
+ *     (this step's among them); query_start_loc NULL: row b is request b's only one
+ *   window >= 1, sinks >= 0; max_query_len >= every request's rows (one with more gets
+ *     outputs that mean nothing, without an access out of bounds); max_seq_len as above
+ *   out [total_query_tokens, num_heads, Dv] in the query dtype: softmax(scale * q . K) V over
+ *     the rows seen, K and V dec(code) * row scale; a row that sees nothing and rows of no
+ *     request get zeros (batch > 0).  What is not seen has no influence, whatever it holds,
+ *     and pages that no query row sees are not read: their table entries may be anything.
+ *     Cache rows whose block id lies outside [0, num_blocks) are left out.  Weights meet V
+ *     in 16 bits as in hif8_tree_attention.
+ *   workspace  at least hif8_window_attention_workspace_size(...) bytes, 16-byte aligned; its
+ *              size depends on these arguments alone
+ * D = Dv of 64, 128 or 256 over pages of a multiple of 16 rows, with 16-byte aligned query and
+ * out, runs on the matrix cores; any other shape takes a kernel that is many times slower.
+ */
+size_t hif8_window_attention_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
+                                            int64_t head_size_v, int64_t block_size, int64_t total_query_tokens,
+                                            int64_t max_query_len, int64_t max_seq_len, int64_t window, int64_t sinks);
+int hif8_window_attention(const void *query, int q_dtype, const uint8_t *key_cache, const uint8_t *value_cache,
+                          int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_size,
+                          int64_t head_size_v, const void *block_table, int block_table_dtype,
+                          int64_t max_blocks_per_seq, const int32_t *query_start_loc, const int32_t *seq_lens,
+                          int64_t batch, int64_t num_heads, int64_t total_query_tokens, int64_t max_query_len,
+                          int64_t max_seq_len, int64_t window, int64_t sinks, float scale, void *out, void *workspace,
+                          size_t workspace_bytes, hif8_stream_t stream);
+
+/*
+ * Verification of drafted tokens against the target model's probabilities (no counterpart
+ * in the reference; follows attention over the drafts, precedes hif8_accept_drafts).  Row i
+ * of a request is a node of its drafts: p_i = target_probs[row] what the target gives for
+ * the token behind it, x_i = draft_tokens[row], u_i = uniforms[row] in [0, 1).  Row 0's token
+ * is known (accepted); from there
+ *   with draft_probs (q_i: what x_i was drawn from; row 0's is not read; a chain): row i + 1
+ *     is accepted after row i where u_{i+1} q_{i+1}(x_{i+1}) < p_i(x_{i+1}); the residual of the
+ *     row that is not followed is max(p_i - q_{i+1}, 0), of the chain's last row p_i;
+ *   without (tokens that were not drawn; a chain, or a tree by parents): the children of row
+ *     i in rising order, with rest = 1 - the p_i of those refused before: j is accepted where
+ *     u_j rest < p_i(x_j); where none is, the residual is p_i without the children's tokens.
+ * next_tokens[b] is the first v whose running sum of the residual passes u_0 times its total.
+ * All of it in FP64.  Entries that are no positive finite number weigh nothing; a residual
+ * without weight is replaced by p_i, and -1 is the answer where that has none either.  A token
+ * outside [0, vocab), or one that an earlier sibling had, is refused.
+ *   target_probs, draft_probs [total_query_tokens, stride >= vocab] float32, draft_probs may be
+ *     NULL; parents [total_query_tokens] int32 (index within the request, below the row's own;
+ *     others are never reached) or NULL for a chain; draft_tokens int32/int64
+ *   query_start_loc [batch + 1]; rows past max_query_len (at most 1024) of a request are ignored
+ *   accepted [batch, max_query_len] int32: the path's rows in rising order, then -1;
+ *   accepted_counts [batch] int32 (0 and next token -1 for a request without rows);
+ *   next_tokens [batch] int64
+ */
+size_t hif8_verify_drafts_workspace_size(int64_t batch, int64_t vocab);
+int hif8_verify_drafts(const float *target_probs, int64_t target_stride, const float *draft_probs,
+                       int64_t draft_stride, int64_t vocab, const void *draft_tokens, int tokens_dtype,
+                       const int32_t *parents, const float *uniforms, const int32_t *query_start_loc, int64_t batch,
+                       int64_t total_query_tokens, int64_t max_query_len, int32_t *accepted, int32_t *accepted_counts,
+                       int64_t *next_tokens, void *workspace, size_t workspace_bytes, hif8_stream_t stream);
+
+/*
+ * Pages for the new tokens of a step, and their slots (no counterpart in the reference,
+ * whose scheduler builds both on the host).  Request b has context_lens[b] cached rows and
+ * query_start_loc[b + 1] - query_start_loc[b] new ones.  Every column of its row of the block
+ * table that the new rows reach and whose entry is below zero gets a page id, taken from the
+ * end of the stack free_blocks[0 .. *free_count) in the order (request, column); the table
+ * and *free_count change in place.
+ *   slot_mapping, positions [total_query_tokens] int64: table entry * block_size + offset, or
+ *     -1 where there is no page, and the position in the request; both -1 for rows of no request
+ *   seq_lens [batch] int32: context_lens + the new rows
+ *   missing [batch] int32: columns that got no page (the stack was empty, or the table too narrow)
+ */
+int hif8_extend_block_tables(void *block_table, int block_table_dtype, int64_t max_blocks_per_seq,
+                             const int32_t *free_blocks, int64_t free_capacity, int32_t *free_count,
+                             const int32_t *context_lens, const int32_t *query_start_loc, int64_t batch,
+                             int64_t total_query_tokens, int64_t block_size, int64_t *slot_mapping,
+                             int64_t *positions, int32_t *seq_lens, int32_t *missing, hif8_stream_t stream);
+
+/*
+ * The way back: page ids that no later token of a request of seq_lens[b] cached rows needs
+ * become -1 in the table and go onto the stack, in the order (request, column).  The page of
+ * column j stays where j * block_size < seq_lens[b] and, with a window (0: none),
+ * j * block_size < sinks or (j + 1) * block_size > seq_lens[b] + 1 - window.  A stack that is
+ * full (free_capacity) leaves the rest in the table.  seq_lens[b] 0 releases all of a request.
+ * Pages must belong to one request.
+ *   workspace  at least hif8_release_blocks_workspace_size(...) bytes, 4-byte aligned
+ */
+size_t hif8_release_blocks_workspace_size(int64_t batch, int64_t max_blocks_per_seq);
+int hif8_release_blocks(void *block_table, int block_table_dtype, int64_t max_blocks_per_seq, int32_t *free_blocks,
+                        int64_t free_capacity, int32_t *free_count, const int32_t *seq_lens, int64_t batch,
+                        int64_t block_size, int64_t window, int64_t sinks, void *workspace, size_t workspace_bytes,
+                        hif8_stream_t stream);
+
+/*
  * Decode-step glue of the synthetic hybrid model (the end-to-end workload).
  * These have no counterpart among the reference's operators: they fuse the
  * bf16 / fp32 model parts that the reference leaves to vLLM (norms, the MLP
