@@ -38,7 +38,9 @@ struct RowAttnParams {
   // query rows of all of them (a KV head's), ceil(2^31 / group).
   int workers, row_tiles, rows_cap, heads_together;
   uint32_t group_magic;
-  int window, sinks, most_rows;  // window 0: none; most_rows: bound of WindowRows::rows
+  int window, sinks;           // window 0: none
+  int most_rows;               // window: bound of WindowRows::rows
+  int long_rows;               // window: requests of more (token, head) rows per KV head are not these kernels'
   float scale_log2;            // softmax scale * log2(e)
 };
 
@@ -68,6 +70,11 @@ __device__ __forceinline__ WindowRows window_rows(const RowAttnParams &p, int le
 // Whether the query row at position `at` sees cache row t.
 __device__ __forceinline__ bool window_sees(const RowAttnParams &p, int at, int t) {
   return t <= at && (int64_t(t) > int64_t(at) - p.window || t < p.sinks);
+}
+
+// Query rows that another kernel takes.
+__device__ __forceinline__ bool left_out(const RowAttnParams &p, int count) {
+  return p.window && int64_t(count) * p.group > p.long_rows;
 }
 
 // Query rows of request b, clipped to the query tensor (start_loc is caller data).

@@ -190,7 +190,7 @@ constexpr int max_of(int a, int b) { return a > b ? a : b; }
 // drafts of 16 heads over 8 x 16k: 111 us against 73).
 constexpr int tile_rows_of(int d, int row_blocks) { return d == 256 && row_blocks <= 2 ? 64 : 128; }
 
-template <int kD, bool kBf16, int kRB, bool kX, typename BtT>
+template <int kD, bool kBf16, int kRB, bool kX, bool kWin, typename BtT>
 __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(const RowAttnParams p,
                                                                             const uint32_t page_magic) {
   constexpr int kW = waves_of(kRB);       // wavefronts
@@ -245,11 +245,15 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     Request r;
     request_rows(p, i, r.begin, r.count);
     r.ctx = clamp_rows(p.lens[i], p.max_len);
+    if (kWin && left_out(p, r.count)) r.count = 0;
     return r;
   };
-  auto tiles_of = [&](const Request &r) {
-    return int((uint32_t(rows_seen(p, r.ctx, r.count)) + uint32_t(kT) - 1) / kT);
+  // Cache rows that a request's query rows see, pushed together under a window.
+  auto rows_of = [&](const Request &r) {
+    if constexpr (kWin) return r.count > 0 ? window_rows(p, r.ctx, r.count).rows : 0;
+    else return rows_seen(p, r.ctx, r.count);
   };
+  auto tiles_of = [&](const Request &r) { return int((uint32_t(rows_of(r)) + uint32_t(kT) - 1) / kT); };
   int total = 0, incl = 0;
   Request early{};  // lane i: request i
   for (int base = 0; base < p.batch; base += kWave) {
@@ -330,7 +334,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   const int begin = now.begin, count = now.count;
   const int rows = count * p.group;
   const int ctx = now.ctx;
-  const int len = rows_seen(p, ctx, count);
+  const int len = rows_of(now);
+  const WindowRows win = kWin ? window_rows(p, ctx, count) : WindowRows{0, 0, 0};
   const int tile_first = cur - first;
   const int seg_tiles = min(run_end - cur, int((uint32_t(len) + kT - 1) / kT) - tile_first);
   cur += seg_tiles;
@@ -363,7 +368,10 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   const BtT *bt = static_cast<const BtT *>(p.block_table) + size_t(b) * p.bt_stride;
   // Lane i % kGroups looks up 16-row group i of a tile; the entry is loaded a
   // tile ahead of its use.
-  auto group_of = [&](int t0) { return min(t0 + 16 * (lane & (kGroups - 1)), t_end - 1) >> 4; };
+  auto group_of = [&](int t0) {
+    const int t = min(t0 + 16 * (lane & (kGroups - 1)), t_end - 1);
+    return (kWin ? win.real(t) : t) >> 4;
+  };
   auto block_at = [&](int t0) {
     const int gr = group_of(t0);
     return bt[__umulhi(2u * uint32_t(gr), page_magic)];  // not widened here: that would wait for it
@@ -504,14 +512,37 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     const int t0 = t_begin + it * kT;
     const uint32_t ok_now = ok_groups;
     // Every row of the tile lies in the cache and every query row sees it (uniform).
-    const bool full = t0 + kT <= min(ctx, t_end) && (ok_now & ((1u << kGroups) - 1u)) == (1u << kGroups) - 1u;
+    bool full = (ok_now & ((1u << kGroups) - 1u)) == (1u << kGroups) - 1u;
+    if constexpr (kWin) {
+      // Behind the first rows the tile starts in the last query row's window and ends at or before the first one.
+      full = full && t0 + kT <= t_end && t0 >= win.head && int64_t(win.real(t0)) > int64_t(ctx) - 1 - p.window &&
+             win.real(t0) + kT - 1 <= ctx - count;
+    } else {
+      full = full && t0 + kT <= min(ctx, t_end);
+    }
     // The rows each query row sees: bit 4 kb + e for cache row 4 g + e of block kb.  All
     // mask bytes are loaded before one is used (clamped into the row; what is no
     // draft does not look at its byte).
     uint32_t seen[kRB];
 #pragma unroll
     for (int rb = 0; rb < kRB; ++rb) seen[rb] = 0xFFFFFFFFu;
-    if (!full) {
+    if (kWin && !full) {
+#pragma unroll
+      for (int rb = 0; rb < kRB; ++rb) {
+        const int at = ctx - count + (row_at(rb).query - begin);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int kb = 0; kb < kKB; ++kb) {
+          const int t = t0 + 16 * (wave * kKB + kb) + 4 * g, real = win.real(t);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool vis = bool((ok_now >> (wave * kKB + kb)) & 1u) & (t + e < t_end) & window_sees(p, at, real + e);
+            bits |= uint32_t(vis) << (4 * kb + e);
+          }
+        }
+        seen[rb] = bits;
+      }
+    } else if (!full) {
       const int base = t0 + 16 * wave * kKB + 4 * g;
       uint32_t byte[kRB][kKB][4];
       if (p.mask) {  // uniform
@@ -702,8 +733,8 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     // O^T += V^T P^T: slots 8 g + e of a 32-row step are rows 4 g + e of its
     // first 16, then of its second 16, as P lies in LDS.
     if (!full) {
-      // Rows that are not there, then infinities and NaN among the drafts: a
-      // query row that does not see one must not meet it in the product.
+      // Rows that are not there, then infinities and NaN among the drafts (or at a
+      // window's edges): a query row that does not see one must not meet it in the product.
       bool odd = false;
 #pragma unroll
       for (int j = 0; j < kVR / 16; ++j)
@@ -712,7 +743,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
           uint32_t &w = vraw[j >> 1][4 * (j & 1) + e];
           const int t = t0 + kVR * vgroup + 16 * j + 4 * g + e;
           w = bool((ok_now >> (kVR / 16 * vgroup + j)) & 1u) & (t < t_end) ? w : 0u;
-          odd |= (t >= ctx) & some_not_finite(w);
+          odd |= (kWin | (t >= ctx)) & some_not_finite(w);
         }
       if (__any(odd)) {
 #pragma unroll 1
@@ -725,7 +756,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
 #pragma unroll 1
           for (int byte = 0; byte < 4; ++byte) {
             const uint32_t c = (w >> (8 * byte)) & 0xFFu;
-            const bool bad = t_lane >= ctx && ((c & 0x7Fu) == 0x6Fu || c == 0x80u);
+            const bool bad = (kWin || t_lane >= ctx) && ((c & 0x7Fu) == 0x6Fu || c == 0x80u);
             uint64_t left = __ballot(bad);
             if (bad) w &= ~(0xFFu << (8 * byte));
             while (left) {
@@ -739,7 +770,9 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
               for (int rb = 0; rb < kRB; ++rb) {
                 // (t, dim) is element sn % 4 of accumulator `byte` in the lanes of group sn / 4.
                 const Row row = row_at(rb);
-                const bool vis = g == (sn >> 2) && row.ok && p.mask[size_t(row.query) * p.mask_stride + (t - ctx)] != 0;
+                bool vis = g == (sn >> 2) && row.ok;
+                if constexpr (kWin) vis = vis && window_sees(p, ctx - count + (row.query - begin), win.real(t));
+                else vis = vis && p.mask[size_t(row.query) * p.mask_stride + (t - ctx)] != 0;
                 const uint16_t pb = pt[(16 * rb + n) * kPStride + at];
                 const float add = vis ? ((pb & 0x8000u) ? -v : v) : 0.f;
 #pragma unroll
@@ -946,6 +979,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     }
     int begin, count;
     request_rows(p, b, begin, count);
+    if (left_out(p, count)) return;
     const Parts parts = parts_of(p, b, row, row - begin, int(r) - row * p.hq);
     if (written(p, parts)) return;
     float m, inv;
@@ -975,6 +1009,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_join(const RowAttnPara
     }
     int begin, count;
     request_rows(p, b, begin, count);
+    if (left_out(p, count)) return;  // uniform
     const Parts parts = parts_of(p, b, row, row - begin, r - row * p.hq);
     if (written(p, parts)) return;  // uniform
     float m, inv;
@@ -1129,8 +1164,9 @@ template <int kD, bool kBf16, int kRB, typename BtT>
 void launch_rows(const RowAttnParams &p, uint32_t magic, hipStream_t s) {
   const unsigned threads = 64 * waves_of(kRB);
   const dim3 blocks = row_grid(p);
-  if (p.x) row_attention_mfma<kD, kBf16, kRB, true, BtT><<<blocks, threads, 0, s>>>(p, magic);
-  else row_attention_mfma<kD, kBf16, kRB, false, BtT><<<blocks, threads, 0, s>>>(p, magic);
+  if (p.window) row_attention_mfma<kD, kBf16, kRB, false, true, BtT><<<blocks, threads, 0, s>>>(p, magic);
+  else if (p.x) row_attention_mfma<kD, kBf16, kRB, true, false, BtT><<<blocks, threads, 0, s>>>(p, magic);
+  else row_attention_mfma<kD, kBf16, kRB, false, false, BtT><<<blocks, threads, 0, s>>>(p, magic);
 }
 
 template <bool kBf16, typename BtT>
@@ -1208,7 +1244,7 @@ int row_attention(const char *name, const RowArgs &a) {
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", name);
 
   const int64_t group = a.heads / a.hkv, longest = std::max<int64_t>(a.max_query, 1);
-  const bool mfma = !a.window && mfma_rows(a.d, a.dv, a.hkv, a.block_size, a.max_len) && aligned(a.query, 16) && aligned(a.out, 16) &&
+  const bool mfma = mfma_rows(a.d, a.dv, a.hkv, a.block_size, a.max_len) && aligned(a.query, 16) && aligned(a.out, 16) &&
                     longest * group < 0xFFFF * 16 && (longest * group + 64) * group < (int64_t(1) << 31);  // the grid's y, token_of
   if (mfma && a.batch * (a.max_len / 64 + 1) > 0x7FFFFFFFll / 2)
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
@@ -1241,6 +1277,7 @@ int row_attention(const char *name, const RowArgs &a) {
   p.window = int(a.window);
   p.sinks = int(a.sinks);
   p.most_rows = int(most_rows);
+  p.long_rows = 0x7FFFFFFF;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   const size_t rows = size_t(a.total_q) * a.heads;
   const RowSpace space = row_space(pl, a.batch, a.total_q, a.heads, a.dv, most_rows, a.weights != nullptr);
