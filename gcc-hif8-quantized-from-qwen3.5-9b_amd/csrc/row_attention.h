@@ -4,6 +4,8 @@
 // sliding window.
 #pragma once
 
+#include <stddef.h>
+
 #include "hif8_common.h"
 
 namespace hif8 {
@@ -101,5 +103,39 @@ __device__ __forceinline__ int request_of_row(const RowAttnParams &p, int row) {
   request_rows(p, lo, begin, count);
   return row >= begin && row - begin < count ? lo : -1;
 }
+
+// Host side: a call's arguments, and the call (row_attention.hip).  long_rows: requests
+// of more (token, head) rows per KV head are left to another kernel (window; 0: none).
+struct RowArgs {
+  const void *query;
+  int q_dtype;
+  const uint8_t *key_cache, *value_cache;
+  int64_t num_blocks, block_size, hkv, d, dv;
+  const void *block_table;
+  int bt_dtype;
+  int64_t max_blocks;
+  const int32_t *start_loc, *lens;
+  const uint8_t *mask;
+  int64_t mask_stride, batch, heads, total_q, max_query, max_len;
+  float scale;
+  void *out;
+  float *weights;
+  int64_t w_stride;
+  int accumulate;
+  int zero_rest;
+  void *workspace;
+  size_t workspace_bytes;
+  hif8_stream_t stream;
+  int64_t window, sinks, long_rows;
+};
+
+int check_row_args(const char *name, const RowArgs &a);  // the arguments alone, without the workspace
+int row_attention(const char *name, const RowArgs &a);
+// Its workspace; max_len as rows_bound gives it.
+size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv, int64_t d, int64_t dv,
+                     int64_t block_size, int64_t max_query, int64_t max_len, bool weights);
+// Cache rows of a request that its query rows can see: all of them, or the window's
+// (WindowRows: whole groups of 16).
+int64_t rows_bound(int64_t max_len, int64_t max_query, int64_t window, int64_t sinks);
 
 }  // namespace hif8

@@ -46,6 +46,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
   if (b < 0) return;  // a row behind the last request (uniform)
   int begin, count;
   request_rows(p, b, begin, count);
+  if (left_out(p, count)) return;  // uniform
   const int ctx = clamp_rows(p.lens[b], p.max_len);
   const WindowRows win = p.window ? window_rows(p, ctx, count) : WindowRows{ctx, 0, 0};
   const int at = ctx - count + (row - begin);  // window: this query row's position
@@ -1136,24 +1137,6 @@ RowSpace row_space(const RowPlan &pl, int64_t batch, int64_t total_q, int64_t he
   return w;
 }
 
-// Cache rows of a request that its query rows can see: all of them, or the window's
-// (WindowRows: whole groups of 16).
-int64_t rows_bound(int64_t max_len, int64_t max_query, int64_t window, int64_t sinks) {
-  return window ? std::min(max_len, (sinks + 15) / 16 * 16 + window + max_query + 15) : max_len;
-}
-
-// Bytes for either kernel: the query's alignment, which also decides, is not known here.
-size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv, int64_t d, int64_t dv,
-                     int64_t block_size, int64_t max_query, int64_t max_len, bool weights) {
-  size_t need = 0;
-  for (const bool mfma : {false, true}) {
-    if (mfma && !mfma_rows(d, dv, hkv, block_size, max_len)) continue;
-    const RowPlan pl = plan_rows(mfma, batch, total_q, heads, hkv, d, block_size, max_query, max_len);
-    need = std::max(need, row_space(pl, batch, total_q, heads, dv, max_len, weights).total());
-  }
-  return need;
-}
-
 // x: XCDs; y: blocks that share a worker's cache rows; z: the workers (by KV head) in eights.
 dim3 row_grid(const RowAttnParams &p) {
   const int outer = p.heads_together ? p.workers : p.workers * p.hkv;
@@ -1186,30 +1169,25 @@ void launch_row_attention(const RowAttnParams &p, const RowPlan &pl, hipStream_t
   else with_dim(std::integral_constant<int, 256>{});
 }
 
-struct RowArgs {
-  const void *query;
-  int q_dtype;
-  const uint8_t *key_cache, *value_cache;
-  int64_t num_blocks, block_size, hkv, d, dv;
-  const void *block_table;
-  int bt_dtype;
-  int64_t max_blocks;
-  const int32_t *start_loc, *lens;
-  const uint8_t *mask;
-  int64_t mask_stride, batch, heads, total_q, max_query, max_len;
-  float scale;
-  void *out;
-  float *weights;
-  int64_t w_stride;
-  int accumulate;
-  int zero_rest;
-  void *workspace;
-  size_t workspace_bytes;
-  hif8_stream_t stream;
-  int64_t window, sinks;
-};
+}  // namespace
 
-int row_attention(const char *name, const RowArgs &a) {
+int64_t rows_bound(int64_t max_len, int64_t max_query, int64_t window, int64_t sinks) {
+  return window ? std::min(max_len, (sinks + 15) / 16 * 16 + window + max_query + 15) : max_len;
+}
+
+// Bytes for either kernel: the query's alignment, which also decides, is not known here.
+size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv, int64_t d, int64_t dv,
+                     int64_t block_size, int64_t max_query, int64_t max_len, bool weights) {
+  size_t need = 0;
+  for (const bool mfma : {false, true}) {
+    if (mfma && !mfma_rows(d, dv, hkv, block_size, max_len)) continue;
+    const RowPlan pl = plan_rows(mfma, batch, total_q, heads, hkv, d, block_size, max_query, max_len);
+    need = std::max(need, row_space(pl, batch, total_q, heads, dv, max_len, weights).total());
+  }
+  return need;
+}
+
+int check_row_args(const char *name, const RowArgs &a) {
   if (a.batch < 0 || a.heads <= 0 || a.hkv <= 0 || a.d <= 0 || a.dv <= 0 || a.num_blocks <= 0 || a.block_size <= 0 ||
       a.max_blocks <= 0 || a.max_len < 0 || a.total_q < 0)
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions must be positive", name);
@@ -1234,6 +1212,12 @@ int row_attention(const char *name, const RowArgs &a) {
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: caches must be 4-byte aligned", name);
   if (!aligned(a.query, 2) || !aligned(a.out, 2))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: query/out must be 2-byte aligned", name);
+  return HIF8_OK;
+}
+
+int row_attention(const char *name, const RowArgs &a) {
+  if (const int st = check_row_args(name, a)) return st;
+  if (a.batch == 0 || a.total_q == 0) return HIF8_OK;
   const int64_t most_rows = rows_bound(a.max_len, a.max_query, a.window, a.sinks);
   const size_t need = row_workspace(a.batch, a.total_q, a.heads, a.hkv, a.d, a.dv, a.block_size, a.max_query, most_rows,
                                     a.weights != nullptr);
@@ -1277,7 +1261,7 @@ int row_attention(const char *name, const RowArgs &a) {
   p.window = int(a.window);
   p.sinks = int(a.sinks);
   p.most_rows = int(most_rows);
-  p.long_rows = 0x7FFFFFFF;
+  p.long_rows = a.long_rows ? int(a.long_rows) : 0x7FFFFFFF;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   const size_t rows = size_t(a.total_q) * a.heads;
   const RowSpace space = row_space(pl, a.batch, a.total_q, a.heads, a.dv, most_rows, a.weights != nullptr);
@@ -1320,7 +1304,6 @@ int row_attention(const char *name, const RowArgs &a) {
   return check_launch(name);
 }
 
-}  // namespace
 }  // namespace hif8
 
 using namespace hif8;
@@ -1414,47 +1397,4 @@ extern "C" int hif8_paged_decode_attention_weights(const void *query, int q_dtyp
                                       head_size, head_size_v, block_table, block_table_dtype, max_blocks_per_seq,
                                       nullptr, seq_lens, nullptr, 0, batch, num_heads, batch, 1, max_seq_len, scale, out,
                                       key_weights, weights_stride, accumulate, 0, workspace, workspace_bytes, stream});
-}
-
-extern "C" size_t hif8_window_attention_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
-                                                       int64_t head_size, int64_t head_size_v, int64_t block_size,
-                                                       int64_t total_query_tokens, int64_t max_query_len,
-                                                       int64_t max_seq_len, int64_t window, int64_t sinks) {
-  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0 || head_size_v <= 0 || block_size <= 0 ||
-      total_query_tokens <= 0 || max_query_len <= 0 || max_seq_len < 0 || window <= 0 || sinks < 0 ||
-      num_heads % num_kv_heads)
-    return 0;
-  window = std::min<int64_t>(window, 0x7FFFFFFF), sinks = std::min<int64_t>(sinks, 0x7FFFFFFF);
-  return row_workspace(batch, total_query_tokens, num_heads, num_kv_heads, head_size, head_size_v, block_size,
-                       max_query_len, rows_bound(max_seq_len, max_query_len, window, sinks), false);
-}
-
-extern "C" int hif8_window_attention(const void *query, int q_dtype, const uint8_t *key_cache,
-                                     const uint8_t *value_cache, int64_t num_blocks, int64_t block_size,
-                                     int64_t num_kv_heads, int64_t head_size, int64_t head_size_v,
-                                     const void *block_table, int block_table_dtype, int64_t max_blocks_per_seq,
-                                     const int32_t *query_start_loc, const int32_t *seq_lens, int64_t batch,
-                                     int64_t num_heads, int64_t total_query_tokens, int64_t max_query_len,
-                                     int64_t max_seq_len, int64_t window, int64_t sinks, float scale, void *out,
-                                     void *workspace, size_t workspace_bytes, hif8_stream_t stream) {
-  static const char *kName = "hif8_window_attention";
-  clear_error();
-  if (window <= 0 || sinks < 0)
-    return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: window must be positive and sinks not negative", kName);
-  if (max_query_len < 0) return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions must be positive", kName);
-  if (batch > 0 && total_query_tokens > 0) {
-    if (max_query_len == 0)
-      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: max_query_len must cover the query rows", kName);
-    if (!query_start_loc && (max_query_len != 1 || total_query_tokens != batch))
-      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: without query_start_loc every request has one query row", kName);
-    if (max_query_len > 0x7FFFFFFF)
-      return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", kName);
-  }
-  // Past the lengths' range a window or a count of first rows means the same.
-  window = std::min<int64_t>(window, 0x7FFFFFFF), sinks = std::min<int64_t>(sinks, 0x7FFFFFFF);
-  return row_attention(kName, RowArgs{query, q_dtype, key_cache, value_cache, num_blocks, block_size, num_kv_heads,
-                                      head_size, head_size_v, block_table, block_table_dtype, max_blocks_per_seq,
-                                      query_start_loc, seq_lens, nullptr, 0, batch, num_heads, total_query_tokens,
-                                      max_query_len, max_seq_len, scale, out, nullptr, 0, 0, 1, workspace,
-                                      workspace_bytes, stream, window, sinks});
 }

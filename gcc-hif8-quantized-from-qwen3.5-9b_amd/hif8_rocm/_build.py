@@ -29,7 +29,8 @@ ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 HIP_SOURCES = ["capi.hip", "static_quant.hip", "gemv.hip", "gemm.hip", "gemm_skinny.hip",
                "static_operand.hip", "linear_api.hip", "kv_cache.hip",
                "embedding.hip", "model_ops.hip", "gdn_prefill.hip", "prefill_attention.hip",
-               "row_attention.hip", "key_weights.hip", "cache_edit.hip", "page_tables.hip", "verify.hip"]
+               "row_attention.hip", "key_weights.hip", "cache_edit.hip",
+               "window_attention.hip", "page_tables.hip", "verify.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
