@@ -9,8 +9,8 @@
 //     request sees into an image: the MFMA operands of K and of V^T as fragments
 //     of 1 KiB, 16 bytes a lane, and the row scales beside them.  Codes are exact in
 //     bf16 and fp16, so nothing is rounded;
-//   * window_attention_kernel: a workgroup of four wavefronts owns (request, KV
-//     head, 128 (token, head) rows), 32 rows a wavefront, and walks the images of
+//   * window_attention_kernel: a workgroup owns (request, KV head, up to 256 (token,
+//     head) rows), 32 rows a wavefront, and walks the images of
 //     the rows it sees.  Per image S^T = K Q^T and O^T += V^T P^T on
 //     v_mfma_f32_32x32x16, a softmax with a running maximum between them.
 // The rows seen are pushed together in groups of 16 (WindowRows), so the first rows
@@ -35,25 +35,36 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
-constexpr int kThreads = 256;  // four wavefronts
-constexpr int kRows = 128;     // (token, head) rows of a workgroup, 32 a wavefront
+constexpr int kThreads = 256;  // of the kernels around the attention
 constexpr int kKeys = 32;      // cached rows of an image
-constexpr int kMaxSplits = 64;
+// Wavefronts of the attention's workgroups, 32 (token, head) rows each, and workgroups per
+// CU: as many wavefronts as the registers hold, in few workgroups, since every one copies
+// the images into its own LDS.
+constexpr int waves_of(int d) { return d == 128 ? 12 : 8; }
+constexpr int groups_per_cu(int d) { return d == 64 ? 2 : 1; }
+constexpr int rows_of(int d) { return 32 * waves_of(d); }
+constexpr int kStages = 4;     // images in LDS: two that are worked on, two on their way
+constexpr int kMaxSlots = 1024;  // requests of a pass
 
 // An image: K fragments [D / 16], V fragments [D / 32][2], then K's scales (times the
-// softmax scale, base 2) [32], V's [32], and two words: rows that are there, rows whose V
-// holds an infinity or NaN.
+// softmax scale, base 2) [32], V's [32], and three words: rows that are there, rows whose V
+// holds an infinity or NaN, the largest of V's scales.
 constexpr int frag_bytes(int d) { return 2 * kKeys * d * 2; }
 constexpr int img_bytes(int d) { return (frag_bytes(d) + 8 * kKeys + 16 + 1023) / 1024 * 1024; }
 
 struct WindowParams {
   RowAttnParams r;       // request split, lengths, table, caches, window
   uint8_t *img;          // [slots][hkv][tiles]
-  float *part_o;         // [slots][hkv][q_tiles][splits][kRows][D]
-  float *part_ml;        // [slots][hkv][q_tiles][splits][kRows][2]
+  int4 *items;           // [most_items][2] of each item: (request, slot, KV head, first query row), (request's first row, rows, cached rows, 0)
+  int32_t *plan;         // [items + 1] images before each item, kStart more for each, the last entry all of them
+  int32_t *plan_items;   // [1] items of the pass
+  int32_t *plan_first;   // [workers] the item in which each run begins
+  float *part_o;         // [2 workers][rows_of(D)][D]
+  float *part_ml;        // [2 workers][rows_of(D)][2]
   int tiles;             // images per (slot, KV head)
   int slots, first_slot; // requests of this pass; slot s holds the (first_slot + s)-th long request
-  int tokens, q_tiles, splits;  // tokens of a workgroup, workgroups of the longest request, parts of its rows
+  int tokens;            // of an item
+  int most_items, workers;
   int zero_rest;         // one request: rows of the query outside it get zeros here
 };
 
@@ -78,6 +89,118 @@ __device__ __forceinline__ int long_request(const RowAttnParams &p, int s) {
   return -1;
 }
 
+// The work of a pass: items (KV head, rows_of(D) rows of it) of its requests, one request after
+// the other, and the images that each sees.  The images of all items, one item after the
+// other, are dealt out to the workers in equal runs, one worker for each workgroup that
+// fits on the GPU: an item that does not end in its worker's run goes on in the next
+// one's, and its parts are joined afterwards.  An item counts kStart images more than it
+// sees, for its start and end (with none a run of fifteen short items took 399 us where
+// the others took 262 to 320).  Whole items in two rounds left CUs idle for
+// a fifth of the time (8192 rows within 2048: 343 us, of which the workgroups ran 270).
+
+constexpr int kStart = 4;
+
+// The images that the query rows tok0 .. of a request see: the first `sinks` of them, and
+// those from `near` on, `total` in all.
+struct Walk {
+  int sinks, near, total;
+  __device__ int image(int i) const { return i < sinks ? i : i - sinks + near; }
+};
+
+__device__ __forceinline__ Walk walk_of(const WindowParams &p, int len, int count, const WindowRows &win, int tok0) {
+  const int first_at = len - count;  // position of the request's first query row
+  const int last = min(win.rows, max(0, first_at + min(tok0 + p.tokens, count) - win.skip));
+  const int low = int(max(int64_t(first_at) + tok0 + 1 - p.r.window, int64_t(win.skip))) - win.skip;
+  const int sinks = (min(p.r.sinks, last) + kKeys - 1) / kKeys;
+  const int near = max(low / kKeys, sinks);
+  return Walk{sinks, near, sinks + max((last + kKeys - 1) / kKeys - near, 0)};
+}
+
+// Worker w of `workers` has the images floor(total w / workers) on.
+__device__ __forceinline__ int run_begin(int total, int w, int workers) { return int(int64_t(total) * w / workers); }
+
+// The plan, by one workgroup.
+__device__ void make_plan(const WindowParams &p) {
+  __shared__ int first[kMaxSlots], owner[kMaxSlots];  // items before each slot's request, the request
+  __shared__ int sums[kThreads / kWave];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int items = 0, rank = -p.first_slot, slots = 0;
+  for (int base = 0; base < p.r.batch; base += kWave) {
+    const int b = base + lane;
+    const bool lng = b < p.r.batch && is_long(p.r, b);
+    const uint64_t mask = __ballot(lng);
+    const int slot = rank + __popcll(mask & ((uint64_t(1) << lane) - 1));
+    rank += __popcll(mask);
+    int n = 0;
+    const bool mine = lng && slot >= 0 && slot < p.slots;
+    if (mine) {
+      int begin, count;
+      request_rows(p.r, b, begin, count);
+      n = (count + p.tokens - 1) / p.tokens * p.r.hkv;
+    }
+    const int upto = items + wave_prefix(n);
+    if (mine && wave == 0) {
+      first[slot] = upto - n;
+      owner[slot] = b;
+    }
+    items = __builtin_amdgcn_readlane(upto, kWave - 1);
+    slots += __popcll(__ballot(mine));
+  }
+  items = min(items, p.most_items);
+  __syncthreads();
+  int before = 0;
+  for (int base = 0; base < items; base += kThreads) {
+    const int item = base + tid;
+    int mine = 0;
+    if (item < items) {
+      int s = 0, hi = slots - 1;
+      while (s < hi) {
+        const int mid = (s + hi + 1) / 2;
+        if (first[mid] <= item) s = mid;
+        else hi = mid - 1;
+      }
+      int begin, count;
+      request_rows(p.r, owner[s], begin, count);
+      const int len = clamp_rows(p.r.lens[owner[s]], p.r.max_len);
+      // The last query rows, which see most, first.
+      const int tiles = (count + p.tokens - 1) / p.tokens, in = item - first[s];
+      const int tok0 = (tiles - 1 - in % tiles) * p.tokens;
+      mine = walk_of(p, len, count, window_rows(p.r, len, count), tok0).total;
+      if (mine) mine += kStart;
+      p.items[2 * item] = make_int4(owner[s], s, in / tiles, tok0);
+      p.items[2 * item + 1] = make_int4(begin, count, len, 0);
+    }
+    const int upto = wave_prefix(mine);
+    if (lane == kWave - 1) sums[wave] = upto;
+    __syncthreads();
+    int left = before;
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) {
+      left += w < wave ? sums[w] : 0;
+      before += sums[w];
+    }
+    if (item < items) p.plan[item] = left + upto - mine;
+    __syncthreads();
+  }
+  if (tid == 0) {
+    p.plan[items] = before;
+    *p.plan_items = items;
+  }
+  __syncthreads();
+  // The last item that starts at or before a run does; it has images.
+  const int workers = min(p.workers, before);
+  for (int w = tid; w < workers; w += kThreads) {
+    const int at = run_begin(before, w, workers);
+    int lo = 0, hi = items - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (p.plan[mid] <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    p.plan_first[w] = lo;
+  }
+}
+
 // ------------------------------------------------------------------ images
 
 // A workgroup per (slot, KV head, kThreads / D * 32 rows): threads take 16 codes of a K
@@ -92,9 +215,13 @@ __global__ __launch_bounds__(kThreads) void window_image_kernel(const WindowPara
   constexpr int kLoads = kKeys * kChunks / kPerTile;
   static_assert(kPerTile == kD && kD % 64 == 0, "a wavefront works on one image");
   __shared__ uint32_t dec[256];  // the query's type below, fp16 (0 where not finite) above
-  __shared__ uint32_t odd[kTiles];
+  __shared__ uint32_t odd[kTiles], top[kTiles];
   const int tid = threadIdx.x;
-  const int xcd = int(blockIdx.x) & 7, rest = int(blockIdx.x) >> 3;
+  if (blockIdx.x < 8) {  // the first eight make the plan or nothing
+    if (blockIdx.x == 0) make_plan(p);
+    return;
+  }
+  const int xcd = int(blockIdx.x) & 7, rest = (int(blockIdx.x) >> 3) - 1;
   const int h = rest % p.r.hkv;
   const int group = (rest / p.r.hkv) * 8 + xcd;  // tiles of one slot after the other
   const int groups = (p.tiles + kTiles - 1) / kTiles;
@@ -113,7 +240,7 @@ __global__ __launch_bounds__(kThreads) void window_image_kernel(const WindowPara
     const bool finite = (tid & 0x7F) != 0x6F && tid != 0x80;
     const uint32_t half = float_to_f16_bits(__uint_as_float(f));
     dec[tid] = (kBf16 ? f >> 16 : half) | (finite ? half << 16 : 0u);
-    if (tid < kTiles) odd[tid] = 0;
+    if (tid < kTiles) odd[tid] = top[tid] = 0;
   }
   const int tile = first + tid / kPerTile, at = tid % kPerTile;
   const BtT *bt = static_cast<const BtT *>(p.r.block_table) + size_t(b) * p.r.bt_stride;
@@ -195,12 +322,14 @@ __global__ __launch_bounds__(kThreads) void window_image_kernel(const WindowPara
       sc[at] = ksc;
       sc[kKeys + at] = finite ? vsc : 0.f;
       if (!finite) atomicOr(&odd[tid / kPerTile], 1u << at);
+      else atomicMax(&top[tid / kPerTile], __float_as_uint(fabsf(vsc)));
     }
     const uint64_t seen = __ballot(there);  // the image's first wavefront
     if (at == 0) reinterpret_cast<uint32_t *>(im + frag_bytes(kD))[2 * kKeys] = uint32_t(seen);
   }
   __syncthreads();
-  if (mine && at == 0) reinterpret_cast<uint32_t *>(im + frag_bytes(kD))[2 * kKeys + 1] = odd[tid / kPerTile];
+  if (mine && at == 0)
+    *reinterpret_cast<u32x2 *>(im + frag_bytes(kD) + 8 * kKeys + 4) = u32x2{odd[tid / kPerTile], top[tid / kPerTile]};
 }
 
 // --------------------------------------------------------------- attention
@@ -235,100 +364,143 @@ __device__ __forceinline__ float sum_of_halves(float x) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// A value that is the same in all lanes, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Of all lanes, without a trip through LDS.
+__device__ __forceinline__ float max_over_lanes(float x) {
+  x = fmaxf(x, rotated<8>(x));
+  x = fmaxf(x, rotated<4>(x));
+  x = fmaxf(x, rotated<2>(x));
+  return max_over_groups(fmaxf(x, rotated<1>(x)));
+}
+
 // Weights are 2^(x - m + kBias - e), m a maximum of the row that moves once a logit passes
 // it by kLazy, 2^e the power of two above the largest of V's scales (held within 2^+-96, so
 // that sums of weights stay in range): P = weight * V's scale stays below 2^14 and starts
 // high in fp16's range, so that small weights keep their bits.
 constexpr float kBias = 6.f, kLazy = 8.f;
 
+// 32 rows that a wavefront holds as S^T and O^T lie (row lane % 32, value(db, q): dims 32 db
+// + 8 q + 4 (lane / 32) + [0, 4)) to their places in out, at(row) or -1: through LDS, since
+// their eight-byte pieces in 32 rows at a time kept the next item waiting for 8 us.
+template <int kD>
+constexpr int kRowsLds = 32 * (2 * kD + 16);
+
+template <int kD, bool kBf16, typename Value, typename At>
+__device__ __forceinline__ void store_rows(uint8_t *lds, uint16_t *out, Value value, At at) {
+  constexpr int kPitch = 2 * kD + 16, kPerRow = kD / 8;  // 16-byte pieces of a row
+  const int lane = threadIdx.x & 63, n = lane & 31, hf = lane >> 5;
+#pragma unroll
+  for (int db = 0; db < kD / 32; ++db)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4_t v = value(db, q);
+      *reinterpret_cast<u32x2 *>(lds + n * kPitch + 64 * db + 16 * q + 8 * hf) =
+          u32x2{pack_out<kBf16>(v[0], v[1]), pack_out<kBf16>(v[2], v[3])};
+    }
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll 4
+  for (int i = 0; i < 32; i += kWave / kPerRow) {
+    const int row = i + lane / kPerRow, piece = lane % kPerRow;
+    const u32x4 v = *reinterpret_cast<const u32x4 *>(lds + row * kPitch + 16 * piece);
+    const int64_t to = at(row);
+    if (to >= 0) *reinterpret_cast<u32x4 *>(out + to + 8 * piece) = v;
+  }
+}
+
 template <int kD, bool kBf16, typename BtT>
-__global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void window_attention_kernel(const WindowParams p) {
+__global__ __launch_bounds__(64 * waves_of(kD), waves_of(kD) * groups_per_cu(kD) / 4) void window_attention_kernel(const WindowParams p) {
   constexpr int kQS = kD / 16;   // MFMA steps over the head dims
   constexpr int kDB = kD / 32;   // 32-dim blocks of O^T
   constexpr int kImg = img_bytes(kD);
   constexpr int kCopies = kImg / 1024;
-  constexpr int kAhead = 2;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // two images
-  __shared__ int top;
+  constexpr int kAheadK = 2, kAheadV = 2;
+  constexpr int kWaves = waves_of(kD), kRows = rows_of(kD);
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // kStages images
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, hf = lane >> 5;
-  // Neighbouring query tiles of one KV head see nearly the same images: they run on
-  // one XCD, one after the other.
-  const int items = p.slots * p.r.hkv * p.q_tiles * p.splits;
-  const int per_xcd = (items + 7) / 8;
-  const int item = (int(blockIdx.x) & 7) * per_xcd + (int(blockIdx.x) >> 3);
-  if ((int(blockIdx.x) >> 3) >= per_xcd || item >= items) return;  // padding block (uniform)
-  const int split = item % p.splits, qt = (item / p.splits) % p.q_tiles;
-  const int sh = item / (p.splits * p.q_tiles);
-  const int slot = sh / p.r.hkv, h = sh - slot * p.r.hkv;
-  const int b = long_request(p.r, p.first_slot + slot);
-  int begin = 0, count = 0;
-  if (b >= 0) request_rows(p.r, b, begin, count);
-  const int tok0 = qt * p.tokens;
-  if (p.zero_rest && split == 0) {  // rows of the query outside the only request
-    for (int i = tid; i < p.tokens * p.r.group * (kD / 2); i += kThreads) {
-      const int row = tok0 + i / (p.r.group * (kD / 2)), in_row = i % (p.r.group * (kD / 2));
-      if (row < p.r.total_q && (row < begin || row - begin >= count))
-        reinterpret_cast<uint32_t *>(p.r.out)[(size_t(row) * p.r.hq + h * p.r.group) * (kD / 2) + in_row] = 0;
+  if (p.zero_rest) {  // rows of the query outside the only request
+    int begin, count;
+    request_rows(p.r, 0, begin, count);
+    const int words = p.r.hq * (kD / 2);
+    const int64_t all = int64_t(p.r.total_q - min(count, p.r.total_q)) * words;
+    for (int64_t i = int64_t(blockIdx.x) * 64 * kWaves + tid; i < all; i += int64_t(gridDim.x) * 64 * kWaves) {
+      const int row = int(i / words);
+      static_cast<uint32_t *>(p.r.out)[i + (row < begin ? 0 : int64_t(count) * words)] = 0;
     }
   }
-  if (b < 0 || tok0 >= count) return;  // uniform
-  const int len = clamp_rows(p.r.lens[b], p.r.max_len);
+  // Neighbouring runs see nearly the same images: they are one XCD's.
+  const int per_xcd = p.workers / 8, worker = (int(blockIdx.x) & 7) * per_xcd + (int(blockIdx.x) >> 3);
+  const int items = uniform(*p.plan_items), images = uniform(p.plan[items]);
+  const int workers = min(p.workers, images);  // an image each at least
+  if (worker >= workers) return;               // uniform
+  int cur = run_begin(images, worker, workers);
+  const int run_end = run_begin(images, worker + 1, workers);
+  int item = uniform(p.plan_first[worker]);
+  const uint32_t lds0 = lds_address(smem);
+
+  for (; cur < run_end; ++item) {
+  // This segment: the run's images of one item.
+  const int item_first = uniform(p.plan[item]), item_end = uniform(p.plan[item + 1]);
+  const int4 it = p.items[2 * item], of = p.items[2 * item + 1];
+  if (item_end <= cur) continue;  // an item without images (uniform)
+  const int seen = item_end - item_first - kStart;
+  const int t_begin = cur - item_first, t_end = min(min(run_end, item_end) - item_first, seen);
+  cur = min(run_end, item_end);
+  if (t_begin >= t_end) continue;  // uniform
+  const bool whole = t_begin == 0 && t_end == seen;
+  const int part = 2 * worker + (cur >= run_end ? 1 : 0);
+  const int b = uniform(it.x), slot = uniform(it.y), h = uniform(it.z), tok0 = uniform(it.w);
+  const int begin = uniform(of.x), count = uniform(of.y), len = uniform(of.z);
   const WindowRows win = window_rows(p.r, len, count);
-  const int first_at = len - count;  // position of the request's first query row
+  const Walk walk = walk_of(p, len, count, win, tok0);
+  const int first_at = len - count;
   const int tok_end = min(tok0 + p.tokens, count);
 
-  // The images that this workgroup's rows see: those of the first rows, and from the one
-  // on in which its first row's window begins.
-  const int last_t = min(win.rows, max(0, first_at + tok_end - win.skip));
-  const int tiles_end = (last_t + kKeys - 1) / kKeys;
-  const int low_t = int(max(int64_t(first_at) + tok0 + 1 - p.r.window, int64_t(win.skip))) - win.skip;
-  const int sink_tiles = (min(p.r.sinks, last_t) + kKeys - 1) / kKeys;
-  const int near = max(low_t / kKeys, sink_tiles);
-  const int total = sink_tiles + max(tiles_end - near, 0);
-  const int t_begin = int(int64_t(total) * split / p.splits), t_end = int(int64_t(total) * (split + 1) / p.splits);
-  auto image_of = [&](int i) { return i < sink_tiles ? i : i - sink_tiles + near; };
-
-  // This lane's query row: column n of the wavefront's 32.
-  const int row = wave * 32 + n;
-  const int tok = tok0 + int(__umulhi(2u * uint32_t(row), p.r.group_magic));
-  const int in_group = row - (tok - tok0) * p.r.group;
-  const bool ok = tok < tok_end;
-  const int at = ok ? first_at + tok : -1;
-  const int qhead = h * p.r.group + (ok ? in_group : 0);
-  const size_t out_row = (size_t(begin + (ok ? tok : 0)) * p.r.hq + qhead) * kD;
+  // This lane's query row, column n of the wavefront's 32: whether there is one, its token
+  // and where it lies in query and output.  Worked out where it is needed: held over the
+  // loop it costs registers.
+  struct Row {
+    bool ok;
+    int tok;
+    size_t at;
+  };
+  auto row_of = [&]() {
+    int row = wave * 32 + n;
+    asm volatile("" : "+v"(row));
+    const int in_tile = int(__umulhi(2u * uint32_t(row), p.r.group_magic)), tok = tok0 + in_tile;
+    const bool ok = tok < tok_end;
+    return Row{ok, tok, (size_t(begin + (ok ? tok : 0)) * p.r.hq + h * p.r.group + (ok ? row - in_tile * p.r.group : 0)) * kD};
+  };
+  const Row mine = row_of();
+  const int at = mine.ok ? first_at + mine.tok : -1;  // its position
   // Positions of the wavefront's rows (it may have none).
   const int at_lo = first_at + tok0 + int(__umulhi(2u * uint32_t(wave * 32), p.r.group_magic));
   const int at_hi = min(first_at + tok0 + int(__umulhi(2u * uint32_t(wave * 32 + 31), p.r.group_magic)), first_at + tok_end - 1);
 
   const uint8_t *img = p.img + (size_t(slot) * p.r.hkv + h) * p.tiles * kImg;
-  const uint32_t lds0 = lds_address(smem);
   auto copy = [&](int i, int stage) {
-    const uint8_t *src = img + size_t(image_of(i)) * kImg + 16 * lane;
-    for (int j = wave; j < kCopies; j += kThreads / kWave) dma16(src + 1024 * j, lds0 + uint32_t(stage) * kImg + 1024u * j);
+    const uint8_t *src = img + size_t(walk.image(i)) * kImg;
+    for (int j = wave; j < kCopies; j += kWaves)
+      dma16_offset(src + 1024 * j, uint32_t(16 * lane), lds0 + uint32_t(stage) * kImg + 1024u * j);
   };
   u32x4 qf[kQS];  // lane: dims 16 i + 8 hf + [0, 8) of row n
   {
-    const uint16_t *q = static_cast<const uint16_t *>(p.r.query) + out_row + 8 * hf;
+    const uint16_t *q = static_cast<const uint16_t *>(p.r.query) + mine.at + 8 * hf;
 #pragma unroll
     for (int i = 0; i < kQS; ++i) qf[i] = *reinterpret_cast<const u32x4 *>(q + 16 * i);
   }
-  if (t_begin < t_end) copy(t_begin, 0);
+  lds_barrier();  // the segment before is done with both stages
+  copy(t_begin, 0);
+  if (t_begin + 1 < t_end) copy(t_begin + 1, 1);
   // The power of two of the largest of V's scales.
-  if (tid == 0) top = 0;
-  __syncthreads();
-  {
-    float most = 0.f;
-    for (int i = t_begin * kKeys + tid; i < t_end * kKeys; i += kThreads) {
-      const uint8_t *im = img + size_t(image_of(i / kKeys)) * kImg + frag_bytes(kD);
-      most = fmaxf(most, fabsf(reinterpret_cast<const float *>(im)[kKeys + i % kKeys]));
-    }
-    atomicMax(&top, int(__float_as_uint(most)));
-  }
-  __syncthreads();
-  const float largest = __uint_as_float(uint32_t(__builtin_amdgcn_readfirstlane(top)));
+  float largest = 0.f;
+  for (int i = t_begin + lane; i < t_end; i += kWave)
+    largest = fmaxf(largest, reinterpret_cast<const float *>(img + size_t(walk.image(i)) * kImg + frag_bytes(kD))[2 * kKeys + 2]);
+  largest = max_over_lanes(largest);
   const float base = kBias - float(min(max(largest > 0.f ? int(__builtin_amdgcn_frexp_expf(largest)) : 0, -96), 96));
 
   f32x16_t oacc[kDB];
@@ -338,12 +510,19 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void window_attention_
     for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
   float m = -__builtin_inff(), l = 0.f;
   uint32_t odd_seen = 0;
+  // The query rows have arrived: without this the loop would wait for them, and with them
+  // for the copies behind them, at every image.
+#pragma unroll
+  for (int k = 0; k < kQS; ++k) asm volatile("" : "+v"(qf[k]));
 
   for (int i = t_begin; i < t_end; ++i) {
-    const int stage = (i - t_begin) & 1;
-    wait_vmcnt<0>();  // this wavefront's part of image i
-    lds_barrier();    // every wavefront's; and all are done with the other stage
-    if (i + 1 < t_end) copy(i + 1, stage ^ 1);
+    const int stage = (i - t_begin) % kStages;
+    if (stage % 2 == 0) {
+      wait_vmcnt<0>();  // this wavefront's part of images i and i + 1
+      lds_barrier();    // every wavefront's; and all are done with the other two stages
+      if (i + 2 < t_end) copy(i + 2, stage ^ 2);
+      if (i + 3 < t_end) copy(i + 3, (stage ^ 2) + 1);
+    }
     if (at_lo > at_hi) continue;  // a wavefront without rows (uniform)
     const uint8_t *im = smem + stage * kImg;
     const u32x4 *kf = reinterpret_cast<const u32x4 *>(im) + lane;
@@ -355,41 +534,38 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void window_attention_
     f32x16_t s;
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0.f;
-    // Fragments are read kAhead steps before their products, no earlier: more would spill.
-    u32x4 ka[2][kAhead];
+    // A ring of fragments: each is read kAhead products (32 cycles apiece) before its own,
+    // which is about what LDS takes; further ahead they would spill.
+    u32x4 ka[kAheadK + 1];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) ka[0][k] = kf[64 * k];
+    for (int k = 0; k < kAheadK; ++k) ka[k] = kf[64 * k];
 #pragma unroll
-    for (int k0 = 0; k0 < kQS; k0 += kAhead) {
+    for (int k = 0; k < kQS; ++k) {
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (k0 + kAhead < kQS) ka[(k0 / kAhead + 1) & 1][k] = kf[64 * (k0 + kAhead + k)];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) s = mfma32<kBf16>(ka[(k0 / kAhead) & 1][k], qf[k0 + k], s);
+      if (k + kAheadK < kQS) ka[(k + kAheadK) % (kAheadK + 1)] = kf[64 * (k + kAheadK)];
+      s = mfma32<kBf16>(ka[k % (kAheadK + 1)], qf[k], s);
     }
+    f32x4_t ks[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) ks[q] = *reinterpret_cast<const f32x4_t *>(sc + 8 * q + 4 * hf);
     __builtin_amdgcn_sched_barrier(0);
     // Cache rows of the image's two groups of 16.
-    const int t0 = image_of(i) * kKeys, r0 = win.real(t0), r1 = win.real(t0 + 16);
+    const int t0 = walk.image(i) * kKeys, r0 = win.real(t0), r1 = win.real(t0 + 16);
     const bool full = there == 0xFFFFFFFFu && r1 + 15 <= at_lo && (int64_t(min(r0, r1)) > int64_t(at_hi) - p.r.window ||
                                                                    r1 + 15 < p.r.sinks);
     float x[16];
     float tmax = -__builtin_inff();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4_t ks = *reinterpret_cast<const f32x4_t *>(sc + 8 * q + 4 * hf);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * q + j] = s[4 * q + j] * ks[j];
-    }
+    for (int e = 0; e < 16; ++e) x[e] = s[e] * ks[e >> 2][e & 3];
     if (!full) {
+      // Bit k: row k of the image is there and this lane's query row sees it.
+      auto below = [](int64_t end) { return (1u << min(max(end, int64_t(0)), int64_t(16))) - 1u; };
+      auto seen16 = [&](int r) {
+        return below(int64_t(at) + 1 - r) & (~below(int64_t(at) + 1 - p.r.window - r) | below(int64_t(p.r.sinks) - r));
+      };
+      const uint32_t seen = ((seen16(r0) | (seen16(r1) << 16)) & there) >> (4 * hf);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = 8 * q + 4 * hf + j, real = (q < 2 ? r0 : r1 - 16) + key;
-          const bool vis = bool((there >> key) & 1u) & window_sees(p.r, at, real);
-          x[4 * q + j] = vis ? x[4 * q + j] : -__builtin_inff();
-        }
+      for (int e = 0; e < 16; ++e) x[e] = (seen >> (8 * (e >> 2) + (e & 3))) & 1u ? x[e] : -__builtin_inff();
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, x[e]);
@@ -422,28 +598,25 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void window_attention_
       pf[q >> 1][2 * (q & 1) + 1] = pack_f16(w[2], w[3]);
     }
     l += sum;
-    u32x4 va[2][2];
-    va[0][0] = vf[0], va[0][1] = vf[64];
+    u32x4 va[kAheadV + 1];
 #pragma unroll
-    for (int db = 0; db < kDB; ++db) {
+    for (int k = 0; k < kAheadV; ++k) va[k] = vf[64 * k];
+#pragma unroll
+    for (int k = 0; k < 2 * kDB; ++k) {
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int st = 0; st < 2; ++st)
-        if (db + 1 < kDB) va[(db + 1) & 1][st] = vf[64 * (2 * db + 2 + st)];
-#pragma unroll
-      for (int st = 0; st < 2; ++st) oacc[db] = mfma32<false>(va[db & 1][st], pf[st], oacc[db]);
+      if (k + kAheadV < 2 * kDB) va[(k + kAheadV) % (kAheadV + 1)] = vf[64 * (k + kAheadV)];
+      oacc[k >> 1] = mfma32<false>(va[k % (kAheadV + 1)], pf[k & 1], oacc[k >> 1]);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  if (at_lo > at_hi) return;
   if (odd_seen) {
     // Infinities and NaN of V lie as zeros in the images: the rows that see them get them
     // here.  (In the loop above this would hold a second copy of O.)
 #pragma unroll 1
     for (int i = t_begin; i < t_end; ++i) {
-      const int t0 = image_of(i) * kKeys, r0 = win.real(t0), r1 = win.real(t0 + 16);
+      const int t0 = walk.image(i) * kKeys, r0 = win.real(t0), r1 = win.real(t0 + 16);
       uint32_t left = __builtin_amdgcn_readfirstlane(
-          reinterpret_cast<const uint32_t *>(img + size_t(image_of(i)) * kImg + frag_bytes(kD))[2 * kKeys + 1]);
+          reinterpret_cast<const uint32_t *>(img + size_t(walk.image(i)) * kImg + frag_bytes(kD))[2 * kKeys + 1]);
 #pragma unroll 1
       for (; left; left &= left - 1) {
         const int key = __builtin_ctz(left);
@@ -470,79 +643,111 @@ __global__ __launch_bounds__(kThreads, kD == 256 ? 2 : 3) void window_attention_
     }
   }
   l = sum_of_halves(l);
-  if (!ok) return;
   const float inv = l != 0.f ? 1.f / l : 0.f;
-  if (p.splits == 1) {
-    uint16_t *o = static_cast<uint16_t *>(p.r.out) + out_row + 4 * hf;
+  lds_barrier();  // every wavefront is done with the images: their place takes the rows
+  if (whole) {
+    if (at_lo <= at_hi)
+      store_rows<kD, kBf16>(smem + wave * kRowsLds<kD>, static_cast<uint16_t *>(p.r.out), [&](int db, int q) {
+        return f32x4_t{oacc[db][4 * q] * inv, oacc[db][4 * q + 1] * inv, oacc[db][4 * q + 2] * inv, oacc[db][4 * q + 3] * inv};
+      }, [&](int i) {
+        const int row = wave * 32 + i, in_tile = int(__umulhi(2u * uint32_t(row), p.r.group_magic)), tok = tok0 + in_tile;
+        return tok < tok_end ? (int64_t(begin + tok) * p.r.hq + h * p.r.group + (row - in_tile * p.r.group)) * kD : int64_t(-1);
+      });
+  } else {
+    // As the registers hold it: 1 KiB for each of the wavefront's quads of dims.
+    const size_t rows = size_t(part) * kRows + wave * 32;
+    if (hf == 0) {
+      p.part_ml[2 * (rows + n)] = m;
+      p.part_ml[2 * (rows + n) + 1] = l * __builtin_amdgcn_exp2f(-base);
+    }
+    f32x4_t *o = reinterpret_cast<f32x4_t *>(p.part_o + rows * kD) + lane;
 #pragma unroll
     for (int db = 0; db < kDB; ++db)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x16_t &a = oacc[db];
-        *reinterpret_cast<u32x2 *>(o + 32 * db + 8 * q) =
-            u32x2{pack_out<kBf16>(a[4 * q] * inv, a[4 * q + 1] * inv),
-                  pack_out<kBf16>(a[4 * q + 2] * inv, a[4 * q + 3] * inv)};
-      }
-    return;
+      for (int q = 0; q < 4; ++q)
+        o[64 * (4 * db + q)] =
+            f32x4_t{oacc[db][4 * q] * inv, oacc[db][4 * q + 1] * inv, oacc[db][4 * q + 2] * inv, oacc[db][4 * q + 3] * inv};
   }
-  const size_t part = size_t(item) * kRows + row;
-  if (hf == 0) {
-    p.part_ml[2 * part] = m;
-    p.part_ml[2 * part + 1] = l;
   }
-  if (l == 0.f) return;  // saw nothing: its outputs are not read
-  float *o = p.part_o + part * kD + 4 * hf;
-#pragma unroll
-  for (int db = 0; db < kDB; ++db)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x16_t &a = oacc[db];
-      *reinterpret_cast<f32x4_t *>(o + 32 * db + 8 * q) =
-          f32x4_t{a[4 * q] * inv, a[4 * q + 1] * inv, a[4 * q + 2] * inv, a[4 * q + 3] * inv};
-    }
 }
 
-// Joins the parts of every row: M = max m_s, out = sum_s 2^(m_s - M) l_s o_s / sum_s
-// 2^(m_s - M) l_s, o_s a part's own attention.  A wavefront per row, four dims a lane.
+// Joins the parts of items that lie in several runs: M = max m_s, out = sum_s 2^(m_s - M)
+// l_s o_s / sum_s 2^(m_s - M) l_s, o_s a part's own attention.  Per run a workgroup for
+// every 32 rows takes the item that reaches into it from the one before, if that is
+// where it begins; a wavefront takes a quarter of the dims.  The workgroups behind them
+// give the rows of items without images their zeros.
 template <int kD, bool kBf16>
 __global__ __launch_bounds__(kThreads) void window_join_kernel(const WindowParams p) {
-  const int item = int(blockIdx.x), lane = threadIdx.x & 63;  // (slot, KV head, query tile)
-  const int row = int(blockIdx.y) * (kThreads / kWave) + (threadIdx.x >> 6);
-  const int qt = item % p.q_tiles, sh = item / p.q_tiles, slot = sh / p.r.hkv, h = sh - slot * p.r.hkv;
-  const int b = long_request(p.r, p.first_slot + slot);
-  if (b < 0) return;  // uniform
-  int begin, count;
-  request_rows(p.r, b, begin, count);
-  const int in_tile = int(__umulhi(2u * uint32_t(row), p.r.group_magic)), tok = qt * p.tokens + in_tile;
-  if (in_tile >= p.tokens || tok >= count) return;  // uniform
-  const size_t base = size_t(item) * p.splits * kRows + row;
-  const bool have = lane < p.splits;
-  const float ms = have ? p.part_ml[2 * (base + size_t(have ? lane : 0) * kRows)] : -__builtin_inff();
-  const float ls = have ? p.part_ml[2 * (base + size_t(have ? lane : 0) * kRows) + 1] : 0.f;
-  const float mx = wave_max(ms);
-  // A part that saw nothing has l = 0; one with a NaN logit l = NaN, whatever its maximum.
-  const float w = ls != 0.f ? __builtin_amdgcn_exp2f(ms - (mx == -__builtin_inff() ? 0.f : mx)) * ls : 0.f;
-  const float total = wave_sum(w);
-  const float inv = total != 0.f ? 1.f / total : 0.f;
-  f32x4_t acc{0.f, 0.f, 0.f, 0.f};
-  const bool dims = 4 * lane < kD;
-  for (int s0 = 0; s0 < p.splits; s0 += 8) {
-    float ws[8];
-    f32x4_t v[8];
+  constexpr int kQuads = kD / 32;  // quads of dims of a wavefront
+  constexpr int kRows = rows_of(kD), kBlocks = kRows / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t rows_lds[kRowsLds<kD>];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hf = lane >> 5;
+  const int items = *p.plan_items, images = p.plan[items], workers = min(p.workers, images);
+  if (int(blockIdx.x) >= p.workers * kBlocks) {
+    const int i0 = (int(blockIdx.x) - p.workers * kBlocks) * kThreads;
+    for (int item = i0; item < min(i0 + kThreads, items); ++item) {
+      if (p.plan[item + 1] > p.plan[item]) continue;
+      const int4 it = p.items[2 * item];
+      const int begin = p.items[2 * item + 1].x, count = p.items[2 * item + 1].y;
+      const int words = p.r.group * (kD / 2), rows = min(p.tokens, count - it.w);
+      for (int i = tid; i < rows * words; i += kThreads)
+        static_cast<uint32_t *>(p.r.out)[(size_t(begin + it.w + i / words) * p.r.hq + it.z * p.r.group) * (kD / 2) + i % words] = 0;
+    }
+    return;
+  }
+  const int w = int(blockIdx.x) / kBlocks, block = int(blockIdx.x) % kBlocks;
+  if (w == 0 || w >= workers) return;  // uniform, as what follows
+  const int at = run_begin(images, w, workers), item = p.plan_first[w];
+  const int lo = p.plan[item], hi = p.plan[item + 1] - kStart;
+  if (lo == at || hi <= at || run_begin(images, w - 1, workers) > lo) return;
+  const int w0 = w - 1, w1 = int((int64_t(hi) * workers - 1) / images);
+  const bool ends = run_begin(images, w1 + 1, workers) <= hi + kStart;  // else w1's run goes on with other items
+  const int4 it = p.items[2 * item];
+  const int begin = p.items[2 * item + 1].x, count = p.items[2 * item + 1].y;
+  auto rows_of_part = [&](int s) { return size_t(2 * s + (s < w1 || ends ? 1 : 0)) * kRows + block * 32; };
+  float m = -__builtin_inff();
+  for (int s = w0; s <= w1; ++s) m = fmaxf(m, p.part_ml[2 * (rows_of_part(s) + n)]);
+  if (m == -__builtin_inff()) m = 0.f;
+  float total = 0.f;
+  f32x4_t acc[kQuads];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      ws[j] = s0 + j < p.splits ? __shfl(w, s0 + j, kWave) : 0.f;
-      v[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      if (dims && ws[j] != 0.f)
-        v[j] = *reinterpret_cast<const f32x4_t *>(p.part_o + (base + size_t(s0 + j) * kRows) * kD + 4 * lane);
+  for (int k = 0; k < kQuads; ++k) acc[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = w0; s0 <= w1; s0 += 2) {
+    float f[2];
+    f32x4_t v[2][kQuads];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int s = min(s0 + i, w1);
+      const f32x4_t *o = reinterpret_cast<const f32x4_t *>(p.part_o + rows_of_part(s) * kD) + 64 * kQuads * wave + lane;
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) v[i][k] = o[64 * k];
+      const float ms = p.part_ml[2 * (rows_of_part(s) + n)], ls = p.part_ml[2 * (rows_of_part(s) + n) + 1];
+      // A part that saw nothing has l = 0; one with a NaN logit l = NaN, whatever its maximum.
+      f[i] = s0 + i <= w1 && ls != 0.f ? __builtin_amdgcn_exp2f(ms - m) * ls : 0.f;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc += ws[j] * inv * v[j];
+    for (int i = 0; i < 2; ++i) {
+      total += f[i];
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) acc[k] += f[i] != 0.f ? f[i] * v[i][k] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
   }
-  if (!dims) return;
-  uint16_t *o = static_cast<uint16_t *>(p.r.out) +
-                (size_t(begin + tok) * p.r.hq + h * p.r.group + (row - in_tile * p.r.group)) * kD + 4 * lane;
-  *reinterpret_cast<u32x2 *>(o) = u32x2{pack_out<kBf16>(acc[0], acc[1]), pack_out<kBf16>(acc[2], acc[3])};
+  const float inv = total != 0.f ? 1.f / total : 0.f;
+#pragma unroll
+  for (int k = 0; k < kQuads; ++k) {
+    const int quad = kQuads * wave + k;  // dims 8 quad + 4 hf + [0, 4)
+    *reinterpret_cast<u32x2 *>(rows_lds + n * (2 * kD + 16) + 16 * quad + 8 * hf) =
+        u32x2{pack_out<kBf16>(acc[k][0] * inv, acc[k][1] * inv), pack_out<kBf16>(acc[k][2] * inv, acc[k][3] * inv)};
+  }
+  __syncthreads();
+  for (int i = tid; i < 32 * (kD / 8); i += kThreads) {
+    const int in = i / (kD / 8), piece = i % (kD / 8), row = block * 32 + in;
+    const int in_tile = int(__umulhi(2u * uint32_t(row), p.r.group_magic)), tok = it.w + in_tile;
+    if (in_tile < p.tokens && tok < count)
+      *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p.r.out) +
+                                 (size_t(begin + tok) * p.r.hq + it.z * p.r.group + (row - in_tile * p.r.group)) * kD + 8 * piece) =
+          *reinterpret_cast<const u32x4 *>(rows_lds + in * (2 * kD + 16) + 16 * piece);
+  }
 }
 
 // ------------------------------------------------------------- host side
@@ -555,10 +760,10 @@ constexpr int64_t kImageBytes = int64_t(512) << 20;
 struct WindowPlan {
   int64_t long_rows;   // 0: the only request, whatever its length
   int64_t requests;    // that can be long
-  int64_t slots, tiles, tokens, q_tiles, splits;
+  int64_t slots, tiles, tokens, items, workers;
   bool others;         // short requests may be among them
-  size_t images, parts_o, parts_ml, rows;  // bytes
-  size_t total() const { return std::max(rows, images + parts_o + parts_ml); }
+  size_t images, parts_o, parts_ml, plan, rows;  // bytes
+  size_t total() const { return std::max(rows, images + parts_o + parts_ml + plan); }
 };
 
 bool image_shape(int64_t d, int64_t dv, int64_t group, int64_t block_size) {
@@ -581,18 +786,16 @@ WindowPlan plan_window(int64_t batch, int64_t heads, int64_t hkv, int64_t d, int
     const int64_t seen = rows_bound(max_len, max_query, window, sinks);
     pl.tiles = (seen + kKeys - 1) / kKeys;
     const int64_t per_slot = hkv * pl.tiles * img_bytes(int(d));
-    pl.slots = std::max<int64_t>(1, std::min(pl.requests, kImageBytes / per_slot));
-    pl.tokens = kRows / group;
-    pl.q_tiles = ((batch > 1 ? max_query : std::max(max_query, total_q)) + pl.tokens - 1) / pl.tokens;
-    // Two workgroups a CU, parts of at least eight images.
-    const int64_t items = pl.slots * hkv * pl.q_tiles;
-    const int64_t walk = std::min(pl.tiles, (rows_bound(max_len, pl.tokens, window, sinks) + kKeys - 1) / kKeys + 1);
-    pl.splits = std::max<int64_t>(1, std::min({512 / items, walk / 8, int64_t(kMaxSplits)}));
+    pl.slots = std::max<int64_t>(1, std::min({pl.requests, kImageBytes / per_slot, int64_t(kMaxSlots)}));
+    pl.tokens = rows_of(int(d)) / group;
+    // At most: every request's rows in whole items.
+    pl.items = hkv * (pl.slots * std::min((max_query + pl.tokens - 1) / pl.tokens, total_q / pl.tokens + 1));
+    if (batch > 1) pl.items = std::min(pl.items, hkv * (total_q / pl.tokens + pl.slots));
+    pl.workers = 256 * groups_per_cu(int(d));
     pl.images = size_t(pl.slots) * per_slot;
-    if (pl.splits > 1) {
-      pl.parts_o = size_t(items) * pl.splits * kRows * d * sizeof(float);
-      pl.parts_ml = size_t(items) * pl.splits * kRows * 2 * sizeof(float);
-    }
+    pl.parts_o = size_t(2 * pl.workers) * rows_of(int(d)) * d * sizeof(float);
+    pl.parts_ml = size_t(2 * pl.workers) * rows_of(int(d)) * 2 * sizeof(float);
+    pl.plan = size_t(pl.items) * 2 * sizeof(int4) + size_t(pl.items + 2 + pl.workers) * sizeof(int32_t);
   }
   if (pl.others)
     pl.rows = row_workspace(batch, total_q, heads, hkv, d, dv, block_size, row_queries,
@@ -601,30 +804,29 @@ WindowPlan plan_window(int64_t batch, int64_t heads, int64_t hkv, int64_t d, int
 }
 
 template <int kD, bool kBf16, typename BtT>
-int launch_images(const char *name, WindowParams p, int64_t requests, hipStream_t s) {
+int launch_images(const char *name, WindowParams p, const WindowPlan &pl, hipStream_t s) {
   constexpr int kTiles = kThreads / kD;
-  constexpr size_t kSmem = 2 * size_t(img_bytes(kD));
+  // The images, and the rows in their place.
+  constexpr size_t kSmem = std::max(kStages * size_t(img_bytes(kD)), size_t(waves_of(kD)) * kRowsLds<kD>);
   if (const int st = reserve_dynamic_lds(reinterpret_cast<const void *>(&window_attention_kernel<kD, kBf16, BtT>), kSmem,
                                          name))
     return st;
   const int64_t groups = int64_t(p.slots) * ((p.tiles + kTiles - 1) / kTiles);
-  const int64_t items = int64_t(p.slots) * p.r.hkv * p.q_tiles;
-  for (p.first_slot = 0; p.first_slot < requests; p.first_slot += p.slots) {
-    window_image_kernel<kD, kBf16, BtT><<<unsigned((groups + 7) / 8 * 8 * p.r.hkv), kThreads, 0, s>>>(p);
-    window_attention_kernel<kD, kBf16, BtT>
-        <<<unsigned((items * p.splits + 7) / 8 * 8), kThreads, kSmem, s>>>(p);
-    if (p.splits > 1)
-      window_join_kernel<kD, kBf16><<<dim3(unsigned(items), kRows / (kThreads / kWave)), kThreads, 0, s>>>(p);
+  for (p.first_slot = 0; p.first_slot < pl.requests; p.first_slot += p.slots) {
+    window_image_kernel<kD, kBf16, BtT><<<unsigned((groups + 7) / 8 * 8 * p.r.hkv + 8), kThreads, 0, s>>>(p);
+    window_attention_kernel<kD, kBf16, BtT><<<unsigned(p.workers), 64 * waves_of(kD), kSmem, s>>>(p);
+    window_join_kernel<kD, kBf16>
+        <<<unsigned(p.workers * (rows_of(kD) / 32) + (pl.items + kThreads - 1) / kThreads), kThreads, 0, s>>>(p);
     if (const int st = check_launch(name)) return st;
   }
   return HIF8_OK;
 }
 
 template <bool kBf16, typename BtT>
-int launch_images_of(const char *name, const WindowParams &p, int64_t requests, hipStream_t s) {
-  if (p.r.d == 64) return launch_images<64, kBf16, BtT>(name, p, requests, s);
-  if (p.r.d == 128) return launch_images<128, kBf16, BtT>(name, p, requests, s);
-  return launch_images<256, kBf16, BtT>(name, p, requests, s);
+int launch_images_of(const char *name, const WindowParams &p, const WindowPlan &pl, hipStream_t s) {
+  if (p.r.d == 64) return launch_images<64, kBf16, BtT>(name, p, pl, s);
+  if (p.r.d == 128) return launch_images<128, kBf16, BtT>(name, p, pl, s);
+  return launch_images<256, kBf16, BtT>(name, p, pl, s);
 }
 
 }  // namespace
@@ -689,8 +891,7 @@ extern "C" int hif8_window_attention(const void *query, int q_dtype, const uint8
   if (pl.requests == 0 || !aligned(query, 16) || !aligned(out, 16)) return row_attention(kName, a);
   if (!aligned(workspace, 16))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", kName);
-  const int64_t items = pl.slots * num_kv_heads * pl.q_tiles;
-  if (items * pl.splits > 0xFFFFFF || pl.slots * num_kv_heads * (pl.tiles + 8) > 0xFFFFFF)  // threads of a launch
+  if (pl.items > 0x1FFFFF || pl.items * pl.tiles > 0x7FFFFFFF || pl.slots * num_kv_heads * (pl.tiles + 8) > 0xFFFFFF)  // threads of a launch
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", kName);
   const int64_t group = num_heads / num_kv_heads;
   if (pl.others) {
@@ -730,14 +931,18 @@ extern "C" int hif8_window_attention(const void *query, int q_dtype, const uint8
   p.tiles = int(pl.tiles);
   p.slots = int(pl.slots);
   p.tokens = int(pl.tokens);
-  p.q_tiles = int(pl.q_tiles);
-  p.splits = int(pl.splits);
+  p.items = reinterpret_cast<int4 *>(ws + pl.images + pl.parts_o + pl.parts_ml);
+  p.plan = reinterpret_cast<int32_t *>(p.items + 2 * pl.items);
+  p.plan_items = p.plan + pl.items + 1;
+  p.plan_first = p.plan_items + 1;
+  p.most_items = int(pl.items);
+  p.workers = int(pl.workers);
   p.zero_rest = pl.others ? 0 : 1;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool i64 = block_table_dtype == HIF8_INDEX_INT64;
   if (q_dtype == HIF8_DTYPE_BF16)
-    return i64 ? launch_images_of<true, int64_t>(kName, p, pl.requests, s)
-               : launch_images_of<true, int32_t>(kName, p, pl.requests, s);
-  return i64 ? launch_images_of<false, int64_t>(kName, p, pl.requests, s)
-             : launch_images_of<false, int32_t>(kName, p, pl.requests, s);
+    return i64 ? launch_images_of<true, int64_t>(kName, p, pl, s)
+               : launch_images_of<true, int32_t>(kName, p, pl, s);
+  return i64 ? launch_images_of<false, int64_t>(kName, p, pl, s)
+             : launch_images_of<false, int32_t>(kName, p, pl, s);
 }
