@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kMaxNodes = 1024;  // rows of a request: their tokens, parents and numbers lie in LDS
+constexpr int kMaxNodes = 1024;  // rows of a request
 constexpr int kChunk = 1024;     // entries whose sum is kept: sixteen per lane
 
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -47,14 +47,24 @@ struct VerifyParams {
   int batch, total, width, chunks;
 };
 
+// A request's rows, in LDS for as many as the call's longest one has.
 struct Nodes {
-  double p[kMaxNodes];       // the target's probability of a row's token after its parent; 0: never taken
-  int64_t token[kMaxNodes];
-  float u[kMaxNodes];
-  int parent[kMaxNodes];
-  int path[kMaxNodes];
-  int count;                 // rows accepted
-  int last;
+  double *p;       // the target's probability of a row's token after its parent; 0: never taken
+  double *q;       // u times what it was drawn with; u of a given token
+  int64_t *token;
+  int64_t *gone;   // tokens of the last row's children
+  int *parent, *path;
+  int *count;      // rows accepted, then the last of them, then the refused tokens
+  static constexpr int kBytes = 4 * 8 + 2 * 4;  // per row
+  __device__ Nodes(void *lds, int rows) {
+    p = static_cast<double *>(lds);
+    q = p + rows;
+    token = reinterpret_cast<int64_t *>(q + rows);
+    gone = token + rows;
+    parent = reinterpret_cast<int *>(gone + rows);
+    path = parent + rows;
+    count = path + rows;
+  }
 };
 
 // The request's rows, clipped to the call's and to its width.
@@ -63,78 +73,104 @@ __device__ __forceinline__ void rows_of(const VerifyParams &p, int b, int &begin
   count = max(min(min(p.start_loc[b + 1], p.total) - begin, p.width), 0);
 }
 
+__device__ __forceinline__ int parent_of(const VerifyParams &p, int begin, int i) {
+  const int par = p.parents ? p.parents[begin + i] : i - 1;
+  return par < 0 || par >= i ? -1 : par;  // follows nothing: never reached
+}
+
 template <typename TokT>
-__device__ __forceinline__ void load_nodes(const VerifyParams &p, int begin, int n, Nodes &nd) {
+__device__ __forceinline__ void load_nodes(const VerifyParams &p, int begin, int n, const Nodes &nd) {
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int64_t x = int64_t(static_cast<const TokT *>(p.tokens)[begin + i]);
-    int par = p.parents ? p.parents[begin + i] : i - 1;
-    if (i == 0 || par < 0 || par >= i) par = -1;  // follows nothing: never reached
-    float pv = 0.f;
-    if (par >= 0 && x >= 0 && x < p.vocab) pv = p.probs[int64_t(begin + par) * p.ld_probs + x];
+    const int par = parent_of(p, begin, i);
+    float pv = 0.f, qv = 1.f;
+    if (par >= 0 && x >= 0 && x < p.vocab) {
+      pv = p.probs[int64_t(begin + par) * p.ld_probs + x];
+      if (p.draft) qv = p.draft[int64_t(begin + i) * p.ld_draft + x];
+    }
     nd.token[i] = x;
     nd.parent[i] = par;
-    nd.u[i] = p.uniforms[begin + i];
-    nd.p[i] = pv > 0.f ? double(pv) : 0.;  // NaN too is never taken
+    nd.q[i] = double(p.uniforms[begin + i]) * double(qv);  // exact
+    nd.p[i] = pv > 0.f ? double(pv) : 0.;                  // NaN too is never taken
   }
 }
 
-// Whether an earlier row than `child` with its parent has its token (a wavefront).
-__device__ __forceinline__ bool seen_before(const Nodes &nd, int child) {
-  const int lane = threadIdx.x & 63, par = nd.parent[child];
-  const int64_t x = nd.token[child];
-  for (int base = 0; base < child; base += kWave) {
-    const int j = base + lane;
-    if (__any(j < child && nd.parent[j] == par && nd.token[j] == x)) return true;
-  }
-  return false;
-}
-
-// The accepted path, by the first wavefront.  Rows are gone through once: children
-// come after their parent.
-__device__ __forceinline__ void walk(const VerifyParams &p, int begin, int n, Nodes &nd) {
+// The accepted path of a chain, by the first wavefront: up to the first row that is refused.
+__device__ __forceinline__ void follow(int n, const Nodes &nd) {
   const int lane = threadIdx.x & 63;
-  int now = 0, count = 1;
+  int count = 1;
+  for (int base = 1; base < n; base += kWave) {
+    const int i = base + lane;
+    const uint64_t refused = __ballot(i < n && !(nd.p[i] > 0. && nd.q[i] < nd.p[i]));
+    if (refused) {
+      count = base + __builtin_ctzll(refused);
+      break;
+    }
+    count = min(base + kWave, n);
+  }
+  for (int i = lane; i < count; i += kWave) nd.path[i] = i;
+  if (lane == 0) {
+    nd.count[0] = count;
+    nd.count[1] = count - 1;
+    nd.count[2] = count < n ? 1 : 0;
+    if (count < n) nd.gone[0] = nd.token[count];
+  }
+}
+
+// The same of a tree.  Rows are gone through once: children come after their parent.
+__device__ __forceinline__ void walk(int n, const Nodes &nd) {
+  const int lane = threadIdx.x & 63;
+  int now = 0, count = 1, gone = 0;  // gone: children of `now` refused so far
   double rest = 1.;
   if (lane == 0) nd.path[0] = 0;
   for (int base = 0; base < n; base += kWave) {
     const int i = base + lane;
     const int par = i < n ? nd.parent[i] : -1;
+    const int64_t token = i < n ? nd.token[i] : 0;
     int from = 0;
     while (from < kWave) {
       const uint64_t mask = __ballot(par == now) & (~uint64_t(0) << from);
       if (!mask) break;
       const int at = __builtin_ctzll(mask), child = base + at;
       from = at + 1;
-      const double pv = nd.p[child], u = double(nd.u[child]);
+      // One that an earlier sibling had is refused with it.
+      const int64_t x = nd.token[child];
+      bool again = (__ballot(par == now && token == x) & ((uint64_t(1) << at) - 1)) != 0;
+      for (int j0 = 0; j0 < gone && !again && base > 0; j0 += kWave)
+        again = __any(j0 + lane < gone && nd.gone[j0 + lane] == x);
       bool takes = false;
-      if (p.draft) {
-        const int64_t x = nd.token[child];
-        if (pv > 0.) takes = u * double(p.draft[int64_t(begin + child) * p.ld_draft + x]) < pv;
-      } else if (!seen_before(nd, child)) {
-        takes = pv > 0. && u * rest < pv;
-        rest = takes ? 1. : rest - pv;
+      if (!again) {
+        const double pv = nd.p[child];
+        takes = pv > 0. && nd.q[child] * rest < pv;
+        rest -= pv;
       }
       if (takes) {
         if (lane == 0) nd.path[count] = child;
         now = child;
         ++count;
+        gone = 0;
+        rest = 1.;
+      } else {
+        if (lane == 0) nd.gone[gone] = x;
+        ++gone;
       }
     }
   }
   if (lane == 0) {
-    nd.count = count;
-    nd.last = now;
+    nd.count[0] = count;
+    nd.count[1] = now;
+    nd.count[2] = gone;
   }
 }
 
 // What entry v of a chunk weighs: w above, or 0 where it is no positive number.
 __device__ __forceinline__ double positive(double w) { return w > 0. && w < __builtin_inf() ? w : 0.; }
 
-// Sixteen entries from v on: four of each of four rounds of the wavefront.
+// A row of weights, four at a time.
 struct Row {
   const float *probs, *draft;  // draft null: none
   int64_t vocab;
-  __device__ __forceinline__ void weights(int64_t v, double (&w)[4]) const {
+  __device__ __forceinline__ void weights(int64_t v, double *w) const {
     if (v + 4 <= vocab) {
       const f32x4_a4 a = *reinterpret_cast<const f32x4_a4 *>(probs + v);
       if (draft) {
@@ -153,17 +189,6 @@ struct Row {
   }
 };
 
-// Without drafts' probabilities the children of the last row strike their tokens out.
-__device__ __forceinline__ void strike(const Nodes &nd, int n, int64_t v, double (&w)[4]) {
-  for (int j = 1; j < n; ++j) {
-    if (nd.parent[j] != nd.last) continue;
-    const int64_t d = nd.token[j] - v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (d == e) w[e] = 0.;
-  }
-}
-
 __device__ __forceinline__ double wave_sum_double(double v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, kWave);
@@ -180,7 +205,8 @@ __device__ __forceinline__ Row row_of(const VerifyParams &p, int begin, int n, i
 // path for itself and sums its chunks of the weights; the first writes the path.
 template <typename TokT>
 __global__ __launch_bounds__(kThreads) void verify_sum_kernel(const VerifyParams p) {
-  __shared__ Nodes nd;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const Nodes nd(smem, p.width);
   const int b = int(blockIdx.y), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int begin, n;
   rows_of(p, b, begin, n);
@@ -196,166 +222,166 @@ __global__ __launch_bounds__(kThreads) void verify_sum_kernel(const VerifyParams
   }
   load_nodes<TokT>(p, begin, n, nd);
   __syncthreads();
-  if (wave == 0) walk(p, begin, n, nd);
+  if (wave == 0) {
+    if (p.parents) walk(n, nd);
+    else follow(n, nd);
+  }
   __syncthreads();
   if (blockIdx.x == 0) {
-    for (int i = tid; i < p.width; i += kThreads) p.accepted[int64_t(b) * p.width + i] = i < nd.count ? nd.path[i] : -1;
+    for (int i = tid; i < p.width; i += kThreads) p.accepted[int64_t(b) * p.width + i] = i < nd.count[0] ? nd.path[i] : -1;
     if (tid == 0) {
-      p.counts[b] = nd.count;
-      p.last[b] = nd.last;
+      p.counts[b] = nd.count[0];
+      p.last[b] = nd.count[1];
     }
   }
   const int chunk = int(blockIdx.x) * kWaves + wave;
   if (chunk >= p.chunks) return;
-  const Row row = row_of(p, begin, n, nd.last);
+  const Row row = row_of(p, begin, n, nd.count[1]);
+  double w[kChunk / kWave];
+#pragma unroll
+  for (int r = 0; r < kChunk / (4 * kWave); ++r)
+    row.weights(int64_t(chunk) * kChunk + 4 * (lane + kWave * r), w + 4 * r);
+  if (!p.draft) {
+    // Given drafts: the tokens refused are struck out.
+    for (int j = 0; j < nd.count[2]; ++j) {
+      const int64_t d = nd.gone[j] - int64_t(chunk) * kChunk;
+      if (d < 0 || d >= kChunk) continue;  // uniform
+#pragma unroll
+      for (int e = 0; e < kChunk / kWave; ++e)
+        if (d == 4 * (lane + kWave * (e >> 2)) + (e & 3)) w[e] = 0.;
+    }
+  }
   double sum = 0.;
 #pragma unroll
-  for (int r = 0; r < kChunk / (4 * kWave); ++r) {
-    const int64_t v = int64_t(chunk) * kChunk + 4 * (lane + kWave * r);
-    double w[4];
-    row.weights(v, w);
-    if (!p.draft) strike(nd, n, v, w);
-    sum += (w[0] + w[1]) + (w[2] + w[3]);
-  }
+  for (int e = 0; e < kChunk / kWave; e += 4) sum += (w[e] + w[e + 1]) + (w[e + 2] + w[e + 3]);
   sum = wave_sum_double(sum);
   if (lane == 0) p.sums[int64_t(b) * p.chunks + chunk] = sum;
 }
 
-// Inclusive sum over the workgroup; `all` gets the total.  part: kWaves doubles of LDS.
-__device__ __forceinline__ double block_upto(double mine, double *part, double &all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double upto = mine;
+// Inclusive sum over a wavefront.
+__device__ __forceinline__ double wave_upto(double v) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) {
-    const double left = __shfl_up(upto, o, kWave);
-    if (lane >= o) upto += left;
+    const double left = __shfl_up(v, o, kWave);
+    if (lane >= o) v += left;
   }
-  __syncthreads();
-  if (lane == kWave - 1) part[wave] = upto;
-  __syncthreads();
-  double before = 0.;
-  all = 0.;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += part[w];
-    all += part[w];
-  }
-  return before + upto;
+  return v;
 }
 
-// The next token of a request: the chunk in which the running sum passes u_0 times
-// the total, then the entry.  Sums of a chunk and of its entries may round apart:
-// where no entry passes, it is the chunk's last with a weight.
+// The next token of a request, a wavefront each: the chunk in which the running sum
+// passes u_0 times the total, then the entry.  Sums of a chunk and of its entries may
+// round apart: where no entry passes, it is the chunk's last with a weight.
 template <typename TokT>
 __global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyParams p) {
-  __shared__ Nodes nd;
-  __shared__ double part[kWaves];
-  __shared__ double before_s;
-  __shared__ int chunk_s, any_s;
-  __shared__ int64_t pick_s, some_s;
-  const int b = int(blockIdx.x), tid = threadIdx.x;
+  const int b = int(blockIdx.x) * kWaves + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (b >= p.batch) return;
+  const double *sums = p.sums + int64_t(b) * p.chunks;
+  // Each lane's run of chunks.
+  const int per = (p.chunks + kWave - 1) / kWave, c0 = min(lane * per, p.chunks), c1 = min(c0 + per, p.chunks);
   int begin, n;
   rows_of(p, b, begin, n);
   if (n == 0) {  // uniform
-    if (tid == 0) p.next[b] = -1;
+    if (lane == 0) p.next[b] = -1;
     return;
   }
-  if (!p.draft) load_nodes<TokT>(p, begin, n, nd);
-  if (tid == 0) {
-    nd.last = p.last[b];
-    chunk_s = 0x7FFFFFFF;
-    any_s = -1;
-    pick_s = INT64_MAX;
-    some_s = -1;
-    before_s = 0.;
-  }
-  __syncthreads();
-  const Row drawn = row_of(p, begin, n, nd.last);
+  const double u = double(p.uniforms[begin]);
+  const int last = p.last[b];
+  const Row drawn = row_of(p, begin, n, last);
   const Row whole{drawn.probs, nullptr, p.vocab};
-  const double *sums = p.sums + int64_t(b) * p.chunks;
-  // Chunk sums, of p alone where no entry of the residual is left.
-  double total = 0.;
-  for (int c0 = 0; c0 < p.chunks; c0 += kThreads) {
-    double all;
-    block_upto(c0 + tid < p.chunks ? sums[c0 + tid] : 0., part, all);
-    total += all;
-  }
-  const bool residual = total > 0.;  // else total is 0: every weight is
-  auto chunk_weights = [&](int c, double (&w)[4]) {
-    const int64_t v = int64_t(c) * kChunk + 4 * tid;
-    if (residual) {
-      drawn.weights(v, w);
-      if (!p.draft) strike(nd, n, v, w);
-    } else {
-      whole.weights(v, w);
+  double run = 0.;
+  for (int c = c0; c < c1; ++c) run += sums[c];
+  double upto = wave_upto(run);
+  double total = __shfl(upto, kWave - 1, kWave);
+  const bool residual = total > 0.;  // else it is 0: every weight is
+  // Sixteen weights of a chunk, one after the other.
+  auto weights = [&](int c, double (&w)[kChunk / kWave]) {
+    const int64_t v0 = int64_t(c) * kChunk + kChunk / kWave * lane;
+    const Row &row = residual ? drawn : whole;
+#pragma unroll
+    for (int e = 0; e < kChunk / kWave; e += 4) row.weights(v0 + e, w + e);
+    if (!residual || p.draft) return;
+    for (int base = last + 1; base < n; base += kWave) {
+      const int i = base + lane;
+      const bool child = i < n && parent_of(p, begin, i) == last;
+      const int64_t token = child ? int64_t(static_cast<const TokT *>(p.tokens)[begin + i]) : 0;
+      for (uint64_t left = __ballot(child); left; left &= left - 1) {
+        const int64_t d = __shfl(token, __builtin_ctzll(left), kWave) - v0;
+#pragma unroll
+        for (int e = 0; e < kChunk / kWave; ++e)
+          if (d == e) w[e] = 0.;
+      }
     }
   };
-  auto chunk_sum = [&](int c) {  // every thread of the workgroup gets it
-    double w[4], all;
-    chunk_weights(c, w);
-    block_upto((w[0] + w[1]) + (w[2] + w[3]), part, all);
-    return all;
+  auto total_of = [](const double (&w)[kChunk / kWave]) {
+    double s = 0.;
+#pragma unroll
+    for (int e = 0; e < kChunk / kWave; ++e) s += w[e];
+    return s;
   };
-  const double u = double(p.uniforms[begin]);
-  double limit = u * total;
+  int chunk = -1;       // where the running sum passes
+  int some = -1;        // the last chunk with a weight
+  double before = 0., limit = 0.;
   if (residual) {
-    double before = 0.;
-    for (int c0 = 0; c0 < p.chunks; c0 += kThreads) {
-      const int c = c0 + tid;
-      const double mine = c < p.chunks ? sums[c] : 0.;
-      double all;
-      const double upto = before + block_upto(mine, part, all);
-      if (mine > 0.) {
-        atomicMax(&any_s, c);
-        if (upto > limit) atomicMin(&chunk_s, c);
+    limit = u * total;
+    // The lane in whose run it passes, then the chunk of it.
+    const uint64_t past = __ballot(run > 0. && upto > limit), any = __ballot(run > 0.);
+    const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
+    before = __shfl(upto - run, at, kWave);
+    const int first = at * per, end = min(first + per, p.chunks);
+    for (int c = first; c < end; c += kWave) {
+      const double mine = c + lane < end ? sums[c + lane] : 0.;
+      const double here = before + wave_upto(mine);
+      const uint64_t over = __ballot(mine > 0. && here > limit), with = __ballot(mine > 0.);
+      if (with) some = c + 63 - __builtin_clzll(with);
+      if (over && past) {
+        const int i = __builtin_ctzll(over);
+        chunk = c + i;
+        before = __shfl(here - mine, i, kWave);
+        break;
       }
-      __syncthreads();
-      if (chunk_s == c) before_s = upto - mine;
-      if (chunk_s != 0x7FFFFFFF) break;  // uniform
-      before += all;
+      before = __shfl(here, kWave - 1, kWave);
     }
   } else {
-    for (int c = 0; c < p.chunks; ++c) total += chunk_sum(c);
-    limit = u * total;
-    double before = 0.;
+    // Rare: every weight of the residual is zero, and p itself is drawn from, chunk by chunk.
+    double w[kChunk / kWave];
+    total = 0.;
     for (int c = 0; c < p.chunks; ++c) {
-      const double all = chunk_sum(c);
-      if (tid == 0 && all > 0.) any_s = c;
-      if (all > 0. && before + all > limit) {
-        if (tid == 0) {
-          chunk_s = c;
-          before_s = before;
-        }
+      weights(c, w);
+      total += wave_sum_double(total_of(w));
+    }
+    limit = u * total;
+    for (int c = 0; c < p.chunks; ++c) {
+      weights(c, w);
+      const double all = wave_sum_double(total_of(w));
+      if (!(all > 0.)) continue;
+      some = c;
+      if (before + all > limit) {
+        chunk = c;
         break;
       }
       before += all;
     }
   }
-  __syncthreads();
-  const bool found = chunk_s != 0x7FFFFFFF;
-  const int c = found ? chunk_s : any_s;
-  if (c < 0) {  // no entry weighs anything
-    if (tid == 0) p.next[b] = -1;
+  if (some < 0) {  // no entry weighs anything
+    if (lane == 0) p.next[b] = -1;
     return;
   }
-  double w[4], all;
-  chunk_weights(c, w);
-  const double mine = (w[0] + w[1]) + (w[2] + w[3]);
-  double upto = before_s + (block_upto(mine, part, all) - mine);
-  int64_t pick = -1, some = -1;
+  const int c = chunk >= 0 ? chunk : some;
+  double w[kChunk / kWave];
+  weights(c, w);
+  const double mine = total_of(w);
+  double sum = before + (wave_upto(mine) - mine);
+  int pick = -1, final = -1;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    upto += w[e];
-    const int64_t v = int64_t(c) * kChunk + 4 * tid + e;
-    if (w[e] > 0.) {
-      some = v;
-      if (pick < 0 && found && upto > limit) pick = v;
-    }
+  for (int e = 0; e < kChunk / kWave; ++e) {
+    sum += w[e];
+    if (w[e] > 0.) final = e;
+    if (w[e] > 0. && pick < 0 && chunk >= 0 && sum > limit) pick = e;
   }
-  if (pick >= 0) atomicMin(reinterpret_cast<unsigned long long *>(&pick_s), static_cast<unsigned long long>(pick));
-  if (some >= 0) atomicMax(reinterpret_cast<long long *>(&some_s), static_cast<long long>(some));
-  __syncthreads();
-  if (tid == 0) p.next[b] = pick_s != INT64_MAX ? pick_s : some_s;
+  const uint64_t picks = __ballot(pick >= 0), finals = __ballot(final >= 0);
+  if (picks ? lane == __builtin_ctzll(picks) : lane == 63 - __builtin_clzll(finals | 1))
+    p.next[b] = int64_t(c) * kChunk + kChunk / kWave * lane + (picks ? pick : final);
 }
 
 int64_t chunks_of(int64_t vocab) { return (vocab + kChunk - 1) / kChunk; }
@@ -420,13 +446,14 @@ extern "C" int hif8_verify_drafts(const float *target_probs, int64_t target_stri
   p.width = int(max_query_len);
   p.chunks = int(chunks_of(vocab));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const size_t lds = size_t(max_query_len) * Nodes::kBytes + 16;
   const dim3 grid(unsigned((p.chunks + kWaves - 1) / kWaves), unsigned(batch));
   if (tokens_dtype == HIF8_INDEX_INT64) {
-    verify_sum_kernel<int64_t><<<grid, kThreads, 0, s>>>(p);
-    verify_pick_kernel<int64_t><<<unsigned(batch), kThreads, 0, s>>>(p);
+    verify_sum_kernel<int64_t><<<grid, kThreads, lds, s>>>(p);
+    verify_pick_kernel<int64_t><<<unsigned((batch + kWaves - 1) / kWaves), kThreads, 0, s>>>(p);
   } else {
-    verify_sum_kernel<int32_t><<<grid, kThreads, 0, s>>>(p);
-    verify_pick_kernel<int32_t><<<unsigned(batch), kThreads, 0, s>>>(p);
+    verify_sum_kernel<int32_t><<<grid, kThreads, lds, s>>>(p);
+    verify_pick_kernel<int32_t><<<unsigned((batch + kWaves - 1) / kWaves), kThreads, 0, s>>>(p);
   }
   return check_launch(kName);
 }
