@@ -9,8 +9,9 @@
 #include <stddef.h>
 
 #include <algorithm>
+#include <type_traits>
 
-#include "hif8_common.h"
+#include "mfma_lookup.h"  // wave_prefix
 
 namespace hif8 {
 namespace {
@@ -19,7 +20,7 @@ constexpr int kScan = 1024;  // threads of a workgroup that ranks entries: sixte
 constexpr int kScanWaves = kScan / kWave;
 constexpr int kRowThreads = 256;
 
-// A request's new query rows, clipped to the call's rows (start_loc is caller data).
+// A request's new rows, clipped to the call's (start_loc is caller data).
 __device__ __forceinline__ void new_rows(const int32_t *start_loc, int b, int total, int &begin, int &count) {
   begin = max(start_loc[b], 0);
   count = max(min(start_loc[b + 1], total) - begin, 0);
@@ -59,17 +60,39 @@ struct ExtendParams {
   int32_t *new_lens, *missing;
   int64_t width, capacity;
   int batch, total, block_size;
+  int with_slots;            // the workgroup that takes the ids works out the slots too
 };
 
+constexpr int kPerThread = 8;  // columns of a thread where there are more than threads
+// Rows up to which one workgroup does all of a call: 2048 rows more would take it 2.5 us,
+// the launch of another kernel 1.6 us (and 4 of the host's).
+constexpr int kFewRows = 2048;
+
+// Slot and position of a row, from the table as it stands; of a row of no request -1.
+template <typename BtT>
+__device__ __forceinline__ void put_slot(const ExtendParams &p, int row, int b, int begin, int n) {
+  int64_t slot = -1, at = -1;
+  if (row >= begin && row - begin < n) {
+    at = int64_t(max(p.lens[b], 0)) + (row - begin);
+    const int64_t col = uint64_t(at) >> 32 ? at / p.block_size : int64_t(uint32_t(at) / uint32_t(p.block_size));
+    const int64_t page = col < p.width ? int64_t(static_cast<const BtT *>(p.table)[int64_t(b) * p.width + col]) : -1;
+    if (page >= 0) slot = page * p.block_size + (at - col * p.block_size);
+  }
+  p.slots[row] = slot;
+  p.positions[row] = at;
+}
+
 // Ids for the table columns that the new tokens reach.  One workgroup: the rank of
-// a column among those without a page runs over all requests.
+// a column among those without a page runs over all requests.  Bound by the dependent
+// reads of lengths, table and stack (four round trips, 3.6 us); with one column a thread
+// and pass 48 prompts of 4k tokens on 16-token pages (9200 columns) took 19 us.
 template <typename BtT>
 __global__ __launch_bounds__(kScan) void extend_kernel(const ExtendParams p) {
-  __shared__ int first[kScan + 1];  // columns of the chunk's requests before each
+  __shared__ int first[kScan];      // columns of the chunk's requests before each
   __shared__ int low[kScan];        // a request's first column
   __shared__ int lack[kScan];       // pages that it did not get
-  __shared__ int sums[kScanWaves];
-  const int tid = threadIdx.x;
+  __shared__ int sums[kScanWaves], counts[kPerThread * kScanWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int have = int(min(int64_t(max(*p.free_count, 0)), p.capacity));
   int64_t taken = 0;  // columns without a page so far
   for (int base = 0; base < p.batch; base += kScan) {
@@ -92,59 +115,92 @@ __global__ __launch_bounds__(kScan) void extend_kernel(const ExtendParams p) {
     low[tid] = lo;
     lack[tid] = beyond;
     __syncthreads();
-    for (int c0 = 0; c0 < total; c0 += kScan) {
-      const int c = c0 + tid;
-      int r = 0;
-      BtT *entry = nullptr;
-      bool wants = false;
-      if (c < total) {
-        // The last request of the chunk that starts at or before column c.
-        int hi = kScan - 1;
-        while (r < hi) {
-          const int mid = (r + hi + 1) / 2;
-          if (first[mid] <= c) r = mid;
-          else hi = mid - 1;
+    auto columns_of = [&](auto per) {
+      constexpr int kPer = decltype(per)::value;
+      for (int c0 = 0; c0 < total; c0 += kScan * kPer) {
+        // Column c0 + kScan j + tid: its request is the last of the chunk that starts at or before it.
+        int owner[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) owner[j] = 0;
+#pragma unroll
+        for (int step = kScan / 2; step > 0; step /= 2)
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+            if (first[owner[j] + step] <= c0 + kScan * j + tid) owner[j] += step;
+        BtT *entry[kPer], id[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int c = c0 + kScan * j + tid, r = owner[j];
+          entry[j] = static_cast<BtT *>(p.table) + int64_t(base + r) * p.width + (low[r] + c - first[r]);
+          id[j] = c < total ? *entry[j] : BtT(0);
         }
-        entry = static_cast<BtT *>(p.table) + int64_t(base + r) * p.width + (low[r] + c - first[r]);
-        wants = *entry < 0;
+        uint64_t wants[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          wants[j] = __ballot(id[j] < 0);
+          if (lane == 0) counts[j * kScanWaves + wave] = __popcll(wants[j]);
+        }
+        __syncthreads();
+        // Those of the 16 wavefronts, one j after the other: before[i] of count i.
+        constexpr int kCounts = kPer * kScanWaves;
+        int upto[(kCounts + kWave - 1) / kWave], all = 0;
+#pragma unroll
+        for (int i = 0; i < (kCounts + kWave - 1) / kWave; ++i) {
+          const int mine = kWave * i + lane < kCounts ? counts[kWave * i + lane] : 0;
+          upto[i] = all + wave_prefix(mine);
+          all = __builtin_amdgcn_readlane(upto[i], kWave - 1);
+          upto[i] -= mine;
+        }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int i = j * kScanWaves + wave;
+          const int64_t rank = taken + __builtin_amdgcn_readlane(upto[j * kScanWaves / kWave], i % kWave) +
+                               __popcll(wants[j] & ((uint64_t(1) << lane) - 1));
+          if (id[j] >= 0) continue;
+          if (rank < have) *entry[j] = BtT(p.free_ids[have - 1 - rank]);
+          else atomicAdd(&lack[owner[j]], 1);
+        }
+        taken += all;
+        __syncthreads();
       }
-      int here;
-      const int64_t rank = taken + block_exclusive(wants ? 1 : 0, sums, here);
-      if (wants) {
-        if (rank < have) *entry = BtT(p.free_ids[have - 1 - rank]);
-        else atomicAdd(&lack[r], 1);
-      }
-      taken += here;
-    }
+    };
+    if (total <= kScan) columns_of(std::integral_constant<int, 1>{});
+    else columns_of(std::integral_constant<int, kPerThread>{});
     __syncthreads();
     if (b < p.batch) p.missing[b] = lack[tid];
     __syncthreads();
   }
   if (tid == 0) *p.free_count = int32_t(have - min(taken, int64_t(have)));
+  if (!p.with_slots) return;  // uniform; here the batch is one chunk
+  for (int i = tid; i < p.batch; i += kScan) first[i] = p.start_loc[i];
+  __syncthreads();
+  for (int row = tid; row < p.total; row += kScan) {
+    int b = 0, hi = p.batch - 1;
+    while (b < hi) {
+      const int mid = (b + hi + 1) / 2;
+      if (first[mid] <= row) b = mid;
+      else hi = mid - 1;
+    }
+    int begin, n;
+    new_rows(p.start_loc, b, p.total, begin, n);
+    put_slot<BtT>(p, row, b, begin, n);
+  }
 }
 
-// Slot and position of every row, from the table as extend_kernel has left it.
+// Slots and positions of many rows, from the table as extend_kernel has left it.
 template <typename BtT>
 __global__ __launch_bounds__(kRowThreads) void slots_kernel(const ExtendParams p) {
   const int row = int(blockIdx.x) * kRowThreads + threadIdx.x;
   if (row >= p.total) return;
-  int lo = 0, hi = p.batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (p.start_loc[mid] <= row) lo = mid;
+  int b = 0, hi = p.batch - 1;
+  while (b < hi) {
+    const int mid = (b + hi + 1) / 2;
+    if (p.start_loc[mid] <= row) b = mid;
     else hi = mid - 1;
   }
-  int begin, n;
-  new_rows(p.start_loc, lo, p.total, begin, n);
-  int64_t slot = -1, at = -1;  // a row of no request: padding
-  if (row >= begin && row - begin < n) {
-    at = int64_t(max(p.lens[lo], 0)) + (row - begin);
-    const int64_t col = at / p.block_size;
-    const int64_t page = col < p.width ? int64_t(static_cast<const BtT *>(p.table)[int64_t(lo) * p.width + col]) : -1;
-    if (page >= 0) slot = page * p.block_size + (at - col * p.block_size);
-  }
-  p.slots[row] = slot;
-  p.positions[row] = at;
+  int begin = 0, n = 0;
+  if (p.batch > 0) new_rows(p.start_loc, b, p.total, begin, n);
+  put_slot<BtT>(p, row, b, begin, n);
 }
 
 struct ReleaseParams {
@@ -162,9 +218,9 @@ struct ReleaseParams {
 constexpr int kPer = 4;                   // consecutive entries per thread
 constexpr int kChunk = kScan * kPer;
 
-// Whether request b goes on needing the page of its column `col`.
-__device__ __forceinline__ bool stays(const ReleaseParams &p, int64_t b, int64_t col) {
-  const int64_t len = max(p.lens[b], 0), from = col * p.block_size;
+// Whether a request of len rows goes on needing the page of its column `col`.
+__device__ __forceinline__ bool stays(const ReleaseParams &p, int64_t len, int64_t col) {
+  const int64_t from = col * p.block_size;
   if (from >= len) return false;
   return p.window == 0 || from < p.sinks || from + p.block_size > len + 1 - p.window;
 }
@@ -172,15 +228,29 @@ __device__ __forceinline__ bool stays(const ReleaseParams &p, int64_t b, int64_t
 // Bit i: entry first + i holds a page that goes.
 template <typename BtT>
 __device__ __forceinline__ uint32_t goers(const ReleaseParams &p, int64_t first, BtT (&ids)[kPer]) {
-  uint32_t bits = 0;
+  const BtT *table = static_cast<const BtT *>(p.table);
+  if (first + kPer <= p.entries) {
+    typedef BtT vec __attribute__((ext_vector_type(kPer), aligned(sizeof(BtT))));
+    const vec v = *reinterpret_cast<const vec *>(table + first);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) ids[i] = v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) ids[i] = first + i < p.entries ? table[first + i] : BtT(-1);
+  }
+  uint32_t held = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) held |= ids[i] >= 0 ? 1u << i : 0u;
+  if (!held) return 0;  // most of a table is empty
+  uint32_t b = uint32_t(first) / uint32_t(p.width), col = uint32_t(first) - b * uint32_t(p.width), bits = 0;
+  int64_t len = max(p.lens[b], 0);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int64_t e = first + i;
-    ids[i] = -1;
-    if (e >= p.entries) continue;
-    ids[i] = static_cast<const BtT *>(p.table)[e];
-    const int64_t b = e / p.width;
-    if (ids[i] >= 0 && !stays(p, b, e - b * p.width)) bits |= 1u << i;
+    if ((held >> i) & 1u) bits |= stays(p, len, col) ? 0u : 1u << i;
+    if (++col == uint32_t(p.width) && first + i + 1 < p.entries) {
+      col = 0;
+      len = max(p.lens[++b], 0);
+    }
   }
   return bits;
 }
@@ -198,14 +268,19 @@ __global__ __launch_bounds__(kScan) void release_count_kernel(const ReleaseParam
   }
 }
 
+// A workgroup per kChunk entries; what the earlier ones release has been counted, unless
+// one workgroup has them all.
 template <typename BtT>
 __global__ __launch_bounds__(kScan) void release_kernel(const ReleaseParams p) {
   __shared__ int sums[kScanWaves];
-  const int have = int(min(int64_t(max(p.counts[p.chunks], 0)), p.capacity));
-  int mine = 0;
-  for (int i = threadIdx.x; i < int(blockIdx.x); i += kScan) mine += p.counts[i];
-  int before;
-  block_exclusive(mine, sums, before);
+  const int stack = p.chunks > 1 ? p.counts[p.chunks] : *p.free_count;
+  const int have = int(min(int64_t(max(stack, 0)), p.capacity));
+  int before = 0;
+  if (p.chunks > 1) {
+    int mine = 0;
+    for (int i = threadIdx.x; i < int(blockIdx.x); i += kScan) mine += p.counts[i];
+    block_exclusive(mine, sums, before);
+  }
   BtT ids[kPer];
   const int64_t first = int64_t(blockIdx.x) * kChunk + int64_t(threadIdx.x) * kPer;
   const uint32_t bits = goers(p, first, ids);
@@ -253,14 +328,14 @@ extern "C" int hif8_extend_block_tables(void *block_table, int block_table_dtype
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: null pointer argument", kName);
   ExtendParams p{block_table, free_blocks, free_count, context_lens, query_start_loc, slot_mapping, positions,
                  seq_lens, missing, max_blocks_per_seq, free_capacity, int(batch), int(total_query_tokens),
-                 int(block_size)};
+                 int(block_size), batch <= kScan && total_query_tokens <= kFewRows ? 1 : 0};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool i64 = block_table_dtype == HIF8_INDEX_INT64;
   if (batch > 0) {
     if (i64) extend_kernel<int64_t><<<1, kScan, 0, s>>>(p);
     else extend_kernel<int32_t><<<1, kScan, 0, s>>>(p);
   }
-  if (total_query_tokens > 0) {
+  if (total_query_tokens > 0 && (batch == 0 || !p.with_slots)) {
     const unsigned blocks = unsigned((total_query_tokens + kRowThreads - 1) / kRowThreads);
     if (i64) slots_kernel<int64_t><<<blocks, kRowThreads, 0, s>>>(p);
     else slots_kernel<int32_t><<<blocks, kRowThreads, 0, s>>>(p);
@@ -301,10 +376,10 @@ extern "C" int hif8_release_blocks(void *block_table, int block_table_dtype, int
                   int(chunks_of(batch, max_blocks_per_seq))};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (block_table_dtype == HIF8_INDEX_INT64) {
-    release_count_kernel<int64_t><<<unsigned(p.chunks), kScan, 0, s>>>(p);
+    if (p.chunks > 1) release_count_kernel<int64_t><<<unsigned(p.chunks), kScan, 0, s>>>(p);
     release_kernel<int64_t><<<unsigned(p.chunks), kScan, 0, s>>>(p);
   } else {
-    release_count_kernel<int32_t><<<unsigned(p.chunks), kScan, 0, s>>>(p);
+    if (p.chunks > 1) release_count_kernel<int32_t><<<unsigned(p.chunks), kScan, 0, s>>>(p);
     release_kernel<int32_t><<<unsigned(p.chunks), kScan, 0, s>>>(p);
   }
   return check_launch(kName);
