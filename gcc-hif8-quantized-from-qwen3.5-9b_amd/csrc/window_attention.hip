@@ -242,17 +242,22 @@ __global__ __launch_bounds__(kThreads) void window_image_kernel(const WindowPara
     dec[tid] = (kBf16 ? f >> 16 : half) | (finite ? half << 16 : 0u);
     if (tid < kTiles) odd[tid] = top[tid] = 0;
   }
-  const int tile = first + tid / kPerTile, at = tid % kPerTile;
+  // Everything of an image is the same in a whole wavefront.
+  const int in_group = __builtin_amdgcn_readfirstlane(tid / kPerTile), tile = first + in_group, at = tid % kPerTile;
   const BtT *bt = static_cast<const BtT *>(p.r.block_table) + size_t(b) * p.r.bt_stride;
   const int64_t rec = int64_t(p.r.hkv) * (kD + 4);
-  // Offset of this KV head's row `key` of the image, or -1.
-  auto offset_of = [&](int key) -> int64_t {
-    const int t = tile * kKeys + key;
+  // Offset of this KV head's row in the first row of each of the two groups of 16, or -1.
+  auto group_offset = [&](int t) -> int64_t {
     if (t >= win.rows) return -1;
     const int real = win.real(t), col = real / p.r.block_size;
     const int64_t blk = int64_t(bt[col]);
     if (blk < 0 || blk >= p.r.num_blocks) return -1;
     return (blk * p.r.block_size + (real - col * p.r.block_size)) * rec + int64_t(h) * (kD + 4);
+  };
+  const int64_t off0 = group_offset(tile * kKeys), off1 = group_offset(tile * kKeys + 16);
+  auto offset_of = [&](int key) -> int64_t {
+    const int64_t off = key < 16 ? off0 : off1;
+    return off < 0 || tile * kKeys + key >= win.rows ? int64_t(-1) : off + (key & 15) * rec;
   };
   uint8_t *im = p.img + ((size_t(slot) * p.r.hkv + h) * p.tiles + tile) * img_bytes(kD);
   const bool mine = tile * kKeys < win.rows;
@@ -305,7 +310,7 @@ __global__ __launch_bounds__(kThreads) void window_image_kernel(const WindowPara
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (some_not_finite(vraw[j])) bad |= 1u << (16 * vs + 8 * (j >> 2) + 4 * vh + (j & 3));
-    if (bad) atomicOr(&odd[tid / kPerTile], bad);
+    if (bad) atomicOr(&odd[in_group], bad);
     uint8_t *vim = im + frag_bytes(kD) / 2 + 1024 * ((4 * quad / 32) * 2 + vs) + 16 * (4 * quad % 32 + 32 * vh);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -321,15 +326,15 @@ __global__ __launch_bounds__(kThreads) void window_image_kernel(const WindowPara
       float *sc = reinterpret_cast<float *>(im + frag_bytes(kD));
       sc[at] = ksc;
       sc[kKeys + at] = finite ? vsc : 0.f;
-      if (!finite) atomicOr(&odd[tid / kPerTile], 1u << at);
-      else atomicMax(&top[tid / kPerTile], __float_as_uint(fabsf(vsc)));
+      if (!finite) atomicOr(&odd[in_group], 1u << at);
+      else atomicMax(&top[in_group], __float_as_uint(fabsf(vsc)));
     }
     const uint64_t seen = __ballot(there);  // the image's first wavefront
     if (at == 0) reinterpret_cast<uint32_t *>(im + frag_bytes(kD))[2 * kKeys] = uint32_t(seen);
   }
   __syncthreads();
   if (mine && at == 0)
-    *reinterpret_cast<u32x2 *>(im + frag_bytes(kD) + 8 * kKeys + 4) = u32x2{odd[tid / kPerTile], top[tid / kPerTile]};
+    *reinterpret_cast<u32x2 *>(im + frag_bytes(kD) + 8 * kKeys + 4) = u32x2{odd[in_group], top[in_group]};
 }
 
 // --------------------------------------------------------------- attention
