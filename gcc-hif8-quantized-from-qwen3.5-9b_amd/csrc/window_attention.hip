@@ -757,8 +757,17 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(const WindowParam
 
 // ------------------------------------------------------------- host side
 
-// Requests of more (token, head) rows per KV head than this run on images.
-constexpr int64_t kLongRows = 128;
+// Requests of more (token, head) rows per KV head than this run on images: kOnlyRows for a
+// call's only request, which cannot fill the GPU with its images' items, kLongRows for one of
+// several.  Images against the other kernels, us, 8 KV heads of 128, groups of 4, 16-row pages:
+//   requests, window   256 rows     384        512        768
+//   1 of 1024          60 vs 27   61 vs 26   49 vs 30   50 vs 40
+//   1 of 4096          64 vs 35   69 vs 41   60 vs 46   63 vs 69
+//   4 of 4096          70 vs 64   78 vs 92   85 vs 105  107 vs 198
+//   8 of 1024          62 vs 46              77 vs 104
+//   16 of 256          63 vs 53   70 vs 94   87 vs 120  111 vs 235
+//   32 of 1024        182 vs 168            238 vs 356
+constexpr int64_t kLongRows = 256, kOnlyRows = 512;
 // Image bytes of a pass; requests that do not fit wait for the next one.
 constexpr int64_t kImageBytes = int64_t(512) << 20;
 
@@ -781,7 +790,7 @@ WindowPlan plan_window(int64_t batch, int64_t heads, int64_t hkv, int64_t d, int
   const int64_t group = heads / hkv;
   pl.others = true;
   int64_t row_queries = max_query;
-  if (image_shape(d, dv, group, block_size) && max_query * group > kLongRows && max_len > 0) {
+  if (image_shape(d, dv, group, block_size) && max_query * group > (batch > 1 ? kLongRows : kOnlyRows) && max_len > 0) {
     pl.long_rows = batch > 1 ? kLongRows : 0;
     pl.others = batch > 1;
     pl.requests = std::min(batch, batch > 1 ? total_q / (kLongRows / group + 1) : int64_t(1));
@@ -896,7 +905,7 @@ extern "C" int hif8_window_attention(const void *query, int q_dtype, const uint8
   if (pl.requests == 0 || !aligned(query, 16) || !aligned(out, 16)) return row_attention(kName, a);
   if (!aligned(workspace, 16))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", kName);
-  if (pl.items > 0x1FFFFF || pl.items * pl.tiles > 0x7FFFFFFF || pl.slots * num_kv_heads * (pl.tiles + 8) > 0xFFFFFF)  // threads of a launch
+  if (pl.items > 0x1FFFFF || pl.items * (pl.tiles + kStart) > 0x7FFFFFFF || pl.slots * num_kv_heads * (pl.tiles + 8) > 0xFFFFFF)  // threads of a launch
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", kName);
   const int64_t group = num_heads / num_kv_heads;
   if (pl.others) {

@@ -218,6 +218,100 @@ def test_window_request_shorter_than_its_rows(native_ops, device):
     assert not out[:120].any() and out[120:140].any(-1).all() and not out[140].any() and out[141:].any(-1).all()
 
 
+@pytest.mark.parametrize("lens, qlens, window, sinks, hq, hkv, d, page", [
+    ([300, 300, 300], [64, 65, 66], 50, 4, 8, 2, 128, 16),      # 256, 260 and 264 rows per KV head
+    ([600], [128], 90, 4, 8, 2, 64, 16),                        # one request of 512 rows, and of 516
+    ([600], [129], 90, 4, 8, 2, 64, 16),
+    ([700, 650], [600, 300], 33, 0, 4, 4, 64, 32),              # a query head per KV head
+    ([80, 70], [60, 9], 20, 3, 32, 1, 256, 48),                 # 32 query heads per KV head
+    ([80, 70], [60, 9], 20, 3, 33, 1, 64, 48),                  # more than that
+    ([40, 1, 0, 2, 290], [40, 1, 0, 2, 290], 1, 0, 16, 2, 128, 16),
+    ([500, 500], [300, 299], 600, 17, 4, 4, 256, 16),
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_around_the_long_ones(native_ops, device, lens, qlens, window, sinks, hq, hkv, d, page, dtype):
+    _window(device, lens, qlens, window, sinks, hq, hkv, d, page, dtype=dtype, seed=hq + d)
+
+
+@pytest.mark.parametrize("long", [range(0, 150, 7), range(60, 70), range(149, 150), ()])
+def test_window_long_requests_among_many(native_ops, device, long):
+    """More requests than a wavefront has lanes; long ones between short and empty ones."""
+    qlens = [70 if b in long else (0, 1, 3, 2)[b % 4] for b in range(150)]
+    lens = [n and n + 5 * (b % 9) for b, n in enumerate(qlens)]
+    _window(device, lens, qlens, 24, 4, 8, 2, 64, 16, seed=len(long))
+
+
+@pytest.mark.parametrize("most", [44800, 80000, 160000])
+def test_window_long_requests_in_passes(native_ops, device, most):
+    """Requests that may be so long that their images are made in passes; and, as ever, are not."""
+    from hif8_rocm import kv_cache
+
+    lens, qlens = [290, 100, 41, 300, 170], [90, 100, 20, 70, 66]
+    kc, vc, table = build_cache(device, lens, 4, 256, 16, 3)
+    table = torch.cat([table, torch.full((5, most // 16 - table.shape[1]), -1, dtype=I32)], 1)
+    q = randn((sum(qlens), 16, 256), 4)
+    loc = torch.tensor(np.concatenate([[0], np.cumsum(qlens)]), dtype=I32, device=device)
+    out = kv_cache.paged_attention(q.to(device), kc, vc, table.to(device), torch.tensor(lens, dtype=I32, device=device),
+                                   scale=0.0625, query_start_loc=loc, max_query_len=100, max_seq_len=most,
+                                   window=2 ** 30, sinks=2, validate=False)
+    want, bound = window_reference(q.double().numpy(), kc.cpu().numpy(), vc.cpu().numpy(), table.numpy(), lens, qlens,
+                                   2 ** 30, 2, 0.0625, torch.bfloat16)
+    _near(out, want, bound)
+
+
+@pytest.mark.parametrize("starts", [[2, 202], [0, 0], [2, 202, 202, 330], [1, 3, 140, 141]])
+def test_window_rows_around_long_requests_are_zeros(native_ops, device, starts):
+    from hif8_rocm import kv_cache
+
+    lens = [230] * (len(starts) - 1)
+    qlens = [b - a for a, b in zip(starts, starts[1:])]
+    kc, vc, table = build_cache(device, lens, 2, 128, 16, 1)
+    table = table.to(device)
+    q = randn((starts[-1] + 9, 12, 128), 2)
+    out = kv_cache.paged_attention(q.to(device), kc, vc, table, torch.tensor(lens, dtype=I32, device=device), scale=0.1,
+                                   query_start_loc=torch.tensor(starts, dtype=I32, device=device), max_query_len=200,
+                                   max_seq_len=240, window=20, sinks=2, validate=False)
+    assert not out[:starts[0]].any() and not out[starts[-1]:].any()
+    if sum(qlens):
+        want, bound = window_reference(q[starts[0]:starts[-1]].double().numpy(), kc.cpu().numpy(), vc.cpu().numpy(),
+                                       table.cpu().numpy(), lens, qlens, 20, 2, 0.1, torch.bfloat16)
+        _near(out[starts[0]:starts[-1]], want, bound)
+
+
+def test_window_of_prompts_captured(native_ops, device):
+    """Long requests in a captured call: replays follow lengths, tables and queries, and two graphs share nothing."""
+    from hif8_rocm import kv_cache
+
+    kc, vc, table = build_cache(device, [500, 500], 2, 128, 16, 1)
+    table = table.to(device)
+    graphs = []
+    for rows in (160, 300):
+        q = torch.zeros(rows, 8, 128, dtype=torch.bfloat16, device=device)
+        loc, lens = torch.zeros(3, dtype=I32, device=device), torch.zeros(2, dtype=I32, device=device)
+
+        def call(q=q, loc=loc, lens=lens, rows=rows):
+            return kv_cache.paged_attention(q, kc, vc, table, lens, scale=0.1, query_start_loc=loc, max_query_len=rows,
+                                            max_seq_len=500, window=100, sinks=4, validate=False)
+
+        call()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, q, loc, lens, out, call))
+    for i in range(6):
+        for g, q, loc, lens, out, call in graphs:
+            n = q.shape[0]
+            q.copy_(randn(q.shape, 10 + i))
+            split = (0, n, n // 2, n - 3, 70, 1)[i]
+            loc.copy_(torch.tensor([0, split, n]))
+            lens.copy_(torch.tensor([500 - 17 * i, 300 + 20 * i]))
+        for g, *_ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, q, loc, lens, out, call in graphs:
+            assert torch.equal(out, call())
+
+
 def test_window_unaligned_and_strided_queries(native_ops, device):
     from hif8_rocm import kv_cache
 
