@@ -64,8 +64,9 @@ struct ExtendParams {
 };
 
 constexpr int kPerThread = 8;  // columns of a thread where there are more than threads
-// Rows up to which one workgroup does all of a call: 2048 rows more would take it 2.5 us,
-// the launch of another kernel 1.6 us (and 4 of the host's).
+// Rows up to which one workgroup does all of a call.  Against a kernel of its own for the
+// slots, 8 requests in a graph: 8 rows 4.4 and 5.3 us, 1024 4.8 and 5.7, 2048 5.7 and 5.7,
+// 4096 7.4 and 5.7; outside a graph the second launch is also 4 us of the host's.
 constexpr int kFewRows = 2048;
 
 // Slot and position of a row, from the table as it stands; of a row of no request -1.
@@ -84,8 +85,9 @@ __device__ __forceinline__ void put_slot(const ExtendParams &p, int row, int b, 
 
 // Ids for the table columns that the new tokens reach.  One workgroup: the rank of
 // a column among those without a page runs over all requests.  Bound by the dependent
-// reads of lengths, table and stack (four round trips, 3.6 us); with one column a thread
-// and pass 48 prompts of 4k tokens on 16-token pages (9200 columns) took 19 us.
+// reads of lengths, table and stack (four round trips, 4.3 us with a new token each).  48
+// prompts of 4k tokens on 16-token pages, 9200 columns: 12.9 us; with one column a thread
+// and pass 19.
 template <typename BtT>
 __global__ __launch_bounds__(kScan) void extend_kernel(const ExtendParams p) {
   __shared__ int first[kScan];      // columns of the chunk's requests before each
@@ -117,7 +119,7 @@ __global__ __launch_bounds__(kScan) void extend_kernel(const ExtendParams p) {
     __syncthreads();
     auto columns_of = [&](auto per) {
       constexpr int kPer = decltype(per)::value;
-      for (int c0 = 0; c0 < total; c0 += kScan * kPer) {
+      for (uint32_t c0 = 0; c0 < uint32_t(total); c0 += kScan * kPer) {  // unsigned: total may come near 2^31
         // Column c0 + kScan j + tid: its request is the last of the chunk that starts at or before it.
         int owner[kPer];
 #pragma unroll
@@ -126,13 +128,14 @@ __global__ __launch_bounds__(kScan) void extend_kernel(const ExtendParams p) {
         for (int step = kScan / 2; step > 0; step /= 2)
 #pragma unroll
           for (int j = 0; j < kPer; ++j)
-            if (first[owner[j] + step] <= c0 + kScan * j + tid) owner[j] += step;
+            if (uint32_t(first[owner[j] + step]) <= c0 + kScan * j + tid) owner[j] += step;
         BtT *entry[kPer], id[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-          const int c = c0 + kScan * j + tid, r = owner[j];
-          entry[j] = static_cast<BtT *>(p.table) + int64_t(base + r) * p.width + (low[r] + c - first[r]);
-          id[j] = c < total ? *entry[j] : BtT(0);
+          const uint32_t c = c0 + kScan * j + tid;
+          const int r = owner[j];
+          entry[j] = static_cast<BtT *>(p.table) + int64_t(base + r) * p.width + (int64_t(low[r]) + c - first[r]);
+          id[j] = c < uint32_t(total) ? *entry[j] : BtT(0);
         }
         uint64_t wants[kPer];
 #pragma unroll

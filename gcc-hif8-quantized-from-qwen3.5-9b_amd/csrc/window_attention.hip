@@ -136,17 +136,16 @@ __device__ void make_plan(const WindowParams &p) {
     if (mine) {
       int begin, count;
       request_rows(p.r, b, begin, count);
-      n = (count + p.tokens - 1) / p.tokens * p.r.hkv;
+      n = int(min(int64_t((count + p.tokens - 1) / p.tokens) * p.r.hkv, int64_t(p.most_items)));
     }
     const int upto = items + wave_prefix(n);
     if (mine && wave == 0) {
       first[slot] = upto - n;
       owner[slot] = b;
     }
-    items = __builtin_amdgcn_readlane(upto, kWave - 1);
+    items = min(__builtin_amdgcn_readlane(upto, kWave - 1), p.most_items);  // more only where start_loc is wrong
     slots += __popcll(__ballot(mine));
   }
-  items = min(items, p.most_items);
   __syncthreads();
   int before = 0;
   for (int base = 0; base < items; base += kThreads) {
