@@ -272,7 +272,8 @@ __global__ __launch_bounds__(kScan) void release_count_kernel(const ReleaseParam
 }
 
 // A workgroup per kChunk entries; what the earlier ones release has been counted, unless
-// one workgroup has them all.
+// one workgroup has them all (8 requests of 25 columns 3.0 us).  256 requests of 2049 columns,
+// 2.1 MB of table: 4.2 + 6.2 us, two reads of the table and a launch's latency each.
 template <typename BtT>
 __global__ __launch_bounds__(kScan) void release_kernel(const ReleaseParams p) {
   __shared__ int sums[kScanWaves];
