@@ -11,6 +11,12 @@ Mirrors the reference's ``vllm_ascend_hif8.kv_cache`` layout API
   only the pages in the block table and decodes them on chip, instead of
   gathering and materialising bf16 K/V for a fused-attention call.
 
+Beside them stand operators without a counterpart in the reference.  A step of a
+server, in their order: :func:`extend_block_tables`, :func:`write_kv_cache`,
+:func:`paged_attention` (with a window or without) or :func:`tree_attention`,
+:func:`verify_drafts`, :func:`accept_drafts`, :func:`release_blocks`; and
+:func:`evict_kv_rows`, which holds a cache to a size.
+
 K and V are separate uint8 tensors ``[num_blocks, block_size, num_kv_heads,
 head_size + 4]``; a row is HiF8 codes followed by a little-endian FP32 scale.
 """

@@ -278,6 +278,25 @@ def test_window_rows_around_long_requests_are_zeros(native_ops, device, starts):
         _near(out[starts[0]:starts[-1]], want, bound)
 
 
+@pytest.mark.parametrize("d, qlens", [(256, [1, 1]), (128, [9, 4]), (256, [90, 70]), (64, [300, 2])])
+def test_window_of_a_cache_past_32_bits(native_ops, device, d, qlens):
+    """Pages behind the first 4 GiB of the cache answer as the same pages in a small one."""
+    from hif8_rocm import kv_cache
+
+    lens, hkv, page = [330, 150], 4, 16
+    kc, vc, table = build_cache(device, lens, hkv, d, page, 7)
+    q = randn((sum(qlens), 16, d), 8).to(device)
+    opts = {"scale": 0.1, "query_lens": qlens, "window": 100, "sinks": 20}
+    want = kv_cache.paged_attention(q, kc, vc, table.to(device), lens, **opts)
+    blocks = (2 ** 32 + 2 ** 20) // (page * hkv * (d + 4)) + kc.shape[0]
+    big = [torch.empty(blocks, *c.shape[1:], dtype=torch.uint8, device=device) for c in (kc, vc)]
+    for b, c in zip(big, (kc, vc)):
+        b[-c.shape[0]:] = c
+    moved = torch.where(table < 0, table, table + (blocks - kc.shape[0]))
+    got = kv_cache.paged_attention(q, *big, moved.to(device), lens, **opts)
+    assert torch.equal(got, want)
+
+
 def test_window_of_prompts_captured(native_ops, device):
     """Long requests in a captured call: replays follow lengths, tables and queries, and two graphs share nothing."""
     from hif8_rocm import kv_cache
