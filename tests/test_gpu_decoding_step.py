@@ -233,6 +233,16 @@ def test_rows_around_the_long_ones(native_ops, device, lens, qlens, window, sink
     _window(device, lens, qlens, window, sinks, hq, hkv, d, page, dtype=dtype, seed=hq + d)
 
 
+@pytest.mark.parametrize("lens, qlens, hq, hkv, d", [
+    ([70, 40], [60, 9], 64, 1, 128), ([50], [50], 200, 2, 256), ([30, 30], [20, 30], 71, 1, 64),
+    ([20, 9, 30], [20, 2, 3], 127, 1, 128), ([24, 20], [4, 1], 256, 1, 64), ([24, 20], [9, 2], 255, 1, 256),
+    ([12, 9], [5, 2], 257, 1, 128), ([12, 9], [5, 2], 300, 1, 256),
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_window_many_query_heads_per_kv_head(native_ops, device, lens, qlens, hq, hkv, d, dtype):
+    _window(device, lens, qlens, 17, 2, hq, hkv, d, 16, dtype=dtype, seed=hq)
+
+
 @pytest.mark.parametrize("long", [range(0, 150, 7), range(60, 70), range(149, 150), ()])
 def test_window_long_requests_among_many(native_ops, device, long):
     """More requests than a wavefront has lanes; long ones between short and empty ones."""
