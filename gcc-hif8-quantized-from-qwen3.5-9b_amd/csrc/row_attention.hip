@@ -152,7 +152,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
 //     the logits alone and f what is multiplied with V: with one reference for
 //     both, rows whose scales lie 2^126 apart fell out of the sum.  P is rounded
 //     once: 2^-11 of it, or 2^-25 where it is subnormal (below 2^-14), which is at
-//     most 2^-31 of the row's largest;
+//     most 2^-31 of the row's largest; what that leaves may be a second P (rest_of);
 //   * O^T += V^T P^T: every wavefront takes 64 dims of 32 or 64 rows, 4 bytes of
 //     each row per lane, transposed by the lookup itself (byte q of eight words).
 // The next tile's K loads are issued as soon as S is done, its V loads after O.
@@ -187,19 +187,29 @@ constexpr float kMostSum = 0x1p40f;  // weights that add up to more are chosen a
 // eight, one workgroup, since the table and the query rows in LDS leave no room
 // for two and the registers of four none for the rows (24 heads of 128 under 61
 // drafts each: 44 us against 50 in row tiles of 32; 48 now).
-constexpr int waves_of(int row_blocks) { return row_blocks > 2 ? 8 : 4; }
+// With P in two parts of 32 rows its LDS does not let a second workgroup in either.
+constexpr int waves_of(int d, int row_blocks, bool rest) { return row_blocks > 2 || (rest && row_blocks == 2 && d < 256) ? 8 : 4; }
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
 // Cache rows of a tile.  256 of them at D = 64 left one workgroup to a CU (32
 // drafts of 16 heads over 8 x 16k: 111 us against 73).
-constexpr int tile_rows_of(int d, int row_blocks) { return d == 256 && row_blocks <= 2 ? 64 : 128; }
+constexpr int tile_rows_of(int d, int row_blocks, bool rest) {
+  return d == 256 && row_blocks <= 2 ? 64 : 32 * waves_of(d, row_blocks, rest) / (d / 64) > 128 ? 256 : 128;
+}
+// Whether what P's rounding to fp16 leaves is multiplied too, as a second P: under a window with
+// an fp16 output, which rounds no further than P does (error against float64 3.0e-4 without and 2.1e-4
+// with it; a bf16 output's own is 1.7e-3).  8 requests within 4096 rows, 16 / 4 heads of 256: one
+// token 28.1 -> 28.7 us, 6 rows 37.6 -> 38.9, 40 rows 71 -> 81; 32 / 8 heads of 128, 7 rows 41.3
+// -> 39.1 (one workgroup of eight wavefronts), 40 rows 86 -> 101; 16 / 4 of 64, 40 rows 42 -> 53.
+constexpr bool rest_of(bool bf16, bool window) { return window && !bf16; }
 
 template <int kD, bool kBf16, int kRB, bool kX, bool kWin, typename BtT>
-__global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(const RowAttnParams p,
+__global__ __launch_bounds__(64 * waves_of(kD, kRB, rest_of(kBf16, kWin)), 2) void row_attention_mfma(const RowAttnParams p,
                                                                             const uint32_t page_magic) {
-  constexpr int kW = waves_of(kRB);       // wavefronts
+  constexpr bool kRest = rest_of(kBf16, kWin);
+  constexpr int kW = waves_of(kD, kRB, kRest);  // wavefronts
   constexpr bool kQLds = kRB > 2;         // the query rows lie in LDS, in operand order, instead of registers
   constexpr int kRow = kD + 4;
-  constexpr int kT = tile_rows_of(kD, kRB);  // cache rows of a tile
+  constexpr int kT = tile_rows_of(kD, kRB, kRest);  // cache rows of a tile
   constexpr int kKB = kT / 16 / kW;       // 16-row blocks of a wavefront in S
   constexpr int kQS = kD / 32;            // MFMA steps over the head dims
   constexpr int kSlices = kD / 64;        // 64-dim slices of V
@@ -209,12 +219,14 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
   static_assert(kGroups < 32 && kVR % 32 == 0 && kKB * kW * 16 == kT, "a bit per group, whole MFMA steps");
   constexpr int kRows = 16 * kRB;
   constexpr int kPStride = kT + 8;        // fp16 values of a row of P in LDS
-  // Two buffers of P where that leaves room for two workgroups of four wavefronts.
-  constexpr int kBuffers = kW == 8 || kLookupBytes + 4 * kRows * kPStride + 32 * kRows + 64 <= 81920 - 1024 ? 2 : 1;
+  constexpr int kP = kRows * kPStride * (kRest ? 2 : 1);  // values of P, and of its rest behind it
+  // Two buffers of P where that leaves room for two workgroups of four wavefronts, or one of eight.
+  constexpr int kBuffers =
+      (kW == 8 ? !kRest : kLookupBytes + 4 * kP + 32 * kRows + 64 <= 81920 - 1024) ? 2 : 1;
   struct Smem {
     uint32_t table[kLookupBytes / 4];     // at LDS byte 0: a lookup's address needs no addition
     // P of a tile and of the next; at a segment's end the shares of O of wavefronts of one slice.
-    __attribute__((aligned(16))) uint16_t pt[max_of(kBuffers * kRows * kPStride, (kVG - 1) * kSlices * 2048)];
+    __attribute__((aligned(16))) uint16_t pt[max_of(kBuffers * kP, (kVG - 1) * kSlices * 2048)];
     lk_u32x4 q[kQLds ? kRB * kQS * kWave : 1];
     float top[2][kW][kRows];              // a wavefront's largest logit, and logit + log2 of V's scale, per query row
     int grow[2];                          // the last tile (counted from 1) whose P grew too large, by parity
@@ -649,7 +661,7 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     // most tiles: one barrier.  Where some wavefront's rows outgrew them (and in a
     // segment's first tile), all of them meet once more for new ones and write P again.
     ++tile_no;
-    uint16_t *pt = sm.pt + (kBuffers == 2 ? (tile_no & 1) * kRows * kPStride : 0);
+    uint16_t *pt = sm.pt + (kBuffers == 2 ? (tile_no & 1) * kP : 0);
     float psum[kRB];
     bool grow = false;
     auto weights = [&](auto all, int rb) __attribute__((always_inline)) {
@@ -671,9 +683,21 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
         }
         const int j = wave * kKB + kb;
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        *reinterpret_cast<u32x2 *>(pt + (16 * rb + n) * kPStride + 32 * (j >> 1) + 8 * g + 4 * (j & 1)) =
-            u32x2{uint32_t(float_to_f16_bits(w[0])) | (uint32_t(float_to_f16_bits(w[1])) << 16),
-                  uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
+        uint16_t *to = pt + (16 * rb + n) * kPStride + 32 * (j >> 1) + 8 * g + 4 * (j & 1);
+        auto store = [&](uint16_t *at) {
+          *reinterpret_cast<u32x2 *>(at) =
+              u32x2{uint32_t(float_to_f16_bits(w[0])) | (uint32_t(float_to_f16_bits(w[1])) << 16),
+                    uint32_t(float_to_f16_bits(w[2])) | (uint32_t(float_to_f16_bits(w[3])) << 16)};
+        };
+        store(to);
+        if constexpr (kRest) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float high = float(static_cast<_Float16>(w[e]));
+            w[e] = fabsf(high) < __builtin_inff() ? w[e] - high : 0.f;  // exact
+          }
+          store(to + kRows * kPStride);
+        }
       }
       // A row that has seen nothing yet has no maximum: what it sees first sets one.
       grow |= (most > 65504.f) | (psum[rb] > kMostSum) | ((m[rb] == -__builtin_inff()) & (kAll | (seen[rb] != 0)));
@@ -794,10 +818,13 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
     }
 #pragma unroll
     for (int hf = 0; hf < kVR / 32; ++hf) {
-      lk_u32x4 pf[kRB];
+      lk_u32x4 pf[kRB], pr[kRest ? kRB : 1];
 #pragma unroll
-      for (int rb = 0; rb < kRB; ++rb)
-        pf[rb] = *reinterpret_cast<const lk_u32x4 *>(pt + (16 * rb + n) * kPStride + kVR * vgroup + 32 * hf + 8 * g);
+      for (int rb = 0; rb < kRB; ++rb) {
+        const uint16_t *at = pt + (16 * rb + n) * kPStride + kVR * vgroup + 32 * hf + 8 * g;
+        pf[rb] = *reinterpret_cast<const lk_u32x4 *>(at);
+        if constexpr (kRest) pr[rb] = *reinterpret_cast<const lk_u32x4 *>(at + kRows * kPStride);
+      }
       // As above: the next byte's lookups are on their way while one multiplies.
       lk_u32x4 a = look_column<0, true>(vraw[hf], lane4, table);
       auto column = [&](auto byte) {
@@ -806,7 +833,10 @@ __global__ __launch_bounds__(64 * waves_of(kRB), 2) void row_attention_mfma(cons
         lk_u32x4 next = a;
         if constexpr (q < 3) next = look_column<q + 1, true>(vraw[hf], lane4, table);
 #pragma unroll
-        for (int rb = 0; rb < kRB; ++rb) oacc[rb][q] = mfma_16x16x32<false>(a, pf[rb], oacc[rb][q]);
+        for (int rb = 0; rb < kRB; ++rb) {
+          oacc[rb][q] = mfma_16x16x32<false>(a, pf[rb], oacc[rb][q]);
+          if constexpr (kRest) oacc[rb][q] = mfma_16x16x32<false>(a, pr[rb], oacc[rb][q]);
+        }
         a = next;
       };
       column(std::integral_constant<int, 0>{});
@@ -1092,7 +1122,7 @@ bool mfma_rows(int64_t d, int64_t dv, int64_t hkv, int64_t block_size, int64_t m
 }
 
 RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int64_t hkv, int64_t d, int64_t block_size,
-                  int64_t max_query, int64_t max_len) {
+                  int64_t max_query, int64_t max_len, bool rest) {
   RowPlan pl{};
   const int64_t len = std::max<int64_t>(max_len, 1);
   if (!mfma) {
@@ -1111,9 +1141,9 @@ RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int6
   pl.row_tiles = int((rows + 16 * pl.row_blocks - 1) / (16 * pl.row_blocks));
   pl.magic = uint32_t(((int64_t(1) << 31) + block_size / 16 - 1) / (block_size / 16));
   // A workgroup for each slot that the GPU has: eight wavefronts per CU.
-  pl.tile_rows = tile_rows_of(int(d), pl.row_blocks);
+  pl.tile_rows = tile_rows_of(int(d), pl.row_blocks, rest);
   const int64_t tiles = batch * ((len + pl.tile_rows - 1) / pl.tile_rows);
-  const int64_t slots = 2048 / waves_of(pl.row_blocks) / (hkv * pl.row_tiles);
+  const int64_t slots = 2048 / waves_of(int(d), pl.row_blocks, rest) / (hkv * pl.row_tiles);
   pl.workers = int(std::min<int64_t>(std::max<int64_t>(slots, 1), tiles));
   pl.parts = (pl.workers + batch) * hkv * pl.row_tiles * 16 * pl.row_blocks;
   pl.outputs = 2 * pl.workers * hkv * pl.row_tiles * 16 * pl.row_blocks;
@@ -1147,7 +1177,7 @@ dim3 row_grid(const RowAttnParams &p) {
 
 template <int kD, bool kBf16, int kRB, typename BtT>
 void launch_rows(const RowAttnParams &p, uint32_t magic, hipStream_t s) {
-  const unsigned threads = 64 * waves_of(kRB);
+  const unsigned threads = 64 * waves_of(kD, kRB, rest_of(kBf16, p.window != 0));
   const dim3 blocks = row_grid(p);
   if (p.window) row_attention_mfma<kD, kBf16, kRB, false, true, BtT><<<blocks, threads, 0, s>>>(p, magic);
   else if (p.x) row_attention_mfma<kD, kBf16, kRB, true, false, BtT><<<blocks, threads, 0, s>>>(p, magic);
@@ -1183,7 +1213,8 @@ size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv,
   size_t need = 0;
   for (const bool mfma : {false, true}) {
     if (mfma && !mfma_rows(d, dv, hkv, block_size, max_len)) continue;
-    const RowPlan pl = plan_rows(mfma, batch, total_q, heads, hkv, d, block_size, max_query, max_len);
+    // With P's rest there are as many workers or fewer.
+    const RowPlan pl = plan_rows(mfma, batch, total_q, heads, hkv, d, block_size, max_query, max_len, false);
     need = std::max(need, row_space(pl, batch, total_q, heads, dv, max_len, weights).total());
   }
   return need;
@@ -1234,7 +1265,8 @@ int row_attention(const char *name, const RowArgs &a) {
                     longest * group < 0xFFFF * 16 && (longest * group + 64) * group < (int64_t(1) << 31);  // the grid's y, token_of
   if (mfma && a.batch * (a.max_len / 64 + 1) > 0x7FFFFFFFll / 2)
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
-  const RowPlan pl = plan_rows(mfma, a.batch, a.total_q, a.heads, a.hkv, a.d, a.block_size, a.max_query, most_rows);
+  const RowPlan pl = plan_rows(mfma, a.batch, a.total_q, a.heads, a.hkv, a.d, a.block_size, a.max_query, most_rows,
+                               rest_of(a.q_dtype == HIF8_DTYPE_BF16, a.window != 0));
   RowAttnParams p{};
   p.query = a.query;
   p.key_cache = a.key_cache;

@@ -307,6 +307,45 @@ def test_window_of_a_cache_past_32_bits(native_ops, device, d, qlens):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("lens, qlens, hq, hkv, d", [
+    ([900, 400], [1, 1], 16, 4, 256), ([900, 400], [6, 3], 16, 4, 256), ([900, 400], [20, 30], 16, 4, 256),
+    ([900, 400], [7, 8], 16, 4, 128), ([900, 400], [30, 9], 16, 4, 128), ([900, 400], [2, 4], 16, 4, 64),
+    ([900, 400], [7, 8], 16, 4, 64), ([900, 400], [30, 9], 16, 4, 64), ([400, 300], [200, 90], 8, 2, 256),
+    ([400, 300], [200, 90], 8, 2, 128), ([400, 300], [200, 90], 8, 2, 64),
+])
+def test_window_fp16_is_off_by_its_rounding(native_ops, device, lens, qlens, hq, hkv, d):
+    """Root mean squares: rounding the exact answer to fp16 is off by about 2^-12.3 of it, a weight rounded to
+    fp16 would add as much again (1.4 times); with what that leaves multiplied (2^-22) and logits in float32 (off by
+    less than 2^-15, so weights by less than 2^-15) the whole stays within sqrt(1 + 2^-5.4) = 1.012 of the first."""
+    from hif8_rocm import kv_cache
+
+    kc, vc, table = build_cache(device, lens, hkv, d, 16, d)
+    q = randn((sum(qlens), hq, d), 3, 1.0, torch.float16)
+    out = kv_cache.paged_attention(q.to(device), kc, vc, table.to(device), lens, scale=1 / math.sqrt(d),
+                                   query_lens=qlens, window=333, sinks=4)
+    want, _ = window_reference(q.double().numpy(), kc.cpu().numpy(), vc.cpu().numpy(), table.numpy(), lens, qlens, 333,
+                               4, 1 / math.sqrt(d), torch.float16)
+    off, own = (np.sqrt(np.square(x - want).mean()) for x in (out.double().cpu().numpy(), want.astype(np.float16).astype(np.float64)))
+    print(f"  off {off:.3e}, the rounding {own:.3e}", flush=True)
+    assert off <= 1.05 * own
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 6, 20, 140])
+def test_window_infinities_in_fp16(native_ops, device, n, d):
+    """Infinite and NaN codes and infinite scales of V, seen by some rows, hidden from others, where P has two parts."""
+    lens, page, low = [200], 16, max(200 - n + 1 - 60, 20)
+
+    def spoil(kc, vc, table):
+        inf = torch.tensor([0, 0, 0x80, 0x7F], dtype=torch.uint8, device=vc.device)
+        for t, head, code in ((199, 0, 0x6F), (198, 1, 0x80), (low, 0, 0xEF), (low - 1, 0, 0x80), (low - 2, 1, 0x6F)):
+            vc[int(table[0, t // page]), t % page, head, 5] = code
+        vc[int(table[0, 190 // page]), 190 % page, 1, -4:] = inf
+        vc[int(table[0, (low - 3) // page]), (low - 3) % page, 0, -4:] = inf
+
+    _window(device, lens, [n], 60, 20, 8, 2, d, page, dtype=torch.float16, spoil=spoil, seed=d + n)
+
+
 def test_window_of_prompts_captured(native_ops, device):
     """Long requests in a captured call: replays follow lengths, tables and queries, and two graphs share nothing."""
     from hif8_rocm import kv_cache
