@@ -187,29 +187,34 @@ constexpr float kMostSum = 0x1p40f;  // weights that add up to more are chosen a
 // eight, one workgroup, since the table and the query rows in LDS leave no room
 // for two and the registers of four none for the rows (24 heads of 128 under 61
 // drafts each: 44 us against 50 in row tiles of 32; 48 now).
-// With P in two parts of 32 rows its LDS does not let a second workgroup in either.
-constexpr int waves_of(int d, int row_blocks, bool rest) { return row_blocks > 2 || (rest && row_blocks == 2 && d < 256) ? 8 : 4; }
+// One of eight too for P in two parts of 32 rows, which leave a second workgroup no
+// LDS either, and for a window's 32 rows of 128 dims (7 rows of 32 / 8 heads, 8
+// requests within 4096: 39.0 us, in two of four 42.6; 32 within 1024 37.4 and 42.6).
+constexpr int waves_of(int d, int row_blocks, bool win, bool rest) {
+  return row_blocks > 2 || (row_blocks == 2 && ((win && d == 128) || (rest && d == 64))) ? 8 : 4;
+}
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
 // Cache rows of a tile.  256 of them at D = 64 left one workgroup to a CU (32
 // drafts of 16 heads over 8 x 16k: 111 us against 73).
-constexpr int tile_rows_of(int d, int row_blocks, bool rest) {
-  return d == 256 && row_blocks <= 2 ? 64 : 32 * waves_of(d, row_blocks, rest) / (d / 64) > 128 ? 256 : 128;
+constexpr int tile_rows_of(int d, int row_blocks, bool win, bool rest) {
+  return d == 256 && row_blocks <= 2 ? 64 : 32 * waves_of(d, row_blocks, win, rest) / (d / 64) > 128 ? 256 : 128;
 }
-// Whether what P's rounding to fp16 leaves is multiplied too, as a second P: under a window with
-// an fp16 output, which rounds no further than P does (error against float64 3.0e-4 without and 2.1e-4
-// with it; a bf16 output's own is 1.7e-3).  8 requests within 4096 rows, 16 / 4 heads of 256: one
-// token 28.1 -> 28.7 us, 6 rows 37.6 -> 38.9, 40 rows 71 -> 81; 32 / 8 heads of 128, 7 rows 41.3
-// -> 39.1 (one workgroup of eight wavefronts), 40 rows 86 -> 101; 16 / 4 of 64, 40 rows 42 -> 53.
+// Whether what P's rounding to fp16 leaves is multiplied too, as a second P: under a
+// window with an fp16 output, which rounds no further than P does (error against
+// float64 3.0e-4 without and 2.1e-4 with it; a bf16 output's own is 1.7e-3).  8
+// requests within 4096 rows, 16 / 4 heads of 256: one token 28.1 -> 28.7 us, 6 rows
+// 37.6 -> 38.9, 40 rows 71 -> 81; 32 / 8 heads of 128, 40 rows 86 -> 101; 16 / 4 of
+// 64, 40 rows 42 -> 53.
 constexpr bool rest_of(bool bf16, bool window) { return window && !bf16; }
 
 template <int kD, bool kBf16, int kRB, bool kX, bool kWin, typename BtT>
-__global__ __launch_bounds__(64 * waves_of(kD, kRB, rest_of(kBf16, kWin)), 2) void row_attention_mfma(const RowAttnParams p,
+__global__ __launch_bounds__(64 * waves_of(kD, kRB, kWin, rest_of(kBf16, kWin)), 2) void row_attention_mfma(const RowAttnParams p,
                                                                             const uint32_t page_magic) {
   constexpr bool kRest = rest_of(kBf16, kWin);
-  constexpr int kW = waves_of(kD, kRB, kRest);  // wavefronts
+  constexpr int kW = waves_of(kD, kRB, kWin, kRest);  // wavefronts
   constexpr bool kQLds = kRB > 2;         // the query rows lie in LDS, in operand order, instead of registers
   constexpr int kRow = kD + 4;
-  constexpr int kT = tile_rows_of(kD, kRB, kRest);  // cache rows of a tile
+  constexpr int kT = tile_rows_of(kD, kRB, kWin, kRest);  // cache rows of a tile
   constexpr int kKB = kT / 16 / kW;       // 16-row blocks of a wavefront in S
   constexpr int kQS = kD / 32;            // MFMA steps over the head dims
   constexpr int kSlices = kD / 64;        // 64-dim slices of V
@@ -1122,7 +1127,7 @@ bool mfma_rows(int64_t d, int64_t dv, int64_t hkv, int64_t block_size, int64_t m
 }
 
 RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int64_t hkv, int64_t d, int64_t block_size,
-                  int64_t max_query, int64_t max_len, bool rest) {
+                  int64_t max_query, int64_t max_len, bool win, bool rest) {
   RowPlan pl{};
   const int64_t len = std::max<int64_t>(max_len, 1);
   if (!mfma) {
@@ -1141,9 +1146,9 @@ RowPlan plan_rows(bool mfma, int64_t batch, int64_t total_q, int64_t heads, int6
   pl.row_tiles = int((rows + 16 * pl.row_blocks - 1) / (16 * pl.row_blocks));
   pl.magic = uint32_t(((int64_t(1) << 31) + block_size / 16 - 1) / (block_size / 16));
   // A workgroup for each slot that the GPU has: eight wavefronts per CU.
-  pl.tile_rows = tile_rows_of(int(d), pl.row_blocks, rest);
+  pl.tile_rows = tile_rows_of(int(d), pl.row_blocks, win, rest);
   const int64_t tiles = batch * ((len + pl.tile_rows - 1) / pl.tile_rows);
-  const int64_t slots = 2048 / waves_of(int(d), pl.row_blocks, rest) / (hkv * pl.row_tiles);
+  const int64_t slots = 2048 / waves_of(int(d), pl.row_blocks, win, rest) / (hkv * pl.row_tiles);
   pl.workers = int(std::min<int64_t>(std::max<int64_t>(slots, 1), tiles));
   pl.parts = (pl.workers + batch) * hkv * pl.row_tiles * 16 * pl.row_blocks;
   pl.outputs = 2 * pl.workers * hkv * pl.row_tiles * 16 * pl.row_blocks;
@@ -1177,7 +1182,7 @@ dim3 row_grid(const RowAttnParams &p) {
 
 template <int kD, bool kBf16, int kRB, typename BtT>
 void launch_rows(const RowAttnParams &p, uint32_t magic, hipStream_t s) {
-  const unsigned threads = 64 * waves_of(kD, kRB, rest_of(kBf16, p.window != 0));
+  const unsigned threads = 64 * waves_of(kD, kRB, p.window != 0, rest_of(kBf16, p.window != 0));
   const dim3 blocks = row_grid(p);
   if (p.window) row_attention_mfma<kD, kBf16, kRB, false, true, BtT><<<blocks, threads, 0, s>>>(p, magic);
   else if (p.x) row_attention_mfma<kD, kBf16, kRB, true, false, BtT><<<blocks, threads, 0, s>>>(p, magic);
@@ -1213,8 +1218,8 @@ size_t row_workspace(int64_t batch, int64_t total_q, int64_t heads, int64_t hkv,
   size_t need = 0;
   for (const bool mfma : {false, true}) {
     if (mfma && !mfma_rows(d, dv, hkv, block_size, max_len)) continue;
-    // With P's rest there are as many workers or fewer.
-    const RowPlan pl = plan_rows(mfma, batch, total_q, heads, hkv, d, block_size, max_query, max_len, false);
+    // Under a window there are as many workers or fewer.
+    const RowPlan pl = plan_rows(mfma, batch, total_q, heads, hkv, d, block_size, max_query, max_len, false, false);
     need = std::max(need, row_space(pl, batch, total_q, heads, dv, max_len, weights).total());
   }
   return need;
@@ -1266,7 +1271,7 @@ int row_attention(const char *name, const RowArgs &a) {
   if (mfma && a.batch * (a.max_len / 64 + 1) > 0x7FFFFFFFll / 2)
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: dimensions too large", name);
   const RowPlan pl = plan_rows(mfma, a.batch, a.total_q, a.heads, a.hkv, a.d, a.block_size, a.max_query, most_rows,
-                               rest_of(a.q_dtype == HIF8_DTYPE_BF16, a.window != 0));
+                               a.window != 0, rest_of(a.q_dtype == HIF8_DTYPE_BF16, a.window != 0));
   RowAttnParams p{};
   p.query = a.query;
   p.key_cache = a.key_cache;
