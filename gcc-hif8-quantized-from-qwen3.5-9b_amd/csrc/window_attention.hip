@@ -48,8 +48,8 @@ constexpr int kStages = 4;     // images in LDS: two that are worked on, two on 
 constexpr int kMaxSlots = 1024;  // requests of a pass
 
 // An image: K fragments [D / 16], V fragments [D / 32][2], then K's scales (times the
-// softmax scale, base 2) [32], V's [32], and three words: rows that are there, rows whose V
-// holds an infinity or NaN, the largest of V's scales.
+// softmax scale, base 2) [32], V's [32], and four words: rows that are there, rows whose V
+// holds an infinity or NaN, and Room of V's scales.
 constexpr int frag_bytes(int d) { return 2 * kKeys * d * 2; }
 constexpr int img_bytes(int d) { return (frag_bytes(d) + 8 * kKeys + 16 + 1023) / 1024 * 1024; }
 
@@ -203,6 +203,25 @@ __device__ void make_plan(const WindowParams &p) {
 
 // ------------------------------------------------------------------ images
 
+// A query row's P = 2^(x - r) * V's scale, x its logits: r stands until some P could reach
+// 2^kMost (fp16 ends at 2^16), and is then the least at which every P that the row has seen
+// stays below 2^kTop.
+constexpr float kTop = 7.f, kMost = 15.f;
+
+// How far a logit may lie above its row's r over an image whose scales of V are at most
+// `most` and at least `least`; -infinity where some are zero or not within 2^-60 to 2^60:
+// sums of 2^(x - r) could leave float32's range there.  And whether one power of two bounds
+// all of the scales tightly.
+struct Room {
+  float logit;
+  uint32_t even;
+};
+__device__ __forceinline__ Room room_of(float most, float least) {
+  const int e = __builtin_amdgcn_frexp_expf(most);
+  return Room{least >= 0x1p-60f && most <= 0x1p60f ? kMost - float(e) : -__builtin_inff(),
+              e == __builtin_amdgcn_frexp_expf(least) ? 1u : 0u};
+}
+
 // A workgroup per (slot, KV head, kThreads / D * 32 rows): threads take 16 codes of a K
 // row, and 4 codes of eight V rows each.  Bound by the bytes (4 of image and 1 of cache
 // per element): 4 x 4608 rows of 4 KV heads of 256, 114 MB, 31 us (3.7 TB/s).  The KV
@@ -215,7 +234,7 @@ __global__ __launch_bounds__(kThreads) void window_image_kernel(const WindowPara
   constexpr int kLoads = kKeys * kChunks / kPerTile;
   static_assert(kPerTile == kD && kD % 64 == 0, "a wavefront works on one image");
   __shared__ uint32_t dec[256];  // the query's type below, fp16 (0 where not finite) above
-  __shared__ uint32_t odd[kTiles], top[kTiles];
+  __shared__ uint32_t odd[kTiles], top[kTiles], low[kTiles];
   const int tid = threadIdx.x;
   if (blockIdx.x < 8) {  // the first eight make the plan or nothing
     if (blockIdx.x == 0) make_plan(p);
@@ -240,7 +259,10 @@ __global__ __launch_bounds__(kThreads) void window_image_kernel(const WindowPara
     const bool finite = (tid & 0x7F) != 0x6F && tid != 0x80;
     const uint32_t half = float_to_f16_bits(__uint_as_float(f));
     dec[tid] = (kBf16 ? f >> 16 : half) | (finite ? half << 16 : 0u);
-    if (tid < kTiles) odd[tid] = top[tid] = 0;
+    if (tid < kTiles) {
+      odd[tid] = top[tid] = 0;
+      low[tid] = 0x7F800000u;
+    }
   }
   // Everything of an image is the same in a whole wavefront.
   const int in_group = __builtin_amdgcn_readfirstlane(tid / kPerTile), tile = first + in_group, at = tid % kPerTile;
@@ -327,14 +349,23 @@ __global__ __launch_bounds__(kThreads) void window_image_kernel(const WindowPara
       sc[at] = ksc;
       sc[kKeys + at] = finite ? vsc : 0.f;
       if (!finite) atomicOr(&odd[in_group], 1u << at);
-      else atomicMax(&top[in_group], __float_as_uint(fabsf(vsc)));
+      if (there) {
+        const uint32_t size = finite ? __float_as_uint(fabsf(vsc)) : 0u;
+        atomicMax(&top[in_group], size);
+        atomicMin(&low[in_group], size);
+      }
     }
     const uint64_t seen = __ballot(there);  // the image's first wavefront
     if (at == 0) reinterpret_cast<uint32_t *>(im + frag_bytes(kD))[2 * kKeys] = uint32_t(seen);
   }
   __syncthreads();
-  if (mine && at == 0)
-    *reinterpret_cast<u32x2 *>(im + frag_bytes(kD) + 8 * kKeys + 4) = u32x2{odd[in_group], top[in_group]};
+  if (mine && at == 0) {
+    const Room room = room_of(__uint_as_float(top[in_group]), __uint_as_float(low[in_group]));
+    uint32_t *words = reinterpret_cast<uint32_t *>(im + frag_bytes(kD)) + 2 * kKeys;
+    words[1] = odd[in_group];
+    words[2] = __float_as_uint(room.logit);
+    words[3] = room.even;
+  }
 }
 
 // --------------------------------------------------------------- attention
@@ -372,20 +403,9 @@ __device__ __forceinline__ float sum_of_halves(float x) {
 // A value that is the same in all lanes, in a scalar register.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Of all lanes, without a trip through LDS.
-__device__ __forceinline__ float max_over_lanes(float x) {
-  x = fmaxf(x, rotated<8>(x));
-  x = fmaxf(x, rotated<4>(x));
-  x = fmaxf(x, rotated<2>(x));
-  return max_over_groups(fmaxf(x, rotated<1>(x)));
-}
-
-// Weights are 2^(x - m + kBias - e), m a maximum of the row that moves once a logit of the
-// wavefront passes its row's by kLazy, then for every row that has one above it (rows that
-// moved alone came to move O^T again and again: 8192 rows within 2048 took 2 % longer), 2^e the power of two above the largest of V's scales (held within 2^+-96, so
-// that sums of weights stay in range): P = weight * V's scale stays below 2^14 and starts
-// high in fp16's range, so that small weights keep their bits.
-constexpr float kBias = 6.f, kLazy = 8.f;
+// Reference of a query row that has seen nothing: below every logit, and a number, so that
+// no difference of references is a NaN.
+constexpr float kNone = -3.402823466e38f;
 
 // 32 rows that a wavefront holds as S^T and O^T lie (row lane % 32, value(db, q): dims 32 db
 // + 8 q + 4 (lane / 32) + [0, 4)) to their places in out, at(row) or -1: through LDS, since
@@ -512,126 +532,172 @@ __global__ __launch_bounds__(64 * waves_of(kD), waves_of(kD) * groups_per_cu(kD)
   lds_barrier();  // the segment before is done with both stages
   copy(t_begin, 0);
   if (t_begin + 1 < t_end) copy(t_begin + 1, 1);
-  // The power of two of the largest of V's scales.
-  float largest = 0.f;
-  for (int i = t_begin + lane; i < t_end; i += kWave)
-    largest = fmaxf(largest, reinterpret_cast<const float *>(img + size_t(walk.image(i)) * kImg + frag_bytes(kD))[2 * kKeys + 2]);
-  largest = max_over_lanes(largest);
-  const float base = kBias - float(min(max(largest > 0.f ? int(__builtin_amdgcn_frexp_expf(largest)) : 0, -96), 96));
 
   f32x16_t oacc[kDB];
 #pragma unroll
   for (int db = 0; db < kDB; ++db)
 #pragma unroll
     for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
-  float m = -__builtin_inff(), l = 0.f;
+  // P's reference r and the sum of weights l, in units of 2^r.  Both are of what this query
+  // row sees: scales that it does not see would take its P below fp16's range.  Where some of
+  // the images' scales lie far from one, l is in units of 2^m, m the largest logit, so that
+  // neither it nor P leaves float32's range (two loops: one for both took 5 % longer).
+  float r = kNone, m = kNone, l = 0.f;
   uint32_t odd_seen = 0;
   // The query rows have arrived: without this the loop would wait for them, and with them
   // for the copies behind them, at every image.
 #pragma unroll
   for (int k = 0; k < kQS; ++k) asm volatile("" : "+v"(qf[k]));
 
-  for (int i = t_begin; i < t_end; ++i) {
-    const int stage = (i - t_begin) % kStages;
-    if (stage % 2 == 0) {
-      wait_vmcnt<0>();  // this wavefront's part of images i and i + 1
-      lds_barrier();    // every wavefront's; and all are done with the other two stages
-      if (i + 2 < t_end) copy(i + 2, stage ^ 2);
-      if (i + 3 < t_end) copy(i + 3, (stage ^ 2) + 1);
-    }
-    if (at_lo > at_hi) continue;  // a wavefront without rows (uniform)
-    const uint8_t *im = smem + stage * kImg;
-    const u32x4 *kf = reinterpret_cast<const u32x4 *>(im) + lane;
-    const u32x4 *vf = reinterpret_cast<const u32x4 *>(im + frag_bytes(kD) / 2) + lane;
-    const float *sc = reinterpret_cast<const float *>(im + frag_bytes(kD));
-    const uint32_t there = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t *>(sc)[2 * kKeys]);
-    odd_seen |= __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t *>(sc)[2 * kKeys + 1]);
-    // S^T: element e is key 8 (e / 4) + 4 hf + e % 4 of row n.
-    f32x16_t s;
+  auto images_of = [&](auto apart) __attribute__((always_inline)) {
+    constexpr bool kApart = decltype(apart)::value;
+    for (int i = t_begin; i < t_end; ++i) {
+      const int stage = (i - t_begin) % kStages;
+      if (stage % 2 == 0) {
+        wait_vmcnt<0>();  // this wavefront's part of images i and i + 1
+        lds_barrier();    // every wavefront's; and all are done with the other two stages
+        if (i + 2 < t_end) copy(i + 2, stage ^ 2);
+        if (i + 3 < t_end) copy(i + 3, (stage ^ 2) + 1);
+      }
+      if (at_lo > at_hi) continue;  // a wavefront without rows (uniform)
+      const uint8_t *im = smem + stage * kImg;
+      const u32x4 *kf = reinterpret_cast<const u32x4 *>(im) + lane;
+      const u32x4 *vf = reinterpret_cast<const u32x4 *>(im + frag_bytes(kD) / 2) + lane;
+      const float *sc = reinterpret_cast<const float *>(im + frag_bytes(kD));
+      const uint32_t there = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t *>(sc)[2 * kKeys]);
+      odd_seen |= __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t *>(sc)[2 * kKeys + 1]);
+      const float room = __int_as_float(uniform(reinterpret_cast<const int *>(sc)[2 * kKeys + 2]));
+      const int even = uniform(reinterpret_cast<const int *>(sc)[2 * kKeys + 3]);
+      // S^T: element e is key 8 (e / 4) + 4 hf + e % 4 of row n.
+      f32x16_t s;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = 0.f;
-    // A ring of fragments: each is read kAhead products (32 cycles apiece) before its own,
-    // which is about what LDS takes; further ahead they would spill.
-    u32x4 ka[kAheadK + 1];
+      for (int e = 0; e < 16; ++e) s[e] = 0.f;
+      // A ring of fragments: each is read kAhead products (32 cycles apiece) before its own,
+      // which is about what LDS takes; further ahead they would spill.
+      u32x4 ka[kAheadK + 1];
 #pragma unroll
-    for (int k = 0; k < kAheadK; ++k) ka[k] = kf[64 * k];
+      for (int k = 0; k < kAheadK; ++k) ka[k] = kf[64 * k];
 #pragma unroll
-    for (int k = 0; k < kQS; ++k) {
+      for (int k = 0; k < kQS; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (k + kAheadK < kQS) ka[(k + kAheadK) % (kAheadK + 1)] = kf[64 * (k + kAheadK)];
+        s = mfma32<kBf16>(ka[k % (kAheadK + 1)], qf[k], s);
+      }
+      f32x4_t ks[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) ks[q] = *reinterpret_cast<const f32x4_t *>(sc + 8 * q + 4 * hf);
       __builtin_amdgcn_sched_barrier(0);
-      if (k + kAheadK < kQS) ka[(k + kAheadK) % (kAheadK + 1)] = kf[64 * (k + kAheadK)];
-      s = mfma32<kBf16>(ka[k % (kAheadK + 1)], qf[k], s);
-    }
-    f32x4_t ks[4];
+      // Cache rows of the image's two groups of 16.
+      const int t0 = walk.image(i) * kKeys, r0 = win.real(t0), r1 = win.real(t0 + 16);
+      const bool full = there == 0xFFFFFFFFu && r1 + 15 <= at_lo &&
+                        (int64_t(min(r0, r1)) > int64_t(at_hi) - p.r.window || r1 + 15 < p.r.sinks);
+      float x[16];
+      float tmax = -__builtin_inff();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) ks[q] = *reinterpret_cast<const f32x4_t *>(sc + 8 * q + 4 * hf);
-    __builtin_amdgcn_sched_barrier(0);
-    // Cache rows of the image's two groups of 16.
-    const int t0 = walk.image(i) * kKeys, r0 = win.real(t0), r1 = win.real(t0 + 16);
-    const bool full = there == 0xFFFFFFFFu && r1 + 15 <= at_lo && (int64_t(min(r0, r1)) > int64_t(at_hi) - p.r.window ||
-                                                                   r1 + 15 < p.r.sinks);
-    float x[16];
-    float tmax = -__builtin_inff();
+      for (int e = 0; e < 16; ++e) x[e] = s[e] * ks[e >> 2][e & 3];
+      if (!full) {
+        // Bit k: row k of the image is there and this lane's query row sees it.
+        auto below = [](int64_t end) { return (1u << min(max(end, int64_t(0)), int64_t(16))) - 1u; };
+        auto seen16 = [&](int r) {
+          return below(int64_t(at) + 1 - r) & (~below(int64_t(at) + 1 - p.r.window - r) | below(int64_t(p.r.sinks) - r));
+        };
+        const uint32_t seen = ((seen16(r0) | (seen16(r1) << 16)) & there) >> (4 * hf);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = s[e] * ks[e >> 2][e & 3];
-    if (!full) {
-      // Bit k: row k of the image is there and this lane's query row sees it.
-      auto below = [](int64_t end) { return (1u << min(max(end, int64_t(0)), int64_t(16))) - 1u; };
-      auto seen16 = [&](int r) {
-        return below(int64_t(at) + 1 - r) & (~below(int64_t(at) + 1 - p.r.window - r) | below(int64_t(p.r.sinks) - r));
-      };
-      const uint32_t seen = ((seen16(r0) | (seen16(r1) << 16)) & there) >> (4 * hf);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = (seen >> (8 * (e >> 2) + (e & 3))) & 1u ? x[e] : -__builtin_inff();
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, x[e]);
-    tmax = max_of_halves(tmax);
-    if (__any(tmax > m + kLazy)) {
-      const bool grow = tmax > m;  // also the first logit of a row: m is -infinity
-      const float m_new = grow ? tmax : m;
-      const float alpha = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-      if (!__all(!grow || m == -__builtin_inff())) {
-        l *= alpha;
-#pragma unroll
-        for (int db = 0; db < kDB; ++db) oacc[db] *= alpha;
+        for (int e = 0; e < 16; ++e) x[e] = (seen >> (8 * (e >> 2) + (e & 3))) & 1u ? x[e] : -__builtin_inff();
       }
-      m = m_new;
-    }
-    const float ref = m == -__builtin_inff() ? 0.f : m - base;
-    u32x4 pf[2], pr[2];
-    float sum = 0.f;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4_t vsc = *reinterpret_cast<const f32x4_t *>(sc + kKeys + 8 * q + 4 * hf);
-      float w[4];
+      for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, x[e]);
+      tmax = max_of_halves(tmax);
+      if (kApart || __any(tmax > r + room)) {
+        // Every row whose P has outgrown 2^kTop moves (rows that moved alone came to move O^T
+        // again and again: 8192 rows within 2048 took 2 % longer).
+        float ty;  // of logit + log2 of V's scale, rounded up
+        if (!kApart && even) {
+          ty = tmax + (kMost - room);
+        } else {
+          ty = -__builtin_inff();
+          int own = kKeys;  // opaque: loads shared with those below would be held across
+          asm volatile("" : "+v"(own));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float pw = __builtin_amdgcn_exp2f(x[4 * q + j] - ref);
-        sum += pw;
-        w[j] = pw * vsc[j];
+          for (int q = 0; q < 4; ++q) {
+            const f32x4_t vsc = *reinterpret_cast<const f32x4_t *>(sc + own + 8 * q + 4 * hf);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (vsc[j] != 0.f) ty = fmaxf(ty, x[4 * q + j] + float(__builtin_amdgcn_frexp_expf(vsc[j])));
+          }
+          ty = max_of_halves(ty);
+        }
+        float r_new = fmaxf(r, ty - kTop);
+        if constexpr (kApart) {
+          const float m_new = fmaxf(m, tmax);
+          r_new = fmaxf(r_new, m_new - 126.f);
+          l *= __builtin_amdgcn_exp2f(m - m_new);
+          m = m_new;
+        }
+        if (!__all(r == r_new || r == kNone)) {
+          const float alpha = __builtin_amdgcn_exp2f(r - r_new);
+          if constexpr (!kApart) l *= alpha;
+#pragma unroll
+          for (int db = 0; db < kDB; ++db) oacc[db] *= alpha;
+        }
+        r = r_new;
       }
-      pf[q >> 1][2 * (q & 1)] = pack_f16(w[0], w[1]);
-      pf[q >> 1][2 * (q & 1) + 1] = pack_f16(w[2], w[3]);
-      if constexpr (kRest) {
+      const float ref = kApart ? m : r;
+      u32x4 pf[2], pr[2];
+      float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const f16x2_t high = __builtin_bit_cast(f16x2_t, uint32_t(pf[q >> 1][2 * (q & 1) + j]));
-          pr[q >> 1][2 * (q & 1) + j] = pack_f16(w[2 * j] - float(high[0]), w[2 * j + 1] - float(high[1]));  // exact
+      for (int q = 0; q < 4; ++q) {
+        const f32x4_t vsc = *reinterpret_cast<const f32x4_t *>(sc + kKeys + 8 * q + 4 * hf);
+        float w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float pw = __builtin_amdgcn_exp2f(x[4 * q + j] - ref);
+          sum += pw;
+          w[j] = pw * vsc[j];
+          if constexpr (kApart) w[j] *= __builtin_amdgcn_exp2f(m - r);
+        }
+        pf[q >> 1][2 * (q & 1)] = pack_f16(w[0], w[1]);
+        pf[q >> 1][2 * (q & 1) + 1] = pack_f16(w[2], w[3]);
+        if constexpr (kRest) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const f16x2_t high = __builtin_bit_cast(f16x2_t, uint32_t(pf[q >> 1][2 * (q & 1) + j]));
+            pr[q >> 1][2 * (q & 1) + j] = pack_f16(w[2 * j] - float(high[0]), w[2 * j + 1] - float(high[1]));  // exact
+          }
         }
       }
-    }
-    l += sum;
-    u32x4 va[kAheadV + 1];
+      l += sum;
+      u32x4 va[kAheadV + 1];
 #pragma unroll
-    for (int k = 0; k < kAheadV; ++k) va[k] = vf[64 * k];
+      for (int k = 0; k < kAheadV; ++k) va[k] = vf[64 * k];
 #pragma unroll
-    for (int k = 0; k < 2 * kDB; ++k) {
+      for (int k = 0; k < 2 * kDB; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (k + kAheadV < 2 * kDB) va[(k + kAheadV) % (kAheadV + 1)] = vf[64 * (k + kAheadV)];
+        oacc[k >> 1] = mfma32<false>(va[k % (kAheadV + 1)], pf[k & 1], oacc[k >> 1]);
+        if constexpr (kRest) oacc[k >> 1] = mfma32<false>(va[k % (kAheadV + 1)], pr[k & 1], oacc[k >> 1]);
+      }
       __builtin_amdgcn_sched_barrier(0);
-      if (k + kAheadV < 2 * kDB) va[(k + kAheadV) % (kAheadV + 1)] = vf[64 * (k + kAheadV)];
-      oacc[k >> 1] = mfma32<false>(va[k % (kAheadV + 1)], pf[k & 1], oacc[k >> 1]);
-      if constexpr (kRest) oacc[k >> 1] = mfma32<false>(va[k % (kAheadV + 1)], pr[k & 1], oacc[k >> 1]);
     }
-    __builtin_amdgcn_sched_barrier(0);
+  };
+  bool apart = false;
+  for (int i = t_begin + lane; i < t_end; i += kWave)
+    apart |= reinterpret_cast<const float *>(img + size_t(walk.image(i)) * kImg + frag_bytes(kD))[2 * kKeys + 2] ==
+             -__builtin_inff();
+  apart = __any(apart);  // of the whole workgroup: the images are the same
+  float inv;
+  if (apart) {
+    images_of(std::true_type{});
+    l = sum_of_halves(l);
+    inv = l != 0.f ? 1.f / l : 0.f;
+    const float back = __builtin_amdgcn_exp2f(r - m);
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) oacc[db] = oacc[db] * inv * back;  // in this order it stays in range
+    inv = 1.f;
+  } else {
+    images_of(std::false_type{});
+    l = sum_of_halves(l);
+    inv = l != 0.f ? 1.f / l : 0.f;
   }
   if (odd_seen) {
     // Infinities and NaN of V lie as zeros in the images: the rows that see them get them
@@ -666,14 +732,13 @@ __global__ __launch_bounds__(64 * waves_of(kD), waves_of(kD) * groups_per_cu(kD)
       }
     }
   }
-  l = sum_of_halves(l);
-  const float inv = l != 0.f ? 1.f / l : 0.f;
+  auto answer = [&](int db, int q) {
+    return f32x4_t{oacc[db][4 * q] * inv, oacc[db][4 * q + 1] * inv, oacc[db][4 * q + 2] * inv, oacc[db][4 * q + 3] * inv};
+  };
   lds_barrier();  // every wavefront is done with the images: their place takes the rows
   if (whole) {
     if (at_lo <= at_hi)
-      store_rows<kD, kBf16>(smem + wave * kRowsLds<kD>, static_cast<uint16_t *>(p.r.out), [&](int db, int q) {
-        return f32x4_t{oacc[db][4 * q] * inv, oacc[db][4 * q + 1] * inv, oacc[db][4 * q + 2] * inv, oacc[db][4 * q + 3] * inv};
-      }, [&](int i) {
+      store_rows<kD, kBf16>(smem + wave * kRowsLds<kD>, static_cast<uint16_t *>(p.r.out), answer, [&](int i) {
         const int row = wave * 32 + i, in_tile = int(__umulhi(2u * uint32_t(row), p.r.group_magic)), tok = tok0 + in_tile;
         return tok < tok_end ? (int64_t(begin + tok) * p.r.hq + h * p.r.group + (row - in_tile * p.r.group)) * kD : int64_t(-1);
       });
@@ -681,16 +746,16 @@ __global__ __launch_bounds__(64 * waves_of(kD), waves_of(kD) * groups_per_cu(kD)
     // As the registers hold it: 1 KiB for each of the wavefront's quads of dims.
     const size_t rows = size_t(part) * kRows + wave * 32;
     if (hf == 0) {
-      p.part_ml[2 * (rows + n)] = m;
-      p.part_ml[2 * (rows + n) + 1] = l * __builtin_amdgcn_exp2f(-base);
+      // l in [1/2, 1): r may lie far below or above the logits.
+      const int e = __builtin_amdgcn_frexp_expf(l);
+      p.part_ml[2 * (rows + n)] = (apart ? m : r) + float(e);
+      p.part_ml[2 * (rows + n) + 1] = __builtin_amdgcn_ldexpf(l, -e);
     }
     f32x4_t *o = reinterpret_cast<f32x4_t *>(p.part_o + rows * kD) + lane;
 #pragma unroll
     for (int db = 0; db < kDB; ++db)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        o[64 * (4 * db + q)] =
-            f32x4_t{oacc[db][4 * q] * inv, oacc[db][4 * q + 1] * inv, oacc[db][4 * q + 2] * inv, oacc[db][4 * q + 3] * inv};
+      for (int q = 0; q < 4; ++q) o[64 * (4 * db + q)] = answer(db, q);
   }
   }
 }
@@ -730,9 +795,8 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(const WindowParam
   const int4 it = p.items[2 * item];
   const int begin = p.items[2 * item + 1].x, count = p.items[2 * item + 1].y;
   auto rows_of_part = [&](int s) { return size_t(2 * s + (s < w1 || ends ? 1 : 0)) * kRows + block * 32; };
-  float m = -__builtin_inff();
+  float m = kNone;
   for (int s = w0; s <= w1; ++s) m = fmaxf(m, p.part_ml[2 * (rows_of_part(s) + n)]);
-  if (m == -__builtin_inff()) m = 0.f;
   float total = 0.f;
   f32x4_t acc[kQuads];
 #pragma unroll
