@@ -121,6 +121,13 @@ __device__ __forceinline__ int wave_prefix(int v) {
   return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
 }
 
+// Bit 7 of each byte: it is no infinity (0x6F, 0xEF) and no NaN (0x80).  The other bits
+// mean nothing; words are joined by `and`.
+__device__ __forceinline__ uint32_t finite_bytes(uint32_t w) {
+  const uint32_t size = w & 0x7F7F7F7Fu;
+  return ((size ^ 0x6F6F6F6Fu) + 0x7F7F7F7Fu) & ((size + 0x7F7F7F7Fu) | ~w);
+}
+
 // True when some byte of w is an infinity (0x6F, 0xEF) or NaN (0x80); may also
 // be true next to such a byte, never false on one.
 __device__ __forceinline__ bool some_not_finite(uint32_t w) {

@@ -202,9 +202,9 @@ constexpr int tile_rows_of(int d, int row_blocks, bool win, bool rest) {
 // Whether what P's rounding to fp16 leaves is multiplied too, as a second P: under a
 // window with an fp16 output, which rounds no further than P does (error against
 // float64 3.0e-4 without and 2.1e-4 with it; a bf16 output's own is 1.7e-3).  8
-// requests within 4096 rows, 16 / 4 heads of 256: one token 28.1 -> 28.7 us, 6 rows
-// 37.6 -> 38.9, 40 rows 71 -> 81; 32 / 8 heads of 128, 40 rows 86 -> 101; 16 / 4 of
-// 64, 40 rows 42 -> 53.
+// requests within 4096 rows, 16 / 4 heads of 256: one token 28.1 -> 28.9 us, 6 rows
+// 37.6 -> 39.5, 40 rows 71 -> 84; 32 / 8 heads of 128, 40 rows 86 -> 104; 16 / 4 of
+// 64, 40 rows 42 -> 54.  1 to 4 % of a call is the look for infinities in V.
 constexpr bool rest_of(bool bf16, bool window) { return window && !bf16; }
 
 template <int kD, bool kBf16, int kRB, bool kX, bool kWin, typename BtT>
@@ -764,9 +764,20 @@ __global__ __launch_bounds__(64 * waves_of(kD, kRB, kWin, rest_of(kBf16, kWin)),
     for (int rb = 0; rb < kRB; ++rb) l[rb] += psum[rb];
     // O^T += V^T P^T: slots 8 g + e of a 32-row step are rows 4 g + e of its
     // first 16, then of its second 16, as P lies in LDS.
-    if (!full) {
-      // Rows that are not there, then infinities and NaN among the drafts (or at a
-      // window's edges): a query row that does not see one must not meet it in the product.
+    bool apart = !full;
+    if (kRest && full) {
+      // Two products of an infinity, with P and with what its rounding leaves, which is zero or of
+      // the other sign, would be a NaN.
+      uint32_t finite = 0x80808080u;
+#pragma unroll
+      for (int i = 0; i < kVR / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) finite &= finite_bytes(vraw[i][j]);
+      apart = __any(finite != 0x80808080u);
+    }
+    if (apart) {
+      // Rows that are not there, then infinities and NaN among the drafts (or within a
+      // window): a query row that does not see one must not meet it in the product.
       bool odd = false;
 #pragma unroll
       for (int j = 0; j < kVR / 16; ++j)
