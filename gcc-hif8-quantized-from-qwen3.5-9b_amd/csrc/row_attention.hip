@@ -113,11 +113,11 @@ __global__ __launch_bounds__(kThreads) void row_attention_any(const RowAttnParam
     f[w] = red_ml[w][1] != 0.f ? __builtin_amdgcn_exp2f(red_ml[w][0] - mx) : 0.f;
     total += f[w] * red_ml[w][1];
   }
-  if (threadIdx.x == 0) {
+  const bool whole = p.num_splits == 1;      // the join leaves the output to this workgroup
+  if (threadIdx.x == 0 && (!whole || p.x)) { // one split's are read for weights alone, and there is no room for others
     p.part_ml[2 * part] = mx;
     p.part_ml[2 * part + 1] = total;
   }
-  const bool whole = p.num_splits == 1;      // the join leaves the output to this workgroup
   if (!whole && !(total != 0.f)) return;     // nothing seen: this split's outputs are not read
   const float inv = total != 0.f ? 1.f / total : 0.f;
   for (int dim = threadIdx.x; dim < p.dv; dim += kThreads) {
@@ -1179,7 +1179,8 @@ RowSpace row_space(const RowPlan &pl, int64_t batch, int64_t total_q, int64_t he
   auto round = [](size_t v) { return (v + 255) / 256 * 256; };
   RowSpace w{};
   w.o = round(size_t(pl.outputs) * dv * sizeof(float));
-  w.ml = round(size_t(pl.parts) * 2 * sizeof(float));
+  const bool unread = !pl.row_blocks && pl.num_splits == 1 && !weights;
+  w.ml = round(unread ? 1 : size_t(pl.parts) * 2 * sizeof(float));
   if (weights) w.x = round(size_t(total_q) * heads * size_t(x_stride_of(max_len)) * sizeof(float));
   if (pl.row_blocks) w.plan = round(size_t(batch + 1) * sizeof(int32_t));
   return w;

@@ -32,6 +32,9 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+// Query and output rows: global memory takes any alignment in one access.
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32_a2 __attribute__((aligned(2)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
@@ -431,7 +434,7 @@ __device__ __forceinline__ void store_rows(uint8_t *lds, uint16_t *out, Value va
     const int row = i + lane / kPerRow, piece = lane % kPerRow;
     const u32x4 v = *reinterpret_cast<const u32x4 *>(lds + row * kPitch + 16 * piece);
     const int64_t to = at(row);
-    if (to >= 0) *reinterpret_cast<u32x4 *>(out + to + 8 * piece) = v;
+    if (to >= 0) *reinterpret_cast<u32x4_a2 *>(out + to + 8 * piece) = v;
   }
 }
 
@@ -465,7 +468,7 @@ __global__ __launch_bounds__(64 * waves_of(kD), waves_of(kD) * groups_per_cu(kD)
     const int64_t all = int64_t(p.r.total_q - min(count, p.r.total_q)) * words;
     for (int64_t i = int64_t(blockIdx.x) * 64 * kWaves + tid; i < all; i += int64_t(gridDim.x) * 64 * kWaves) {
       const int row = int(i / words);
-      static_cast<uint32_t *>(p.r.out)[i + (row < begin ? 0 : int64_t(count) * words)] = 0;
+      static_cast<u32_a2 *>(p.r.out)[i + (row < begin ? 0 : int64_t(count) * words)] = 0;
     }
   }
   // Neighbouring runs see nearly the same images: they are one XCD's.
@@ -527,7 +530,7 @@ __global__ __launch_bounds__(64 * waves_of(kD), waves_of(kD) * groups_per_cu(kD)
   {
     const uint16_t *q = static_cast<const uint16_t *>(p.r.query) + mine.at + 8 * hf;
 #pragma unroll
-    for (int i = 0; i < kQS; ++i) qf[i] = *reinterpret_cast<const u32x4 *>(q + 16 * i);
+    for (int i = 0; i < kQS; ++i) qf[i] = *reinterpret_cast<const u32x4_a2 *>(q + 16 * i);
   }
   lds_barrier();  // the segment before is done with both stages
   copy(t_begin, 0);
@@ -781,7 +784,7 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(const WindowParam
       const int begin = p.items[2 * item + 1].x, count = p.items[2 * item + 1].y;
       const int words = p.r.group * (kD / 2), rows = min(p.tokens, count - it.w);
       for (int i = tid; i < rows * words; i += kThreads)
-        static_cast<uint32_t *>(p.r.out)[(size_t(begin + it.w + i / words) * p.r.hq + it.z * p.r.group) * (kD / 2) + i % words] = 0;
+        static_cast<u32_a2 *>(p.r.out)[(size_t(begin + it.w + i / words) * p.r.hq + it.z * p.r.group) * (kD / 2) + i % words] = 0;
     }
     return;
   }
@@ -833,8 +836,8 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(const WindowParam
     const int in = i / (kD / 8), piece = i % (kD / 8), row = block * 32 + in;
     const int in_tile = int(__umulhi(2u * uint32_t(row), p.r.group_magic)), tok = it.w + in_tile;
     if (in_tile < p.tokens && tok < count)
-      *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p.r.out) +
-                                 (size_t(begin + tok) * p.r.hq + it.z * p.r.group + (row - in_tile * p.r.group)) * kD + 8 * piece) =
+      *reinterpret_cast<u32x4_a2 *>(static_cast<uint16_t *>(p.r.out) +
+                                    (size_t(begin + tok) * p.r.hq + it.z * p.r.group + (row - in_tile * p.r.group)) * kD + 8 * piece) =
           *reinterpret_cast<const u32x4 *>(rows_lds + in * (2 * kD + 16) + 16 * piece);
   }
 }
@@ -945,12 +948,9 @@ extern "C" size_t hif8_window_attention_workspace_size(int64_t batch, int64_t nu
       num_heads % num_kv_heads)
     return 0;
   window = std::min<int64_t>(window, 0x7FFFFFFF), sinks = std::min<int64_t>(sinks, 0x7FFFFFFF);
-  const WindowPlan pl = plan_window(batch, num_heads, num_kv_heads, head_size, head_size_v, block_size,
-                                    total_query_tokens, max_query_len, max_seq_len, window, sinks);
-  // Bytes for either: the query's alignment, which also decides, is not known here.
-  return std::max(pl.total(), row_workspace(batch, total_query_tokens, num_heads, num_kv_heads, head_size, head_size_v,
-                                            block_size, max_query_len,
-                                            rows_bound(max_seq_len, max_query_len, window, sinks), false));
+  return plan_window(batch, num_heads, num_kv_heads, head_size, head_size_v, block_size, total_query_tokens,
+                     max_query_len, max_seq_len, window, sinks)
+      .total();
 }
 
 extern "C" int hif8_window_attention(const void *query, int q_dtype, const uint8_t *key_cache,
@@ -990,7 +990,7 @@ extern "C" int hif8_window_attention(const void *query, int q_dtype, const uint8
                 workspace_bytes);
   const WindowPlan pl = plan_window(batch, num_heads, num_kv_heads, head_size, head_size_v, block_size,
                                     total_query_tokens, max_query_len, max_seq_len, window, sinks);
-  if (pl.requests == 0 || !aligned(query, 16) || !aligned(out, 16)) return row_attention(kName, a);
+  if (pl.requests == 0) return row_attention(kName, a);
   if (!aligned(workspace, 16))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", kName);
   if (pl.items > 0x1FFFFF || pl.items * (pl.tiles + kStart) > 0x7FFFFFFF || pl.slots * num_kv_heads * (pl.tiles + 8) > 0xFFFFFF)  // threads of a launch

@@ -530,8 +530,10 @@ int hif8_kv_evict(uint8_t *key_cache, uint8_t *value_cache, int64_t num_blocks, 
  *     in 16 bits as in hif8_tree_attention.
  *   workspace  at least hif8_window_attention_workspace_size(...) bytes, 16-byte aligned; its
  *              size depends on these arguments alone
- * D = Dv of 64, 128 or 256 over pages of a multiple of 16 rows, with 16-byte aligned query and
- * out, runs on the matrix cores; any other shape takes a kernel that is many times slower.
+ * D = Dv of 64, 128 or 256 over pages of a multiple of 16 rows runs on the matrix cores: requests
+ * of more than 256 (row, head) pairs per KV head at any alignment (one of 512 or fewer that is alone
+ * counts as few), those of fewer where query and out are 16-byte aligned.  Anything else takes a
+ * kernel that is many times slower.
  */
 size_t hif8_window_attention_workspace_size(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
                                             int64_t head_size_v, int64_t block_size, int64_t total_query_tokens,
