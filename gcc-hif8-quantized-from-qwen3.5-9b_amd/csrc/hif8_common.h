@@ -35,6 +35,14 @@ static __device__ const Tables kDeviceTables = make_tables();
 
 constexpr int kWave = 64;
 
+// Query rows begin .. begin + count - 1 of request b, clipped to the call's `total` (start_loc is
+// caller data).  Neither end is below zero when they are subtracted: the difference of any two
+// 32-bit numbers may wrap to a large count.
+__device__ __forceinline__ void clipped_rows(const int32_t *start_loc, int b, int total, int &begin, int &count) {
+  begin = max(start_loc[b], 0);
+  count = max(min(max(start_loc[b + 1], 0), total) - begin, 0);
+}
+
 template <bool kBf16>
 __device__ __forceinline__ float half_bits_to_float(uint32_t h) {
   if constexpr (kBf16) {

@@ -44,8 +44,8 @@ __device__ __forceinline__ int clamp_rows(int n, int most) { return n < 0 ? 0 : 
 
 // Query rows of request b, clipped to the query tensor and to the longest request told (start_loc is caller data).
 __device__ __forceinline__ void request_rows(const WeightParams &p, int b, int &begin, int &count) {
-  begin = max(p.start_loc[b], 0);
-  count = min(max(min(p.start_loc[b + 1], p.total_q) - begin, 0), p.max_query);
+  clipped_rows(p.start_loc, b, p.total_q, begin, count);
+  count = min(count, p.max_query);
 }
 
 // Rows that query row i of a request with `len` cached rows sees.

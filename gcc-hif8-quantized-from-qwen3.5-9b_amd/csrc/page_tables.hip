@@ -20,12 +20,6 @@ constexpr int kScan = 1024;  // threads of a workgroup that ranks entries: sixte
 constexpr int kScanWaves = kScan / kWave;
 constexpr int kRowThreads = 256;
 
-// A request's new rows, clipped to the call's (start_loc is caller data).
-__device__ __forceinline__ void new_rows(const int32_t *start_loc, int b, int total, int &begin, int &count) {
-  begin = max(start_loc[b], 0);
-  count = max(min(start_loc[b + 1], total) - begin, 0);
-}
-
 // Exclusive sum over the workgroup of what each thread counts; `all` gets the total.
 // sums: kScanWaves + 1 ints of LDS, free again after the next barrier.
 __device__ __forceinline__ int block_exclusive(int mine, int *sums, int &all) {
@@ -102,7 +96,7 @@ __global__ __launch_bounds__(kScan) void extend_kernel(const ExtendParams p) {
     int columns = 0, lo = 0, beyond = 0;
     if (b < p.batch) {
       int begin, n;
-      new_rows(p.start_loc, b, p.total, begin, n);
+      clipped_rows(p.start_loc, b, p.total, begin, n);
       const int64_t ctx = max(p.lens[b], 0), end = ctx + n;
       p.new_lens[b] = int32_t(min(end, int64_t(0x7FFFFFFF)));
       if (n > 0) {
@@ -185,7 +179,7 @@ __global__ __launch_bounds__(kScan) void extend_kernel(const ExtendParams p) {
       else hi = mid - 1;
     }
     int begin, n;
-    new_rows(p.start_loc, b, p.total, begin, n);
+    clipped_rows(p.start_loc, b, p.total, begin, n);
     put_slot<BtT>(p, row, b, begin, n);
   }
 }
@@ -202,7 +196,7 @@ __global__ __launch_bounds__(kRowThreads) void slots_kernel(const ExtendParams p
     else hi = mid - 1;
   }
   int begin = 0, n = 0;
-  if (p.batch > 0) new_rows(p.start_loc, b, p.total, begin, n);
+  if (p.batch > 0) clipped_rows(p.start_loc, b, p.total, begin, n);
   put_slot<BtT>(p, row, b, begin, n);
 }
 

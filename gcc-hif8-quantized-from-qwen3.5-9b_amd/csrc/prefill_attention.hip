@@ -94,8 +94,8 @@ struct PrefillParams {
 // nor cost image bytes.  Every wavefront of a workgroup evaluates these
 // itself from query_start_loc; the results are uniform.
 __device__ __forceinline__ bool request_is_long(const PrefillParams &p, int b) {
-  const int q_begin = max(p.query_start_loc[b], 0);
-  const int ql = min(p.query_start_loc[b + 1], p.total_q) - q_begin;
+  int q_begin, ql;
+  clipped_rows(p.query_start_loc, b, p.total_q, q_begin, ql);
   return ql > 0 && int64_t(ql) * p.group > int64_t(p.long_rows);
 }
 
@@ -391,9 +391,8 @@ __global__ __launch_bounds__(kPThreads, 2) void paged_prefill_attention_kernel(c
   const int b = rb % p.batch;
   const int qt = p.q_tiles - 1 - rb / p.batch;
   if (request_has_images(p, b)) return;  // that request runs on the tile-image path (uniform)
-  // A request's rows, clipped to the query tensor (query_start_loc is caller data).
-  const int q_begin = max(p.query_start_loc[b], 0);
-  const int ql = min(p.query_start_loc[b + 1], p.total_q) - q_begin;
+  int q_begin, ql;
+  clipped_rows(p.query_start_loc, b, p.total_q, q_begin, ql);
   const int tok0 = qt * p.tokens_per_tile;
   if (tok0 >= ql) return;  // a query tile past this request's rows (uniform)
   const int kl = clamp_len(p.seq_lens[b], p.max_len);
@@ -595,8 +594,8 @@ __global__ __launch_bounds__(kWaves * 64) void paged_prefill_attention_img_kerne
   const int qt = p.q_tiles - 1 - rq / p.slots;
   const int b = request_of_slot(p, slot);
   if (b < 0) return;  // an unused slot (uniform)
-  const int q_begin = max(p.query_start_loc[b], 0);
-  const int ql = min(p.query_start_loc[b + 1], p.total_q) - q_begin;
+  int q_begin, ql;
+  clipped_rows(p.query_start_loc, b, p.total_q, q_begin, ql);
   const int tok0 = qt * p.tokens_per_tile;
   if (tok0 >= ql) return;  // uniform
   const int kl = clamp_len(p.seq_lens[b], p.max_len);
@@ -715,8 +714,8 @@ __global__ __launch_bounds__(kPThreads) void prefill_combine_kernel(const Prefil
   const int rq = item / (p.hkv * p.q_tiles);
   const int b = kSlots ? request_of_slot(p, rq) : rq;
   if (b < 0 || (!kSlots && request_has_images(p, b))) return;  // uniform
-  const int q_begin = max(p.query_start_loc[b], 0);
-  const int ql = min(p.query_start_loc[b + 1], p.total_q) - q_begin;
+  int q_begin, ql;
+  clipped_rows(p.query_start_loc, b, p.total_q, q_begin, ql);
   const int tok = qt * p.tokens_per_tile + (r >> p.log2_group);
   if (r >= kRows || tok >= ql) return;  // wavefront-uniform: a row past the request
   const size_t base = size_t(item) * p.num_splits * kRows + r;  // part index of split 0
@@ -766,8 +765,8 @@ __global__ __launch_bounds__(kWave) void paged_prefill_attention_simple(const Pr
     else hi = mid - 1;
   }
   const int b = lo;
-  const int q_begin = p.query_start_loc[b];
-  const int ql = p.query_start_loc[b + 1] - q_begin;
+  int q_begin, ql;
+  clipped_rows(p.query_start_loc, b, total_q, q_begin, ql);
   if (row < q_begin || row - q_begin >= ql) return;  // rows outside every request
   const int kl = clamp_len(p.seq_lens[b], p.max_len);
   const int lim = p.causal ? min(kl, kl - ql + (row - q_begin) + 1) : kl;

@@ -87,8 +87,7 @@ __device__ __forceinline__ void request_rows(const RowAttnParams &p, int b, int 
     count = 1;
     return;
   }
-  begin = max(p.start_loc[b], 0);
-  count = max(min(p.start_loc[b + 1], p.total_q) - begin, 0);
+  clipped_rows(p.start_loc, b, p.total_q, begin, count);
 }
 
 // The request of a query row, or -1: the last b with start_loc[b] <= row.

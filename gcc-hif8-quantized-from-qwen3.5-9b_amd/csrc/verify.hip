@@ -69,8 +69,8 @@ struct Nodes {
 
 // The request's rows, clipped to the call's and to its width.
 __device__ __forceinline__ void rows_of(const VerifyParams &p, int b, int &begin, int &count) {
-  begin = max(p.start_loc[b], 0);
-  count = max(min(min(p.start_loc[b + 1], p.total) - begin, p.width), 0);
+  clipped_rows(p.start_loc, b, p.total, begin, count);
+  count = min(count, p.width);
 }
 
 __device__ __forceinline__ int parent_of(const VerifyParams &p, int begin, int i) {
