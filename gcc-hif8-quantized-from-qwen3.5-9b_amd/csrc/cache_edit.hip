@@ -412,6 +412,8 @@ extern "C" int hif8_accept_drafts(void *const *caches, const int64_t *row_bytes,
   for (int64_t i = 1; i < num_caches; ++i)
     if (spans[i].first - spans[i - 1].first < spans[i - 1].bytes)
       return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: caches must not overlap", kName);
+  if (new_lens && share(context_lens, new_lens, batch))  // other workgroups have yet to read the lengths
+    return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: new_lens must not overlap context_lens", kName);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const auto launch = [&](auto most) {
     constexpr int kCaches = decltype(most)::value;
@@ -482,6 +484,8 @@ extern "C" int hif8_kv_evict(uint8_t *key_cache, uint8_t *value_cache, int64_t n
                 workspace_bytes);
   if (!aligned(workspace, 16))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", kName);
+  if (share(seq_lens, new_lens, batch))  // other KV heads have yet to read the lengths
+    return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: new_lens must not overlap seq_lens", kName);
   EvictParams p{};
   p.key_cache = reinterpret_cast<uint32_t *>(key_cache);
   p.value_cache = reinterpret_cast<uint32_t *>(value_cache);

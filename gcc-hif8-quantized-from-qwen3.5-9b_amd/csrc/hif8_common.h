@@ -25,6 +25,11 @@ void clear_error();
 int reserve_dynamic_lds(const void *kernel, size_t bytes, const char *what);
 
 inline bool is_io_dtype(int d) { return d == HIF8_DTYPE_FP16 || d == HIF8_DTYPE_BF16; }
+// Whether two arrays of n 32-bit numbers share one.
+inline bool share(const int32_t *a, const int32_t *b, int64_t n) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return (x > y ? x - y : y - x) < uintptr_t(n) * sizeof(int32_t);
+}
 inline bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // The constexpr-built tables in device global memory (one ~9.5 KiB copy per

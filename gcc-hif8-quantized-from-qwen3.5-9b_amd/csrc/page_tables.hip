@@ -324,6 +324,8 @@ extern "C" int hif8_extend_block_tables(void *block_table, int block_table_dtype
       (batch && (!block_table || !free_count || !context_lens || !seq_lens || !missing)) ||
       (free_capacity && !free_blocks))
     return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: null pointer argument", kName);
+  if (batch && share(context_lens, seq_lens, batch))  // the slots are worked out from the lengths before
+    return fail(HIF8_ERR_INVALID_ARGUMENT, "%s: seq_lens must not overlap context_lens", kName);
   ExtendParams p{block_table, free_blocks, free_count, context_lens, query_start_loc, slot_mapping, positions,
                  seq_lens, missing, max_blocks_per_seq, free_capacity, int(batch), int(total_query_tokens),
                  int(block_size), batch <= kScan && total_query_tokens <= kFewRows ? 1 : 0};

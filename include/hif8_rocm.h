@@ -481,7 +481,8 @@ int hif8_key_weights(const void *query, int q_dtype, const uint8_t *key_cache, i
  *   accepted [batch, accepted_width] int32: draft indices in strictly rising order (a path
  *     from the root: parents come before children); not rising, the rows' contents are
  *     unspecified, the accesses stay inside the cache
- *   new_lens [batch] int32 (may be NULL): context_lens[b] + accepted_counts[b]
+ *   new_lens [batch] int32 (may be NULL): context_lens[b] + accepted_counts[b]; not in
+ *     context_lens's place
  * Rows outside the table or in a block outside [0, num_blocks) are skipped.  The pages
  * that are written must belong to one request.  Without caches or requests nothing is
  * done: the call succeeds and new_lens is left as it was.
@@ -502,7 +503,7 @@ int hif8_accept_drafts(void *const *caches, const int64_t *row_bytes, int64_t nu
  *   key_weights [batch, Hkv, weights_stride] float32; positions the same shape in int32, or
  *     NULL (then a row's position is its index)
  *   keep [batch] int32, or NULL for keep_all of every request; protect_from [batch] int32 or NULL
- *   new_lens [batch] int32: n
+ *   new_lens [batch] int32: n; not in seq_lens's place
  * Rows in a block outside [0, num_blocks) are not copied.  Pages must belong to one request.
  */
 size_t hif8_kv_evict_workspace_size(int64_t batch, int64_t num_kv_heads, int64_t max_seq_len);
@@ -586,7 +587,7 @@ int hif8_verify_drafts(const float *target_probs, int64_t target_stride, const f
  * and *free_count change in place.
  *   slot_mapping, positions [total_query_tokens] int64: table entry * block_size + offset, or
  *     -1 where there is no page, and the position in the request; both -1 for rows of no request
- *   seq_lens [batch] int32: context_lens + the new rows
+ *   seq_lens [batch] int32: context_lens + the new rows; not in context_lens's place
  *   missing [batch] int32: columns that got no page (the stack was empty, or the table too narrow)
  */
 int hif8_extend_block_tables(void *block_table, int block_table_dtype, int64_t max_blocks_per_seq,
