@@ -128,7 +128,8 @@ __global__ __launch_bounds__(kScan) void extend_kernel(const ExtendParams p) {
         for (int j = 0; j < kPer; ++j) {
           const uint32_t c = c0 + kScan * j + tid;
           const int r = owner[j];
-          entry[j] = static_cast<BtT *>(p.table) + int64_t(base + r) * p.width + (int64_t(low[r]) + c - first[r]);
+          // `first` wraps past 2^31 as c does (starts that go back and forth give every request many rows).
+          entry[j] = static_cast<BtT *>(p.table) + int64_t(base + r) * p.width + low[r] + int64_t(c - uint32_t(first[r]));
           id[j] = c < uint32_t(total) ? *entry[j] : BtT(0);
         }
         uint64_t wants[kPer];
