@@ -136,15 +136,17 @@ def _check_caches(key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
         raise ValueError("key_cache and value_cache must have the same blocks and heads")
 
 
-def _check_window(window: int | None, sinks: int) -> None:
+def _check_window(window: int | None, sinks: int) -> tuple[int | None, int]:
+    """Both as the operators take them: integers of 64 bits, past every length where they were larger."""
     if window is None:
         if sinks:
             raise ValueError("sinks need a window")
-        return
+        return None, 0
     if isinstance(window, bool) or not isinstance(window, int) or window < 1:
         raise ValueError(f"window must be a positive integer, got {window}")
     if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
         raise ValueError(f"sinks must be a non-negative integer, got {sinks}")
+    return min(window, 1 << 62), min(sinks, 1 << 62)
 
 
 def _pages_in_window(lens: torch.Tensor, query_lens, columns: int, block_size: int, window: int, sinks: int):
@@ -230,7 +232,7 @@ def paged_decode_attention(
     them) and the first ``sinks`` alone, as in :func:`paged_attention`.
     """
     _check_caches(key_cache, value_cache)
-    _check_window(window, sinks)
+    window, sinks = _check_window(window, sinks)
     if query.ndim != 3:
         raise ValueError("query must have shape [tokens, num_heads, head_size]")
     batch = query.shape[0]
@@ -325,7 +327,7 @@ def paged_attention(
     fast, are those of :func:`tree_attention`.
     """
     _check_caches(key_cache, value_cache)
-    _check_window(window, sinks)
+    window, sinks = _check_window(window, sinks)
     if window is not None and not causal:
         raise ValueError("a window needs causal attention")
     if query.ndim != 3:
@@ -981,7 +983,7 @@ def release_blocks(
     become -1) for the end of ``free_blocks``, in the order (request, column);
     length 0 gives back all of a request.  Pages must belong to one request.
     """
-    _check_window(window, sinks)
+    window, sinks = _check_window(window, sinks)
     lens = _check_pool(block_table, free_blocks, free_count, seq_lens, "seq_lens", block_size, validate)
     extension = native.load_extension()
     native._operator("hif8_release_blocks", extension)(
