@@ -226,8 +226,9 @@ __device__ __forceinline__ Room room_of(float most, float least) {
 }
 
 // A workgroup per (slot, KV head, kThreads / D * 32 rows): threads take 16 codes of a K
-// row, and 4 codes of eight V rows each.  Bound by the bytes (4 of image and 1 of cache
-// per element): 4 x 4608 rows of 4 KV heads of 256, 114 MB, 31 us (3.7 TB/s).  The KV
+// row, and 4 codes of eight V rows each.  Bound by the bytes (4 of image and 2 of cache
+// per (row, dim), K and V together): 4 x 4608 rows of 4 KV heads of 256, 113 MB, 31 us
+// (3.7 TB/s).  The KV
 // heads of one tile, whose rows share cache lines, have block ids equal modulo 8: one XCD.
 template <int kD, bool kBf16, typename BtT>
 __global__ __launch_bounds__(kThreads) void window_image_kernel(const WindowParams p) {
