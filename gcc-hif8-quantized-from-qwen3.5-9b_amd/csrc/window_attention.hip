@@ -847,7 +847,8 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(const WindowParam
 
 // Requests of more (token, head) rows per KV head than this run on images: kOnlyRows for a
 // call's only request, which cannot fill the GPU with its images' items, kLongRows for one of
-// several.  Images against the other kernels, us, 8 KV heads of 128, groups of 4, 16-row pages:
+// several.  Images against the other kernels, us, 8 KV heads of 128, groups of 4, 16-row pages
+// (the one shape that both were measured at):
 //   requests, window   256 rows     384        512        768
 //   1 of 1024          60 vs 27   61 vs 26   49 vs 30   50 vs 40
 //   1 of 4096          64 vs 35   69 vs 41   60 vs 46   63 vs 69
